@@ -34,6 +34,9 @@ SOURCES = [
     "densify.hip",
     "loss.hip",
     "adam.hip",
+    "lookup.hip",
+    "gated_scan.hip",
+    "grouped.hip",
 ]
 
 ARCH = os.environ.get("R2S_OFFLOAD_ARCH", "gfx950")

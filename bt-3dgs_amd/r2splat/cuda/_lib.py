@@ -125,6 +125,23 @@ _PLAIN = {
     "r2s_hierarchy_workspace_bytes": (_i64, [_i64]),
     "r2s_hierarchy_loss_fwd_f32": (_i32, [_p, _p, _i64, _p, _p, _p, _i64, _f32, _p, _p, _sz, _p]),
     "r2s_hierarchy_loss_bwd_f32": (_i32, [_i64, _p, _p, _p, _sz, _p, _p]),
+    "r2s_group_rows_workspace_bytes": (_i64, [_i64, _i64]),
+    "r2s_group_rows": (_i32, [_p, _i32, _i64, _i64, _p, _p, _p, _sz, _p]),
+    "r2s_embedding_fwd": (_i32, [_p, _i64, _p, _i32, _f32, _i32, _i64, _i64, _i64, _p, _p]),
+    "r2s_embedding_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "r2s_embedding_bwd": (_i32, [_p, _i64, _p, _i32, _f32, _i32, _i64, _i64, _i64, _p, _p, _sz,
+                                 _p]),
+    "r2s_gated_scan_tiles": (_i64, [_i32, _i64, _i64]),
+    "r2s_gated_scan_workspace_bytes": (_i64, [_i32, _i64, _i64, _i32]),
+    "r2s_gated_scan_fwd": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32, _i32,
+                                  _p, _p, _p, _p, _sz, _p]),
+    "r2s_gated_scan_bwd": (_i32, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64,
+                                  _i64, _i32, _i32, _p, _p, _p, _p, _sz, _p]),
+    "r2s_grouped_matmul_fwd": (_i32, [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _p,
+                                      _p]),
+    "r2s_grouped_matmul_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "r2s_grouped_matmul_bwd": (_i32, [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                                      _i32, _p, _p, _p, _p, _sz, _p]),
 }
 
 
@@ -156,10 +173,12 @@ class AdamTensor(ctypes.Structure):
 COL_COPY, COL_ZERO_NEW, COL_MEANS, COL_RAW_SCALES, COL_RAW_OPACITIES, COL_PARENT, COL_LEVEL, \
     COL_HISTORY = range(8)
 DENSIFY_MAX_WIDTH = 16
+# Element types of the latent decoder's operators (R2S_TYPE_*).
+TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
 
 SYMBOLS = sorted(list(_PLAIN) + [f"r2s_{n}_{s}" for n in _FLOAT_OPS for s in ("f32", "f64")])
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 def load(path: str = LIB_PATH) -> ctypes.CDLL:

@@ -21,6 +21,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _backend
+from . import _lib as L
 
 Tensor = torch.Tensor
 
@@ -1534,8 +1535,6 @@ _COLUMN = struct.Struct("@PPPqii")  # _lib.Column, packed in one call
 def _densify_columns(columns, n_rows: int, hist_rows: int, what: str) -> list:
     """Check the columns; each one's values per row.  Nothing here depends on
     how many rows are selected, so it runs while the device counts them."""
-    from . import _lib as L
-
     widths = []
     for i, col in enumerate(columns):
         src, role, extra = col
@@ -1579,8 +1578,6 @@ def _densify_columns(columns, n_rows: int, hist_rows: int, what: str) -> list:
 def _densify_table(columns, widths, main_rows: int, hist_rows: int, n_sel: int):
     """The library's column table and the output tensors for columns that
     :func:`_densify_columns` checked."""
-    from . import _lib as L
-
     table = (L.Column * max(len(columns), 1))()
     outs, used = [], 0
     for (src, role, extra), width in zip(columns, widths):
@@ -1619,8 +1616,6 @@ def densify_split(mask: Tensor, columns, history_rows: int = 0, geometry=None):
     table, required by the MEANS / RAW_SCALES roles.  Returns
     ``(outputs, n_sel)`` with outputs in column order.
     """
-    from . import _lib as L
-
     n = int(mask.shape[0]) if isinstance(mask, torch.Tensor) and mask.dim() == 1 else -1
     m = _densify_mask(mask, n, "densify_split")
     idx, count = _mask_split_enqueue(m)
@@ -1884,3 +1879,282 @@ def hierarchy_loss_bwd(n: int, grad_out: Tensor, out: Tensor, workspace: Tensor)
         _call("r2s_hierarchy_loss_bwd_f32", n, _ptr(g), _ptr(out), _ptr(workspace),
               workspace.numel(), _ptr(v), _stream(dev))
     return v
+
+
+# ------------------------------------------------------------ latent decoder --
+#
+# No reference counterpart.  Activations, tables and weights are float32,
+# bfloat16 or float16 (one type per call); states are float32.  Inputs whose
+# rows are not dense are taken with their row stride where the elements of a
+# row are consecutive, else copied.
+
+_LATENT_TYPES = {torch.float32: L.TYPE_F32, torch.bfloat16: L.TYPE_BF16,
+                 torch.float16: L.TYPE_F16}
+
+
+def _latent_type(t: Tensor, op: str) -> int:
+    code = _LATENT_TYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f'"{op}" not implemented for \'{t.dtype}\'')
+    return code
+
+
+def _check_latent(t, name: str, like: Optional[Tensor] = None, dtype=None) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if like is not None and t.device != like.device:
+        raise RuntimeError(f"{name} must be on the device of the other inputs")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _rows_2d(t: Tensor, align: int = 1):
+    """(tensor, row stride) of a 2-D tensor whose rows' elements are
+    consecutive; a copy where they are not, where rows overlap or where a row
+    does not start at a multiple of ``align`` bytes."""
+    n, d = t.shape
+    stride = t.stride(0) if n > 1 else d
+    if (d > 1 and t.stride(1) != 1) or stride < d or \
+            (align > 1 and (t.data_ptr() % align or (stride * t.element_size()) % align)):
+        t = torch.empty_strided((n, d), (d, 1), dtype=t.dtype, device=t.device).copy_(t)
+        stride = d
+    return t, max(stride, d)
+
+
+def _check_ids(ids: Tensor, name: str, like: Tensor) -> Tensor:
+    _check_latent(ids, name, like)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{name} must be int32 or int64, got {ids.dtype}")
+    return ids.contiguous()
+
+
+def group_rows(ids: Tensor, n_groups: int) -> Tuple[Tensor, Tensor]:
+    """(rows [N] int32, offsets [n_groups + 1] int32): the positions of ids [N]
+    in stable order of their id, those of ids outside [0, n_groups) last;
+    offsets[e] the first of group e, offsets[n_groups] the number inside."""
+    _check_latent(ids, "ids")
+    if ids.dim() != 1:
+        _fail("ids must be [N], got shape ", tuple(ids.shape))
+    if n_groups < 0:
+        _fail("n_groups must not be negative, got ", n_groups)
+    ids = _check_ids(ids, "ids", ids)
+    n, dev = ids.numel(), ids.device
+    lib = _lib()
+    with _on(dev):
+        rows = torch.empty((n,), dtype=torch.int32, device=dev)
+        offsets = torch.empty((n_groups + 1,), dtype=torch.int32, device=dev)
+        need = lib.r2s_group_rows_workspace_bytes(n, n_groups)
+        ws = _workspace(need, dev)
+        _call("r2s_group_rows", _ptr(ids), ids.dtype == torch.int64, n, n_groups, _ptr(rows),
+              _ptr(offsets), _ptr(ws), need, _stream(dev))
+    return rows, offsets
+
+
+def embedding_fwd(table: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
+    """scale * table[ids] ([*ids.shape, D]); zero rows where an id is outside
+    [0, V).  table [V, D], ids int32 or int64 of any shape."""
+    _check_latent(table, "table")
+    if table.dim() != 2:
+        _fail("table must be [V, D], got shape ", tuple(table.shape))
+    code = _latent_type(table, "embedding_fwd")
+    ids = _check_ids(ids, "ids", table)
+    table, stride = _rows_2d(table)
+    v, d = table.shape
+    dev = table.device
+    with _on(dev):
+        out = torch.empty((*ids.shape, d), dtype=table.dtype, device=dev)
+        _call("r2s_embedding_fwd", _ptr(table), stride, _ptr(ids), ids.dtype == torch.int64,
+              float(scale), code, ids.numel(), v, d, _ptr(out), _stream(dev))
+    return out
+
+
+def embedding_bwd(v_out: Tensor, ids: Tensor, n_rows: int, scale: float = 1.0) -> Tensor:
+    """The table's gradient [n_rows, D] from v_out [*ids.shape, D]: for each row
+    the scaled float32 sum over the positions that name it, the same bits from
+    every call."""
+    _check_latent(v_out, "v_out")
+    code = _latent_type(v_out, "embedding_bwd")
+    ids = _check_ids(ids, "ids", v_out)
+    if v_out.shape[:-1] != ids.shape or v_out.dim() == 0:
+        _fail("v_out must be [*ids.shape, D], got shape ", tuple(v_out.shape))
+    if n_rows < 0:
+        _fail("n_rows must not be negative, got ", n_rows)
+    d, n, dev = v_out.shape[-1], ids.numel(), v_out.device
+    v_out, stride = _rows_2d(v_out.reshape(n, d))
+    lib = _lib()
+    with _on(dev):
+        v_table = torch.empty((n_rows, d), dtype=v_out.dtype, device=dev)
+        need = lib.r2s_embedding_bwd_workspace_bytes(n, n_rows, d)
+        ws = _workspace(need, dev)
+        _call("r2s_embedding_bwd", _ptr(v_out), stride, _ptr(ids), ids.dtype == torch.int64,
+              float(scale), code, n, n_rows, d, _ptr(v_table), _ptr(ws), need, _stream(dev))
+    return v_table
+
+
+def _scan_shape(x: Tensor, offsets: Optional[Tensor]):
+    """(tokens, sequences, tokens per sequence) of [B, L, D] or, with offsets
+    [S + 1], [N, D]."""
+    if offsets is None:
+        if x.dim() != 3:
+            _fail("x must be [B, L, D] without offsets, got shape ", tuple(x.shape))
+        b, length, _ = x.shape
+        return b * length, b, length
+    if x.dim() != 2:
+        _fail("x must be [N, D] with offsets, got shape ", tuple(x.shape))
+    _check_latent(offsets, "offsets", x, torch.int32)
+    if offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
+        _fail("offsets must be a contiguous [S + 1], got shape ", tuple(offsets.shape))
+    if offsets.numel() == 1 and x.shape[0] > 0:
+        _fail("offsets name no sequence for ", x.shape[0], " tokens")
+    return x.shape[0], offsets.numel() - 1, 0
+
+
+def _scan_input(t: Tensor, name: str, x: Tensor, n: int):
+    _check_latent(t, name, x, x.dtype)
+    if t.shape != x.shape:
+        _fail(name, " must have the shape of x ", tuple(x.shape), ", got ", tuple(t.shape))
+    d = x.shape[-1]
+    # Rows of 16-bit elements of an even width are read in pairs.
+    align = 4 if x.element_size() == 2 and d % 2 == 0 else 1
+    return _rows_2d(t.reshape(n, d), align)
+
+
+def _scan_state(t: Optional[Tensor], name: str, x: Tensor, sequences: int) -> Optional[Tensor]:
+    if t is None:
+        return None
+    _check_latent(t, name, x, torch.float32)
+    if t.shape != (sequences, x.shape[-1]):
+        _fail(name, " must be [", sequences, ", ", x.shape[-1], "], got shape ", tuple(t.shape))
+    return t.contiguous()
+
+
+def gated_scan_fwd(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
+                   offsets: Optional[Tensor] = None, reverse: bool = False
+                   ) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y, final, carries) of h_t = a_t h_{t-1} + (1 - a_t) x_t with
+    a_t = sigmoid(gate_t): y the states in x's type, final [S, D] float32 each
+    sequence's last state, carries what gated_scan_bwd takes.  x, gate
+    [B, L, D], or [N, D] with offsets [S + 1] (int32, from 0 to N); initial
+    [S, D] float32; reverse: from each sequence's last token to its first."""
+    _check_latent(x, "x")
+    code = _latent_type(x, "gated_scan_fwd")
+    n, sequences, length = _scan_shape(x, offsets)
+    d, dev = x.shape[-1], x.device
+    xr, xs = _scan_input(x, "x", x, n)
+    gr, gs = _scan_input(gate, "gate", x, n)
+    initial = _scan_state(initial, "initial", x, sequences)
+    lib = _lib()
+    with _on(dev):
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        final = torch.empty((sequences, d), dtype=torch.float32, device=dev)
+        carries = torch.empty((lib.r2s_gated_scan_tiles(code, n, d), d), dtype=torch.float32,
+                              device=dev)
+        need = lib.r2s_gated_scan_workspace_bytes(code, n, d, 0)
+        ws = _workspace(need, dev)
+        _call("r2s_gated_scan_fwd", _ptr(xr), xs, _ptr(gr), gs, _ptr(initial), _ptr(offsets),
+              sequences, length, n, d, code, bool(reverse), _ptr(y), _ptr(final), _ptr(carries),
+              _ptr(ws), need, _stream(dev))
+    return y, final, carries
+
+
+def gated_scan_bwd(x: Tensor, gate: Tensor, initial: Optional[Tensor],
+                   offsets: Optional[Tensor], carries: Tensor, v_y: Tensor,
+                   v_final: Optional[Tensor] = None, reverse: bool = False
+                   ) -> Tuple[Tensor, Tensor, Tensor]:
+    """(v_x, v_gate, v_initial) of gated_scan_fwd with the same inputs, whose
+    carries these are, from v_y (x's shape and type) and v_final [S, D]."""
+    _check_latent(x, "x")
+    code = _latent_type(x, "gated_scan_bwd")
+    n, sequences, length = _scan_shape(x, offsets)
+    d, dev = x.shape[-1], x.device
+    xr, xs = _scan_input(x, "x", x, n)
+    gr, gs = _scan_input(gate, "gate", x, n)
+    vr, vs = _scan_input(v_y, "v_y", x, n)
+    initial = _scan_state(initial, "initial", x, sequences)
+    v_final = _scan_state(v_final, "v_final", x, sequences)
+    lib = _lib()
+    _check_latent(carries, "carries", x, torch.float32)
+    if carries.shape != (lib.r2s_gated_scan_tiles(code, n, d), d) or not carries.is_contiguous():
+        _fail("carries are not those of the forward of these inputs: shape ",
+              tuple(carries.shape))
+    with _on(dev):
+        v_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        v_gate = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        v_initial = torch.empty((sequences, d), dtype=torch.float32, device=dev)
+        need = lib.r2s_gated_scan_workspace_bytes(code, n, d, 1)
+        ws = _workspace(need, dev)
+        _call("r2s_gated_scan_bwd", _ptr(xr), xs, _ptr(gr), gs, _ptr(initial), _ptr(offsets),
+              _ptr(carries), _ptr(vr), vs, _ptr(v_final), sequences, length, n, d, code,
+              bool(reverse), _ptr(v_x), _ptr(v_gate), _ptr(v_initial), _ptr(ws), need,
+              _stream(dev))
+    return v_x, v_gate, v_initial
+
+
+def _check_grouped(x: Tensor, weight: Tensor, offsets: Tensor, rows: Optional[Tensor], op: str):
+    """(type code, n, k, m, groups) of a grouped product's inputs."""
+    _check_latent(x, "x")
+    code = _latent_type(x, op)
+    _check_latent(weight, "weight", x, x.dtype)
+    if x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1]:
+        _fail("x must be [N, K] and weight [E, M, K], got shapes ", tuple(x.shape), " and ",
+              tuple(weight.shape))
+    e, m, k = weight.shape
+    _check_latent(offsets, "offsets", x, torch.int32)
+    if offsets.shape != (e + 1,) or not offsets.is_contiguous():
+        _fail("offsets must be a contiguous [", e + 1, "], got shape ", tuple(offsets.shape))
+    if rows is not None:
+        _check_latent(rows, "rows", x, torch.int32)
+        if rows.shape != (x.shape[0],) or not rows.is_contiguous():
+            _fail("rows must be a contiguous [", x.shape[0], "], got shape ", tuple(rows.shape))
+    return code, x.shape[0], k, m, e
+
+
+def grouped_matmul_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Tensor,
+                       rows: Optional[Tensor] = None) -> Tensor:
+    """y [N, M] with y[r] = weight[e] x[r] + bias[e] for the rows r of group e:
+    rows[offsets[e] : offsets[e + 1]], or those numbers themselves without
+    ``rows`` (a permutation of 0..N-1, as group_rows returns).  Rows in no group
+    give zeros.  x [N, K], weight [E, M, K], bias [E, M], offsets [E + 1]."""
+    code, n, k, m, e = _check_grouped(x, weight, offsets, rows, "grouped_matmul_fwd")
+    if bias is not None:
+        _check_latent(bias, "bias", x, x.dtype)
+        if bias.shape != (e, m):
+            _fail("bias must be [", e, ", ", m, "], got shape ", tuple(bias.shape))
+        bias = bias.contiguous()
+    x, xs = _rows_2d(x)
+    weight = weight.contiguous()
+    dev = x.device
+    with _on(dev):
+        y = torch.empty((n, m), dtype=x.dtype, device=dev)
+        _call("r2s_grouped_matmul_fwd", _ptr(x), xs, _ptr(weight), _ptr(bias), _ptr(offsets),
+              _ptr(rows), n, k, m, e, code, _ptr(y), _stream(dev))
+    return y
+
+
+def grouped_matmul_bwd(x: Tensor, weight: Tensor, offsets: Tensor, rows: Optional[Tensor],
+                       v_y: Tensor, with_bias: bool = False, with_x: bool = True,
+                       with_weight: bool = True
+                       ) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """(v_x, v_weight, v_bias) of grouped_matmul_fwd from v_y [N, M]; None for
+    those not wanted."""
+    code, n, k, m, e = _check_grouped(x, weight, offsets, rows, "grouped_matmul_bwd")
+    _check_latent(v_y, "v_y", x, x.dtype)
+    if v_y.shape != (n, m):
+        _fail("v_y must be [", n, ", ", m, "], got shape ", tuple(v_y.shape))
+    x, xs = _rows_2d(x)
+    v_y, vs = _rows_2d(v_y)
+    weight = weight.contiguous()
+    dev = x.device
+    lib = _lib()
+    with _on(dev):
+        new = lambda want, *shape: (  # noqa: E731
+            torch.empty(shape, dtype=x.dtype, device=dev) if want else None)
+        v_x, v_weight, v_bias = new(with_x, n, k), new(with_weight, e, m, k), new(with_bias, e, m)
+        need = 0
+        if with_weight or with_bias:
+            need = lib.r2s_grouped_matmul_bwd_workspace_bytes(n, k, m, e)
+        ws = _workspace(need, dev)
+        _call("r2s_grouped_matmul_bwd", _ptr(x), xs, _ptr(weight), _ptr(offsets), _ptr(rows),
+              _ptr(v_y), vs, n, k, m, e, code, _ptr(v_x), _ptr(v_weight), _ptr(v_bias), _ptr(ws),
+              need, _stream(dev))
+    return v_x, v_weight, v_bias

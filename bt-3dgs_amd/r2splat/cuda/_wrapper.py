@@ -56,6 +56,15 @@ tv_bwd = _make_cuda_func("tv_bwd")
 hierarchy_loss_fwd = _make_cuda_func("hierarchy_loss_fwd")
 hierarchy_loss_bwd = _make_cuda_func("hierarchy_loss_bwd")
 
+# The latent decoder's operators (no reference counterpart).
+group_rows = _make_cuda_func("group_rows")
+embedding_fwd = _make_cuda_func("embedding_fwd")
+embedding_bwd = _make_cuda_func("embedding_bwd")
+gated_scan_fwd = _make_cuda_func("gated_scan_fwd")
+gated_scan_bwd = _make_cuda_func("gated_scan_bwd")
+grouped_matmul_fwd = _make_cuda_func("grouped_matmul_fwd")
+grouped_matmul_bwd = _make_cuda_func("grouped_matmul_bwd")
+
 
 def is_cuda_extension_available() -> bool:
     try:

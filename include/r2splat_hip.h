@@ -1127,6 +1127,91 @@ typedef struct r2s_adam_tensor {
 int r2s_adam_step_f32(const r2s_adam_tensor_t *tensors, int32_t n_tensors,
                       r2s_stream_t stream);
 
+/* ---------------------------------------------------------------------- */
+/* Latent decoder: row lookup, gated scan, products per group              */
+/* ---------------------------------------------------------------------- */
+
+/* No reference counterpart: the operators of a model that decodes its
+ * Gaussians from a codebook (r2splat.ops.latent).  Activations, tables and
+ * weights are of one R2S_TYPE_*; sums, states and statistics are float32.
+ * A stride is that between rows, in elements; a row's elements are
+ * consecutive. */
+#define R2S_TYPE_F32 0
+#define R2S_TYPE_BF16 1
+#define R2S_TYPE_F16 2
+
+/* Positions 0..n-1 grouped by their ids (int32, or int64 with ids_are_64),
+ * stable: rows [n] in ascending (id, position), those of ids outside
+ * [0, n_groups) last; offsets [n_groups + 1] each group's first index in
+ * rows, offsets[n_groups] the number of ids inside. */
+int64_t r2s_group_rows_workspace_bytes(int64_t n, int64_t n_groups);
+int r2s_group_rows(const void *ids, int32_t ids_are_64, int64_t n, int64_t n_groups,
+                   int32_t *rows, int32_t *offsets, void *workspace, size_t workspace_bytes,
+                   r2s_stream_t stream);
+
+/* out[i] = scale table[ids[i]], i < n; a zero row where the id is outside
+ * [0, n_rows).  table [n_rows, width] of stride table_stride, out [n, width]
+ * contiguous. */
+int r2s_embedding_fwd(const void *table, int64_t table_stride, const void *ids,
+                      int32_t ids_are_64, float scale, int32_t type, int64_t n, int64_t n_rows,
+                      int64_t width, void *out, r2s_stream_t stream);
+/* v_table[v] = scale sum of v_out[i] over the i with ids[i] = v, in ascending
+ * blocks of i (no atomics: the same bits from every call); fully written. */
+int64_t r2s_embedding_bwd_workspace_bytes(int64_t n, int64_t n_rows, int64_t width);
+int r2s_embedding_bwd(const void *v_out, int64_t v_out_stride, const void *ids,
+                      int32_t ids_are_64, float scale, int32_t type, int64_t n, int64_t n_rows,
+                      int64_t width, void *v_table, void *workspace, size_t workspace_bytes,
+                      r2s_stream_t stream);
+
+/* The gated recurrence h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(gate_t),
+ * per channel.  x, gate [n, width] hold `sequences` sequences one behind the
+ * other: of `length` tokens each, or (offsets [sequences + 1] given, ascending
+ * from 0 to n) ragged ones, empty ones among them.  reverse: each sequence
+ * from its last token to its first.  initial [sequences, width] (may be NULL:
+ * zeros) is the history of each sequence's first token, final_state
+ * [sequences, width] the state after its last (its initial one if it is
+ * empty); y [n, width] contiguous.  A gate of +inf holds the state whatever x
+ * is, one of -inf forgets it whatever it was.
+ * carries [r2s_gated_scan_tiles(type, n, width), width] receives the states
+ * that the backward starts from; the decode form (offsets NULL, length 1)
+ * leaves it alone.  Rows of 16-bit elements of an even width must start at
+ * multiples of 4 bytes. */
+int64_t r2s_gated_scan_tiles(int32_t type, int64_t n, int64_t width);
+int64_t r2s_gated_scan_workspace_bytes(int32_t type, int64_t n, int64_t width, int32_t backward);
+int r2s_gated_scan_fwd(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
+                       const float *initial, const int32_t *offsets, int64_t sequences,
+                       int64_t length, int64_t n, int64_t width, int32_t type, int32_t reverse,
+                       void *y, float *final_state, float *carries, void *workspace,
+                       size_t workspace_bytes, r2s_stream_t stream);
+/* Its gradient: v_y [n, width], v_final [sequences, width] (may be NULL) ->
+ * v_x, v_gate [n, width] contiguous, v_initial [sequences, width] (may be
+ * NULL: not wanted).  carries as the forward of the same inputs left them. */
+int r2s_gated_scan_bwd(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
+                       const float *initial, const int32_t *offsets, const float *carries,
+                       const void *v_y, int64_t v_y_stride, const float *v_final,
+                       int64_t sequences, int64_t length, int64_t n, int64_t width, int32_t type,
+                       int32_t reverse, void *v_x, void *v_gate, float *v_initial,
+                       void *workspace, size_t workspace_bytes, r2s_stream_t stream);
+
+/* One weight per group of rows: y[r] = weight[e] x[r] + bias[e] for the rows r
+ * of group e, which are rows[offsets[e] .. offsets[e + 1]) (rows NULL: those
+ * numbers themselves); offsets [groups + 1] ascending from 0 to at most n,
+ * groups of any size.  rows is a permutation of 0..n-1 (r2s_group_rows); the
+ * rows past offsets[groups] belong to no group and give zeros.
+ * x [n, k] of stride x_stride, weight [groups, m, k], bias [groups, m] (may be
+ * NULL), y [n, m] contiguous. */
+int r2s_grouped_matmul_fwd(const void *x, int64_t x_stride, const void *weight, const void *bias,
+                           const int32_t *offsets, const int32_t *rows, int64_t n, int64_t k,
+                           int64_t m, int64_t groups, int32_t type, void *y, r2s_stream_t stream);
+/* Its gradient from v_y [n, m]: v_x [n, k], v_weight [groups, m, k], v_bias
+ * [groups, m]; any of them may be NULL (not wanted). */
+int64_t r2s_grouped_matmul_bwd_workspace_bytes(int64_t n, int64_t k, int64_t m, int64_t groups);
+int r2s_grouped_matmul_bwd(const void *x, int64_t x_stride, const void *weight,
+                           const int32_t *offsets, const int32_t *rows, const void *v_y,
+                           int64_t v_y_stride, int64_t n, int64_t k, int64_t m, int64_t groups,
+                           int32_t type, void *v_x, void *v_weight, void *v_bias,
+                           void *workspace, size_t workspace_bytes, r2s_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
