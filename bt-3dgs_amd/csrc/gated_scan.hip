@@ -11,50 +11,66 @@
 // A step is the affine map h -> p h + u with p = a, u = (1 - a) x, and maps
 // compose: (p2, u2) after (p1, u1) is (p2 p1, p2 u1 + u2).  A sequence's first
 // token has p = 0 and its initial state inside u, which cuts the packed axis
-// without any other rule.  The axis is cut into tiles; a thread composes
-// kSteps steps of its channels in registers, the block composes its threads'
-// maps over LDS, and the state that enters each tile comes from the tiles
-// before.
+// without any other rule.  So the axis is cut into strips of equal length
+// whatever the sequences are.  A group of lanes (one vector of channels each)
+// walks one strip, token after token, in registers: once to compose the
+// strip's map, then, with the state that enters the strip, to write the
+// states.  No step of either walk waits for another lane.
+//
+//   resident   a block's strips hold whole sequences (one equal sequence, or
+//              everything there is): the maps meet in LDS and both walks are
+//              one launch; the second finds its tokens in cache.
+//   packed     a launch composes the strips' maps, one adds them up along the
+//              axis, one walks again: for few long sequences and ragged ones.
+//   own        short equal sequences: a strip is a sequence, one walk.
 //
 // The gradient runs the other way.  With F_t the gradient that reaches the
 // state before token t:  F_t = a_t (dy_t + F_{t+1}), again an affine map, cut
 // at each sequence's last token, where F_{t+1} is the final state's gradient.
 // Then with G_t = dy_t + F_{t+1}:
 //   dx_t = (1 - a_t) G_t,  dg_t = a_t (1 - a_t) G_t (h_{t-1} - x_t),
-// and h_{t-1} is composed again from x, g and the forward's state at the
-// tile's start, which the forward keeps (one state per tile, float32).
+// and h_{t-1} is composed again from x, g and the state before each kChunk
+// tokens, which the forward keeps in float32.
 //
 // The reverse order is the same code on mirrored token and sequence numbers.
+// The plain and the careful form of each walk round alike (no contraction but
+// the fmaf written), so a token's bits do not depend on its neighbours'.
+#pragma clang fp contract(off)
+
+#include <algorithm>
+
 #include "r2s_latent.h"
 
 namespace r2s {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSteps = 16;  // tokens per thread
+constexpr int kThreads = 256;    // of a packed block
+constexpr int kResident = 1024;  // of a resident block, at most
+constexpr int kChunk = 8;        // tokens loaded together, and between kept states
 
 // What every kernel of a call needs to know of its tokens.  Tokens and
 // sequences are numbered in scan order; physical numbers are mirrored with
 // `reverse`.  offsets null: sequences of `length` tokens.
+// Strip i of block b holds tokens [b block + i strip, + strip), not past the
+// block's.
 struct Tokens {
   const int32_t *offsets;
   int64_t n, length;
+  int64_t block;       // tokens per block
   int32_t sequences;
   int32_t reverse;
+  int32_t strip;       // tokens per strip
+  int32_t steps;       // the same, to the next multiple of kChunk
   uint32_t width;
-  uint32_t lane_bits;  // 2^lane_bits lanes across a tile's channels
-  int32_t tiles;
+  uint32_t lane_bits;  // 2^lane_bits lanes across a block's channels
 
   __device__ __forceinline__ int64_t start(int64_t s) const {
     if (offsets == nullptr) return s * length;
     return reverse ? n - offsets[sequences - s] : offsets[s];
   }
-  __device__ __forceinline__ int64_t row(int64_t t) const { return reverse ? n - 1 - t : t; }
   __device__ __forceinline__ int64_t state_row(int64_t s) const {
     return reverse ? sequences - 1 - s : s;
   }
-  __device__ __forceinline__ int groups() const { return kThreads >> lane_bits; }
-  __device__ __forceinline__ int tile_tokens() const { return groups() * kSteps; }
 };
 
 // sigmoid(g) and sigmoid(-g), each to a few units in its own last place.
@@ -65,270 +81,690 @@ __device__ __forceinline__ void gate_pair(float g, float &a, float &b) {
   b = g < 0.0f ? r : q;
 }
 
-// factor * value, with a factor of 0 taking any value (also a NaN) to 0.
+// factor * value, with a factor of 0 taking any value (also a NaN) to 0; only
+// with kSafe, where a chunk holds something that is not finite.
+template <bool kSafe>
 __device__ __forceinline__ float scaled(float factor, float value) {
-  return factor == 0.0f ? 0.0f : factor * value;
+  return kSafe && factor == 0.0f ? 0.0f : factor * value;
 }
 // p h + u, likewise.
+template <bool kSafe>
 __device__ __forceinline__ float applied(float p, float h, float u) {
-  return p == 0.0f ? u : fmaf(p, h, u);
+  return kSafe && p == 0.0f ? u : fmaf(p, h, u);
 }
 
-// s_first[t]: the sequence whose first token is the tile's token t, else -1
-// (also for the places of a last tile that no token has); s_last likewise.
-__device__ __forceinline__ void mark_sequences(const Tokens &c, int64_t t0, int32_t *s_first,
-                                               int32_t *s_last) {
-  __shared__ int32_t s_seq;
-  const int places = c.tile_tokens();
-  const int count = static_cast<int>(min(static_cast<int64_t>(places), c.n - t0));
-  for (int t = threadIdx.x; t < places; t += kThreads) s_first[t] = s_last[t] = -1;
-  if (c.offsets == nullptr) {
-    __syncthreads();
-    for (int t = threadIdx.x; t < count; t += kThreads) {
-      const int64_t s = (t0 + t) / c.length, in = t0 + t - s * c.length;
-      if (in == 0) s_first[t] = static_cast<int32_t>(s);
-      if (in == c.length - 1) s_last[t] = static_cast<int32_t>(s);
-    }
-    __syncthreads();
-    return;
-  }
-  if (threadIdx.x < 64) {
-    // The last sequence that starts at or before t0: 64 probes a round.
-    int64_t lo = 0, hi = c.sequences;  // start(lo) <= t0 (or lo = 0), start(hi) > t0 (or the end)
-    while (hi - lo > 1) {
-      const int64_t step = (hi - lo + 63) / 64;
-      const int64_t s = lo + (static_cast<int64_t>(threadIdx.x) + 1) * step;
-      const uint64_t under = ballot(s < hi && c.start(s) <= t0);
-      const int64_t k = __popcll(under);
-      hi = min(hi, lo + (k + 1) * step);
-      lo += k * step;
-    }
-    if (threadIdx.x == 0) s_seq = static_cast<int32_t>(lo);
-  }
-  __syncthreads();
-  // Every sequence with a token in the tile, 256 at a time, to the first that
-  // starts past it.
-  const int64_t end = t0 + count;
-  for (int64_t s = s_seq;; s += kThreads) {
-    const int64_t mine = s + threadIdx.x;
-    int64_t lo = end;
-    if (mine < c.sequences) {
-      lo = c.start(mine);
-      const int64_t hi = c.start(mine + 1);
-      if (lo < hi) {
-        if (lo >= t0 && lo < end) s_first[lo - t0] = static_cast<int32_t>(mine);
-        if (hi - 1 >= t0 && hi - 1 < end) s_last[hi - 1 - t0] = static_cast<int32_t>(mine);
-      }
-    }
-    if (!__syncthreads_or(threadIdx.x == kThreads - 1 && lo < end &&
-                          s + kThreads < c.sequences))
-      break;
-  }
-}
+__device__ __forceinline__ bool finite(float x) { return __builtin_isfinite(x); }
 
-// A thread's place in its tile.
+// A thread's place: its strip and channels.
 struct Place {
-  int group;       // of kSteps tokens
-  uint32_t col;    // its first channel
-  uint32_t lane;   // among the lanes across the channels
-  bool inside;     // the channels exist
-  __device__ __forceinline__ Place(const Tokens &c, int V) {
+  int group;      // strip of the block
+  uint32_t col;   // first channel
+  uint32_t lane;  // among the lanes across the channels
+  bool inside;    // the channels exist
+  int64_t lo, hi; // tokens
+  __device__ __forceinline__ Place(const Tokens &c, int V, int64_t block, uint32_t slice) {
     lane = threadIdx.x & ((1u << c.lane_bits) - 1u);
     group = static_cast<int>(threadIdx.x >> c.lane_bits);
-    col = ((blockIdx.y << c.lane_bits) + lane) * V;
+    col = ((slice << c.lane_bits) + lane) * V;
     inside = col < c.width;
+    const int64_t end = min((block + 1) * c.block, c.n);
+    lo = min(block * c.block + static_cast<int64_t>(group) * c.strip, end);
+    hi = min(lo + c.strip, end);
   }
 };
 
+// Rows of a strip: a wave's strips lie `strip` tokens apart, so the address of
+// step k is a scalar that moves with k and a 32-bit offset per lane that does
+// not.
 template <typename T, int V>
-__device__ __forceinline__ void load_rows(const T *p, int64_t stride, const Tokens &c,
-                                          const Place &at, int64_t t0, Pack<T, V> (&x)[kSteps]) {
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int64_t t = t0 + at.group * kSteps + k;
-    if (at.inside && t < c.n) {
-      x[k] = load_pack<T, V>(p + c.row(t) * stride + at.col);
+struct Rows {
+  const char *base;  // of step 0, wave-uniform
+  int64_t pitch;     // bytes per step, negative in reverse
+  uint32_t offset;
+  __device__ __forceinline__ Rows(const T *p, int64_t stride, const Tokens &c, const Place &at,
+                                  int64_t block) {
+    const int per_wave = 64 >> c.lane_bits;
+    const int first = static_cast<int>(wave_index()) * per_wave, mine = at.group - first;
+    const int64_t row_bytes = stride * static_cast<int64_t>(sizeof(T));
+    const int64_t t0 = block * c.block + static_cast<int64_t>(first) * c.strip;
+    const uint32_t step = static_cast<uint32_t>(c.strip * row_bytes);
+    const uint32_t col = min(at.col, c.width - V) * static_cast<uint32_t>(sizeof(T));
+    if (c.reverse) {
+      base = reinterpret_cast<const char *>(p) +
+             (c.n - 1 - t0 - static_cast<int64_t>(per_wave - 1) * c.strip) * row_bytes;
+      pitch = -row_bytes;
+      offset = static_cast<uint32_t>(per_wave - 1 - mine) * step + col;
     } else {
+      base = reinterpret_cast<const char *>(p) + t0 * row_bytes;
+      pitch = row_bytes;
+      offset = static_cast<uint32_t>(mine) * step + col;
+    }
+  }
+  __device__ __forceinline__ Pack<T, V> load(int64_t k) const {
+    return load_pack<T, V>(reinterpret_cast<const T *>(base + k * pitch + offset));
+  }
+  __device__ __forceinline__ void store(int64_t k, const Pack<T, V> &x) const {
+    store_pack<T, V>(reinterpret_cast<T *>(const_cast<char *>(base + k * pitch + offset)), x);
+  }
+};
+
+// kChunk rows from step j on; the places past `count` tokens are 0.
+template <typename T, int V>
+__device__ __forceinline__ void load_chunk(const Rows<T, V> &r, int64_t j, bool full,
+                                           int64_t count, Pack<T, V> (&x)[kChunk]) {
+  if (full) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[k].v[v] = static_cast<T>(0.0f);
+    for (int k = 0; k < kChunk; ++k) x[k] = r.load(j + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+      if (j + k < count) {
+        x[k] = r.load(j + k);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[k].v[v] = static_cast<T>(0.0f);
+      }
     }
   }
 }
 
-// One forward step's map.  first: the sequence that begins here, or -1.
-__device__ __forceinline__ void forward_step(float x, float g, float h0, bool first, float &p,
-                                             float &u) {
-  float b;
-  gate_pair(g, p, b);
-  u = scaled(b, x);
-  if (first) {
-    u = applied(p, h0, u);
-    p = 0.0f;
+// The sequence that a walk is in: its number and tokens [first, last].
+struct Cursor {
+  int64_t s, first, last;
+
+  // The sequence of token t; none (s = -1) where there is no such token.
+  __device__ __forceinline__ void seek(const Tokens &c, int64_t t, bool some) {
+    s = -1;
+    first = last = -1;
+    if (c.offsets == nullptr) {
+      if (!some) return;
+      s = static_cast<int64_t>(static_cast<uint32_t>(t) / static_cast<uint32_t>(c.length));
+    } else {
+      // The last sequence that starts at or before t, by the lanes of the
+      // group together: 2^lane_bits probes a round.
+      const uint32_t lanes = 1u << c.lane_bits, lane = lane_id() & (lanes - 1u);
+      const uint32_t shift = lane_id() & ~(lanes - 1u);
+      const uint64_t mask = lanes == 64u ? ~0ull : ((1ull << lanes) - 1ull);
+      int64_t lo = 0, hi = c.sequences;
+      while (__any(hi - lo > 1)) {
+        const int64_t step = (hi - lo + lanes) / (lanes + 1);
+        const int64_t q = lo + (static_cast<int64_t>(lane) + 1) * step;
+        const uint64_t under = ballot(step > 0 && q < hi && c.start(q) <= t) >> shift & mask;
+        const int64_t k = __popcll(under);
+        hi = min(hi, lo + (k + 1) * step);
+        lo += k * step;
+        if (hi <= lo) hi = lo + 1;  // offsets that do not ascend
+      }
+      if (!some) return;
+      s = lo;
+    }
+    bounds(c);
   }
+  __device__ __forceinline__ void bounds(const Tokens &c) {
+    first = c.start(s);
+    last = c.start(s + 1) - 1;
+  }
+  // The sequences with a token that follow, and those before.
+  __device__ __forceinline__ void next(const Tokens &c, int64_t t) {
+    do {
+      ++s;
+      if (s >= c.sequences) {
+        s = -1;
+        first = last = -1;
+        return;
+      }
+      bounds(c);
+    } while (last < t);
+  }
+  __device__ __forceinline__ void previous(const Tokens &c, int64_t t) {
+    do {
+      --s;
+      if (s < 0) {
+        first = last = -1;
+        return;
+      }
+      bounds(c);
+    } while (first > t);
+  }
+};
+
+// Whether tokens [t, t + kChunk) of every lane of the wave lie inside one
+// sequence, and none but its first token is not a sequence's first (forward)
+// or none is its last (backward).
+__device__ __forceinline__ bool plain_forward(const Cursor &q, int64_t t, int64_t hi) {
+  return __all(t + kChunk <= hi && t > q.first && t + kChunk - 1 <= q.last);
+}
+__device__ __forceinline__ bool plain_backward(const Cursor &q, int64_t t, int64_t hi) {
+  return __all(t + kChunk <= hi && t > q.first && t + kChunk - 1 < q.last);
+}
+
+template <int V>
+__device__ __forceinline__ void load_state(const float *p, const Tokens &c, const Place &at,
+                                           int64_t s, float (&h)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    h[v] = p != nullptr && at.inside ? p[c.state_row(s) * c.width + at.col + v] : 0.0f;
 }
 
 // ------------------------------------------------------------- forward ---
 
-// The map of each tile: maps [tiles][2][width].
+// The map of the strip: p, u.
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_fwd_maps_kernel(
-    const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
-    const float *__restrict__ initial, Tokens c, float *__restrict__ maps) {
-  __shared__ int32_t s_first[kThreads * kSteps], s_last[kThreads * kSteps];
-  __shared__ float s_p[kThreads * V], s_u[kThreads * V];
-  const Place at(c, V);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * c.tile_tokens();
-  mark_sequences(c, t0, s_first, s_last);
-  Pack<T, V> xs[kSteps], gs[kSteps];
-  load_rows<T, V>(x, x_stride, c, at, t0, xs);
-  load_rows<T, V>(gate, g_stride, c, at, t0, gs);
-  float p[V], u[V];
+__device__ __forceinline__ void compose_forward(const Rows<T, V> &xr, const Rows<T, V> &gr,
+                                                const float *initial, const Tokens &c,
+                                                const Place &at, float (&p)[V], float (&u)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
+  Cursor q;
+  q.seek(c, at.lo, at.lo < at.hi);
+  const int64_t count = at.hi - at.lo;
+  for (int64_t j = 0; __any(j < count); j += kChunk) {
+    const int64_t t = at.lo + j;
+    Pack<T, V> x[kChunk], g[kChunk];
+    const bool full = __all(j + kChunk <= count);
+    load_chunk<T, V>(xr, j, full, count, x);
+    load_chunk<T, V>(gr, j, full, count, g);
+    const bool plain = full && plain_forward(q, t, at.hi);
+    bool fine = plain;
+    float p1[V], u1[V];
+    if (plain) {
 #pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    if (t0 + at.group * kSteps + k < c.n) {
-      const int32_t s = s_first[at.group * kSteps + k];
+      for (int v = 0; v < V; ++v) p1[v] = p[v], u1[v] = u[v];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float h0 = 0.0f, pk, uk;
-        if (s >= 0 && initial != nullptr && at.inside)
-          h0 = initial[c.state_row(s) * c.width + at.col + v];
-        forward_step(static_cast<float>(xs[k].v[v]), static_cast<float>(gs[k].v[v]), h0, s >= 0,
-                     pk, uk);
-        u[v] = applied(pk, u[v], uk);
-        p[v] = p[v] * pk;
+      for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(static_cast<float>(g[k].v[v]), a, b);
+          u1[v] = fmaf(a, u1[v], b * static_cast<float>(x[k].v[v]));
+          p1[v] *= a;
+        }
+      bool ok = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) ok = ok && finite(u1[v]) && finite(p1[v]);
+      fine = __all(ok);
+    }
+    if (fine) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[v] = p1[v], u[v] = u1[v];
+    } else {
+      for (int k = 0; k < kChunk; ++k) {
+        if (j + k >= count) break;
+        if (t + k > q.last) q.next(c, t + k);
+        const bool first = t + k == q.first;
+        float h0[V];
+        if (first) load_state<V>(initial, c, at, q.s, h0);
+        const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(static_cast<float>(gk.v[v]), a, b);
+          const float fresh = scaled<true>(b, static_cast<float>(xk.v[v]));
+          u[v] = applied<true>(a, first ? h0[v] : u[v], fresh);
+          p[v] = first ? 0.0f : p[v] * a;
+        }
       }
     }
   }
-#pragma unroll
-  for (int v = 0; v < V; ++v) s_p[threadIdx.x * V + v] = p[v], s_u[threadIdx.x * V + v] = u[v];
-  __syncthreads();
-  if (at.group != 0 || !at.inside) return;
-  for (int q = 1; q < c.groups(); ++q) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int i = ((q << c.lane_bits) + static_cast<int>(at.lane)) * V + v;
-      u[v] = applied(s_p[i], u[v], s_u[i]);
-      p[v] *= s_p[i];
-    }
-  }
-  float *m = maps + static_cast<int64_t>(blockIdx.x) * 2 * c.width + at.col;
-#pragma unroll
-  for (int v = 0; v < V; ++v) m[v] = p[v], m[c.width + v] = u[v];
 }
 
-// The state that enters each tile, from the tiles' maps in order (from the
-// last tile down with `down`).  A block takes 16 channels; each of its 16
-// rows of threads composes one sixteenth of the tiles, and again with the
-// state that the rows before leave.
-__global__ __launch_bounds__(kThreads) void scan_carry_kernel(const float *__restrict__ maps,
-                                                              int32_t tiles, uint32_t width,
-                                                              int32_t down,
-                                                              float *__restrict__ carries) {
-  __shared__ float s_p[16][16], s_u[16][16];
+// The states of the strip from h, the one before it.  kept: the state before
+// each kChunk tokens (may be null).
+template <typename T, int V>
+__device__ __forceinline__ void walk_forward(const Rows<T, V> &xr, const Rows<T, V> &gr,
+                                             const Rows<T, V> &yr, const float *initial,
+                                             const Tokens &c, const Place &at, float *kept,
+                                             float *final, float (&h)[V]) {
+  Cursor q;
+  q.seek(c, at.lo, at.lo < at.hi);
+  const int64_t count = at.hi - at.lo;
+  for (int64_t j = 0; __any(j < count); j += kChunk) {
+    const int64_t t = at.lo + j;
+    Pack<T, V> x[kChunk], g[kChunk], y[kChunk];
+    const bool full = __all(j + kChunk <= count);
+    load_chunk<T, V>(xr, j, full, count, x);
+    load_chunk<T, V>(gr, j, full, count, g);
+    if (kept != nullptr && j < count && at.inside) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) kept[j / kChunk * c.width + v] = h[v];
+    }
+    // A sequence's last token stores its state: not in the plain form.
+    const bool plain = full && plain_backward(q, t, at.hi);
+    bool fine = plain;
+    float h1[V];
+    if (plain) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h1[v] = h[v];
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(static_cast<float>(g[k].v[v]), a, b);
+          h1[v] = fmaf(a, h1[v], b * static_cast<float>(x[k].v[v]));
+          y[k].v[v] = static_cast<T>(h1[v]);
+        }
+      bool ok = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) ok = ok && finite(h1[v]);
+      fine = __all(ok);
+    }
+    if (fine) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = h1[v];
+      if (at.inside) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) yr.store(j + k, y[k]);
+      }
+    } else {
+      for (int k = 0; k < kChunk; ++k) {
+        if (j + k >= count) break;
+        if (t + k > q.last) q.next(c, t + k);
+        if (t + k == q.first) load_state<V>(initial, c, at, q.s, h);
+        const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k);
+        Pack<T, V> yk;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(static_cast<float>(gk.v[v]), a, b);
+          h[v] = applied<true>(a, h[v], scaled<true>(b, static_cast<float>(xk.v[v])));
+          yk.v[v] = static_cast<T>(h[v]);
+        }
+        if (at.inside) {
+          yr.store(j + k, yk);
+          if (t + k == q.last) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) final[c.state_row(q.s) * c.width + at.col + v] = h[v];
+          }
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ backward ---
+
+// The backward map of the strip, from its last token to its first.
+template <typename T, int V>
+__device__ __forceinline__ void compose_backward(const Rows<T, V> &gr, const Rows<T, V> &vr,
+                                                 const float *v_final, const Tokens &c,
+                                                 const Place &at, float (&p)[V], float (&u)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
+  const int64_t count = at.hi - at.lo;
+  Cursor q;
+  q.seek(c, at.hi - 1, count > 0);
+  for (int64_t j = c.steps - kChunk; j >= 0; j -= kChunk) {
+    if (!__any(j < count)) continue;
+    const int64_t t = at.lo + j;
+    Pack<T, V> g[kChunk], d[kChunk];
+    const bool full = __all(j + kChunk <= count);
+    load_chunk<T, V>(gr, j, full, count, g);
+    load_chunk<T, V>(vr, j, full, count, d);
+    const bool plain = full && plain_backward(q, t, at.hi);
+    bool fine = plain;
+    float p1[V], u1[V];
+    if (plain) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) p1[v] = p[v], u1[v] = u[v];
+#pragma unroll
+      for (int k = kChunk - 1; k >= 0; --k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(static_cast<float>(g[k].v[v]), a, b);
+          u1[v] = a * (static_cast<float>(d[k].v[v]) + u1[v]);
+          p1[v] *= a;
+        }
+      bool ok = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) ok = ok && finite(u1[v]) && finite(p1[v]);
+      fine = __all(ok);
+    }
+    if (fine) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[v] = p1[v], u[v] = u1[v];
+    } else {
+      for (int k = kChunk - 1; k >= 0; --k) {
+        if (j + k >= count) continue;
+        if (t + k < q.first) q.previous(c, t + k);
+        const bool last = t + k == q.last;
+        float f0[V];
+        if (last) load_state<V>(v_final, c, at, q.s, f0);
+        const Pack<T, V> gk = gr.load(j + k), dk = vr.load(j + k);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(static_cast<float>(gk.v[v]), a, b);
+          u[v] = scaled<true>(a, static_cast<float>(dk.v[v]) + (last ? f0[v] : u[v]));
+          p[v] = last ? 0.0f : p[v] * a;
+        }
+      }
+    }
+  }
+}
+
+// The gradients of the strip's tokens from f, the gradient that reaches the
+// state after it.
+template <typename T, int V>
+__device__ __forceinline__ void walk_backward(const Rows<T, V> &xr, const Rows<T, V> &gr,
+                                              const Rows<T, V> &vr, const Rows<T, V> &dxr,
+                                              const Rows<T, V> &dgr, const float *initial,
+                                              const float *v_final, const Tokens &c,
+                                              const Place &at, const float *kept,
+                                              float *v_initial, float (&f)[V]) {
+  const int64_t count = at.hi - at.lo;
+  Cursor q;
+  q.seek(c, at.hi - 1, count > 0);
+  for (int64_t j = c.steps - kChunk; j >= 0; j -= kChunk) {
+    if (!__any(j < count)) continue;
+    const int64_t t = at.lo + j;
+    Pack<T, V> x[kChunk], g[kChunk], d[kChunk];
+    const bool full = __all(j + kChunk <= count);
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      h[v] = j < count && at.inside ? kept[j / kChunk * c.width + v] : 0.0f;
+    load_chunk<T, V>(xr, j, full, count, x);
+    load_chunk<T, V>(gr, j, full, count, g);
+    load_chunk<T, V>(vr, j, full, count, d);
+    const bool plain = full && plain_backward(q, t, at.hi);
+    bool fine = plain;
+    float f1[V];
+    Pack<T, V> dx[kChunk], dg[kChunk];
+    if (plain) {
+      float prior[kChunk][V], a[kChunk][V], b[kChunk][V], h1[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) f1[v] = f[v], h1[v] = h[v];
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          gate_pair(static_cast<float>(g[k].v[v]), a[k][v], b[k][v]);
+          const float xv = static_cast<float>(x[k].v[v]);
+          prior[k][v] = h1[v] - xv;
+          h1[v] = fmaf(a[k][v], h1[v], b[k][v] * xv);
+        }
+#pragma unroll
+      for (int k = kChunk - 1; k >= 0; --k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float gk = static_cast<float>(d[k].v[v]) + f1[v], vx = b[k][v] * gk;
+          f1[v] = a[k][v] * gk;
+          dx[k].v[v] = static_cast<T>(vx);
+          dg[k].v[v] = static_cast<T>(a[k][v] * (vx * prior[k][v]));
+        }
+      bool ok = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) ok = ok && finite(f1[v]) && finite(h1[v]);
+      fine = __all(ok);
+    }
+    if (fine) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) f[v] = f1[v];
+      if (at.inside) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) dxr.store(j + k, dx[k]), dgr.store(j + k, dg[k]);
+      }
+    } else {
+      // The sequences of the chunk's tokens once forwards, for the states
+      // before them, then back.
+      float before[kChunk][V];
+      Cursor w = q;
+      if (j < count) {
+        const int64_t end = min(static_cast<int64_t>(kChunk), count - j);
+        if (t < w.first) w.previous(c, t);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) {
+          if (k >= end) continue;
+          if (t + k > w.last) w.next(c, t + k);
+          if (t + k == w.first) load_state<V>(initial, c, at, w.s, h);
+          const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            float a, b;
+            gate_pair(static_cast<float>(gk.v[v]), a, b);
+            before[k][v] = h[v];
+            h[v] = applied<true>(a, h[v], scaled<true>(b, static_cast<float>(xk.v[v])));
+          }
+        }
+#pragma unroll
+        for (int k = kChunk - 1; k >= 0; --k) {
+          if (k >= end) continue;
+          if (t + k < q.first) q.previous(c, t + k);
+          if (t + k == q.last) load_state<V>(v_final, c, at, q.s, f);
+          const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k), dk = vr.load(j + k);
+          Pack<T, V> vx, vg;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            float a, b;
+            gate_pair(static_cast<float>(gk.v[v]), a, b);
+            const float gv = static_cast<float>(dk.v[v]) + f[v];
+            const float dx = scaled<true>(b, gv);
+            const float dg = a * (dx * (before[k][v] - static_cast<float>(xk.v[v])));
+            vx.v[v] = static_cast<T>(dx);
+            vg.v[v] = static_cast<T>(a == 0.0f || b == 0.0f ? 0.0f : dg);
+            f[v] = scaled<true>(a, gv);
+          }
+          if (at.inside) {
+            dxr.store(j + k, vx);
+            dgr.store(j + k, vg);
+            if (t + k == q.first && v_initial != nullptr) {
+#pragma unroll
+              for (int v = 0; v < V; ++v)
+                v_initial[c.state_row(q.s) * c.width + at.col + v] = f[v];
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// --------------------------------------------------- maps between strips ---
+
+// The strips' maps of a block in LDS, as [group][lane] of V (p, u) pairs.
+template <int V>
+__device__ __forceinline__ void put_map(float *s_map, const float (&p)[V], const float (&u)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    s_map[(threadIdx.x * V + v) * 2] = p[v];
+    s_map[(threadIdx.x * V + v) * 2 + 1] = u[v];
+  }
+}
+
+// h through the maps of the strips before this one (after it with kDown).
+template <int V, bool kDown>
+__device__ __forceinline__ void through_maps(const float *s_map, const Tokens &c, const Place &at,
+                                             int groups, float (&h)[V]) {
+  const int count = kDown ? groups - 1 - at.group : at.group;
+  for (int i = 0; i < count; ++i) {
+    const int q = kDown ? groups - 1 - i : i;
+    const float *m = s_map + ((q << c.lane_bits) + static_cast<int>(at.lane)) * V * 2;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = applied<true>(m[v * 2], h[v], m[v * 2 + 1]);
+  }
+}
+
+// The maps that a packed call keeps between its launches: of every strip,
+// strips [n][width] of (p, u), and of every block of strips, likewise.
+template <int V>
+__device__ __forceinline__ void store_map(float *maps, int64_t row, const Tokens &c,
+                                          const Place &at, const float (&p)[V],
+                                          const float (&u)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float *m = maps + (row * c.width + at.col + v) * 2;
+    m[0] = p[v];
+    m[1] = u[v];
+  }
+}
+
+template <typename T, int V, bool kBack>
+__global__ __launch_bounds__(kThreads) void scan_maps_kernel(
+    const T *__restrict__ a, int64_t a_stride, const T *__restrict__ b, int64_t b_stride,
+    const float *__restrict__ state, Tokens c, float *__restrict__ strips,
+    float *__restrict__ blocks) {
+  extern __shared__ float s_map[];
+  const int groups = kThreads >> c.lane_bits;
+  const Place at(c, V, blockIdx.x, blockIdx.y);
+  const Rows<T, V> ar(a, a_stride, c, at, blockIdx.x), br(b, b_stride, c, at, blockIdx.x);
+  float p[V], u[V];
+  if constexpr (kBack)
+    compose_backward<T, V>(ar, br, state, c, at, p, u);
+  else
+    compose_forward<T, V>(ar, br, state, c, at, p, u);
+  put_map<V>(s_map, p, u);
+  if (at.inside)
+    store_map<V>(strips, static_cast<int64_t>(blockIdx.x) * groups + at.group, c, at, p, u);
+  __syncthreads();
+  // The block's map: everything from its far end, composed by one group.
+  if (at.group != (kBack ? groups - 1 : 0) || !at.inside) return;
+  for (int i = 1; i < groups; ++i) {
+    const int q = kBack ? groups - 1 - i : i;
+    const float *m = s_map + ((q << c.lane_bits) + static_cast<int>(at.lane)) * V * 2;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      u[v] = applied<true>(m[v * 2], u[v], m[v * 2 + 1]);
+      p[v] *= m[v * 2];
+    }
+  }
+  store_map<V>(blocks, blockIdx.x, c, at, p, u);
+}
+
+// The state that enters each block, from the blocks' maps in order (from the
+// last block down with `down`).  16 channels per launch block; each of its 64
+// rows of threads composes one 64th of the blocks, and again with the state
+// that the rows before leave.
+constexpr int kCarryRows = 64;
+__global__ __launch_bounds__(1024) void scan_carry_kernel(const float2 *__restrict__ maps,
+                                                          int32_t blocks, uint32_t width,
+                                                          int32_t down,
+                                                          float *__restrict__ carries) {
+  __shared__ float2 s_map[kCarryRows][16];
   const uint32_t lane = threadIdx.x % 16, row = threadIdx.x / 16;
   const uint32_t col = blockIdx.x * 16 + lane;
-  const int32_t per = (tiles + 15) / 16, i0 = static_cast<int32_t>(row) * per;
-  const int32_t i1 = min(i0 + per, tiles);
+  const int32_t per = (blocks + kCarryRows - 1) / kCarryRows;
+  const int32_t i0 = min(static_cast<int32_t>(row) * per, blocks), i1 = min(i0 + per, blocks);
   const bool inside = col < width;
-  auto at = [&](int32_t i) { return static_cast<int64_t>(down ? tiles - 1 - i : i); };
+  auto at = [&](int32_t i) {
+    return static_cast<int64_t>(down ? blocks - 1 - i : i) * width + col;
+  };
   float p = 1.0f, u = 0.0f;
   if (inside) {
 #pragma unroll 8
     for (int32_t i = i0; i < i1; ++i) {
-      const float *m = maps + at(i) * 2 * width + col;
-      u = applied(m[0], u, m[width]);
-      p *= m[0];
+      const float2 m = maps[at(i)];
+      u = applied<true>(m.x, u, m.y);
+      p *= m.x;
     }
   }
-  s_p[row][lane] = p;
-  s_u[row][lane] = u;
+  s_map[row][lane] = make_float2(p, u);
   __syncthreads();
   if (!inside) return;
   float h = 0.0f;
-  for (uint32_t r = 0; r < row; ++r) h = applied(s_p[r][lane], h, s_u[r][lane]);
+  for (uint32_t r = 0; r < row; ++r) h = applied<true>(s_map[r][lane].x, h, s_map[r][lane].y);
 #pragma unroll 8
   for (int32_t i = i0; i < i1; ++i) {
-    const float *m = maps + at(i) * 2 * width + col;
-    carries[at(i) * width + col] = h;
-    h = applied(m[0], h, m[width]);
+    const float2 m = maps[at(i)];
+    carries[at(i)] = h;
+    h = applied<true>(m.x, h, m.y);
   }
 }
 
-// The threads' own incoming values from the block's: composes the maps that
-// the threads left in s_p, s_u, in group order (downwards with kDown).
+// The state that enters the thread's strip in a packed call: the block's,
+// through the maps of the block's strips before.
 template <int V, bool kDown>
-__device__ __forceinline__ void enter(const Tokens &c, const Place &at, const float *s_p,
-                                      const float *s_u, float (&h)[V]) {
-  const int count = kDown ? c.groups() - 1 - at.group : at.group;
-  for (int i = 0; i < count; ++i) {
-    const int q = kDown ? c.groups() - 1 - i : i;
+__device__ __forceinline__ void enter_strip(const float *strips, const float *carries,
+                                            const Tokens &c, const Place &at, int groups,
+                                            int64_t block, float (&h)[V]) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int j = ((q << c.lane_bits) + static_cast<int>(at.lane)) * V + v;
-      h[v] = applied(s_p[j], h[v], s_u[j]);
-    }
+  for (int v = 0; v < V; ++v) h[v] = at.inside ? carries[block * c.width + at.col + v] : 0.0f;
+  if (!at.inside) return;
+  const int count = kDown ? groups - 1 - at.group : at.group;
+  for (int i = 0; i < count; ++i) {
+    const int q = kDown ? groups - 1 - i : i;
+    const float *m = strips + ((block * groups + q) * c.width + at.col) * 2;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = applied<true>(m[v * 2], h[v], m[v * 2 + 1]);
   }
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_fwd_apply_kernel(
+// How a walk gets the state that enters its strip.
+enum Mode { kPacked, kResidentMode, kOwn };
+
+// Blocks of a resident or own launch that share rows' cache lines (slices of
+// one block of tokens) run on one XCD.
+__device__ __forceinline__ void block_and_slice(uint32_t slices, int64_t &block,
+                                                uint32_t &slice) {
+  const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
+  block = id / slices;
+  slice = id - static_cast<uint32_t>(block) * slices;
+}
+
+// kept [strips][steps / kChunk][width].
+template <typename T, int V, int kMode, int kBlock>
+__global__ __launch_bounds__(kBlock) void scan_fwd_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
-    const float *__restrict__ initial, Tokens c, const float *__restrict__ carries,
+    const float *__restrict__ initial, Tokens c, uint32_t slices,
+    const float *__restrict__ strips, const float *__restrict__ carries, float *__restrict__ kept,
     T *__restrict__ y, float *__restrict__ final) {
-  __shared__ int32_t s_first[kThreads * kSteps], s_last[kThreads * kSteps];
-  __shared__ float s_p[kThreads * V], s_u[kThreads * V];
-  const Place at(c, V);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * c.tile_tokens();
-  mark_sequences(c, t0, s_first, s_last);
-  Pack<T, V> xs[kSteps], gs[kSteps];
-  load_rows<T, V>(x, x_stride, c, at, t0, xs);
-  load_rows<T, V>(gate, g_stride, c, at, t0, gs);
-  // Each step's map composed with the thread's steps before it.
-  float p[kSteps][V], u[kSteps][V];
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int32_t s = s_first[at.group * kSteps + k];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float h0 = 0.0f;
-      if (s >= 0 && initial != nullptr && at.inside)
-        h0 = initial[c.state_row(s) * c.width + at.col + v];
-      forward_step(static_cast<float>(xs[k].v[v]), static_cast<float>(gs[k].v[v]), h0, s >= 0,
-                   p[k][v], u[k][v]);
-      if (k > 0) {
-        u[k][v] = applied(p[k][v], u[k - 1][v], u[k][v]);
-        p[k][v] *= p[k - 1][v];
-      }
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    s_p[threadIdx.x * V + v] = p[kSteps - 1][v];
-    s_u[threadIdx.x * V + v] = u[kSteps - 1][v];
-  }
-  __syncthreads();
-  if (!at.inside) return;
+  extern __shared__ float s_map[];
+  int64_t block;
+  uint32_t slice;
+  block_and_slice(slices, block, slice);
+  const int groups = static_cast<int>(blockDim.x >> c.lane_bits);
+  const Place at(c, V, block, slice);
+  const Rows<T, V> xr(x, x_stride, c, at, block), gr(gate, g_stride, c, at, block);
+  const Rows<T, V> yr(y, c.width, c, at, block);
   float h[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    h[v] = carries[static_cast<int64_t>(blockIdx.x) * c.width + at.col + v];
-  enter<V, false>(c, at, s_p, s_u, h);
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    const int64_t t = t0 + at.group * kSteps + k;
-    if (t >= c.n) break;
-    Pack<T, V> out;
-    const int32_t s = s_last[at.group * kSteps + k];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float state = applied(p[k][v], h[v], u[k][v]);
-      out.v[v] = static_cast<T>(state);
-      if (s >= 0) final[c.state_row(s) * c.width + at.col + v] = state;
-    }
-    store_pack<T, V>(y + c.row(t) * c.width + at.col, out);
+  for (int v = 0; v < V; ++v) h[v] = 0.0f;
+  if constexpr (kMode == kResidentMode) {
+    float p[V], u[V];
+    compose_forward<T, V>(xr, gr, initial, c, at, p, u);
+    put_map<V>(s_map, p, u);
+    __syncthreads();
+    through_maps<V, false>(s_map, c, at, groups, h);
+  } else if constexpr (kMode == kPacked) {
+    enter_strip<V, false>(strips, carries, c, at, groups, block, h);
   }
+  if (kept != nullptr)
+    kept += (block * groups + at.group) * (c.steps / kChunk) * c.width + at.col;
+  walk_forward<T, V>(xr, gr, yr, initial, c, at, kept, final, h);
+}
+
+template <typename T, int V, int kMode, int kBlock>
+__global__ __launch_bounds__(kBlock) void scan_bwd_kernel(
+    const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
+    const float *__restrict__ initial, const T *__restrict__ v_y, int64_t v_stride,
+    const float *__restrict__ v_final, Tokens c, uint32_t slices,
+    const float *__restrict__ strips, const float *__restrict__ carries,
+    const float *__restrict__ kept, T *__restrict__ v_x, T *__restrict__ v_gate,
+    float *__restrict__ v_initial) {
+  extern __shared__ float s_map[];
+  int64_t block;
+  uint32_t slice;
+  block_and_slice(slices, block, slice);
+  const int groups = static_cast<int>(blockDim.x >> c.lane_bits);
+  const Place at(c, V, block, slice);
+  const Rows<T, V> xr(x, x_stride, c, at, block), gr(gate, g_stride, c, at, block);
+  const Rows<T, V> vr(v_y, v_stride, c, at, block);
+  const Rows<T, V> dxr(v_x, c.width, c, at, block), dgr(v_gate, c.width, c, at, block);
+  float f[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v] = 0.0f;
+  if constexpr (kMode == kResidentMode) {
+    float p[V], u[V];
+    compose_backward<T, V>(gr, vr, v_final, c, at, p, u);
+    put_map<V>(s_map, p, u);
+    __syncthreads();
+    through_maps<V, true>(s_map, c, at, groups, f);
+  } else if constexpr (kMode == kPacked) {
+    enter_strip<V, true>(strips, carries, c, at, groups, block, f);
+  }
+  kept += (block * groups + at.group) * (c.steps / kChunk) * c.width + at.col;
+  walk_backward<T, V>(xr, gr, vr, dxr, dgr, initial, v_final, c, at, kept, v_initial, f);
 }
 
 // Sequences without a token: the state they end in (or its gradient) is the
@@ -359,242 +795,113 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const float h0 = initial != nullptr ? initial[t * width + col + v] : 0.0f;
-    float p, u;
-    forward_step(static_cast<float>(xs.v[v]), static_cast<float>(gs.v[v]), h0, true, p, u);
-    out.v[v] = static_cast<T>(u);
-    final[t * width + col + v] = u;
+    float a, b;
+    gate_pair(static_cast<float>(gs.v[v]), a, b);
+    const float h = applied<true>(a, h0, scaled<true>(b, static_cast<float>(xs.v[v])));
+    out.v[v] = static_cast<T>(h);
+    final[t * width + col + v] = h;
   }
   store_pack<T, V>(y + t * width + col, out);
 }
 
-// ------------------------------------------------------------ backward ---
-
-// F_t = a_t (dy_t + F_{t+1}) as a map of F_{t+1}; the last token of a
-// sequence takes the final state's gradient and no other.
-__device__ __forceinline__ void backward_step(float a, float dy, float last_grad, bool last,
-                                              float &p, float &u) {
-  p = last ? 0.0f : a;
-  u = scaled(a, last ? dy + last_grad : dy);
-}
-
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_bwd_maps_kernel(
-    const T *__restrict__ gate, int64_t g_stride, const T *__restrict__ v_y, int64_t v_stride,
-    const float *__restrict__ v_final, Tokens c, float *__restrict__ maps) {
-  __shared__ int32_t s_first[kThreads * kSteps], s_last[kThreads * kSteps];
-  __shared__ float s_p[kThreads * V], s_u[kThreads * V];
-  const Place at(c, V);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * c.tile_tokens();
-  mark_sequences(c, t0, s_first, s_last);
-  Pack<T, V> gs[kSteps], vs[kSteps];
-  load_rows<T, V>(gate, g_stride, c, at, t0, gs);
-  load_rows<T, V>(v_y, v_stride, c, at, t0, vs);
-  float p[V], u[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
-#pragma unroll
-  for (int k = kSteps - 1; k >= 0; --k) {
-    if (t0 + at.group * kSteps + k < c.n) {
-      const int32_t s = s_last[at.group * kSteps + k];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float vf = 0.0f, a, b, pk, uk;
-        if (s >= 0 && v_final != nullptr && at.inside)
-          vf = v_final[c.state_row(s) * c.width + at.col + v];
-        gate_pair(static_cast<float>(gs[k].v[v]), a, b);
-        backward_step(a, static_cast<float>(vs[k].v[v]), vf, s >= 0, pk, uk);
-        u[v] = applied(pk, u[v], uk);
-        p[v] *= pk;
-      }
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) s_p[threadIdx.x * V + v] = p[v], s_u[threadIdx.x * V + v] = u[v];
-  __syncthreads();
-  if (at.group != c.groups() - 1 || !at.inside) return;
-  for (int q = c.groups() - 2; q >= 0; --q) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int i = ((q << c.lane_bits) + static_cast<int>(at.lane)) * V + v;
-      u[v] = applied(s_p[i], u[v], s_u[i]);
-      p[v] *= s_p[i];
-    }
-  }
-  float *m = maps + static_cast<int64_t>(blockIdx.x) * 2 * c.width + at.col;
-#pragma unroll
-  for (int v = 0; v < V; ++v) m[v] = p[v], m[c.width + v] = u[v];
-}
-
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void scan_bwd_apply_kernel(
-    const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
-    const float *__restrict__ initial, const T *__restrict__ v_y, int64_t v_stride,
-    const float *__restrict__ v_final, Tokens c, const float *__restrict__ carries,
-    const float *__restrict__ flows, T *__restrict__ v_x, T *__restrict__ v_gate,
-    float *__restrict__ v_initial) {
-  __shared__ int32_t s_first[kThreads * kSteps], s_last[kThreads * kSteps];
-  __shared__ float s_p[kThreads * V], s_u[kThreads * V];
-  const Place at(c, V);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * c.tile_tokens();
-  mark_sequences(c, t0, s_first, s_last);
-  Pack<T, V> xs[kSteps], gs[kSteps], vs[kSteps];
-  load_rows<T, V>(x, x_stride, c, at, t0, xs);
-  load_rows<T, V>(gate, g_stride, c, at, t0, gs);
-  load_rows<T, V>(v_y, v_stride, c, at, t0, vs);
-  const int32_t *first = s_first + at.group * kSteps, *last = s_last + at.group * kSteps;
-  auto state0 = [&](int k, int v) {
-    return first[k] >= 0 && initial != nullptr && at.inside
-               ? initial[c.state_row(first[k]) * c.width + at.col + v]
-               : 0.0f;
-  };
-  auto grad0 = [&](int k, int v) {
-    return last[k] >= 0 && v_final != nullptr && at.inside
-               ? v_final[c.state_row(last[k]) * c.width + at.col + v]
-               : 0.0f;
-  };
-  // Both scans' maps over the thread's tokens.
-  float hp[V], hu[V], fp[V], fu[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) hp[v] = fp[v] = 1.0f, hu[v] = fu[v] = 0.0f;
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float p, u;
-      forward_step(static_cast<float>(xs[k].v[v]), static_cast<float>(gs[k].v[v]), state0(k, v),
-                   first[k] >= 0, p, u);
-      hu[v] = applied(p, hu[v], u);
-      hp[v] *= p;
-    }
-  }
-#pragma unroll
-  for (int k = kSteps - 1; k >= 0; --k) {
-    if (t0 + at.group * kSteps + k < c.n) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a, b, p, u;
-        gate_pair(static_cast<float>(gs[k].v[v]), a, b);
-        backward_step(a, static_cast<float>(vs[k].v[v]), grad0(k, v), last[k] >= 0, p, u);
-        fu[v] = applied(p, fu[v], u);
-        fp[v] *= p;
-      }
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) s_p[threadIdx.x * V + v] = hp[v], s_u[threadIdx.x * V + v] = hu[v];
-  __syncthreads();
-  float h[V], f[V];
-  const int64_t tile = static_cast<int64_t>(blockIdx.x) * c.width + at.col;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    h[v] = at.inside ? carries[tile + v] : 0.0f;
-    f[v] = at.inside ? flows[tile + v] : 0.0f;
-  }
-  enter<V, false>(c, at, s_p, s_u, h);
-  __syncthreads();
-#pragma unroll
-  for (int v = 0; v < V; ++v) s_p[threadIdx.x * V + v] = fp[v], s_u[threadIdx.x * V + v] = fu[v];
-  __syncthreads();
-  enter<V, true>(c, at, s_p, s_u, f);
-  if (!at.inside) return;
-  // The states before each token, then the tokens from the last to the first.
-  float prior[kSteps][V];
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float a, b;
-      gate_pair(static_cast<float>(gs[k].v[v]), a, b);
-      prior[k][v] = first[k] >= 0 ? state0(k, v) : h[v];
-      h[v] = applied(a, prior[k][v], scaled(b, static_cast<float>(xs[k].v[v])));
-    }
-  }
-#pragma unroll
-  for (int k = kSteps - 1; k >= 0; --k) {
-    const int64_t t = t0 + at.group * kSteps + k;
-    if (t < c.n) {
-      Pack<T, V> vx, vg;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a, b;
-        gate_pair(static_cast<float>(gs[k].v[v]), a, b);
-        const float g = static_cast<float>(vs[k].v[v]) + (last[k] >= 0 ? grad0(k, v) : f[v]);
-        vx.v[v] = static_cast<T>(scaled(b, g));
-        vg.v[v] = static_cast<T>(
-            scaled(a * b, g * (prior[k][v] - static_cast<float>(xs[k].v[v]))));
-        f[v] = scaled(a, g);
-        if (first[k] >= 0 && v_initial != nullptr)
-          v_initial[c.state_row(first[k]) * c.width + at.col + v] = f[v];
-      }
-      store_pack<T, V>(v_x + c.row(t) * c.width + at.col, vx);
-      store_pack<T, V>(v_gate + c.row(t) * c.width + at.col, vg);
-    }
-  }
-}
-
 // ---------------------------------------------------------------- host ---
 
-// Lanes across the channels, for vectors of V.
-uint32_t lane_bits_for(int64_t width, int V) {
-  const int64_t vpr = ceil_div(width, V);
-  uint32_t bits = 0;
-  while (bits < 6 && (1 << bits) < vpr) ++bits;
-  return bits;
-}
+// The threads that a packed call spreads the tokens over: 256 CUs of 24
+// waves.
+constexpr int64_t kSpread = 256 * 24 * 64;
 
-int vector_for(int type, int64_t width) {
-  // 4 bytes of 16-bit elements where the width is even; see the strides' check
-  // of the caller.
-  return type == R2S_TYPE_F32 ? 1 : (width % 2 == 0 ? 2 : 1);
-}
-
-int64_t tile_count(int type, int64_t n, int64_t width) {
-  const int V = vector_for(type, width);
-  return ceil_div(n, static_cast<int64_t>(kThreads >> lane_bits_for(width, V)) * kSteps);
-}
-
-struct ScanSpace {
-  float *maps, *flows;
+struct Plan {
+  Mode mode;
+  int V;
+  uint32_t slices;
+  int64_t blocks;
+  int threads;
+  Tokens c;
+  int64_t groups() const { return threads >> c.lane_bits; }
+  int64_t strips() const { return blocks * groups(); }
+  int64_t kept_rows() const { return strips() * (c.steps / kChunk); }
 };
-ScanSpace carve_scan(Carver &cv, int64_t tiles, int64_t width, bool backward) {
-  ScanSpace s;
-  s.maps = cv.take<float>(tiles * 2 * width);
-  s.flows = backward ? cv.take<float>(tiles * width) : nullptr;
-  return s;
-}
 
-int check_scan(const char *what, int type, const int32_t *offsets, int64_t n, int64_t sequences,
-               int64_t length, int64_t width) {
-  R2S_REQUIRE(known_type(type), "%s: unknown element type %d", what, type);
-  R2S_REQUIRE(n >= 0 && sequences >= 0 && length >= 0 && width >= 0, "%s: negative size", what);
-  R2S_REQUIRE(offsets != nullptr || n == sequences * length,
-              "%s: %lld tokens are not %lld sequences of %lld", what, (long long)n,
-              (long long)sequences, (long long)length);
-  R2S_REQUIRE(sequences > 0 || n == 0, "%s: tokens without a sequence", what);
-  if (n > kInt32Max || sequences >= kInt32Max || width > (1 << 20)) {
-    set_error("%s: more than 2^31 - 1 tokens or sequences, or more than 2^20 channels", what);
-    return R2S_ERANGE;
-  }
-  return R2S_OK;
-}
-
-Tokens tokens_of(int type, const int32_t *offsets, int64_t n, int64_t sequences, int64_t length,
-                 int64_t width, int32_t reverse) {
-  Tokens c{};
+// The plan depends on sizes and types alone, so a backward call finds its
+// forward's.
+Plan plan_of(int type, const int32_t *offsets, int64_t n, int64_t sequences, int64_t length,
+             int64_t width, bool ragged, int32_t reverse) {
+  Plan p{};
+  Tokens &c = p.c;
   c.offsets = offsets;
   c.n = n;
   c.length = length;
   c.sequences = static_cast<int32_t>(sequences);
   c.reverse = reverse != 0;
   c.width = static_cast<uint32_t>(width);
-  c.lane_bits = lane_bits_for(width, vector_for(type, width));
-  c.tiles = static_cast<int32_t>(tile_count(type, n, width));
-  return c;
+  // 4 bytes per lane where 16-bit rows allow; 64 bytes of a row per block.
+  p.V = type != R2S_TYPE_F32 && width % 2 == 0 ? 2 : 1;
+  const int64_t vpr = width / p.V;
+  while (c.lane_bits < 4 && (1 << c.lane_bits) < vpr) ++c.lane_bits;
+  const int64_t lanes = int64_t{1} << c.lane_bits;
+  p.slices = static_cast<uint32_t>(ceil_div(vpr, lanes));
+  if (!ragged && length <= 128) {
+    p.mode = kOwn;
+    p.threads = kThreads;
+    c.strip = static_cast<int32_t>(length);
+    c.block = p.groups() * length;
+  } else if ((!ragged && sequences * p.slices >= 192) || n * lanes <= kResident * 32) {
+    p.mode = kResidentMode;
+    c.block = ragged || sequences * p.slices < 192 ? n : length;
+    p.threads = 64;
+    while (p.threads < kResident && p.groups() * 16 < c.block) p.threads *= 2;
+    c.strip = static_cast<int32_t>(align_up(ceil_div(c.block, p.groups()), kChunk));
+  } else {
+    p.mode = kPacked;
+    p.threads = kThreads;
+    const int64_t even = ceil_div(n * lanes * p.slices, kSpread);
+    c.strip = static_cast<int32_t>(
+        align_up(std::min<int64_t>(std::max<int64_t>(even, 16), 128), kChunk));
+    c.block = p.groups() * c.strip;
+  }
+  c.steps = static_cast<int32_t>(align_up(c.strip, kChunk));
+  p.blocks = ceil_div(n, c.block);
+  return p;
 }
 
-dim3 scan_grid(const Tokens &c, int V) {
-  return dim3(static_cast<uint32_t>(c.tiles),
-              static_cast<uint32_t>(ceil_div(c.width, static_cast<int64_t>(V) << c.lane_bits)));
+struct ScanSpace {
+  float *strips, *blocks, *carries;
+};
+ScanSpace carve_scan(Carver &cv, const Plan &p) {
+  ScanSpace s{};
+  if (p.mode != kPacked) return s;
+  s.strips = cv.take<float>(p.strips() * 2 * p.c.width);
+  s.blocks = cv.take<float>(p.blocks * 2 * p.c.width);
+  s.carries = cv.take<float>(p.blocks * p.c.width);
+  return s;
+}
+
+int check_scan(const char *what, int type, const int32_t *offsets, int64_t n, int64_t sequences,
+               int64_t length, int64_t width, std::initializer_list<int64_t> strides) {
+  R2S_REQUIRE(known_type(type), "%s: unknown element type %d", what, type);
+  R2S_REQUIRE(n >= 0 && sequences >= 0 && length >= 0 && width >= 0, "%s: negative size", what);
+  R2S_REQUIRE(offsets != nullptr || n == sequences * length,
+              "%s: %lld tokens are not %lld sequences of %lld", what, (long long)n,
+              (long long)sequences, (long long)length);
+  R2S_REQUIRE(sequences > 0 || n == 0, "%s: tokens without a sequence", what);
+  if (n > kInt32Max || sequences >= kInt32Max || width > (1 << 16)) {
+    set_error("%s: more than 2^31 - 1 tokens or sequences, or more than 2^16 channels", what);
+    return R2S_ERANGE;
+  }
+  for (int64_t s : strides) R2S_REQUIRE(s >= width, "%s: rows overlap", what);
+  return R2S_OK;
+}
+
+// The limits of a plan: grid sizes, and the 32-bit lane offsets of Rows.
+int check_plan(const char *what, int type, const Plan &p, std::initializer_list<int64_t> strides) {
+  bool fits = p.blocks * p.slices <= kInt32Max && p.slices <= 65535;
+  for (int64_t s : strides)
+    fits &= s * type_size(type) * p.c.strip * (64 >> p.c.lane_bits) <= 0xffffffffll;
+  if (!fits) {
+    set_error("%s: rows too far apart or too many tokens", what);
+    return R2S_ERANGE;
+  }
+  return R2S_OK;
 }
 
 int empty_states(const Tokens &c, const float *in, float *out, hipStream_t stream) {
@@ -605,17 +912,29 @@ int empty_states(const Tokens &c, const float *in, float *out, hipStream_t strea
   return check_launch("gated_scan empty sequences");
 }
 
-int carry(const Tokens &c, const float *maps, bool down, float *out, hipStream_t stream) {
-  scan_carry_kernel<<<dim3(static_cast<uint32_t>(ceil_div(c.width, 16))), dim3(kThreads), 0,
-                      stream>>>(maps, c.tiles, c.width, down, out);
+// The maps of a packed call's strips and blocks, and the states that enter
+// the blocks.
+template <typename T, int V, bool kBack>
+int packed_maps(const Plan &p, const T *a, int64_t as, const T *b, int64_t bs, const float *state,
+                const ScanSpace &s, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(p.blocks), p.slices);
+  scan_maps_kernel<T, V, kBack><<<grid, dim3(kThreads), kThreads * V * 2 * sizeof(float),
+                                  stream>>>(a, as, b, bs, state, p.c, s.strips, s.blocks);
+  R2S_RETURN_IF(check_launch("gated_scan maps"));
+  scan_carry_kernel<<<dim3(static_cast<uint32_t>(ceil_div(p.c.width, 16))), dim3(1024), 0,
+                      stream>>>(reinterpret_cast<const float2 *>(s.blocks),
+                                static_cast<int32_t>(p.blocks), p.c.width, kBack ? 1 : 0,
+                                s.carries);
   return check_launch("gated_scan carries");
 }
 
 template <typename T, int V>
-int scan_fwd(const Tokens &c, const void *x, int64_t xs, const void *g, int64_t gs,
-             const float *initial, void *y, float *final, float *carries, const ScanSpace &s,
+int scan_fwd(const Plan &p, const void *x, int64_t xs, const void *g, int64_t gs,
+             const float *initial, void *y_, float *final, float *kept, const ScanSpace &s,
              hipStream_t stream) {
+  const Tokens &c = p.c;
   const T *xt = static_cast<const T *>(x), *gt = static_cast<const T *>(g);
+  T *y = static_cast<T *>(y_);
   if (c.offsets == nullptr && c.length == 1) {
     const int64_t blocks = ceil_div(c.n * (c.width / V), kThreads);
     if (blocks > kInt32Max) {
@@ -623,34 +942,50 @@ int scan_fwd(const Tokens &c, const void *x, int64_t xs, const void *g, int64_t 
       return R2S_ERANGE;
     }
     scan_step_kernel<T, V><<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream>>>(
-        xt, xs, gt, gs, initial, c.n, c.width, static_cast<T *>(y), final);
+        xt, xs, gt, gs, initial, c.n, c.width, y, final);
     return check_launch("gated_scan_fwd");
   }
-  const dim3 grid = scan_grid(c, V);
-  scan_fwd_maps_kernel<T, V><<<grid, dim3(kThreads), 0, stream>>>(xt, xs, gt, gs, initial, c,
-                                                                  s.maps);
-  R2S_RETURN_IF(check_launch("gated_scan_fwd"));
-  R2S_RETURN_IF(carry(c, s.maps, false, carries, stream));
-  scan_fwd_apply_kernel<T, V><<<grid, dim3(kThreads), 0, stream>>>(
-      xt, xs, gt, gs, initial, c, carries, static_cast<T *>(y), final);
+  const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices)), block(p.threads);
+  if (p.mode == kPacked) {
+    R2S_RETURN_IF((packed_maps<T, V, false>(p, xt, xs, gt, gs, initial, s, stream)));
+    scan_fwd_kernel<T, V, kPacked, kThreads><<<grid, block, 0, stream>>>(
+        xt, xs, gt, gs, initial, c, p.slices, s.strips, s.carries, kept, y, final);
+  } else if (p.mode == kOwn) {
+    scan_fwd_kernel<T, V, kOwn, kThreads><<<grid, block, 0, stream>>>(
+        xt, xs, gt, gs, initial, c, p.slices, nullptr, nullptr, kept, y, final);
+  } else {
+    scan_fwd_kernel<T, V, kResidentMode, kResident>
+        <<<grid, block, p.threads * V * 2 * sizeof(float), stream>>>(
+            xt, xs, gt, gs, initial, c, p.slices, nullptr, nullptr, kept, y, final);
+  }
   return check_launch("gated_scan_fwd");
 }
 
 template <typename T, int V>
-int scan_bwd(const Tokens &c, const void *x, int64_t xs, const void *g, int64_t gs,
-             const float *initial, const float *carries, const void *v_y, int64_t vs,
+int scan_bwd(const Plan &p, const void *x, int64_t xs, const void *g, int64_t gs,
+             const float *initial, const float *kept, const void *v_y, int64_t vs,
              const float *v_final, void *v_x, void *v_gate, float *v_initial, const ScanSpace &s,
              hipStream_t stream) {
+  const Tokens &c = p.c;
   const T *xt = static_cast<const T *>(x), *gt = static_cast<const T *>(g);
   const T *vt = static_cast<const T *>(v_y);
-  const dim3 grid = scan_grid(c, V);
-  scan_bwd_maps_kernel<T, V><<<grid, dim3(kThreads), 0, stream>>>(gt, gs, vt, vs, v_final, c,
-                                                                  s.maps);
-  R2S_RETURN_IF(check_launch("gated_scan_bwd"));
-  R2S_RETURN_IF(carry(c, s.maps, true, s.flows, stream));
-  scan_bwd_apply_kernel<T, V><<<grid, dim3(kThreads), 0, stream>>>(
-      xt, xs, gt, gs, initial, vt, vs, v_final, c, carries, s.flows, static_cast<T *>(v_x),
-      static_cast<T *>(v_gate), v_initial);
+  T *dx = static_cast<T *>(v_x), *dg = static_cast<T *>(v_gate);
+  const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices)), block(p.threads);
+  if (p.mode == kPacked) {
+    R2S_RETURN_IF((packed_maps<T, V, true>(p, gt, gs, vt, vs, v_final, s, stream)));
+    scan_bwd_kernel<T, V, kPacked, kThreads><<<grid, block, 0, stream>>>(
+        xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, s.strips, s.carries, kept, dx, dg,
+        v_initial);
+  } else if (p.mode == kOwn) {
+    scan_bwd_kernel<T, V, kOwn, kThreads><<<grid, block, 0, stream>>>(
+        xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, nullptr, nullptr, kept, dx, dg,
+        v_initial);
+  } else {
+    scan_bwd_kernel<T, V, kResidentMode, kResident>
+        <<<grid, block, p.threads * V * 2 * sizeof(float), stream>>>(
+            xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, nullptr, nullptr, kept, dx, dg,
+            v_initial);
+  }
   return check_launch("gated_scan_bwd");
 }
 
@@ -668,93 +1003,110 @@ bool pairs_fit(std::initializer_list<const void *> bases, std::initializer_list<
 
 extern "C" {
 
-int64_t r2s_gated_scan_tiles(int32_t type, int64_t n, int64_t width) {
+int64_t r2s_gated_scan_kept_rows(int32_t type, int32_t ragged, int64_t sequences, int64_t length,
+                                 int64_t n, int64_t width) {
   if (!r2s::known_type(type) || n <= 0 || width <= 0) return 0;
-  return r2s::tile_count(type, n, width);
+  return r2s::plan_of(type, nullptr, n, sequences, length, width, ragged != 0, 0).kept_rows();
 }
 
-int64_t r2s_gated_scan_workspace_bytes(int32_t type, int64_t n, int64_t width, int32_t backward) {
+int64_t r2s_gated_scan_workspace_bytes(int32_t type, int32_t ragged, int64_t sequences,
+                                       int64_t length, int64_t n, int64_t width) {
+  if (!r2s::known_type(type) || n <= 0 || width <= 0) return 0;
   r2s::Carver cv(nullptr);
-  r2s::carve_scan(cv, r2s_gated_scan_tiles(type, n, width), width > 0 ? width : 0, backward != 0);
+  r2s::carve_scan(cv, r2s::plan_of(type, nullptr, n, sequences, length, width, ragged != 0, 0));
   return static_cast<int64_t>(cv.used);
 }
 
 int r2s_gated_scan_fwd(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
                        const float *initial, const int32_t *offsets, int64_t sequences,
                        int64_t length, int64_t n, int64_t width, int32_t type, int32_t reverse,
-                       void *y, float *final_state, float *carries, void *ws, size_t ws_bytes,
+                       void *y, float *final_state, float *kept, void *ws, size_t ws_bytes,
                        r2s_stream_t st) {
   using namespace r2s;
   clear_error();
-  R2S_RETURN_IF(check_scan("gated_scan_fwd", type, offsets, n, sequences, length, width));
+  R2S_RETURN_IF(check_scan("gated_scan_fwd", type, offsets, n, sequences, length, width,
+                           {x_stride, gate_stride}));
   if (width == 0 || sequences == 0) return R2S_OK;
-  R2S_REQUIRE(x_stride >= width && gate_stride >= width, "gated_scan_fwd: rows overlap");
   R2S_REQUIRE(final_state != nullptr, "gated_scan_fwd: null final states");
-  const Tokens c = tokens_of(type, offsets, n, sequences, length, width, reverse);
+  const bool ragged = offsets != nullptr;
   hipStream_t stream = as_stream(st);
-  R2S_RETURN_IF(empty_states(c, initial, final_state, stream));
+  Tokens all{};
+  all.offsets = offsets;
+  all.length = length;
+  all.sequences = static_cast<int32_t>(sequences);
+  all.width = static_cast<uint32_t>(width);
+  R2S_RETURN_IF(empty_states(all, initial, final_state, stream));
   if (n == 0) return R2S_OK;
-  R2S_REQUIRE(x != nullptr && gate != nullptr && y != nullptr && carries != nullptr,
-              "gated_scan_fwd: null tokens, outputs or carries");
-  const int64_t need = r2s_gated_scan_workspace_bytes(type, n, width, 0);
-  if (ws == nullptr || static_cast<int64_t>(ws_bytes) < need) {
+  const Plan p = plan_of(type, offsets, n, sequences, length, width, ragged, reverse);
+  R2S_RETURN_IF(check_plan("gated_scan_fwd", type, p, {x_stride, gate_stride, width}));
+  R2S_REQUIRE(x != nullptr && gate != nullptr && y != nullptr,
+              "gated_scan_fwd: null tokens or output");
+  const int64_t need =
+      r2s_gated_scan_workspace_bytes(type, ragged, sequences, length, n, width);
+  if (need > 0 && (ws == nullptr || static_cast<int64_t>(ws_bytes) < need)) {
     set_error("gated_scan_fwd: workspace of %zu bytes, %lld required", ws_bytes, (long long)need);
     return R2S_EWORKSPACE;
   }
   Carver cv(ws);
-  const ScanSpace s = carve_scan(cv, c.tiles, width, false);
-  const int V = vector_for(type, width);
-  R2S_REQUIRE(V == 1 || pairs_fit({x, gate, y}, {x_stride, gate_stride}),
+  const ScanSpace s = carve_scan(cv, p);
+  R2S_REQUIRE(p.V == 1 || pairs_fit({x, gate, y}, {x_stride, gate_stride}),
               "gated_scan_fwd: rows of 16-bit elements must start at multiples of 4 bytes");
   R2S_BY_TYPE(type, {
     if constexpr (sizeof(T) == 2) {
-      if (V == 2)
-        return scan_fwd<T, 2>(c, x, x_stride, gate, gate_stride, initial, y, final_state, carries,
-                              s, stream);
+      if (p.V == 2)
+        return scan_fwd<T, 2>(p, x, x_stride, gate, gate_stride, initial, y, final_state, kept, s,
+                              stream);
     }
-    return scan_fwd<T, 1>(c, x, x_stride, gate, gate_stride, initial, y, final_state, carries, s,
+    return scan_fwd<T, 1>(p, x, x_stride, gate, gate_stride, initial, y, final_state, kept, s,
                           stream);
   });
   return R2S_OK;
 }
 
 int r2s_gated_scan_bwd(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
-                       const float *initial, const int32_t *offsets, const float *carries,
+                       const float *initial, const int32_t *offsets, const float *kept,
                        const void *v_y, int64_t v_y_stride, const float *v_final,
                        int64_t sequences, int64_t length, int64_t n, int64_t width, int32_t type,
                        int32_t reverse, void *v_x, void *v_gate, float *v_initial, void *ws,
                        size_t ws_bytes, r2s_stream_t st) {
   using namespace r2s;
   clear_error();
-  R2S_RETURN_IF(check_scan("gated_scan_bwd", type, offsets, n, sequences, length, width));
+  R2S_RETURN_IF(check_scan("gated_scan_bwd", type, offsets, n, sequences, length, width,
+                           {x_stride, gate_stride, v_y_stride}));
   if (width == 0 || sequences == 0) return R2S_OK;
-  R2S_REQUIRE(x_stride >= width && gate_stride >= width && v_y_stride >= width,
-              "gated_scan_bwd: rows overlap");
-  const Tokens c = tokens_of(type, offsets, n, sequences, length, width, reverse);
+  const bool ragged = offsets != nullptr;
   hipStream_t stream = as_stream(st);
-  if (v_initial != nullptr) R2S_RETURN_IF(empty_states(c, v_final, v_initial, stream));
+  Tokens all{};
+  all.offsets = offsets;
+  all.length = length;
+  all.sequences = static_cast<int32_t>(sequences);
+  all.width = static_cast<uint32_t>(width);
+  if (v_initial != nullptr) R2S_RETURN_IF(empty_states(all, v_final, v_initial, stream));
   if (n == 0) return R2S_OK;
-  R2S_REQUIRE(x != nullptr && gate != nullptr && v_y != nullptr && carries != nullptr &&
+  const Plan p = plan_of(type, offsets, n, sequences, length, width, ragged, reverse);
+  R2S_RETURN_IF(check_plan("gated_scan_bwd", type, p,
+                           {x_stride, gate_stride, v_y_stride, width}));
+  R2S_REQUIRE(x != nullptr && gate != nullptr && v_y != nullptr && kept != nullptr &&
                   v_x != nullptr && v_gate != nullptr,
-              "gated_scan_bwd: null tokens, gradients or carries");
-  const int64_t need = r2s_gated_scan_workspace_bytes(type, n, width, 1);
-  if (ws == nullptr || static_cast<int64_t>(ws_bytes) < need) {
+              "gated_scan_bwd: null tokens, gradients or kept states");
+  const int64_t need =
+      r2s_gated_scan_workspace_bytes(type, ragged, sequences, length, n, width);
+  if (need > 0 && (ws == nullptr || static_cast<int64_t>(ws_bytes) < need)) {
     set_error("gated_scan_bwd: workspace of %zu bytes, %lld required", ws_bytes, (long long)need);
     return R2S_EWORKSPACE;
   }
   Carver cv(ws);
-  const ScanSpace s = carve_scan(cv, c.tiles, width, true);
-  const int V = vector_for(type, width);
-  R2S_REQUIRE(V == 1 || pairs_fit({x, gate, v_y, v_x, v_gate},
-                                  {x_stride, gate_stride, v_y_stride}),
+  const ScanSpace s = carve_scan(cv, p);
+  R2S_REQUIRE(p.V == 1 || pairs_fit({x, gate, v_y, v_x, v_gate},
+                                    {x_stride, gate_stride, v_y_stride}),
               "gated_scan_bwd: rows of 16-bit elements must start at multiples of 4 bytes");
   R2S_BY_TYPE(type, {
     if constexpr (sizeof(T) == 2) {
-      if (V == 2)
-        return scan_bwd<T, 2>(c, x, x_stride, gate, gate_stride, initial, carries, v_y, v_y_stride,
+      if (p.V == 2)
+        return scan_bwd<T, 2>(p, x, x_stride, gate, gate_stride, initial, kept, v_y, v_y_stride,
                               v_final, v_x, v_gate, v_initial, s, stream);
     }
-    return scan_bwd<T, 1>(c, x, x_stride, gate, gate_stride, initial, carries, v_y, v_y_stride,
+    return scan_bwd<T, 1>(p, x, x_stride, gate, gate_stride, initial, kept, v_y, v_y_stride,
                           v_final, v_x, v_gate, v_initial, s, stream);
   });
   return R2S_OK;

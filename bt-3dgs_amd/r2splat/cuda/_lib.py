@@ -131,8 +131,8 @@ _PLAIN = {
     "r2s_embedding_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "r2s_embedding_bwd": (_i32, [_p, _i64, _p, _i32, _f32, _i32, _i64, _i64, _i64, _p, _p, _sz,
                                  _p]),
-    "r2s_gated_scan_tiles": (_i64, [_i32, _i64, _i64]),
-    "r2s_gated_scan_workspace_bytes": (_i64, [_i32, _i64, _i64, _i32]),
+    "r2s_gated_scan_kept_rows": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64]),
+    "r2s_gated_scan_workspace_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64]),
     "r2s_gated_scan_fwd": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32, _i32,
                                   _p, _p, _p, _p, _sz, _p]),
     "r2s_gated_scan_bwd": (_i32, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64,

@@ -1910,11 +1910,11 @@ def _check_latent(t, name: str, like: Optional[Tensor] = None, dtype=None) -> No
 
 def _rows_2d(t: Tensor, align: int = 1):
     """(tensor, row stride) of a 2-D tensor whose rows' elements are
-    consecutive; a copy where they are not, where rows overlap or where a row
-    does not start at a multiple of ``align`` bytes."""
+    consecutive; a copy where they are not, where rows overlap or lie very far
+    apart, or where a row does not start at a multiple of ``align`` bytes."""
     n, d = t.shape
     stride = t.stride(0) if n > 1 else d
-    if (d > 1 and t.stride(1) != 1) or stride < d or \
+    if (d > 1 and t.stride(1) != 1) or stride < d or stride > 4 * max(d, 4096) or \
             (align > 1 and (t.data_ptr() % align or (stride * t.element_size()) % align)):
         t = torch.empty_strided((n, d), (d, 1), dtype=t.dtype, device=t.device).copy_(t)
         stride = d
@@ -2029,11 +2029,12 @@ def _scan_state(t: Optional[Tensor], name: str, x: Tensor, sequences: int) -> Op
 
 
 def gated_scan_fwd(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
-                   offsets: Optional[Tensor] = None, reverse: bool = False
-                   ) -> Tuple[Tensor, Tensor, Tensor]:
-    """(y, final, carries) of h_t = a_t h_{t-1} + (1 - a_t) x_t with
+                   offsets: Optional[Tensor] = None, reverse: bool = False, keep: bool = True
+                   ) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
+    """(y, final, kept) of h_t = a_t h_{t-1} + (1 - a_t) x_t with
     a_t = sigmoid(gate_t): y the states in x's type, final [S, D] float32 each
-    sequence's last state, carries what gated_scan_bwd takes.  x, gate
+    sequence's last state, kept what gated_scan_bwd takes (None without
+    ``keep``).  x, gate
     [B, L, D], or [N, D] with offsets [S + 1] (int32, from 0 to N); initial
     [S, D] float32; reverse: from each sequence's last token to its first."""
     _check_latent(x, "x")
@@ -2047,22 +2048,25 @@ def gated_scan_fwd(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
     with _on(dev):
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
         final = torch.empty((sequences, d), dtype=torch.float32, device=dev)
-        carries = torch.empty((lib.r2s_gated_scan_tiles(code, n, d), d), dtype=torch.float32,
-                              device=dev)
-        need = lib.r2s_gated_scan_workspace_bytes(code, n, d, 0)
-        ws = _workspace(need, dev)
+        sizes = (code, offsets is not None, sequences, length, n, d)
+        kept = None
+        if keep:
+            kept = torch.empty((lib.r2s_gated_scan_kept_rows(*sizes), d), dtype=torch.float32,
+                               device=dev)
+        need = lib.r2s_gated_scan_workspace_bytes(*sizes)
+        ws = _workspace(need, dev) if need else None
         _call("r2s_gated_scan_fwd", _ptr(xr), xs, _ptr(gr), gs, _ptr(initial), _ptr(offsets),
-              sequences, length, n, d, code, bool(reverse), _ptr(y), _ptr(final), _ptr(carries),
+              sequences, length, n, d, code, bool(reverse), _ptr(y), _ptr(final), _ptr(kept),
               _ptr(ws), need, _stream(dev))
-    return y, final, carries
+    return y, final, kept
 
 
 def gated_scan_bwd(x: Tensor, gate: Tensor, initial: Optional[Tensor],
-                   offsets: Optional[Tensor], carries: Tensor, v_y: Tensor,
+                   offsets: Optional[Tensor], kept: Tensor, v_y: Tensor,
                    v_final: Optional[Tensor] = None, reverse: bool = False
                    ) -> Tuple[Tensor, Tensor, Tensor]:
     """(v_x, v_gate, v_initial) of gated_scan_fwd with the same inputs, whose
-    carries these are, from v_y (x's shape and type) and v_final [S, D]."""
+    ``kept`` this is, from v_y (x's shape and type) and v_final [S, D]."""
     _check_latent(x, "x")
     code = _latent_type(x, "gated_scan_bwd")
     n, sequences, length = _scan_shape(x, offsets)
@@ -2073,18 +2077,18 @@ def gated_scan_bwd(x: Tensor, gate: Tensor, initial: Optional[Tensor],
     initial = _scan_state(initial, "initial", x, sequences)
     v_final = _scan_state(v_final, "v_final", x, sequences)
     lib = _lib()
-    _check_latent(carries, "carries", x, torch.float32)
-    if carries.shape != (lib.r2s_gated_scan_tiles(code, n, d), d) or not carries.is_contiguous():
-        _fail("carries are not those of the forward of these inputs: shape ",
-              tuple(carries.shape))
+    sizes = (code, offsets is not None, sequences, length, n, d)
+    _check_latent(kept, "kept", x, torch.float32)
+    if kept.shape != (lib.r2s_gated_scan_kept_rows(*sizes), d) or not kept.is_contiguous():
+        _fail("kept is not that of the forward of these inputs: shape ", tuple(kept.shape))
     with _on(dev):
         v_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
         v_gate = torch.empty(x.shape, dtype=x.dtype, device=dev)
         v_initial = torch.empty((sequences, d), dtype=torch.float32, device=dev)
-        need = lib.r2s_gated_scan_workspace_bytes(code, n, d, 1)
-        ws = _workspace(need, dev)
+        need = lib.r2s_gated_scan_workspace_bytes(*sizes)
+        ws = _workspace(need, dev) if need else None
         _call("r2s_gated_scan_bwd", _ptr(xr), xs, _ptr(gr), gs, _ptr(initial), _ptr(offsets),
-              _ptr(carries), _ptr(vr), vs, _ptr(v_final), sequences, length, n, d, code,
+              _ptr(kept), _ptr(vr), vs, _ptr(v_final), sequences, length, n, d, code,
               bool(reverse), _ptr(v_x), _ptr(v_gate), _ptr(v_initial), _ptr(ws), need,
               _stream(dev))
     return v_x, v_gate, v_initial

@@ -68,18 +68,18 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, initial, offsets, reverse):
         ctx.set_materialize_grads(False)
-        y, final, carries = W.gated_scan_fwd(x, gate, initial, offsets, reverse)
-        ctx.save_for_backward(x, gate, initial, offsets, carries)
+        y, final, kept = W.gated_scan_fwd(x, gate, initial, offsets, reverse)
+        ctx.save_for_backward(x, gate, initial, offsets, kept)
         ctx.reverse = reverse
         return y, final
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, v_y, v_final):
-        x, gate, initial, offsets, carries = ctx.saved_tensors
+        x, gate, initial, offsets, kept = ctx.saved_tensors
         if v_y is None:
             v_y = torch.zeros_like(x)
-        v_x, v_gate, v_initial = W.gated_scan_bwd(x, gate, initial, offsets, carries, v_y, v_final,
+        v_x, v_gate, v_initial = W.gated_scan_bwd(x, gate, initial, offsets, kept, v_y, v_final,
                                                   ctx.reverse)
         return v_x, v_gate, v_initial if ctx.needs_input_grad[2] else None, None, None
 
@@ -99,7 +99,7 @@ def gated_scan(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
     gate of -inf or until the gates' product leaves float32's range."""
     offsets = _index32(offsets)
     if not _wants_grad(x, gate, initial):
-        return W.gated_scan_fwd(x, gate, initial, offsets, reverse)[:2]
+        return W.gated_scan_fwd(x, gate, initial, offsets, reverse, keep=False)[:2]
     return _GatedScan.apply(x, gate, initial, offsets, bool(reverse))
 
 

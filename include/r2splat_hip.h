@@ -1172,22 +1172,24 @@ int r2s_embedding_bwd(const void *v_out, int64_t v_out_stride, const void *ids,
  * [sequences, width] the state after its last (its initial one if it is
  * empty); y [n, width] contiguous.  A gate of +inf holds the state whatever x
  * is, one of -inf forgets it whatever it was.
- * carries [r2s_gated_scan_tiles(type, n, width), width] receives the states
- * that the backward starts from; the decode form (offsets NULL, length 1)
- * leaves it alone.  Rows of 16-bit elements of an even width must start at
- * multiples of 4 bytes. */
-int64_t r2s_gated_scan_tiles(int32_t type, int64_t n, int64_t width);
-int64_t r2s_gated_scan_workspace_bytes(int32_t type, int64_t n, int64_t width, int32_t backward);
+ * kept [r2s_gated_scan_kept_rows(...), width] (may be NULL: no backward
+ * follows) receives the states that the backward starts from; the decode form
+ * (offsets NULL, length 1) leaves it alone.  ragged: offsets are given.  Rows
+ * of 16-bit elements of an even width must start at multiples of 4 bytes. */
+int64_t r2s_gated_scan_kept_rows(int32_t type, int32_t ragged, int64_t sequences, int64_t length,
+                                 int64_t n, int64_t width);
+int64_t r2s_gated_scan_workspace_bytes(int32_t type, int32_t ragged, int64_t sequences,
+                                       int64_t length, int64_t n, int64_t width);
 int r2s_gated_scan_fwd(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
                        const float *initial, const int32_t *offsets, int64_t sequences,
                        int64_t length, int64_t n, int64_t width, int32_t type, int32_t reverse,
-                       void *y, float *final_state, float *carries, void *workspace,
+                       void *y, float *final_state, float *kept, void *workspace,
                        size_t workspace_bytes, r2s_stream_t stream);
 /* Its gradient: v_y [n, width], v_final [sequences, width] (may be NULL) ->
  * v_x, v_gate [n, width] contiguous, v_initial [sequences, width] (may be
- * NULL: not wanted).  carries as the forward of the same inputs left them. */
+ * NULL: not wanted).  kept as the forward of the same inputs left it. */
 int r2s_gated_scan_bwd(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
-                       const float *initial, const int32_t *offsets, const float *carries,
+                       const float *initial, const int32_t *offsets, const float *kept,
                        const void *v_y, int64_t v_y_stride, const float *v_final,
                        int64_t sequences, int64_t length, int64_t n, int64_t width, int32_t type,
                        int32_t reverse, void *v_x, void *v_gate, float *v_initial,

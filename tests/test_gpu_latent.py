@@ -622,7 +622,7 @@ def test_refusals():
         (lambda: W.gated_scan_fwd(x3, x3, f[:1].bfloat16()), "initial must be torch.float32"),
         (lambda: W.gated_scan_fwd(f, f, None, off.long()), "offsets must be torch.int32"),
         (lambda: W.gated_scan_fwd(f, f, None, off[:1]), "offsets name no sequence"),
-        (lambda: W.gated_scan_bwd(x3, x3, None, None, f[:0], x3), "carries are not those"),
+        (lambda: W.gated_scan_bwd(x3, x3, None, None, f[:0], x3), "kept is not that"),
         (lambda: W.grouped_matmul_fwd(f, w[:, :, :7], None, off), "x must be"),
         (lambda: W.grouped_matmul_fwd(f, w.half(), None, off), "weight must be torch.float32"),
         (lambda: W.grouped_matmul_fwd(f, w, f, off), "bias must be"),
