@@ -101,14 +101,15 @@ struct Place {
   uint32_t col;   // first channel
   uint32_t lane;  // among the lanes across the channels
   bool inside;    // the channels exist
-  int64_t lo, hi; // tokens
+  int32_t lo, hi; // tokens
   __device__ __forceinline__ Place(const Tokens &c, int V, int64_t block, uint32_t slice) {
     lane = threadIdx.x & ((1u << c.lane_bits) - 1u);
     group = static_cast<int>(threadIdx.x >> c.lane_bits);
     col = ((slice << c.lane_bits) + lane) * V;
     inside = col < c.width;
-    const int64_t end = min((block + 1) * c.block, c.n);
-    lo = min(block * c.block + static_cast<int64_t>(group) * c.strip, end);
+    const int32_t end = static_cast<int32_t>(min((block + 1) * c.block, c.n));
+    lo = static_cast<int32_t>(
+        min(block * c.block + static_cast<int64_t>(group) * c.strip, static_cast<int64_t>(end)));
     hi = min(lo + c.strip, end);
   }
 };
@@ -118,7 +119,9 @@ struct Place {
 // not.
 template <typename T, int V>
 struct Rows {
-  const char *base;  // of step 0, wave-uniform
+  using Global = __attribute__((address_space(1))) char *;
+  using Word = typename std::conditional<sizeof(T) * V == 4, uint32_t, uint16_t>::type;
+  Global base;       // of step 0, wave-uniform
   int64_t pitch;     // bytes per step, negative in reverse
   uint32_t offset;
   __device__ __forceinline__ Rows(const T *p, int64_t stride, const Tokens &c, const Place &at,
@@ -130,82 +133,116 @@ struct Rows {
     const uint32_t step = static_cast<uint32_t>(c.strip * row_bytes);
     const uint32_t col = min(at.col, c.width - V) * static_cast<uint32_t>(sizeof(T));
     if (c.reverse) {
-      base = reinterpret_cast<const char *>(p) +
-             (c.n - 1 - t0 - static_cast<int64_t>(per_wave - 1) * c.strip) * row_bytes;
+      base = (Global)p + (c.n - 1 - t0 - static_cast<int64_t>(per_wave - 1) * c.strip) * row_bytes;
       pitch = -row_bytes;
       offset = static_cast<uint32_t>(per_wave - 1 - mine) * step + col;
     } else {
-      base = reinterpret_cast<const char *>(p) + t0 * row_bytes;
+      base = (Global)p + t0 * row_bytes;
       pitch = row_bytes;
       offset = static_cast<uint32_t>(mine) * step + col;
     }
   }
-  __device__ __forceinline__ Pack<T, V> load(int64_t k) const {
-    return load_pack<T, V>(reinterpret_cast<const T *>(base + k * pitch + offset));
+  // Step k's address without the lane's part, kept in scalar registers.
+  __device__ __forceinline__ Global step(int64_t k) const {
+    Global s = base + k * pitch;
+    asm("" : "+s"(s));
+    return s;
   }
-  __device__ __forceinline__ void store(int64_t k, const Pack<T, V> &x) const {
-    store_pack<T, V>(reinterpret_cast<T *>(const_cast<char *>(base + k * pitch + offset)), x);
+  // The lane's offset, known to be 32 bits wide where it is added (else the
+  // address is a 64-bit vector sum).
+  __device__ __forceinline__ uint32_t lane_offset() const {
+    uint32_t o = offset;
+    asm("" : "+v"(o));
+    return o;
+  }
+  __device__ __forceinline__ Word load(Global s, uint32_t o) const {
+    return *(const __attribute__((address_space(1))) Word *)(s + o);
+  }
+  __device__ __forceinline__ void store(Global s, uint32_t o, Word x) const {
+    *(__attribute__((address_space(1))) Word *)(s + o) = x;
+  }
+  __device__ __forceinline__ Word load(int64_t k) const { return load(step(k), lane_offset()); }
+  __device__ __forceinline__ void store(int64_t k, Word x) const {
+    store(step(k), lane_offset(), x);
+  }
+  // Element v of a word.
+  static __device__ __forceinline__ float value(Word x, int v) {
+    return static_cast<float>(__builtin_bit_cast(Pack<T, V>, x).v[v]);
   }
 };
 
-// kChunk rows from step j on; the places past `count` tokens are 0.
-template <typename T, int V>
-__device__ __forceinline__ void load_chunk(const Rows<T, V> &r, int64_t j, bool full,
-                                           int64_t count, Pack<T, V> (&x)[kChunk]) {
-  if (full) {
-#pragma unroll
-    for (int k = 0; k < kChunk; ++k) x[k] = r.load(j + k);
-  } else {
+// kChunk rows from step j on, of which this lane has `count` in all; 0 past
+// them.
+template <typename R, typename Word>
+__device__ __forceinline__ void load_chunk(const R &r, int32_t j, int32_t count,
+                                           Word (&x)[kChunk]) {
+  typename R::Global s = r.step(j);
+  const uint32_t o = r.lane_offset();
+  if (__all(j + kChunk <= count)) {
 #pragma unroll
     for (int k = 0; k < kChunk; ++k) {
-      if (j + k < count) {
-        x[k] = r.load(j + k);
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) x[k].v[v] = static_cast<T>(0.0f);
-      }
+      x[k] = r.load(s, o);
+      s += r.pitch;
+      asm("" : "+s"(s));
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) x[k] = j + k < count ? r.load(j + k) : Word(0);
+  }
+}
+template <typename R, typename T, int V>
+__device__ __forceinline__ void store_chunk(const R &r, int32_t j,
+                                            const Pack<T, V> (&x)[kChunk]) {
+  typename R::Global s = r.step(j);
+  const uint32_t o = r.lane_offset();
+#pragma unroll
+  for (int k = 0; k < kChunk; ++k) {
+    r.store(s, o, __builtin_bit_cast(typename R::Word, x[k]));
+    s += r.pitch;
+    asm("" : "+s"(s));
   }
 }
 
 // The sequence that a walk is in: its number and tokens [first, last].
 struct Cursor {
-  int64_t s, first, last;
+  int32_t s, first, last;
 
   // The sequence of token t; none (s = -1) where there is no such token.
-  __device__ __forceinline__ void seek(const Tokens &c, int64_t t, bool some) {
+  __device__ __forceinline__ void seek(const Tokens &c, int32_t t, bool some) {
     s = -1;
     first = last = -1;
     if (c.offsets == nullptr) {
       if (!some) return;
-      s = static_cast<int64_t>(static_cast<uint32_t>(t) / static_cast<uint32_t>(c.length));
+      s = static_cast<int32_t>(static_cast<uint32_t>(t) / static_cast<uint32_t>(c.length));
     } else {
       // The last sequence that starts at or before t, by the lanes of the
       // group together: 2^lane_bits probes a round.
       const uint32_t lanes = 1u << c.lane_bits, lane = lane_id() & (lanes - 1u);
       const uint32_t shift = lane_id() & ~(lanes - 1u);
       const uint64_t mask = lanes == 64u ? ~0ull : ((1ull << lanes) - 1ull);
-      int64_t lo = 0, hi = c.sequences;
+      uint32_t lo = 0, hi = static_cast<uint32_t>(c.sequences);
       while (__any(hi - lo > 1)) {
-        const int64_t step = (hi - lo + lanes) / (lanes + 1);
-        const int64_t q = lo + (static_cast<int64_t>(lane) + 1) * step;
-        const uint64_t under = ballot(step > 0 && q < hi && c.start(q) <= t) >> shift & mask;
-        const int64_t k = __popcll(under);
-        hi = min(hi, lo + (k + 1) * step);
+        const uint32_t step = (hi - lo - 1) / (lanes + 1) + 1;
+        const uint64_t q = lo + (static_cast<uint64_t>(lane) + 1) * step;
+        const uint64_t under =
+            ballot(q < hi && c.start(static_cast<int64_t>(q)) <= t) >> shift & mask;
+        const uint32_t k = static_cast<uint32_t>(__popcll(under));
+        hi = static_cast<uint32_t>(
+            min(static_cast<uint64_t>(hi), lo + (static_cast<uint64_t>(k) + 1) * step));
         lo += k * step;
         if (hi <= lo) hi = lo + 1;  // offsets that do not ascend
       }
       if (!some) return;
-      s = lo;
+      s = static_cast<int32_t>(lo);
     }
     bounds(c);
   }
   __device__ __forceinline__ void bounds(const Tokens &c) {
-    first = c.start(s);
-    last = c.start(s + 1) - 1;
+    first = static_cast<int32_t>(c.start(s));
+    last = static_cast<int32_t>(c.start(s + 1) - 1);
   }
   // The sequences with a token that follow, and those before.
-  __device__ __forceinline__ void next(const Tokens &c, int64_t t) {
+  __device__ __forceinline__ void next(const Tokens &c, int32_t t) {
     do {
       ++s;
       if (s >= c.sequences) {
@@ -216,7 +253,7 @@ struct Cursor {
       bounds(c);
     } while (last < t);
   }
-  __device__ __forceinline__ void previous(const Tokens &c, int64_t t) {
+  __device__ __forceinline__ void previous(const Tokens &c, int32_t t) {
     do {
       --s;
       if (s < 0) {
@@ -231,10 +268,10 @@ struct Cursor {
 // Whether tokens [t, t + kChunk) of every lane of the wave lie inside one
 // sequence, and none but its first token is not a sequence's first (forward)
 // or none is its last (backward).
-__device__ __forceinline__ bool plain_forward(const Cursor &q, int64_t t, int64_t hi) {
+__device__ __forceinline__ bool plain_forward(const Cursor &q, int32_t t, int32_t hi) {
   return __all(t + kChunk <= hi && t > q.first && t + kChunk - 1 <= q.last);
 }
-__device__ __forceinline__ bool plain_backward(const Cursor &q, int64_t t, int64_t hi) {
+__device__ __forceinline__ bool plain_backward(const Cursor &q, int32_t t, int32_t hi) {
   return __all(t + kChunk <= hi && t > q.first && t + kChunk - 1 < q.last);
 }
 
@@ -257,17 +294,15 @@ __device__ __forceinline__ void compose_forward(const Rows<T, V> &xr, const Rows
   for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
   Cursor q;
   q.seek(c, at.lo, at.lo < at.hi);
-  const int64_t count = at.hi - at.lo;
-  for (int64_t j = 0; __any(j < count); j += kChunk) {
-    const int64_t t = at.lo + j;
-    Pack<T, V> x[kChunk], g[kChunk];
-    const bool full = __all(j + kChunk <= count);
-    load_chunk<T, V>(xr, j, full, count, x);
-    load_chunk<T, V>(gr, j, full, count, g);
-    const bool plain = full && plain_forward(q, t, at.hi);
-    bool fine = plain;
-    float p1[V], u1[V];
-    if (plain) {
+  const int32_t count = at.hi - at.lo;
+  using R = Rows<T, V>;
+  typename R::Word x[kChunk], g[kChunk];
+  for (int32_t j = 0; __any(j < count); j += kChunk) {
+    const int32_t t = at.lo + j;
+    load_chunk(xr, j, count, x);
+    load_chunk(gr, j, count, g);
+    if (plain_forward(q, t, at.hi)) {
+      float p1[V], u1[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) p1[v] = p[v], u1[v] = u[v];
 #pragma unroll
@@ -275,31 +310,34 @@ __device__ __forceinline__ void compose_forward(const Rows<T, V> &xr, const Rows
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float a, b;
-          gate_pair(static_cast<float>(g[k].v[v]), a, b);
-          u1[v] = fmaf(a, u1[v], b * static_cast<float>(x[k].v[v]));
+          gate_pair(R::value(g[k], v), a, b);
+          u1[v] = fmaf(a, u1[v], b * R::value(x[k], v));
           p1[v] *= a;
         }
-      bool ok = true;
+      bool fine = true;
 #pragma unroll
-      for (int v = 0; v < V; ++v) ok = ok && finite(u1[v]) && finite(p1[v]);
-      fine = __all(ok);
+      for (int v = 0; v < V; ++v) fine = fine && finite(u1[v]) && finite(p1[v]);
+      if (__all(fine)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[v] = p1[v], u[v] = u1[v];
+        continue;
+      }
+      // Loaded again rather than held through the form above.
+      load_chunk(xr, j, count, x);
+      load_chunk(gr, j, count, g);
     }
-    if (fine) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) p[v] = p1[v], u[v] = u1[v];
-    } else {
-      for (int k = 0; k < kChunk; ++k) {
-        if (j + k >= count) break;
+    for (int k = 0; k < kChunk; ++k) {
+      if (j + k < count) {
         if (t + k > q.last) q.next(c, t + k);
         const bool first = t + k == q.first;
         float h0[V];
         if (first) load_state<V>(initial, c, at, q.s, h0);
-        const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float a, b;
-          gate_pair(static_cast<float>(gk.v[v]), a, b);
-          const float fresh = scaled<true>(b, static_cast<float>(xk.v[v]));
+          gate_pair(R::value(g[k], v), a, b);
+          const float fresh = scaled<true>(b, R::value(x[k], v));
           u[v] = applied<true>(a, first ? h0[v] : u[v], fresh);
           p[v] = first ? 0.0f : p[v] * a;
         }
@@ -317,22 +355,21 @@ __device__ __forceinline__ void walk_forward(const Rows<T, V> &xr, const Rows<T,
                                              float *final, float (&h)[V]) {
   Cursor q;
   q.seek(c, at.lo, at.lo < at.hi);
-  const int64_t count = at.hi - at.lo;
-  for (int64_t j = 0; __any(j < count); j += kChunk) {
-    const int64_t t = at.lo + j;
-    Pack<T, V> x[kChunk], g[kChunk], y[kChunk];
-    const bool full = __all(j + kChunk <= count);
-    load_chunk<T, V>(xr, j, full, count, x);
-    load_chunk<T, V>(gr, j, full, count, g);
+  const int32_t count = at.hi - at.lo;
+  using R = Rows<T, V>;
+  typename R::Word x[kChunk], g[kChunk];
+  for (int32_t j = 0; __any(j < count); j += kChunk) {
+    const int32_t t = at.lo + j;
+    load_chunk(xr, j, count, x);
+    load_chunk(gr, j, count, g);
     if (kept != nullptr && j < count && at.inside) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) kept[j / kChunk * c.width + v] = h[v];
+      for (int v = 0; v < V; ++v) kept[static_cast<int64_t>(j / kChunk) * c.width + v] = h[v];
     }
     // A sequence's last token stores its state: not in the plain form.
-    const bool plain = full && plain_backward(q, t, at.hi);
-    bool fine = plain;
-    float h1[V];
-    if (plain) {
+    if (plain_backward(q, t, at.hi)) {
+      float h1[V];
+      Pack<T, V> y[kChunk];
 #pragma unroll
       for (int v = 0; v < V; ++v) h1[v] = h[v];
 #pragma unroll
@@ -340,38 +377,37 @@ __device__ __forceinline__ void walk_forward(const Rows<T, V> &xr, const Rows<T,
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float a, b;
-          gate_pair(static_cast<float>(g[k].v[v]), a, b);
-          h1[v] = fmaf(a, h1[v], b * static_cast<float>(x[k].v[v]));
+          gate_pair(R::value(g[k], v), a, b);
+          h1[v] = fmaf(a, h1[v], b * R::value(x[k], v));
           y[k].v[v] = static_cast<T>(h1[v]);
         }
-      bool ok = true;
+      bool fine = true;
 #pragma unroll
-      for (int v = 0; v < V; ++v) ok = ok && finite(h1[v]);
-      fine = __all(ok);
-    }
-    if (fine) {
+      for (int v = 0; v < V; ++v) fine = fine && finite(h1[v]);
+      if (__all(fine)) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = h1[v];
-      if (at.inside) {
-#pragma unroll
-        for (int k = 0; k < kChunk; ++k) yr.store(j + k, y[k]);
+        for (int v = 0; v < V; ++v) h[v] = h1[v];
+        if (at.inside) store_chunk(yr, j, y);
+        continue;
       }
-    } else {
-      for (int k = 0; k < kChunk; ++k) {
-        if (j + k >= count) break;
+      load_chunk(xr, j, count, x);
+      load_chunk(gr, j, count, g);
+    }
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+      if (j + k < count) {
         if (t + k > q.last) q.next(c, t + k);
         if (t + k == q.first) load_state<V>(initial, c, at, q.s, h);
-        const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k);
-        Pack<T, V> yk;
+        Pack<T, V> y;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float a, b;
-          gate_pair(static_cast<float>(gk.v[v]), a, b);
-          h[v] = applied<true>(a, h[v], scaled<true>(b, static_cast<float>(xk.v[v])));
-          yk.v[v] = static_cast<T>(h[v]);
+          gate_pair(R::value(g[k], v), a, b);
+          h[v] = applied<true>(a, h[v], scaled<true>(b, R::value(x[k], v)));
+          y.v[v] = static_cast<T>(h[v]);
         }
         if (at.inside) {
-          yr.store(j + k, yk);
+          yr.store(j + k, __builtin_bit_cast(typename R::Word, y));
           if (t + k == q.last) {
 #pragma unroll
             for (int v = 0; v < V; ++v) final[c.state_row(q.s) * c.width + at.col + v] = h[v];
@@ -391,20 +427,18 @@ __device__ __forceinline__ void compose_backward(const Rows<T, V> &gr, const Row
                                                  const Place &at, float (&p)[V], float (&u)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
-  const int64_t count = at.hi - at.lo;
+  const int32_t count = at.hi - at.lo;
   Cursor q;
   q.seek(c, at.hi - 1, count > 0);
-  for (int64_t j = c.steps - kChunk; j >= 0; j -= kChunk) {
+  using R = Rows<T, V>;
+  typename R::Word g[kChunk], d[kChunk];
+  for (int32_t j = c.steps - kChunk; j >= 0; j -= kChunk) {
     if (!__any(j < count)) continue;
-    const int64_t t = at.lo + j;
-    Pack<T, V> g[kChunk], d[kChunk];
-    const bool full = __all(j + kChunk <= count);
-    load_chunk<T, V>(gr, j, full, count, g);
-    load_chunk<T, V>(vr, j, full, count, d);
-    const bool plain = full && plain_backward(q, t, at.hi);
-    bool fine = plain;
-    float p1[V], u1[V];
-    if (plain) {
+    const int32_t t = at.lo + j;
+    load_chunk(gr, j, count, g);
+    load_chunk(vr, j, count, d);
+    if (plain_backward(q, t, at.hi)) {
+      float p1[V], u1[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) p1[v] = p[v], u1[v] = u[v];
 #pragma unroll
@@ -412,31 +446,33 @@ __device__ __forceinline__ void compose_backward(const Rows<T, V> &gr, const Row
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float a, b;
-          gate_pair(static_cast<float>(g[k].v[v]), a, b);
-          u1[v] = a * (static_cast<float>(d[k].v[v]) + u1[v]);
+          gate_pair(R::value(g[k], v), a, b);
+          u1[v] = a * (R::value(d[k], v) + u1[v]);
           p1[v] *= a;
         }
-      bool ok = true;
+      bool fine = true;
 #pragma unroll
-      for (int v = 0; v < V; ++v) ok = ok && finite(u1[v]) && finite(p1[v]);
-      fine = __all(ok);
+      for (int v = 0; v < V; ++v) fine = fine && finite(u1[v]) && finite(p1[v]);
+      if (__all(fine)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[v] = p1[v], u[v] = u1[v];
+        continue;
+      }
+      load_chunk(gr, j, count, g);
+      load_chunk(vr, j, count, d);
     }
-    if (fine) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) p[v] = p1[v], u[v] = u1[v];
-    } else {
-      for (int k = kChunk - 1; k >= 0; --k) {
-        if (j + k >= count) continue;
+    for (int k = kChunk - 1; k >= 0; --k) {
+      if (j + k < count) {
         if (t + k < q.first) q.previous(c, t + k);
         const bool last = t + k == q.last;
         float f0[V];
         if (last) load_state<V>(v_final, c, at, q.s, f0);
-        const Pack<T, V> gk = gr.load(j + k), dk = vr.load(j + k);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float a, b;
-          gate_pair(static_cast<float>(gk.v[v]), a, b);
-          u[v] = scaled<true>(a, static_cast<float>(dk.v[v]) + (last ? f0[v] : u[v]));
+          gate_pair(R::value(g[k], v), a, b);
+          u[v] = scaled<true>(a, R::value(d[k], v) + (last ? f0[v] : u[v]));
           p[v] = last ? 0.0f : p[v] * a;
         }
       }
@@ -452,108 +488,107 @@ __device__ __forceinline__ void walk_backward(const Rows<T, V> &xr, const Rows<T
                                               const Rows<T, V> &dgr, const float *initial,
                                               const float *v_final, const Tokens &c,
                                               const Place &at, const float *kept,
-                                              float *v_initial, float (&f)[V]) {
-  const int64_t count = at.hi - at.lo;
+                                              float *v_initial, float *s_before,
+                                              float (&f)[V]) {
+  const int32_t count = at.hi - at.lo;
   Cursor q;
   q.seek(c, at.hi - 1, count > 0);
-  for (int64_t j = c.steps - kChunk; j >= 0; j -= kChunk) {
+  using R = Rows<T, V>;
+  typename R::Word x[kChunk], g[kChunk], d[kChunk];
+  for (int32_t j = c.steps - kChunk; j >= 0; j -= kChunk) {
     if (!__any(j < count)) continue;
-    const int64_t t = at.lo + j;
-    Pack<T, V> x[kChunk], g[kChunk], d[kChunk];
-    const bool full = __all(j + kChunk <= count);
+    const int32_t t = at.lo + j;
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      h[v] = j < count && at.inside ? kept[j / kChunk * c.width + v] : 0.0f;
-    load_chunk<T, V>(xr, j, full, count, x);
-    load_chunk<T, V>(gr, j, full, count, g);
-    load_chunk<T, V>(vr, j, full, count, d);
-    const bool plain = full && plain_backward(q, t, at.hi);
-    bool fine = plain;
-    float f1[V];
-    Pack<T, V> dx[kChunk], dg[kChunk];
-    if (plain) {
-      float prior[kChunk][V], a[kChunk][V], b[kChunk][V], h1[V];
+      h[v] = j < count && at.inside ? kept[static_cast<int64_t>(j / kChunk) * c.width + v] : 0.0f;
+    load_chunk(xr, j, count, x);
+    load_chunk(gr, j, count, g);
+    load_chunk(vr, j, count, d);
+    if (plain_backward(q, t, at.hi)) {
+      float prior[kChunk][V], a[kChunk][V], b[kChunk][V], f1[V], h1[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) f1[v] = f[v], h1[v] = h[v];
 #pragma unroll
       for (int k = 0; k < kChunk; ++k)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          gate_pair(static_cast<float>(g[k].v[v]), a[k][v], b[k][v]);
-          const float xv = static_cast<float>(x[k].v[v]);
+          gate_pair(R::value(g[k], v), a[k][v], b[k][v]);
+          const float xv = R::value(x[k], v);
           prior[k][v] = h1[v] - xv;
           h1[v] = fmaf(a[k][v], h1[v], b[k][v] * xv);
         }
+      // Stored as they come; where the chunk turns out not to be finite, the
+      // other form stores again.
 #pragma unroll
-      for (int k = kChunk - 1; k >= 0; --k)
+      for (int k = kChunk - 1; k >= 0; --k) {
+        Pack<T, V> dx, dg;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float gk = static_cast<float>(d[k].v[v]) + f1[v], vx = b[k][v] * gk;
+          const float gk = R::value(d[k], v) + f1[v], vx = b[k][v] * gk;
           f1[v] = a[k][v] * gk;
-          dx[k].v[v] = static_cast<T>(vx);
-          dg[k].v[v] = static_cast<T>(a[k][v] * (vx * prior[k][v]));
+          dx.v[v] = static_cast<T>(vx);
+          dg.v[v] = static_cast<T>(a[k][v] * (vx * prior[k][v]));
         }
-      bool ok = true;
-#pragma unroll
-      for (int v = 0; v < V; ++v) ok = ok && finite(f1[v]) && finite(h1[v]);
-      fine = __all(ok);
-    }
-    if (fine) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) f[v] = f1[v];
-      if (at.inside) {
-#pragma unroll
-        for (int k = 0; k < kChunk; ++k) dxr.store(j + k, dx[k]), dgr.store(j + k, dg[k]);
+        if (at.inside) {
+          dxr.store(j + k, __builtin_bit_cast(typename R::Word, dx));
+          dgr.store(j + k, __builtin_bit_cast(typename R::Word, dg));
+        }
       }
-    } else {
-      // The sequences of the chunk's tokens once forwards, for the states
-      // before them, then back.
-      float before[kChunk][V];
-      Cursor w = q;
-      if (j < count) {
-        const int64_t end = min(static_cast<int64_t>(kChunk), count - j);
-        if (t < w.first) w.previous(c, t);
+      bool fine = true;
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) {
-          if (k >= end) continue;
-          if (t + k > w.last) w.next(c, t + k);
-          if (t + k == w.first) load_state<V>(initial, c, at, w.s, h);
-          const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k);
+      for (int v = 0; v < V; ++v) fine = fine && finite(f1[v]) && finite(h1[v]);
+      if (__all(fine)) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            float a, b;
-            gate_pair(static_cast<float>(gk.v[v]), a, b);
-            before[k][v] = h[v];
-            h[v] = applied<true>(a, h[v], scaled<true>(b, static_cast<float>(xk.v[v])));
-          }
+        for (int v = 0; v < V; ++v) f[v] = f1[v];
+        continue;
+      }
+      load_chunk(xr, j, count, x);
+      load_chunk(gr, j, count, g);
+      load_chunk(vr, j, count, d);
+    }
+    // Token by token: the states before them first (in LDS, so that the other
+    // form keeps its registers), then back.
+    Cursor w = q;
+    if (j < count && t < w.first) w.previous(c, t);
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+      if (j + k < count) {
+        if (t + k > w.last) w.next(c, t + k);
+        if (t + k == w.first) load_state<V>(initial, c, at, w.s, h);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(R::value(g[k], v), a, b);
+          s_before[(k * V + v) * blockDim.x + threadIdx.x] = h[v];
+          h[v] = applied<true>(a, h[v], scaled<true>(b, R::value(x[k], v)));
         }
+      }
+    }
 #pragma unroll
-        for (int k = kChunk - 1; k >= 0; --k) {
-          if (k >= end) continue;
-          if (t + k < q.first) q.previous(c, t + k);
-          if (t + k == q.last) load_state<V>(v_final, c, at, q.s, f);
-          const Pack<T, V> xk = xr.load(j + k), gk = gr.load(j + k), dk = vr.load(j + k);
-          Pack<T, V> vx, vg;
+    for (int k = kChunk - 1; k >= 0; --k) {
+      if (j + k < count) {
+        if (t + k < q.first) q.previous(c, t + k);
+        if (t + k == q.last) load_state<V>(v_final, c, at, q.s, f);
+        Pack<T, V> dx, dg;
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            float a, b;
-            gate_pair(static_cast<float>(gk.v[v]), a, b);
-            const float gv = static_cast<float>(dk.v[v]) + f[v];
-            const float dx = scaled<true>(b, gv);
-            const float dg = a * (dx * (before[k][v] - static_cast<float>(xk.v[v])));
-            vx.v[v] = static_cast<T>(dx);
-            vg.v[v] = static_cast<T>(a == 0.0f || b == 0.0f ? 0.0f : dg);
-            f[v] = scaled<true>(a, gv);
-          }
-          if (at.inside) {
-            dxr.store(j + k, vx);
-            dgr.store(j + k, vg);
-            if (t + k == q.first && v_initial != nullptr) {
+        for (int v = 0; v < V; ++v) {
+          float a, b;
+          gate_pair(R::value(g[k], v), a, b);
+          const float gk = R::value(d[k], v) + f[v], vx = scaled<true>(b, gk);
+          const float before = s_before[(k * V + v) * blockDim.x + threadIdx.x];
+          const float vg = a * (vx * (before - R::value(x[k], v)));
+          dx.v[v] = static_cast<T>(vx);
+          dg.v[v] = static_cast<T>(a == 0.0f || b == 0.0f ? 0.0f : vg);
+          f[v] = scaled<true>(a, gk);
+        }
+        if (at.inside) {
+          dxr.store(j + k, __builtin_bit_cast(typename R::Word, dx));
+          dgr.store(j + k, __builtin_bit_cast(typename R::Word, dg));
+          if (t + k == q.first && v_initial != nullptr) {
 #pragma unroll
-              for (int v = 0; v < V; ++v)
-                v_initial[c.state_row(q.s) * c.width + at.col + v] = f[v];
-            }
+            for (int v = 0; v < V; ++v)
+              v_initial[c.state_row(q.s) * c.width + at.col + v] = f[v];
           }
         }
       }
@@ -600,15 +635,27 @@ __device__ __forceinline__ void store_map(float *maps, int64_t row, const Tokens
   }
 }
 
+// Blocks that share rows' cache lines (slices of one block of tokens) run on
+// one XCD.
+__device__ __forceinline__ void block_and_slice(uint32_t slices, int64_t &block,
+                                                uint32_t &slice) {
+  const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
+  block = id / slices;
+  slice = id - static_cast<uint32_t>(block) * slices;
+}
+
 template <typename T, int V, bool kBack>
 __global__ __launch_bounds__(kThreads) void scan_maps_kernel(
     const T *__restrict__ a, int64_t a_stride, const T *__restrict__ b, int64_t b_stride,
-    const float *__restrict__ state, Tokens c, float *__restrict__ strips,
+    const float *__restrict__ state, Tokens c, uint32_t slices, float *__restrict__ strips,
     float *__restrict__ blocks) {
   extern __shared__ float s_map[];
+  int64_t block;
+  uint32_t slice;
+  block_and_slice(slices, block, slice);
   const int groups = kThreads >> c.lane_bits;
-  const Place at(c, V, blockIdx.x, blockIdx.y);
-  const Rows<T, V> ar(a, a_stride, c, at, blockIdx.x), br(b, b_stride, c, at, blockIdx.x);
+  const Place at(c, V, block, slice);
+  const Rows<T, V> ar(a, a_stride, c, at, block), br(b, b_stride, c, at, block);
   float p[V], u[V];
   if constexpr (kBack)
     compose_backward<T, V>(ar, br, state, c, at, p, u);
@@ -616,7 +663,7 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(
     compose_forward<T, V>(ar, br, state, c, at, p, u);
   put_map<V>(s_map, p, u);
   if (at.inside)
-    store_map<V>(strips, static_cast<int64_t>(blockIdx.x) * groups + at.group, c, at, p, u);
+    store_map<V>(strips, block * groups + at.group, c, at, p, u);
   __syncthreads();
   // The block's map: everything from its far end, composed by one group.
   if (at.group != (kBack ? groups - 1 : 0) || !at.inside) return;
@@ -629,46 +676,83 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(
       p[v] *= m[v * 2];
     }
   }
-  store_map<V>(blocks, blockIdx.x, c, at, p, u);
+  store_map<V>(blocks, block, c, at, p, u);
+}
+
+// Sequences without a token: the state they end in (or its gradient) is the
+// one they began with.
+__device__ __forceinline__ void empty_state(const Tokens &c, int64_t i, const float *in,
+                                            float *out) {
+  const int64_t s = i / c.width;
+  if (s >= c.sequences || (c.offsets != nullptr && c.offsets[s] < c.offsets[s + 1])) return;
+  out[i] = in != nullptr ? in[i] : 0.0f;
 }
 
 // The state that enters each block, from the blocks' maps in order (from the
-// last block down with `down`).  16 channels per launch block; each of its 64
-// rows of threads composes one 64th of the blocks, and again with the state
-// that the rows before leave.
-constexpr int kCarryRows = 64;
+// last block down with `down`).  A launch block takes kCarryCols channels, and
+// kCarryRows x kCarryPer maps of each at a time: a thread composes kCarryPer of
+// them in registers, the rows of a wave meet by lane shifts, the waves in LDS.
+// Launch blocks past the channels' look after the sequences without a token.
+constexpr int kCarryCols = 4, kCarryRows = 1024 / kCarryCols, kCarryPer = 4;
 __global__ __launch_bounds__(1024) void scan_carry_kernel(const float2 *__restrict__ maps,
-                                                          int32_t blocks, uint32_t width,
-                                                          int32_t down,
-                                                          float *__restrict__ carries) {
-  __shared__ float2 s_map[kCarryRows][16];
-  const uint32_t lane = threadIdx.x % 16, row = threadIdx.x / 16;
-  const uint32_t col = blockIdx.x * 16 + lane;
-  const int32_t per = (blocks + kCarryRows - 1) / kCarryRows;
-  const int32_t i0 = min(static_cast<int32_t>(row) * per, blocks), i1 = min(i0 + per, blocks);
-  const bool inside = col < width;
-  auto at = [&](int32_t i) {
-    return static_cast<int64_t>(down ? blocks - 1 - i : i) * width + col;
-  };
-  float p = 1.0f, u = 0.0f;
-  if (inside) {
-#pragma unroll 8
-    for (int32_t i = i0; i < i1; ++i) {
-      const float2 m = maps[at(i)];
-      u = applied<true>(m.x, u, m.y);
-      p *= m.x;
-    }
+                                                          int32_t blocks, Tokens c, int32_t down,
+                                                          uint32_t channel_blocks,
+                                                          float *__restrict__ carries,
+                                                          const float *__restrict__ empty_in,
+                                                          float *__restrict__ empty_out) {
+  if (blockIdx.x >= channel_blocks) {
+    empty_state(c, static_cast<int64_t>(blockIdx.x - channel_blocks) * 1024 + threadIdx.x,
+                empty_in, empty_out);
+    return;
   }
-  s_map[row][lane] = make_float2(p, u);
-  __syncthreads();
-  if (!inside) return;
-  float h = 0.0f;
-  for (uint32_t r = 0; r < row; ++r) h = applied<true>(s_map[r][lane].x, h, s_map[r][lane].y);
-#pragma unroll 8
-  for (int32_t i = i0; i < i1; ++i) {
-    const float2 m = maps[at(i)];
-    carries[at(i)] = h;
-    h = applied<true>(m.x, h, m.y);
+  __shared__ float2 s_map[16][kCarryCols];
+  const uint32_t lane = threadIdx.x % kCarryCols, wave = threadIdx.x / 64;
+  const int32_t row = static_cast<int32_t>(threadIdx.x / kCarryCols);
+  const uint32_t col = min(blockIdx.x * kCarryCols + lane, c.width - 1);
+  const bool inside = blockIdx.x * kCarryCols + lane < c.width;
+  float h = 0.0f;  // the state that enters the round
+  for (int32_t r0 = 0; r0 < blocks; r0 += kCarryRows * kCarryPer) {
+    const int32_t i0 = r0 + row * kCarryPer;
+    float2 m[kCarryPer];
+#pragma unroll
+    for (int k = 0; k < kCarryPer; ++k) {
+      const int32_t i = min(i0 + k, blocks - 1);
+      m[k] = maps[static_cast<int64_t>(down ? blocks - 1 - i : i) * c.width + col];
+    }
+    float p = 1.0f, u = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kCarryPer; ++k) {
+      if (i0 + k >= blocks) m[k] = make_float2(1.0f, 0.0f);
+      u = applied<true>(m[k].x, u, m[k].y);
+      p *= m[k].x;
+    }
+#pragma unroll
+    for (int off = kCarryCols; off < 64; off *= 2) {
+      const float pb = __shfl_up(p, off, 64), ub = __shfl_up(u, off, 64);
+      if (static_cast<int>(threadIdx.x % 64) >= off) {
+        u = applied<true>(p, ub, u);
+        p *= pb;
+      }
+    }
+    if (threadIdx.x % 64 >= 64 - kCarryCols) s_map[wave][lane] = make_float2(p, u);
+    float before_p = __shfl_up(p, kCarryCols, 64), before_u = __shfl_up(u, kCarryCols, 64);
+    if (threadIdx.x % 64 < kCarryCols) before_p = 1.0f, before_u = 0.0f;
+    __syncthreads();
+    float mine = h;
+#pragma unroll
+    for (uint32_t w = 0; w < 16; ++w) {
+      if (w == wave) mine = h;
+      h = applied<true>(s_map[w][lane].x, h, s_map[w][lane].y);
+    }
+    __syncthreads();
+    mine = applied<true>(before_p, mine, before_u);
+#pragma unroll
+    for (int k = 0; k < kCarryPer; ++k) {
+      const int32_t i = i0 + k;
+      if (inside && i < blocks)
+        carries[static_cast<int64_t>(down ? blocks - 1 - i : i) * c.width + col] = mine;
+      mine = applied<true>(m[k].x, mine, m[k].y);
+    }
   }
 }
 
@@ -692,15 +776,6 @@ __device__ __forceinline__ void enter_strip(const float *strips, const float *ca
 
 // How a walk gets the state that enters its strip.
 enum Mode { kPacked, kResidentMode, kOwn };
-
-// Blocks of a resident or own launch that share rows' cache lines (slices of
-// one block of tokens) run on one XCD.
-__device__ __forceinline__ void block_and_slice(uint32_t slices, int64_t &block,
-                                                uint32_t &slice) {
-  const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
-  block = id / slices;
-  slice = id - static_cast<uint32_t>(block) * slices;
-}
 
 // kept [strips][steps / kChunk][width].
 template <typename T, int V, int kMode, int kBlock>
@@ -764,18 +839,14 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(
     enter_strip<V, true>(strips, carries, c, at, groups, block, f);
   }
   kept += (block * groups + at.group) * (c.steps / kChunk) * c.width + at.col;
-  walk_backward<T, V>(xr, gr, vr, dxr, dgr, initial, v_final, c, at, kept, v_initial, f);
+  walk_backward<T, V>(xr, gr, vr, dxr, dgr, initial, v_final, c, at, kept, v_initial,
+                      s_map + (kMode == kResidentMode ? blockDim.x * V * 2 : 0), f);
 }
 
-// Sequences without a token: the state they end in (or its gradient) is the
-// one they began with.
 __global__ __launch_bounds__(kThreads) void scan_empty_kernel(Tokens c,
                                                               const float *__restrict__ in,
                                                               float *__restrict__ out) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t s = i / c.width;
-  if (s >= c.sequences || (c.offsets != nullptr && c.offsets[s] < c.offsets[s + 1])) return;
-  out[i] = in != nullptr ? in[i] : 0.0f;
+  empty_state(c, static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, in, out);
 }
 
 // One token per sequence, the decode form: nothing to scan.
@@ -806,9 +877,11 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(
 
 // ---------------------------------------------------------------- host ---
 
-// The threads that a packed call spreads the tokens over: 256 CUs of 24
-// waves.
-constexpr int64_t kSpread = 256 * 24 * 64;
+// The threads that a packed call spreads the tokens over, in waves per CU.  A
+// lane of 16-bit rows holds two channels, so half the waves have as much in
+// flight: 500k x 64 bf16 74.6 us with 16 and 82.8 us with 32, 200k x 99 f32
+// (forward and backward) 328 and 315 us.
+constexpr int64_t kSpread16 = 256 * 16 * 64, kSpread32 = 256 * 32 * 64;
 
 struct Plan {
   Mode mode;
@@ -837,9 +910,13 @@ Plan plan_of(int type, const int32_t *offsets, int64_t n, int64_t sequences, int
   // 4 bytes per lane where 16-bit rows allow; 64 bytes of a row per block.
   p.V = type != R2S_TYPE_F32 && width % 2 == 0 ? 2 : 1;
   const int64_t vpr = width / p.V;
-  while (c.lane_bits < 4 && (1 << c.lane_bits) < vpr) ++c.lane_bits;
+  auto set_lanes = [&](uint32_t most) {
+    c.lane_bits = 0;
+    while (c.lane_bits < most && (1 << c.lane_bits) < vpr) ++c.lane_bits;
+    p.slices = static_cast<uint32_t>(ceil_div(vpr, 1 << c.lane_bits));
+  };
+  set_lanes(4);
   const int64_t lanes = int64_t{1} << c.lane_bits;
-  p.slices = static_cast<uint32_t>(ceil_div(vpr, lanes));
   if (!ragged && length <= 128) {
     p.mode = kOwn;
     p.threads = kThreads;
@@ -854,7 +931,9 @@ Plan plan_of(int type, const int32_t *offsets, int64_t n, int64_t sequences, int
   } else {
     p.mode = kPacked;
     p.threads = kThreads;
-    const int64_t even = ceil_div(n * lanes * p.slices, kSpread);
+    set_lanes(5);
+    const int64_t even = ceil_div(n * (int64_t{p.slices} << c.lane_bits),
+                                  p.V == 2 ? kSpread16 : kSpread32);
     c.strip = static_cast<int32_t>(
         align_up(std::min<int64_t>(std::max<int64_t>(even, 16), 128), kChunk));
     c.block = p.groups() * c.strip;
@@ -884,8 +963,9 @@ int check_scan(const char *what, int type, const int32_t *offsets, int64_t n, in
               "%s: %lld tokens are not %lld sequences of %lld", what, (long long)n,
               (long long)sequences, (long long)length);
   R2S_REQUIRE(sequences > 0 || n == 0, "%s: tokens without a sequence", what);
-  if (n > kInt32Max || sequences >= kInt32Max || width > (1 << 16)) {
-    set_error("%s: more than 2^31 - 1 tokens or sequences, or more than 2^16 channels", what);
+  // Token numbers are 32 bits wide, with room for a strip past the last.
+  if (n > kInt32Max - (1 << 24) || sequences >= kInt32Max || width > (1 << 16)) {
+    set_error("%s: more than 2^31 - 2^24 tokens, 2^31 - 1 sequences or 2^16 channels", what);
     return R2S_ERANGE;
   }
   for (int64_t s : strides) R2S_REQUIRE(s >= width, "%s: rows overlap", what);
@@ -894,7 +974,7 @@ int check_scan(const char *what, int type, const int32_t *offsets, int64_t n, in
 
 // The limits of a plan: grid sizes, and the 32-bit lane offsets of Rows.
 int check_plan(const char *what, int type, const Plan &p, std::initializer_list<int64_t> strides) {
-  bool fits = p.blocks * p.slices <= kInt32Max && p.slices <= 65535;
+  bool fits = p.blocks * p.slices <= kInt32Max && p.c.strip < (1 << 23);
   for (int64_t s : strides)
     fits &= s * type_size(type) * p.c.strip * (64 >> p.c.lane_bits) <= 0xffffffffll;
   if (!fits) {
@@ -904,27 +984,36 @@ int check_plan(const char *what, int type, const Plan &p, std::initializer_list<
   return R2S_OK;
 }
 
+int64_t states(const Tokens &c) { return static_cast<int64_t>(c.sequences) * c.width; }
+
+// A launch for the sequences without a token, where there can be any.
 int empty_states(const Tokens &c, const float *in, float *out, hipStream_t stream) {
-  const int64_t blocks = ceil_div(static_cast<int64_t>(c.sequences) * c.width, kThreads);
-  if (blocks == 0 || (c.offsets == nullptr && c.length > 0)) return R2S_OK;
+  const int64_t blocks = ceil_div(states(c), kThreads);
+  if (out == nullptr || blocks == 0 || (c.offsets == nullptr && c.length > 0)) return R2S_OK;
   scan_empty_kernel<<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream>>>(c, in,
                                                                                          out);
   return check_launch("gated_scan empty sequences");
 }
 
 // The maps of a packed call's strips and blocks, and the states that enter
-// the blocks.
+// the blocks; empty_out [sequences][width] receives empty_in for the sequences
+// without a token.
 template <typename T, int V, bool kBack>
 int packed_maps(const Plan &p, const T *a, int64_t as, const T *b, int64_t bs, const float *state,
-                const ScanSpace &s, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(p.blocks), p.slices);
+                const float *empty_in, float *empty_out, const ScanSpace &s, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices));
   scan_maps_kernel<T, V, kBack><<<grid, dim3(kThreads), kThreads * V * 2 * sizeof(float),
-                                  stream>>>(a, as, b, bs, state, p.c, s.strips, s.blocks);
+                                  stream>>>(a, as, b, bs, state, p.c, p.slices, s.strips,
+                                            s.blocks);
   R2S_RETURN_IF(check_launch("gated_scan maps"));
-  scan_carry_kernel<<<dim3(static_cast<uint32_t>(ceil_div(p.c.width, 16))), dim3(1024), 0,
+  const int64_t channel_blocks = ceil_div(p.c.width, kCarryCols);
+  const int64_t empty_blocks =
+      p.c.offsets != nullptr && empty_out != nullptr ? ceil_div(states(p.c), 1024) : 0;
+  scan_carry_kernel<<<dim3(static_cast<uint32_t>(channel_blocks + empty_blocks)), dim3(1024), 0,
                       stream>>>(reinterpret_cast<const float2 *>(s.blocks),
-                                static_cast<int32_t>(p.blocks), p.c.width, kBack ? 1 : 0,
-                                s.carries);
+                                static_cast<int32_t>(p.blocks), p.c, kBack ? 1 : 0,
+                                static_cast<uint32_t>(channel_blocks), s.carries, empty_in,
+                                empty_out);
   return check_launch("gated_scan carries");
 }
 
@@ -947,7 +1036,7 @@ int scan_fwd(const Plan &p, const void *x, int64_t xs, const void *g, int64_t gs
   }
   const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices)), block(p.threads);
   if (p.mode == kPacked) {
-    R2S_RETURN_IF((packed_maps<T, V, false>(p, xt, xs, gt, gs, initial, s, stream)));
+    R2S_RETURN_IF((packed_maps<T, V, false>(p, xt, xs, gt, gs, initial, initial, final, s, stream)));
     scan_fwd_kernel<T, V, kPacked, kThreads><<<grid, block, 0, stream>>>(
         xt, xs, gt, gs, initial, c, p.slices, s.strips, s.carries, kept, y, final);
   } else if (p.mode == kOwn) {
@@ -971,18 +1060,19 @@ int scan_bwd(const Plan &p, const void *x, int64_t xs, const void *g, int64_t gs
   const T *vt = static_cast<const T *>(v_y);
   T *dx = static_cast<T *>(v_x), *dg = static_cast<T *>(v_gate);
   const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices)), block(p.threads);
+  const size_t priors = static_cast<size_t>(p.threads) * V * kChunk * sizeof(float);
   if (p.mode == kPacked) {
-    R2S_RETURN_IF((packed_maps<T, V, true>(p, gt, gs, vt, vs, v_final, s, stream)));
-    scan_bwd_kernel<T, V, kPacked, kThreads><<<grid, block, 0, stream>>>(
+    R2S_RETURN_IF((packed_maps<T, V, true>(p, gt, gs, vt, vs, v_final, v_final, v_initial, s, stream)));
+    scan_bwd_kernel<T, V, kPacked, kThreads><<<grid, block, priors, stream>>>(
         xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, s.strips, s.carries, kept, dx, dg,
         v_initial);
   } else if (p.mode == kOwn) {
-    scan_bwd_kernel<T, V, kOwn, kThreads><<<grid, block, 0, stream>>>(
+    scan_bwd_kernel<T, V, kOwn, kThreads><<<grid, block, priors, stream>>>(
         xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, nullptr, nullptr, kept, dx, dg,
         v_initial);
   } else {
     scan_bwd_kernel<T, V, kResidentMode, kResident>
-        <<<grid, block, p.threads * V * 2 * sizeof(float), stream>>>(
+        <<<grid, block, priors + p.threads * V * 2 * sizeof(float), stream>>>(
             xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, nullptr, nullptr, kept, dx, dg,
             v_initial);
   }
@@ -1035,8 +1125,7 @@ int r2s_gated_scan_fwd(const void *x, int64_t x_stride, const void *gate, int64_
   all.length = length;
   all.sequences = static_cast<int32_t>(sequences);
   all.width = static_cast<uint32_t>(width);
-  R2S_RETURN_IF(empty_states(all, initial, final_state, stream));
-  if (n == 0) return R2S_OK;
+  if (n == 0) return empty_states(all, initial, final_state, stream);
   const Plan p = plan_of(type, offsets, n, sequences, length, width, ragged, reverse);
   R2S_RETURN_IF(check_plan("gated_scan_fwd", type, p, {x_stride, gate_stride, width}));
   R2S_REQUIRE(x != nullptr && gate != nullptr && y != nullptr,
@@ -1051,6 +1140,7 @@ int r2s_gated_scan_fwd(const void *x, int64_t x_stride, const void *gate, int64_
   const ScanSpace s = carve_scan(cv, p);
   R2S_REQUIRE(p.V == 1 || pairs_fit({x, gate, y}, {x_stride, gate_stride}),
               "gated_scan_fwd: rows of 16-bit elements must start at multiples of 4 bytes");
+  if (p.mode != kPacked) R2S_RETURN_IF(empty_states(p.c, initial, final_state, stream));
   R2S_BY_TYPE(type, {
     if constexpr (sizeof(T) == 2) {
       if (p.V == 2)
@@ -1081,8 +1171,7 @@ int r2s_gated_scan_bwd(const void *x, int64_t x_stride, const void *gate, int64_
   all.length = length;
   all.sequences = static_cast<int32_t>(sequences);
   all.width = static_cast<uint32_t>(width);
-  if (v_initial != nullptr) R2S_RETURN_IF(empty_states(all, v_final, v_initial, stream));
-  if (n == 0) return R2S_OK;
+  if (n == 0) return empty_states(all, v_final, v_initial, stream);
   const Plan p = plan_of(type, offsets, n, sequences, length, width, ragged, reverse);
   R2S_RETURN_IF(check_plan("gated_scan_bwd", type, p,
                            {x_stride, gate_stride, v_y_stride, width}));
@@ -1100,6 +1189,7 @@ int r2s_gated_scan_bwd(const void *x, int64_t x_stride, const void *gate, int64_
   R2S_REQUIRE(p.V == 1 || pairs_fit({x, gate, v_y, v_x, v_gate},
                                     {x_stride, gate_stride, v_y_stride}),
               "gated_scan_bwd: rows of 16-bit elements must start at multiples of 4 bytes");
+  if (p.mode != kPacked) R2S_RETURN_IF(empty_states(p.c, v_final, v_initial, stream));
   R2S_BY_TYPE(type, {
     if constexpr (sizeof(T) == 2) {
       if (p.V == 2)
