@@ -34,6 +34,7 @@ SOURCES = [
     "densify.hip",
     "loss.hip",
     "adam.hip",
+    "group.hip",
     "lookup.hip",
     "gated_scan.hip",
     "grouped.hip",

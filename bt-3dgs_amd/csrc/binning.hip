@@ -28,7 +28,6 @@
 #include <utility>
 
 #include "r2s_common.h"
-#include "r2s_latent.h"
 #include "r2s_scan.h"
 
 namespace r2s {
@@ -933,25 +932,6 @@ int radix_sort(SortSpace &s, const int64_t *n_dev, int64_t cap, uint32_t key_bit
   return R2S_OK;
 }
 
-// ------------------------------------------------------------ plain ids ---
-
-// The sort's input from a caller's ids: key = id, or n_groups for an id
-// outside [0, n_groups); gid = position.  Also the count the sort kernels
-// read from the device.
-template <typename I>
-__global__ __launch_bounds__(256) void id_keys_kernel(const I *__restrict__ ids, int64_t n,
-                                                      int64_t n_groups,
-                                                      uint32_t *__restrict__ keys,
-                                                      uint32_t *__restrict__ gid,
-                                                      int64_t *__restrict__ n_dev) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i == 0) *n_dev = n;
-  if (i >= n) return;
-  const int64_t id = static_cast<int64_t>(ids[i]);
-  keys[i] = static_cast<uint32_t>(id >= 0 && id < n_groups ? id : n_groups);
-  gid[i] = static_cast<uint32_t>(i);
-}
-
 // ---------------------------------------------------------------- host ---
 
 int check_workspace(void *ws, size_t have, int64_t need, const char *name) {
@@ -1130,64 +1110,10 @@ int layer_counts_3d_impl(const T *means3d, const int32_t *radii, int64_t N, uint
   return check_launch(name);
 }
 
-// The workspace of sort_ids: the record count, then the sort's own.
-int64_t *carve_ids(Carver &cv, int64_t n, int64_t n_groups, SortSpace &s) {
-  int64_t *n_dev = cv.take<int64_t>(1);
-  s = carve_sort(cv, n, key_bits_for(n_groups + 1));
-  return n_dev;
-}
-
 }  // namespace
-
-int64_t sort_ids_bytes(int64_t n, int64_t n_groups) {
-  Carver cv(nullptr);
-  SortSpace s;
-  carve_ids(cv, n, n_groups, s);
-  return static_cast<int64_t>(cv.used);
-}
-
-int sort_ids(const void *ids, bool wide, int64_t n, int64_t n_groups, int32_t *order,
-             int32_t *offsets, void *workspace, hipStream_t stream) {
-  if (n == 0) return device_fill<int32_t>(offsets, n_groups + 1, 0, stream, "group_rows");
-  Carver cv(workspace);
-  SortSpace s;
-  int64_t *n_dev = carve_ids(cv, n, n_groups, s);
-  s.gid0 = s.g0;
-  const dim3 grid(static_cast<uint32_t>(ceil_div(n, 256)));
-  if (wide)
-    id_keys_kernel<int64_t><<<grid, dim3(256), 0, stream>>>(static_cast<const int64_t *>(ids), n,
-                                                            n_groups, s.k0, s.g0, n_dev);
-  else
-    id_keys_kernel<int32_t><<<grid, dim3(256), 0, stream>>>(static_cast<const int32_t *>(ids), n,
-                                                            n_groups, s.k0, s.g0, n_dev);
-  R2S_RETURN_IF(check_launch("group_rows"));
-  return radix_sort(s, n_dev, n, key_bits_for(n_groups + 1), nullptr, order, false, nullptr,
-                    offsets, n_groups + 1, stream);
-}
-
 }  // namespace r2s
 
 extern "C" {
-
-int64_t r2s_group_rows_workspace_bytes(int64_t n, int64_t n_groups) {
-  return n > 0 && n_groups >= 0 ? r2s::sort_ids_bytes(n, n_groups) : 0;
-}
-
-int r2s_group_rows(const void *ids, int32_t ids_are_64, int64_t n, int64_t n_groups,
-                   int32_t *rows, int32_t *offsets, void *ws, size_t ws_bytes, r2s_stream_t st) {
-  r2s::clear_error();
-  R2S_REQUIRE(n >= 0 && n_groups >= 0, "group_rows: negative size");
-  if (n > r2s::kInt32Max || n_groups >= r2s::kInt32Max) {
-    r2s::set_error("group_rows: more than 2^31 - 1 rows or groups");
-    return R2S_ERANGE;
-  }
-  R2S_REQUIRE(offsets != nullptr && (n == 0 || (ids != nullptr && rows != nullptr)),
-              "group_rows: null ids, rows or offsets");
-  R2S_RETURN_IF(r2s::check_workspace(ws, ws_bytes, r2s_group_rows_workspace_bytes(n, n_groups),
-                                     "group_rows"));
-  return r2s::sort_ids(ids, ids_are_64 != 0, n, n_groups, rows, offsets, ws,
-                       r2s::as_stream(st));
-}
 
 int64_t r2s_isect_workspace_bytes(int64_t n_items, int64_t n_isects, uint32_t end_bit) {
   const int64_t a = n_items > 0 ? r2s::count_space_bytes(n_items) : 0;

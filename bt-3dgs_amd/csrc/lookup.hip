@@ -4,7 +4,7 @@
 //             addresses and strides allow).  Ids outside the table give zero
 //             rows, so no id reads out of range.
 //   backward  dT_v = s sum_{id_i = v} dy_i, without atomics: the positions are
-//             sorted by id (stable, binning.hip), the sorted list is cut into
+//             sorted by id (stable, group.hip), the sorted list is cut into
 //             chunks of equal length whatever the ids are, and each chunk sums
 //             its runs of equal ids in float32.  A run inside one chunk is a
 //             finished row; a run that crosses chunk ends leaves one partial
@@ -12,6 +12,8 @@
 //             writes the rows that no id names as zeros.  Chunks keep the work
 //             even when a few ids own almost every position, and fix the order
 //             of the sums.
+#include <algorithm>
+
 #include "r2s_latent.h"
 
 namespace r2s {
@@ -21,32 +23,37 @@ constexpr int kThreads = 256;
 
 // ------------------------------------------------------------- forward ---
 
-constexpr int kFwdVectors = 4;  // vectors per thread
+// Vectors per thread: as many bytes of the narrow ones.
+constexpr int fwd_vectors(int bytes) { return bytes <= 4 ? 8 : 4; }
 
-// Block b writes vectors [b, b + 1) * kThreads * kFwdVectors of the output,
-// row-major.  vpr: vectors per row.
+// A block takes `rows` whole rows (of at most kThreads fwd_vectors vectors
+// together), or in a longer row one run of that many.  vpr: vectors per row;
+// magic: 2^32 / vpr rounded up, the quotient of every vector number of a block
+// (below 2^13, so exact) by one multiplication.  Bound by the writes: 64 MB of
+// 500k x 64 bf16 rows in 16 us, 3.9 TB/s.
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
     const T *__restrict__ table, int64_t stride, const I *__restrict__ ids, float scale,
-    int64_t n, int64_t n_rows, uint32_t vpr, T *__restrict__ out) {
-  const int64_t total = n * vpr;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads * kFwdVectors);
-  // Row and vector of the block's first one; the rest from there in 32 bits.
-  const int64_t row0 = base / vpr;
-  const uint32_t vec0 = static_cast<uint32_t>(base - row0 * vpr);
-  int64_t id[kFwdVectors];
-  uint32_t vec[kFwdVectors];
+    int64_t n, int64_t n_rows, uint32_t vpr, uint32_t rows, uint32_t magic,
+    T *__restrict__ out) {
+  constexpr int kVectors = fwd_vectors(V * sizeof(T));
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows;
+  const uint32_t vec0 = blockIdx.y * (kThreads * kVectors);
+  const uint32_t count = static_cast<uint32_t>(min(static_cast<int64_t>(rows), n - row0));
+  int64_t id[kVectors], at[kVectors];
+  uint32_t vec[kVectors];
 #pragma unroll
-  for (int k = 0; k < kFwdVectors; ++k) {
-    const uint32_t q = vec0 + k * kThreads + threadIdx.x;
-    const uint32_t r = q / vpr;
-    vec[k] = q - r * vpr;
-    const int64_t row = row0 + r;
-    id[k] = row < n ? static_cast<int64_t>(ids[row]) : -1;
+  for (int k = 0; k < kVectors; ++k) {
+    const uint32_t q = k * kThreads + threadIdx.x;
+    const uint32_t r = rows > 1 ? __umulhi(q, magic) : 0u;
+    vec[k] = vec0 + q - r * vpr;
+    const bool inside = r < count && vec[k] < vpr;
+    at[k] = inside ? (row0 + r) * vpr + vec[k] : -1;
+    id[k] = inside ? static_cast<int64_t>(ids[row0 + r]) : -1;
   }
-  Pack<T, V> x[kFwdVectors];
+  Pack<T, V> x[kVectors];
 #pragma unroll
-  for (int k = 0; k < kFwdVectors; ++k) {
+  for (int k = 0; k < kVectors; ++k) {
     if (id[k] >= 0 && id[k] < n_rows) {
       x[k] = load_pack<T, V>(table + id[k] * stride + static_cast<int64_t>(vec[k]) * V);
     } else {
@@ -55,53 +62,59 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
     }
   }
 #pragma unroll
-  for (int k = 0; k < kFwdVectors; ++k) {
-    const int64_t at = base + k * kThreads + threadIdx.x;
-    if (at < total) {
+  for (int k = 0; k < kVectors; ++k) {
+    if (at[k] >= 0) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         x[k].v[j] = static_cast<T>(static_cast<float>(x[k].v[j]) * scale);
-      store_pack<T, V>(out + at * V, x[k]);
+      store_pack<T, V>(out + at[k] * V, x[k]);
     }
   }
 }
 
 // ------------------------------------------------------------ backward ---
 
-constexpr int kChunk = 32;     // sorted positions per chunk
-constexpr int kInFlight = 8;   // rows loaded before their first use
-constexpr int kLongRow = 64;   // chunks: longer rows are added by a whole block
+// Threads of the second kernel's blocks: a long row of narrow vectors needs the
+// more lane groups (45 f32 columns: 15.4 us with 1024 threads, 19.8 with 512),
+// wide vectors the less LDS (64 bf16 columns: 7.1 us with 512, 13.9 with 1024).
+constexpr int row_threads(int V) { return V <= 2 ? 1024 : 512; }
+constexpr int kLongRow = 32;       // chunks: longer rows are added by a whole block
+constexpr int64_t kSpread = 1 << 18;  // lanes that the chunks are spread over
 
-// The backward's view of the sorted list.
+// The sorted ids (n_rows for those outside the table), their positions and each
+// row's first entry.
 struct Sorted {
-  const int32_t *order;    // position of each sorted entry
-  const int32_t *offsets;  // [n_rows + 1]; offsets[n_rows]: entries in all
+  const uint32_t *keys;
+  const int32_t *order, *offsets;
+  uint32_t n;
+  uint32_t chunk;  // entries per chunk
 };
 
-// lanes = 2^lane_bits lanes hold one row's columns [c0, c0 + lanes V) and walk
-// one chunk; partial [chunks][2][width]: slot 0 the chunk's part of a run that
-// began in an earlier chunk, slot 1 its part of one that goes on into the
-// next (a run that does both is in slot 0).
-template <typename T, int V, typename I>
+// 2^lane_bits lanes hold one row's columns [c0, c0 + lanes V) and walk one
+// chunk; partial [chunks][2][width]: slot 0 the chunk's part of a run that began
+// in an earlier chunk, slot 1 its part of one that goes on into the next (a run
+// that does both is in slot 0).
+template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void lookup_bwd_chunks_kernel(
-    const T *__restrict__ v_out, int64_t stride, const I *__restrict__ ids, Sorted list,
-    float scale, int64_t n_rows, uint32_t width, uint32_t lane_bits, T *__restrict__ v_table,
-    float *__restrict__ partial) {
+    const T *__restrict__ v_out, int64_t stride, Sorted list, float scale, uint32_t n_rows,
+    uint32_t width, uint32_t lane_bits, T *__restrict__ v_table, float *__restrict__ partial) {
   const uint32_t col = (blockIdx.y << lane_bits) * V + (threadIdx.x & ((1u << lane_bits) - 1u)) * V;
-  const int64_t chunk = (static_cast<int64_t>(blockIdx.x) << (8 - lane_bits)) +
-                        (threadIdx.x >> lane_bits);
-  const int64_t j0 = chunk * kChunk;
-  const int64_t n = list.offsets[n_rows];
-  if (j0 >= n || col >= width) return;
-  const int64_t j1 = min(j0 + kChunk, n);
-  const int64_t before = j0 > 0 ? static_cast<int64_t>(ids[list.order[j0 - 1]]) : -1;
-  const int64_t after = j1 < n ? static_cast<int64_t>(ids[list.order[j1]]) : -1;
+  const uint64_t chunk = (static_cast<uint64_t>(blockIdx.x) << (8 - lane_bits)) +
+                         (threadIdx.x >> lane_bits);
+  const uint64_t begin = chunk * list.chunk;
+  if (begin >= list.n || col >= width) return;
+  const uint32_t j0 = static_cast<uint32_t>(begin);
+  const uint32_t j1 = static_cast<uint32_t>(min(begin + list.chunk, uint64_t{list.n}));
+  // No id is n_rows + 1: nothing runs past the list's ends.
+  const uint32_t before = j0 > 0 ? list.keys[j0 - 1] : n_rows + 1;
+  const uint32_t after = j1 < list.n ? list.keys[j1] : n_rows + 1;
   float acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-  int64_t run = static_cast<int64_t>(ids[list.order[j0]]);
+  uint32_t run = list.keys[j0];
   bool first = true;  // the run that began at j0
   auto flush = [&](bool last) {
+    if (run == n_rows) return;
     if ((first && run == before) || (last && run == after)) {
       const int slot = first && run == before ? 0 : 1;
       float *p = partial + (chunk * 2 + slot) * width + col;
@@ -111,17 +124,19 @@ __global__ __launch_bounds__(kThreads) void lookup_bwd_chunks_kernel(
       Pack<T, V> r;
 #pragma unroll
       for (int v = 0; v < V; ++v) r.v[v] = static_cast<T>(acc[v] * scale);
-      store_pack<T, V>(v_table + run * width + col, r);
+      store_pack<T, V>(v_table + static_cast<int64_t>(run) * width + col, r);
     }
   };
-  for (int64_t j = j0; j < j1; j += kInFlight) {
-    int64_t id[kInFlight];
+  // Rows loaded before their first use: as many bytes of the narrow vectors.
+  constexpr int kInFlight = sizeof(T) * V <= 4 ? 16 : 8;
+  for (uint32_t j = j0; j < j1; j += kInFlight) {
+    uint32_t id[kInFlight];
     Pack<T, V> x[kInFlight];
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
-      const int64_t at = list.order[min(j + k, j1 - 1)];
-      id[k] = static_cast<int64_t>(ids[at]);
-      x[k] = load_pack<T, V>(v_out + at * stride + col);
+      const uint32_t i = min(j + k, j1 - 1);
+      id[k] = list.keys[i];
+      x[k] = load_pack<T, V>(v_out + static_cast<int64_t>(list.order[i]) * stride + col);
     }
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
@@ -141,48 +156,68 @@ __global__ __launch_bounds__(kThreads) void lookup_bwd_chunks_kernel(
   flush(true);
 }
 
+// acc += the parts of chunks c, c + step, ... up to `last` of a row whose first
+// chunk is `first`.
+template <int V>
+__device__ __forceinline__ void add_parts(const float *__restrict__ partial, uint32_t width,
+                                          uint32_t col, uint32_t first, uint32_t c, uint32_t last,
+                                          uint32_t step, float (&acc)[V]) {
+  constexpr int kParts = V <= 2 ? 16 : 8;  // loaded before their first use
+  for (; c <= last; c += step * kParts) {
+    float p[kParts][V];
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+      const uint32_t i = min(c + k * step, last);
+      const float *q = partial + (uint64_t{i} * 2 + (i == first ? 1 : 0)) * width + col;
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[k][v] = q[v];
+    }
+#pragma unroll
+    for (int k = 0; k < kParts; ++k)
+      if (c + k * step <= last) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] += p[k][v];
+      }
+  }
+}
+
 // Blocks from n_long on: one row per lane group -- zeros without an entry,
 // the sum of its parts if it crosses a chunk end, nothing to do otherwise.
 // Blocks before: block b looks at the row that holds the first entry of chunk
 // (b + 1) kLongRow and adds its parts if it spans more than kLongRow chunks
 // and no smaller b sees it.
-template <typename T, int V, typename I>
-__global__ __launch_bounds__(kThreads) void lookup_bwd_rows_kernel(
-    const I *__restrict__ ids, Sorted list, float scale, int64_t n_rows, uint32_t width,
-    uint32_t lane_bits, uint32_t n_long, const float *__restrict__ partial,
-    T *__restrict__ v_table) {
+template <typename T, int V>
+__global__ __launch_bounds__(row_threads(V)) void lookup_bwd_rows_kernel(
+    Sorted list, float scale, uint32_t n_rows, uint32_t width, uint32_t lane_bits,
+    uint32_t n_long, const float *__restrict__ partial, T *__restrict__ v_table) {
   const uint32_t lane = threadIdx.x & ((1u << lane_bits) - 1u), group = threadIdx.x >> lane_bits;
-  const uint32_t groups = kThreads >> lane_bits;
+  constexpr int kRowThreads = row_threads(V);
+  const uint32_t groups = kRowThreads >> lane_bits;
   const uint32_t col = (blockIdx.y << lane_bits) * V + lane * V;
   const bool inside = col < width;
-  __shared__ float sums[kThreads * V];
-  int64_t row;
-  bool whole = blockIdx.x < n_long;
+  __shared__ float sums[kRowThreads * V];
+  const bool whole = blockIdx.x < n_long;
+  uint32_t row;
   if (whole) {
-    const int64_t j = (static_cast<int64_t>(blockIdx.x) + 1) * kLongRow * kChunk;
-    if (j >= list.offsets[n_rows]) return;
-    row = static_cast<int64_t>(ids[list.order[j]]);
+    const uint64_t j = (uint64_t{blockIdx.x} + 1) * kLongRow * list.chunk;
+    row = list.keys[j];  // j < n: see n_long
+    if (row == n_rows) return;
   } else {
-    row = (static_cast<int64_t>(blockIdx.x) - n_long) * groups + group;
+    row = (blockIdx.x - n_long) * groups + group;
     if (row >= n_rows) return;
   }
-  const int64_t o0 = list.offsets[row], o1 = list.offsets[row + 1];
-  const int64_t c0 = o0 / kChunk, c1 = o1 > o0 ? (o1 - 1) / kChunk : c0;
+  const uint32_t o0 = static_cast<uint32_t>(list.offsets[row]);
+  const uint32_t o1 = static_cast<uint32_t>(list.offsets[row + 1]);
+  const uint32_t c0 = o0 / list.chunk, c1 = o1 > o0 ? (o1 - 1) / list.chunk : c0;
   const bool is_long = c1 - c0 > kLongRow;
   float acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
   if (whole) {
-    // Uniform over the block: every thread of a block reads the same row.
-    const int64_t smaller = static_cast<int64_t>(blockIdx.x) * kLongRow * kChunk;
+    // Uniform over the block: every thread of a block has the same row.
+    const uint64_t smaller = uint64_t{blockIdx.x} * kLongRow * list.chunk;
     if (!is_long || (blockIdx.x > 0 && o0 <= smaller)) return;
-    for (int64_t c = c0 + group; c <= c1; c += groups) {
-      if (inside) {
-        const float *p = partial + (c * 2 + (c == c0 ? 1 : 0)) * width + col;
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += p[v];
-      }
-    }
+    if (inside) add_parts<V>(partial, width, col, c0, c0 + group, c1, groups, acc);
 #pragma unroll
     for (int v = 0; v < V; ++v) sums[threadIdx.x * V + v] = acc[v];
     __syncthreads();
@@ -193,25 +228,32 @@ __global__ __launch_bounds__(kThreads) void lookup_bwd_rows_kernel(
     }
   } else {
     if (o1 > o0 && (c0 == c1 || is_long)) return;
-    if (inside && o1 > o0) {
-      for (int64_t c = c0; c <= c1; ++c) {
-        const float *p = partial + (c * 2 + (c == c0 ? 1 : 0)) * width + col;
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += p[v];
-      }
-    }
+    if (inside && o1 > o0) add_parts<V>(partial, width, col, c0, c0, c1, 1, acc);
   }
   if (!inside) return;
   Pack<T, V> r;
 #pragma unroll
   for (int v = 0; v < V; ++v) r.v[v] = static_cast<T>(acc[v] * scale);
-  store_pack<T, V>(v_table + row * width + col, r);
+  store_pack<T, V>(v_table + static_cast<int64_t>(row) * width + col, r);
 }
 
 // ---------------------------------------------------------------- host ---
 
+// Entries per chunk, for rows of `lanes` lanes: as many chunks as keep the
+// device busy and no more, since a row of many entries has a part per chunk to
+// add afterwards.  With the fewest lanes that a width can have (16-byte
+// vectors), the most chunks, which the workspace has to hold.
+uint32_t chunk_entries(int64_t n, int64_t lanes) {
+  const int64_t even = ceil_div(n * lanes, kSpread);
+  return static_cast<uint32_t>(std::min<int64_t>(std::max<int64_t>(align_up(even, 8), 16), 1024));
+}
+int64_t most_chunks(int64_t n, int64_t width) {
+  return ceil_div(n, chunk_entries(n, std::max<int64_t>(width / 8, 1)));
+}
+
 struct BwdSpace {
   int32_t *order, *offsets;
+  uint32_t *keys;
   float *partial;
   char *sort;
 };
@@ -220,7 +262,8 @@ BwdSpace carve_bwd(Carver &cv, int64_t n, int64_t n_rows, int64_t width) {
   BwdSpace s;
   s.order = cv.take<int32_t>(n);
   s.offsets = cv.take<int32_t>(n_rows + 1);
-  s.partial = cv.take<float>(ceil_div(n, kChunk) * 2 * width);
+  s.keys = cv.take<uint32_t>(n);
+  s.partial = cv.take<float>(most_chunks(n, width) * 2 * width);
   s.sort = cv.take<char>(sort_ids_bytes(n, n_rows));
   return s;
 }
@@ -242,42 +285,54 @@ int check_lookup(const char *what, int64_t n, int64_t n_rows, int64_t width, int
 template <typename T, int V, typename I>
 int lookup_fwd(const void *table, int64_t stride, const void *ids, float scale, int64_t n,
                int64_t n_rows, int64_t width, void *out, hipStream_t stream) {
-  const uint32_t vpr = static_cast<uint32_t>(width / V);
-  const int64_t blocks = ceil_div(n * vpr, kThreads * kFwdVectors);
-  if (blocks > kInt32Max) {
+  constexpr int64_t per_block = kThreads * fwd_vectors(V * static_cast<int>(sizeof(T)));
+  static_assert(per_block <= 4096, "vector numbers of a block below 2^13");
+  const int64_t vpr = width / V;
+  const int64_t rows = std::max<int64_t>(per_block / vpr, 1), slices = ceil_div(vpr, per_block);
+  if (ceil_div(n, rows) > kInt32Max || slices > 65535) {
     set_error("embedding_fwd: output too large");
     return R2S_ERANGE;
   }
-  lookup_fwd_kernel<T, V, I><<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream>>>(
-      static_cast<const T *>(table), stride, static_cast<const I *>(ids), scale, n, n_rows, vpr,
-      static_cast<T *>(out));
+  const uint32_t magic =
+      rows > 1 ? static_cast<uint32_t>(std::min<uint64_t>(((uint64_t{1} << 32) + vpr - 1) / vpr,
+                                                          0xffffffffull))
+               : 0u;
+  lookup_fwd_kernel<T, V, I>
+      <<<dim3(static_cast<uint32_t>(ceil_div(n, rows)), static_cast<uint32_t>(slices)),
+         dim3(kThreads), 0, stream>>>(static_cast<const T *>(table), stride,
+                                      static_cast<const I *>(ids), scale, n, n_rows,
+                                      static_cast<uint32_t>(vpr), static_cast<uint32_t>(rows),
+                                      magic, static_cast<T *>(out));
   return check_launch("embedding_fwd");
 }
 
-template <typename T, int V, typename I>
-int lookup_bwd(const void *v_out, int64_t stride, const void *ids_, float scale, int64_t n,
-               int64_t n_rows, int64_t width_, void *v_table_, const BwdSpace &s,
-               hipStream_t stream) {
-  const I *ids = static_cast<const I *>(ids_);
+template <typename T, int V>
+int lookup_bwd(const void *v_out, int64_t stride, float scale, int64_t n, int64_t n_rows,
+               int64_t width_, void *v_table_, const BwdSpace &s, hipStream_t stream) {
   T *v_table = static_cast<T *>(v_table_);
   const uint32_t width = static_cast<uint32_t>(width_), vpr = width / V;
   uint32_t bits = 0;
   while (bits < 6 && (1u << bits) < vpr) ++bits;
   const uint32_t slices = static_cast<uint32_t>(ceil_div(vpr, 1 << bits));
-  const int64_t groups = kThreads >> bits, chunks = ceil_div(n, kChunk);
-  const Sorted list{s.order, s.offsets};
+  const Sorted list{s.keys, s.order, s.offsets, static_cast<uint32_t>(n),
+                    chunk_entries(n, int64_t{slices} << bits)};
+  const int64_t chunks = ceil_div(n, list.chunk);
   if (n > 0) {
-    lookup_bwd_chunks_kernel<T, V, I>
-        <<<dim3(static_cast<uint32_t>(ceil_div(chunks, groups)), slices), dim3(kThreads), 0,
-           stream>>>(static_cast<const T *>(v_out), stride, ids, list, scale, n_rows, width, bits,
-                     v_table, s.partial);
+    lookup_bwd_chunks_kernel<T, V>
+        <<<dim3(static_cast<uint32_t>(ceil_div(chunks, kThreads >> bits)), slices),
+           dim3(kThreads), 0, stream>>>(static_cast<const T *>(v_out), stride, list, scale,
+                                        static_cast<uint32_t>(n_rows), width, bits, v_table,
+                                        s.partial);
     R2S_RETURN_IF(check_launch("embedding_bwd"));
   }
+  // Block b < n_long reads entry (b + 1) kLongRow chunk, the first of a chunk
+  // that there is.
   const int64_t n_long = chunks > 0 ? (chunks - 1) / kLongRow : 0;
-  lookup_bwd_rows_kernel<T, V, I>
-      <<<dim3(static_cast<uint32_t>(n_long + ceil_div(n_rows, groups)), slices), dim3(kThreads),
-         0, stream>>>(ids, list, scale, n_rows, width, bits, static_cast<uint32_t>(n_long),
-                      s.partial, v_table);
+  lookup_bwd_rows_kernel<T, V>
+      <<<dim3(static_cast<uint32_t>(n_long + ceil_div(n_rows, row_threads(V) >> bits)),
+              slices),
+         dim3(row_threads(V)), 0, stream>>>(list, scale, static_cast<uint32_t>(n_rows), width, bits,
+                                         static_cast<uint32_t>(n_long), s.partial, v_table);
   return check_launch("embedding_bwd rows");
 }
 
@@ -350,16 +405,14 @@ int r2s_embedding_bwd(const void *v_out, int64_t v_out_stride, const void *ids,
   Carver cv(ws);
   const BwdSpace s = carve_bwd(cv, n, n_rows, width);
   hipStream_t stream = as_stream(st);
-  R2S_RETURN_IF(sort_ids(ids, ids_are_64 != 0, n, n_rows, s.order, s.offsets, s.sort, stream));
+  R2S_RETURN_IF(
+      sort_ids(ids, ids_are_64 != 0, n, n_rows, s.order, s.offsets, s.keys, s.sort, stream));
   const uint64_t size = type_size(type);
   const int bytes = vector_bytes({address(v_out), address(v_table), v_out_stride * size,
                                   width * size},
                                  static_cast<int>(size));
   R2S_BY_TYPE(type, R2S_BY_VECTOR(T, bytes, {
-    return ids_are_64 ? (lookup_bwd<T, V, int64_t>(v_out, v_out_stride, ids, scale, n, n_rows,
-                                                   width, v_table, s, stream))
-                      : (lookup_bwd<T, V, int32_t>(v_out, v_out_stride, ids, scale, n, n_rows,
-                                                   width, v_table, s, stream));
+    return (lookup_bwd<T, V>(v_out, v_out_stride, scale, n, n_rows, width, v_table, s, stream));
   }));
   return R2S_OK;
 }

@@ -45,13 +45,14 @@ inline int vector_bytes(std::initializer_list<uint64_t> all, int least) {
 }
 inline uint64_t address(const void *p) { return reinterpret_cast<uint64_t>(p); }
 
-// Stable grouping of n ids by value (binning.hip): order [n] receives the
-// positions sorted by (id, position), ids outside [0, n_groups) last;
-// offsets [n_groups + 1] each group's first index in it, offsets[n_groups]
-// the number of ids inside.
+// Stable grouping of n ids by value (group.hip): order [n] receives the
+// positions sorted by (id, position), ids outside [0, n_groups) last; keys [n]
+// (may be null) the sorted ids, n_groups for those outside; offsets
+// [n_groups + 1] (may be null) each group's first index in order,
+// offsets[n_groups] the number of ids inside.
 int64_t sort_ids_bytes(int64_t n, int64_t n_groups);
 int sort_ids(const void *ids, bool wide, int64_t n, int64_t n_groups, int32_t *order,
-             int32_t *offsets, void *workspace, hipStream_t stream);
+             int32_t *offsets, uint32_t *keys, void *workspace, hipStream_t stream);
 
 // The expression `call` with T bound to the element type.
 #define R2S_BY_TYPE(type, ...)                   \
