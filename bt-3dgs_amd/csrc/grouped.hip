@@ -10,39 +10,56 @@
 // last tile return.  Rows are read and written through `rows` where the
 // groups' rows do not lie together, so no permuted copy is made.
 //
-// Every product is a 64 x 64 tile per block of four waves on the matrix cores,
-// operands staged in LDS with the summed index innermost; sums are float32.
-// dW sums over rows: its blocks take a fixed number of rows of one group each
-// and leave float32 parts, which a second kernel adds in row order.
+// A block of four waves makes a tile of 128 output rows by 64 or 128 columns on
+// the matrix cores, each wave half of both, from operands staged in LDS 128
+// bytes of the summed index at a time, the next stage's loads in flight while
+// one is multiplied.  An operand whose summed index is innermost in memory
+// ("along": rows of x, of W forward) is staged as it lies; one whose tile
+// index is innermost ("across": W backward, both operands of dW) is staged as
+// it lies too and transposed by the LDS reads.  The columns are the matrix
+// cores' rows, so that a lane ends with four neighbouring columns of one output
+// row.  Sums are float32.
+//
+// dW sums over rows: its blocks take a fixed number of rows of one group each.
+// A group of one such part is stored at once; the others leave float32 parts,
+// which a second kernel adds in row order.
+#include <algorithm>
+
 #include "r2s_latent.h"
 
 namespace r2s {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 64;        // rows and columns of a block's tile
+constexpr int kRows = 128;      // output rows of a block's tile
 constexpr int kSlabBytes = 128;  // of the summed index per stage
-constexpr int kPitch = kSlabBytes + 16;
+constexpr int kSlots = kSlabBytes / 16;
+constexpr int kHalves = kSlabBytes / 64;  // what one matrix instruction, or four, sum over
+constexpr int kWindow = 512;     // row numbers of a weights' gradient block in LDS, twice
+constexpr int kStages = 2;       // in LDS: one is multiplied, the other is on its way
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using i16x4 = __attribute__((ext_vector_type(4))) short;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using Lds = __attribute__((address_space(3))) char *;
 
 // acc += A B over the 16 bytes per lane of the summed index (which elements
 // they are does not matter, as long as both operands hold the same).
 template <typename T>
-__device__ __forceinline__ void multiply(const void *a, const void *b, f32x4 &acc) {
+__device__ __forceinline__ void multiply(u32x4 a, u32x4 b, f32x4 &acc) {
   if constexpr (sizeof(T) == 4) {
-    const f32x4 x = *static_cast<const f32x4 *>(a), y = *static_cast<const f32x4 *>(b);
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], acc, 0, 0, 0);
   } else if constexpr (std::is_same<T, bf16_t>::value) {
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*static_cast<const bf16x8 *>(a),
-                                                  *static_cast<const bf16x8 *>(b), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                  __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
   } else {
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(*static_cast<const f16x8 *>(a),
-                                                 *static_cast<const f16x8 *>(b), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                 __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
   }
 }
 
@@ -56,11 +73,12 @@ struct Groups {
   }
 };
 
-// Part `slot` of the groups cut into parts of `per` rows each: its group and
-// rows [r0, r1).  With `rest` the rows past the last group follow as group
-// `count`.  False past the last part.  Called by whole waves.
+// Part `slot` of the groups cut into parts of `per` rows each: its group, rows
+// [r0, r1), and whether it is the group's only part.  With `rest` the rows past
+// the last group follow as group `count`.  False past the last part.  Called by
+// whole waves.
 __device__ __forceinline__ bool find_part(const Groups &g, bool rest, uint32_t per, uint32_t slot,
-                                          int32_t &group, int64_t &r0, int64_t &r1) {
+                                          int32_t &group, int64_t &r0, int64_t &r1, bool &only) {
   uint32_t before = 0;
   const int32_t total = g.count + (rest ? 1 : 0);
   for (int32_t e0 = 0; e0 < total; e0 += 64) {
@@ -76,9 +94,10 @@ __device__ __forceinline__ bool find_part(const Groups &g, bool rest, uint32_t p
     if (past != 0) {
       const uint32_t src = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(past))) - 1u;
       group = static_cast<int32_t>(readlane_u32(static_cast<uint32_t>(e), src));
-      const uint32_t first = readlane_u32(end - parts, src);
+      const uint32_t count = readlane_u32(parts, src), first = readlane_u32(end, src) - count;
       r0 = readlane_i64(lo, src) + static_cast<int64_t>(slot - first) * per;
       r1 = min(readlane_i64(hi, src), r0 + per);
+      only = count == 1;
       return true;
     }
     before = readlane_u32(end, 63);
@@ -88,194 +107,504 @@ __device__ __forceinline__ bool find_part(const Groups &g, bool rest, uint32_t p
 
 // ------------------------------------------------------------- staging ---
 
-// Stages [kTile][slab] of an operand whose summed index is innermost in
-// memory: element (r, c) at base + row(r) * stride + c0 + c; rows < 0 and
-// c0 + c >= c_end are zero.
-template <typename T, bool kVec, typename Row>
-__device__ __forceinline__ void stage_along(char *lds, const T *base, int64_t stride, Row row,
-                                            int64_t c0, int64_t c_end) {
-  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-  constexpr int kChunks = kTile * kSlabBytes / 16 / kThreads;
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int q = threadIdx.x + i * kThreads, r = q / (kSlabBytes / 16), s = q % (kSlabBytes / 16);
-    const int64_t at = row(r), c = c0 + s * kPer;
-    Pack<T, kPer> x;
-    if (kVec && at >= 0 && c + kPer <= c_end) {
-      x = load_pack<T, kPer>(base + at * stride + c);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        x.v[j] = at >= 0 && c + j < c_end ? base[at * stride + c + j] : static_cast<T>(0.0f);
-    }
-    *reinterpret_cast<Pack<T, kPer> *>(lds + r * kPitch + s * 16) = x;
-  }
+// Waits until all but the wave's last `kLeft` loads have arrived, then for the
+// block's other waves: the stage before those is in LDS, and the one that was
+// multiplied last is free.
+template <int kLeft>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
-// The same of an operand whose tile rows are innermost in memory: element
-// (r, c) at base + row(c) * stride + r0 + r; r0 + r >= r_end is zero.
-template <typename T, bool kVec, typename Row>
-__device__ __forceinline__ void stage_across(char *lds, const T *base, int64_t stride, Row row,
-                                             int64_t r0, int64_t r_end) {
-  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-  constexpr int kChunks = kTile * kSlabBytes / 16 / kThreads;
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int q = threadIdx.x + i * kThreads, c = q / (kTile / kPer), s = q % (kTile / kPer);
-    const int64_t at = row(c), r = r0 + s * kPer;
-    Pack<T, kPer> x;
-    if (kVec && at >= 0 && r + kPer <= r_end) {
-      x = load_pack<T, kPer>(base + at * stride + r);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        x.v[j] = at >= 0 && r + j < r_end ? base[at * stride + r + j] : static_cast<T>(0.0f);
-    }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      *reinterpret_cast<T *>(lds + (s * kPer + j) * kPitch + c * sizeof(T)) = x.v[j];
-  }
+// An operand's stage is R x 128 bytes of LDS in 16-byte slots:
+//   along   [R rows][kSlots], slot s of row r at s ^ swizzle(r);
+//   across  [kSlab summed][R sizeof(T) / 16 slots], slot s of index c at
+//           s ^ swizzle(c),
+// so that the lanes that read together (8 rows of one slot; 4 or 2 summed
+// indices of 32 or 64 bytes) hit different banks although LDS is filled in
+// order by loads that go straight there.
+__device__ __forceinline__ int along_swizzle(int r) {
+  return kSlots == 8 ? r & 7 : (r >> 1) & 3;
 }
-
-// The staged slab's products: wave (wm, wn) of the 2 x 2 has 32 x 32.
 template <typename T>
-__device__ __forceinline__ void multiply_slab(const char *a, const char *b, f32x4 (&acc)[2][2]) {
-  const int lane = threadIdx.x % 64, wm = threadIdx.x / 128, wn = (threadIdx.x / 64) % 2;
+__device__ __forceinline__ int across_swizzle(int c) {
+  return sizeof(T) == 4 ? ((c >> 2) & 1) << 2 : (c & 3) << 1;
+}
+
+// The slots that a thread fills: q = i kThreads + threadIdx.x.
+template <typename T, bool kAcross, int R>
+struct Slot {
+  static constexpr int kCount = R * kSlots / kThreads;
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements
+  int index;   // tile row (along) or summed index (across)
+  int offset;  // elements from the stage's first, in the other direction
+  __device__ __forceinline__ explicit Slot(int i) {
+    const int q = i * kThreads + static_cast<int>(threadIdx.x);
+    if constexpr (kAcross) {
+      constexpr int kRow = R * static_cast<int>(sizeof(T)) / 16;
+      index = q / kRow;
+      offset = ((q % kRow) ^ across_swizzle<T>(index)) * kPer;
+    } else {
+      index = q / kSlots;
+      offset = ((q % kSlots) ^ along_swizzle(index)) * kPer;
+    }
+  }
+};
+
+// Fills slot i of the thread from 16 bytes at p.
+__device__ __forceinline__ void load_slot(char *lds, int i, const void *p) {
+  const int wave = static_cast<int>(wave_index());
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) void *)p,
+      (__attribute__((address_space(3))) void *)(lds + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+}
+// The same, or with zeros.
+__device__ __forceinline__ void fill_slot(char *lds, int i, const void *p, bool some) {
+  if (some) {
+    load_slot(lds, i, p);
+  } else {
+    *reinterpret_cast<u32x4 *>(lds + (i * kThreads + threadIdx.x) * 16) = u32x4{0, 0, 0, 0};
+  }
+}
+// The same from single elements, of which the first `count` exist.
+template <typename T>
+__device__ __forceinline__ void fill_slot_by_elements(char *lds, int i, const T *p, int64_t count) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  Pack<T, kPer> x;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int at = half * 64 + lane / 16 * 16;
-    const char *pa = a + (wm * 32 + lane % 16) * kPitch + at;
-    const char *pb = b + (wn * 32 + lane % 16) * kPitch + at;
+  for (int j = 0; j < kPer; ++j) x.v[j] = j < count ? p[j] : static_cast<T>(0.0f);
+  *reinterpret_cast<Pack<T, kPer> *>(lds + (i * kThreads + threadIdx.x) * 16) = x;
+}
+
+// Where this lane reads its 16 bytes of the summed index in a staged operand,
+// for the N tiles of 16 rows from `first` on (a multiple of 16 N, so that a
+// tile's number only adds to, or moves within, what the swizzle touches).
+template <typename T, bool kAcross, int R, int N>
+struct Fragments {
+  // along: one place per half; the tiles lie 16 rows apart.  across: one place
+  // per tile; the halves lie half a slab apart.
+  int at[kAcross ? N : kHalves];
+  __device__ __forceinline__ explicit Fragments(int first) {
+    const int lane = static_cast<int>(lane_id()), i = lane % 16, q = lane / 16;
+    if constexpr (!kAcross) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int h = 0; h < kHalves; ++h)
+        at[h] = (first + i) * kSlabBytes + ((h * 4 + q) ^ along_swizzle(i)) * 16;
+    } else {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        multiply<T>(pa + i * 16 * kPitch, pb + j * 16 * kPitch, acc[i][j]);
+      for (int n = 0; n < N; ++n) {
+        if constexpr (sizeof(T) == 2) {
+          // Sixteen lanes read 4 summed indices of 16 neighbours, 8 bytes each,
+          // and get 4 indices of one neighbour each.
+          const int c = q * 8 + i / 4, slot = (first + n * 16) / 8 + i % 4 / 2;
+          at[n] = c * (R * 2) + (slot ^ across_swizzle<T>(c)) * 16 + i % 2 * 8;
+        } else {
+          const int c = q * 4, r = first + n * 16 + i;
+          at[n] = c * (R * 4) + ((r / 4) ^ across_swizzle<T>(c)) * 16 + r % 4 * 4;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ u32x4 load(const char *lds, int n, int half) const {
+    if constexpr (!kAcross) {
+      return *reinterpret_cast<const u32x4 *>(lds + at[half] + n * (16 * kSlabBytes));
+    } else if constexpr (sizeof(T) == 2) {
+      const char *p = lds + at[n] + half * (32 * R * 2);
+      const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) i16x4 *)p);
+      const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) i16x4 *)(p + 4 * R * 2));
+      u32x4 out;
+      __builtin_memcpy(&out, &x, 8);
+      __builtin_memcpy(reinterpret_cast<char *>(&out) + 8, &y, 8);
+      return out;
+    } else {
+      const char *p = lds + at[n] + half * (16 * R * 4);
+      u32x4 out;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        out[j] = *reinterpret_cast<const uint32_t *>(p + j * R * 4);
+      return out;
+    }
+  }
+};
+
+// A wave's part of the tile: 64 rows by kCols / 2 columns.
+template <int kCols>
+struct Accumulator {
+  static constexpr int kA = kCols / 32, kB = kRows / 32;
+  f32x4 v[kA][kB];
+  __device__ __forceinline__ Accumulator() {
+#pragma unroll
+    for (int a = 0; a < kA; ++a)
+#pragma unroll
+      for (int b = 0; b < kB; ++b) v[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  static __device__ __forceinline__ int first_col() {
+    return static_cast<int>(wave_index()) % 2 * (kCols / 2);
+  }
+  static __device__ __forceinline__ int first_row() {
+    return static_cast<int>(wave_index()) / 2 * (kRows / 2);
+  }
+  // The tile row, and the first of the four columns, that a lane has of v[a][b].
+  static __device__ __forceinline__ int row(int b) {
+    return first_row() + b * 16 + static_cast<int>(lane_id()) % 16;
+  }
+  static __device__ __forceinline__ int column(int a) {
+    return first_col() + a * 16 + static_cast<int>(lane_id()) / 16 * 4;
+  }
+};
+
+// acc += the products of a stage at `lds` (columns, then rows); kSums: sums +=
+// the summed index's total of the row operand's rows, per lane its share.
+template <typename T, bool kSums, int kCols, typename ColFragments, typename RowFragments>
+__device__ __forceinline__ void multiply_stage(const char *lds, const ColFragments &cols,
+                                               const RowFragments &rows, Accumulator<kCols> &acc,
+                                               float (&sums)[Accumulator<kCols>::kB]) {
+  using Acc = Accumulator<kCols>;
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) {
+    u32x4 a[Acc::kA], b[Acc::kB];
+#pragma unroll
+    for (int i = 0; i < Acc::kA; ++i) a[i] = cols.load(lds, i, h);
+#pragma unroll
+    for (int i = 0; i < Acc::kB; ++i) b[i] = rows.load(lds + kCols * kSlabBytes, i, h);
+#pragma unroll
+    for (int i = 0; i < Acc::kA; ++i)
+#pragma unroll
+      for (int j = 0; j < Acc::kB; ++j) multiply<T>(a[i], b[j], acc.v[i][j]);
+    if constexpr (kSums) {
+#pragma unroll
+      for (int j = 0; j < Acc::kB; ++j) {
+        const Pack<T, 16 / sizeof(T)> x = __builtin_bit_cast(Pack<T, 16 / sizeof(T)>, b[j]);
+#pragma unroll
+        for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k)
+          sums[j] += static_cast<float>(x.v[k]);
+      }
+    }
   }
 }
 
-// store(row, column, value) for each element of the block's tile.
-template <typename Store>
-__device__ __forceinline__ void store_tile(const f32x4 (&acc)[2][2], Store store) {
-  const int lane = threadIdx.x % 64, wm = threadIdx.x / 128, wn = (threadIdx.x / 64) % 2;
+// The product over `steps` stages, each put on its way by stage(lds, step), the
+// steps in order: kLoads of them per thread, fewer in the last step.  Step i's
+// stage is at lds + i % kStages * kStageBytes.
+template <int kLoads, int kStageBytes, typename Stage, typename Multiply>
+__device__ __forceinline__ void pipeline(char *lds, int steps, Stage stage, Multiply multiply) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < kStages - 1; ++i)
+    if (i < steps) stage(lds + i * kStageBytes, i);
+  // Step i, whose stage is the s-th in LDS; more: the step kStages - 1 ahead is
+  // none past the end.
+  auto turn = [&](int i, int s, bool more) {
+    // Behind step i are kStages - 2 steps' loads, as long as none is the last.
+    if (kStages > 2 && i + kStages - 2 < steps - 1)
+      stage_barrier<(kStages - 2) * kLoads>();
+    else
+      stage_barrier<0>();
+    if (more) stage(lds + (s + kStages - 1) % kStages * kStageBytes, i + kStages - 1);
+    multiply(lds + s * kStageBytes);
+  };
+  int i0 = 0;
+  for (; i0 + 2 * kStages - 2 < steps; i0 += kStages) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int s = 0; s < kStages; ++s) turn(i0 + s, s, true);
+  }
+  // At most 2 kStages - 2 steps more.
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        store(wm * 32 + i * 16 + lane / 16 * 4 + k, wn * 32 + j * 16 + lane % 16, acc[i][j][k]);
+  for (int s = 0; s < 2 * kStages - 2; ++s)
+    if (i0 + s < steps) turn(i0 + s, s % kStages, i0 + s + kStages - 1 < steps);
+}
+
+// Four neighbouring columns of an output row of `width`: one store where the
+// row's vectors allow.
+template <typename T>
+__device__ __forceinline__ void store_four(T *row, int64_t col, int64_t width, bool vector,
+                                           const f32x4 &v) {
+  if (vector && col + 4 <= width) {
+    Pack<T, 4> x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[j] = static_cast<T>(v[j]);
+    store_pack<T, 4>(row + col, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < width) row[col + j] = static_cast<T>(v[j]);
+  }
 }
 
 // ------------------------------------------------------------- kernels ---
 
 // Rows times weights: out[r][j] = sum_c in[r][c] w(c, j), the forward
 // (weight [m, k], summed over k) or with kBack the input's gradient (summed
-// over m).
-template <typename T, bool kBack, bool kVec>
+// over m).  Blocks of one row tile are neighbours, and neighbours share an XCD:
+// they read the same rows and weight.
+template <typename T, bool kBack, bool kVec, int kCols>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const T *__restrict__ in, int64_t stride,
                                                         const T *__restrict__ weight,
                                                         const T *__restrict__ bias, Groups g,
                                                         const int32_t *__restrict__ rows,
-                                                        int64_t k, int64_t m,
+                                                        int64_t k, int64_t m, uint32_t col_tiles,
+                                                        uint32_t vector_out,
                                                         T *__restrict__ out) {
-  __shared__ __attribute__((aligned(16))) char s_a[kTile * kPitch], s_b[kTile * kPitch];
-  __shared__ int64_t s_row[kTile];
+  extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [stages][cols, rows]
+  __shared__ int32_t s_row[kRows];
   constexpr int kSlab = kSlabBytes / static_cast<int>(sizeof(T));
+  constexpr int kColBytes = kCols * kSlabBytes, kStage = (kCols + kRows) * kSlabBytes;
+  using RowSlot = Slot<T, false, kRows>;
+  using ColSlot = Slot<T, kBack, kCols>;
   const int64_t inner = kBack ? m : k, outer = kBack ? k : m;
+  const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int64_t j0 = static_cast<int64_t>(id % col_tiles) * kCols;
   int32_t e;
   int64_t r0, r1;
-  if (!find_part(g, true, kTile, blockIdx.x, e, r0, r1)) return;
-  if (threadIdx.x < kTile) {
+  bool only;
+  if (!find_part(g, true, kRows, id / col_tiles, e, r0, r1, only)) return;
+  if (threadIdx.x < kRows) {
     const int64_t i = r0 + threadIdx.x;
     int64_t r = -1;
     if (i < r1) {
       r = rows != nullptr ? rows[i] : i;
-      if (r >= g.n) r = -1;
+      if (r < 0 || r >= g.n) r = -1;
     }
-    s_row[threadIdx.x] = r;
+    s_row[threadIdx.x] = static_cast<int32_t>(r);
   }
   __syncthreads();
-  const int64_t j0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  f32x4 acc[2][2] = {};
-  if (e < g.count) {
+  Accumulator<kCols> acc;
+  if (e < g.count && inner > 0) {
     const T *w = weight + static_cast<int64_t>(e) * m * k;
-    for (int64_t c0 = 0; c0 < inner; c0 += kSlab) {
-      stage_along<T, kVec>(s_a, in, stride, [&](int r) { return s_row[r]; }, c0, inner);
-      if constexpr (kBack)
-        stage_across<T, kVec>(
-            s_b, w, k, [&](int c) { return c0 + c < m ? c0 + c : int64_t{-1}; }, j0, k);
-      else
-        stage_along<T, kVec>(
-            s_b, w, k, [&](int r) { return j0 + r < m ? j0 + r : int64_t{-1}; }, c0, k);
-      __syncthreads();
-      multiply_slab<T>(s_a, s_b, acc);
-      __syncthreads();
+    // Addresses of the thread's slots in the next stage.  Rows and columns past
+    // the tile's are some others: nothing of theirs is stored.
+    const T *row_at[RowSlot::kCount], *col_at[ColSlot::kCount];
+#pragma unroll
+    for (int i = 0; i < RowSlot::kCount; ++i) {
+      const RowSlot s(i);
+      row_at[i] = in + static_cast<int64_t>(max(s_row[s.index], 0)) * stride + s.offset;
     }
+#pragma unroll
+    for (int i = 0; i < ColSlot::kCount; ++i) {
+      const ColSlot s(i);
+      if constexpr (kBack)
+        col_at[i] = w + s.index * k + (j0 + s.offset < k ? j0 + s.offset : 0);
+      else
+        col_at[i] = w + min(j0 + s.index, m - 1) * k + s.offset;
+    }
+    const int64_t col_step = kBack ? kSlab * k : kSlab;
+    auto stage = [&](char *lds, int step) {
+      const int64_t c0 = static_cast<int64_t>(step) * kSlab;
+      if (kVec && c0 + kSlab <= inner) {
+#pragma unroll
+        for (int i = 0; i < ColSlot::kCount; ++i) load_slot(lds, i, col_at[i]);
+#pragma unroll
+        for (int i = 0; i < RowSlot::kCount; ++i) load_slot(lds + kColBytes, i, row_at[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < ColSlot::kCount; ++i) {
+          const ColSlot s(i);
+          if constexpr (kVec) {
+            fill_slot(lds, i, col_at[i], c0 + (kBack ? s.index : s.offset) < inner);
+          } else {
+            const int64_t count = !kBack            ? k - (c0 + s.offset)
+                                  : c0 + s.index < m ? k - (j0 + s.offset)
+                                                     : 0;
+            fill_slot_by_elements<T>(lds, i, col_at[i], count);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < RowSlot::kCount; ++i) {
+          const RowSlot s(i);
+          if constexpr (kVec)
+            fill_slot(lds + kColBytes, i, row_at[i], c0 + s.offset < inner);
+          else
+            fill_slot_by_elements<T>(lds + kColBytes, i, row_at[i], inner - (c0 + s.offset));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ColSlot::kCount; ++i) col_at[i] += col_step;
+#pragma unroll
+      for (int i = 0; i < RowSlot::kCount; ++i) row_at[i] += kSlab;
+    };
+    const Fragments<T, kBack, kCols, Accumulator<kCols>::kA> col_fragments(acc.first_col());
+    const Fragments<T, false, kRows, Accumulator<kCols>::kB> row_fragments(acc.first_row());
+    float none[Accumulator<kCols>::kB];
+    pipeline<kVec ? RowSlot::kCount + ColSlot::kCount : 0, kStage>(
+        s_stage, static_cast<int>((inner + kSlab - 1) / kSlab), stage, [&](const char *lds) {
+          multiply_stage<T, false>(lds, col_fragments, row_fragments, acc, none);
+        });
   }
-  store_tile(acc, [&](int r, int c, float v) {
-    const int64_t at = s_row[r], j = j0 + c;
-    if (at < 0 || j >= outer) return;
-    if (!kBack && bias != nullptr && e < g.count)
-      v += static_cast<float>(bias[static_cast<int64_t>(e) * m + j]);
-    out[at * outer + j] = static_cast<T>(v);
-  });
+  // The biases of the lane's columns.
+  f32x4 add[Accumulator<kCols>::kA] = {};
+  if (!kBack && bias != nullptr && e < g.count) {
+    const T *b = bias + static_cast<int64_t>(e) * m;
+#pragma unroll
+    for (int a = 0; a < Accumulator<kCols>::kA; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        add[a][i] = static_cast<float>(b[min(j0 + acc.column(a) + i, m - 1)]);
+  }
+#pragma unroll
+  for (int b = 0; b < Accumulator<kCols>::kB; ++b) {
+    const int64_t at = s_row[acc.row(b)];
+    if (at < 0) continue;
+#pragma unroll
+    for (int a = 0; a < Accumulator<kCols>::kA; ++a)
+      store_four<T>(out + at * outer, j0 + acc.column(a), outer, vector_out != 0,
+                    acc.v[a][b] + add[a]);
+  }
 }
 
-// Parts of dW (and db): part s of `per` rows of one group, tile (y, z) of
-// [m, k], into parts [slots][m][k] and bias_parts [slots][m] (may be null).
-template <typename T, bool kVec>
+// dW[m0 + row][k0 + col] (and db) of part `slot`: `per` rows of one group.  The
+// group's only part goes to v_weight and v_bias, others to parts
+// [slots][m][k] and bias_parts [slots][m].
+template <typename T, bool kVec, int kCols>
 __global__ __launch_bounds__(kThreads) void weights_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ v_y, int64_t v_stride,
     Groups g, const int32_t *__restrict__ rows, int64_t k, int64_t m, uint32_t per,
-    float *__restrict__ parts, float *__restrict__ bias_parts) {
-  __shared__ __attribute__((aligned(16))) char s_a[kTile * kPitch], s_b[kTile * kPitch];
+    uint32_t m_tiles, uint32_t k_tiles, uint32_t vector_out, float *__restrict__ parts,
+    float *__restrict__ bias_parts, T *__restrict__ v_weight, T *__restrict__ v_bias) {
+  extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [kStages][cols, rows]
+  // The rows' numbers, two windows by turns.
+  __shared__ __attribute__((aligned(16))) int32_t s_row[2][kWindow];
   constexpr int kSlab = kSlabBytes / static_cast<int>(sizeof(T));
-  __shared__ int64_t s_row[kSlab];
+  constexpr int kColBytes = kCols * kSlabBytes, kStage = (kCols + kRows) * kSlabBytes;
+  static_assert(kWindow % kSlab == 0 && kWindow % kThreads == 0, "whole slabs and waves");
+  using RowSlot = Slot<T, true, kRows>;
+  using ColSlot = Slot<T, true, kCols>;
+  const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x), tiles = m_tiles * k_tiles;
+  const uint32_t slot = id / tiles, tile = id - slot * tiles;
+  const int64_t m0 = static_cast<int64_t>(tile / k_tiles) * kRows;
+  const int64_t k0 = static_cast<int64_t>(tile % k_tiles) * kCols;
   int32_t e;
   int64_t r0, r1;
-  if (!find_part(g, false, per, blockIdx.x, e, r0, r1)) return;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  const int64_t k0 = static_cast<int64_t>(blockIdx.z) * kTile;
-  f32x4 acc[2][2] = {};
-  float bias_sum = 0.0f;
-  for (int64_t c0 = r0; c0 < r1; c0 += kSlab) {
-    if (threadIdx.x < kSlab) {
-      const int64_t i = c0 + threadIdx.x;
-      int64_t r = -1;
-      if (i < r1) {
-        r = rows != nullptr ? rows[i] : i;
-        if (r >= g.n) r = -1;
+  bool only;
+  if (!find_part(g, false, per, slot, e, r0, r1, only)) return;
+  const int count = static_cast<int>(r1 - r0);
+  // Window w's numbers on their way to LDS; past the part's end the last one's.
+  auto fetch_rows = [&](int w) {
+    if (rows == nullptr || w * kWindow >= count) return;
+#pragma unroll
+    for (int i = 0; i < kWindow / kThreads; ++i) {
+      const int at = i * kThreads + static_cast<int>(wave_index()) * 64;
+      const int32_t *p =
+          rows + r0 + min(w * kWindow + at + static_cast<int>(lane_id()), count - 1);
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)p,
+          (__attribute__((address_space(3))) void *)(s_row[w & 1] + at), 4, 0, 0);
+    }
+  };
+  fetch_rows(0);
+  stage_barrier<0>();
+  Accumulator<kCols> acc;
+  float sums[Accumulator<kCols>::kB] = {};
+  const bool with_bias = v_bias != nullptr && k0 == 0 && Accumulator<kCols>::first_col() == 0;
+  // The row of the part's place c < count.
+  auto row_of = [&](int c) -> int64_t {
+    if (rows == nullptr) return r0 + c;
+    return min(max(static_cast<int64_t>(s_row[c / kWindow & 1][c % kWindow]), int64_t{0}),
+               g.n - 1);
+  };
+  auto stage = [&](char *lds, int step) {
+    const int c0 = step * kSlab;
+    // The next window, kWindow / kSlab steps before its first use.
+    if (c0 % kWindow == 0) fetch_rows(c0 / kWindow + 1);
+    if (kVec && c0 + kSlab <= count) {
+#pragma unroll
+      for (int i = 0; i < ColSlot::kCount; ++i) {
+        const ColSlot s(i);
+        const int64_t c = k0 + s.offset;
+        load_slot(lds, i, x + row_of(c0 + s.index) * x_stride + (c < k ? c : 0));
       }
-      s_row[threadIdx.x] = r;
+#pragma unroll
+      for (int i = 0; i < RowSlot::kCount; ++i) {
+        const RowSlot s(i);
+        const int64_t c = m0 + s.offset;
+        load_slot(lds + kColBytes, i, v_y + row_of(c0 + s.index) * v_stride + (c < m ? c : 0));
+      }
+      return;
     }
-    __syncthreads();
-    stage_across<T, kVec>(s_a, v_y, v_stride, [&](int c) { return s_row[c]; }, m0, m);
-    stage_across<T, kVec>(s_b, x, x_stride, [&](int c) { return s_row[c]; }, k0, k);
-    __syncthreads();
-    multiply_slab<T>(s_a, s_b, acc);
-    if (bias_parts != nullptr && blockIdx.z == 0 && threadIdx.x < kTile) {
-      for (int c = 0; c < kSlab; ++c)
-        bias_sum += static_cast<float>(
-            *reinterpret_cast<const T *>(s_a + threadIdx.x * kPitch + c * sizeof(T)));
+#pragma unroll
+    for (int i = 0; i < ColSlot::kCount; ++i) {
+      const ColSlot s(i);
+      const bool some = c0 + s.index < count;
+      const int64_t c = k0 + s.offset;
+      const T *p = x + row_of(min(c0 + s.index, count - 1)) * x_stride;
+      if constexpr (kVec)
+        fill_slot(lds, i, p + (c < k ? c : 0), some);
+      else
+        fill_slot_by_elements<T>(lds, i, p + c, some ? k - c : 0);
     }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RowSlot::kCount; ++i) {
+      const RowSlot s(i);
+      const bool some = c0 + s.index < count;
+      const int64_t c = m0 + s.offset;
+      const T *p = v_y + row_of(min(c0 + s.index, count - 1)) * v_stride;
+      if constexpr (kVec)
+        fill_slot(lds + kColBytes, i, p + (c < m ? c : 0), some);
+      else
+        fill_slot_by_elements<T>(lds + kColBytes, i, p + c, some ? m - c : 0);
+    }
+  };
+  const Fragments<T, true, kCols, Accumulator<kCols>::kA> col_fragments(acc.first_col());
+  const Fragments<T, true, kRows, Accumulator<kCols>::kB> row_fragments(acc.first_row());
+  constexpr int kLoads = kVec ? RowSlot::kCount + ColSlot::kCount : 0;
+  const int steps = (count + kSlab - 1) / kSlab;
+  if (with_bias)
+    pipeline<kLoads, kStage>(s_stage, steps, stage, [&](const char *lds) {
+      multiply_stage<T, true>(lds, col_fragments, row_fragments, acc, sums);
+    });
+  else
+    pipeline<kLoads, kStage>(s_stage, steps, stage, [&](const char *lds) {
+      multiply_stage<T, false>(lds, col_fragments, row_fragments, acc, sums);
+    });
+  if (v_weight != nullptr) {
+    float *p = parts + static_cast<int64_t>(slot) * m * k;
+    T *w = v_weight + static_cast<int64_t>(e) * m * k;
+#pragma unroll
+    for (int b = 0; b < Accumulator<kCols>::kB; ++b) {
+      const int64_t r = m0 + acc.row(b);
+      if (r >= m) continue;
+#pragma unroll
+      for (int a = 0; a < Accumulator<kCols>::kA; ++a) {
+        const int64_t c = k0 + acc.column(a);
+        if (only)
+          store_four<T>(w + r * k, c, k, vector_out != 0, acc.v[a][b]);
+        else
+          store_four<float>(p + r * k, c, k, vector_out != 0, acc.v[a][b]);
+      }
+    }
   }
-  float *p = parts + static_cast<int64_t>(blockIdx.x) * m * k;
-  store_tile(acc, [&](int r, int c, float v) {
-    if (m0 + r < m && k0 + c < k) p[(m0 + r) * k + k0 + c] = v;
-  });
-  if (bias_parts != nullptr && blockIdx.z == 0 && threadIdx.x < kTile && m0 + threadIdx.x < m)
-    bias_parts[static_cast<int64_t>(blockIdx.x) * m + m0 + threadIdx.x] = bias_sum;
+  if (with_bias) {
+    const int lane = static_cast<int>(lane_id());
+#pragma unroll
+    for (int j = 0; j < Accumulator<kCols>::kB; ++j) {
+      // The four lanes of a row hold the slab's quarters.
+      float sum = sums[j];
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      const int64_t r = m0 + Accumulator<kCols>::first_row() + j * 16 + lane % 16;
+      if (lane < 16 && r < m) {
+        if (only)
+          v_bias[static_cast<int64_t>(e) * m + r] = static_cast<T>(sum);
+        else
+          bias_parts[static_cast<int64_t>(slot) * m + r] = sum;
+      }
+    }
+  }
 }
 
-// out[e][i] = the sum of group e's parts, in row order.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void add_parts_kernel(const float *__restrict__ parts,
-                                                             Groups g, uint32_t per,
-                                                             uint32_t slots, int64_t size,
-                                                             T *__restrict__ out) {
+// The weights' (blocks below weight_blocks) and biases' gradient of the groups
+// that have no part or more than one: zeros, or the parts' sum.  kShare threads
+// per element each add every kShare-th part, in row order, and meet in LDS:
+// eight for small weights, whose parts are many, one for large ones.
+template <typename T, int kShare>
+__global__ __launch_bounds__(kThreads) void add_parts_kernel(
+    const float *__restrict__ parts, const float *__restrict__ bias_parts, Groups g, uint32_t per,
+    uint32_t slots, int64_t weight_size, int64_t bias_size, uint32_t weight_blocks,
+    uint32_t bias_blocks, T *__restrict__ v_weight, T *__restrict__ v_bias) {
+  constexpr int kElements = kThreads / kShare;
+  __shared__ float s_sum[kShare][kElements];
   const int32_t e = static_cast<int32_t>(blockIdx.y);
+  const bool is_bias = blockIdx.x >= weight_blocks;
+  const int64_t size = is_bias ? bias_size : weight_size;
   uint32_t before = 0, mine = 0;
   for (int32_t e0 = 0; e0 <= e; e0 += 64) {
     const int32_t q = e0 + static_cast<int32_t>(lane_id());
@@ -288,27 +617,59 @@ __global__ __launch_bounds__(kThreads) void add_parts_kernel(const float *__rest
     mine = readlane_u32(n, static_cast<uint32_t>(min(e - e0, 63)));
     before = readlane_u32(end, 63);
   }
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= size) return;
+  if (mine == 1) return;
   // Offsets that do not ascend could name more parts than there are.
   const uint32_t first = min(before - mine, slots);
   mine = min(mine, slots - first);
-  const float *p = parts + static_cast<int64_t>(first) * size + i;
-  float sum = 0.0f;
-#pragma unroll 4
-  for (uint32_t s = 0; s < mine; ++s) sum += p[static_cast<int64_t>(s) * size];
-  out[static_cast<int64_t>(e) * size + i] = static_cast<T>(sum);
+  const uint32_t share = threadIdx.x / kElements, lane = threadIdx.x % kElements;
+  const uint32_t block = blockIdx.x - (is_bias ? weight_blocks : 0);
+  const int64_t stride = static_cast<int64_t>(is_bias ? bias_blocks : weight_blocks) * kElements;
+  for (int64_t i0 = static_cast<int64_t>(block) * kElements; i0 < size; i0 += stride) {
+    const int64_t i = i0 + lane;
+    float sum = 0.0f;
+    if (i < size) {
+      const float *p = (is_bias ? bias_parts : parts) + static_cast<int64_t>(first) * size + i;
+      for (uint32_t s = share; s < mine; s += kShare * 8) {
+        float v[8];
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q)
+          v[q] = p[static_cast<int64_t>(min(s + q * kShare, mine - 1)) * size];
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) sum += s + q * kShare < mine ? v[q] : 0.0f;
+      }
+    }
+    if constexpr (kShare > 1) {
+      s_sum[share][lane] = sum;
+      __syncthreads();
+      if (share == 0) {
+#pragma unroll
+        for (int q = 1; q < kShare; ++q) sum += s_sum[q][lane];
+      }
+      __syncthreads();
+    }
+    if (share == 0 && i < size)
+      (is_bias ? v_bias : v_weight)[static_cast<int64_t>(e) * size + i] = static_cast<T>(sum);
+  }
 }
 
 // ---------------------------------------------------------------- host ---
 
-uint32_t rows_per_part(int64_t k, int64_t m) {
-  return ceil_div(k, kTile) * ceil_div(m, kTile) >= 64 ? 4096 : 1024;
+int64_t weight_tiles(int64_t k, int64_t m) {
+  return ceil_div(m, kRows) * ceil_div(std::max<int64_t>(k, 1), kRows);
+}
+
+// Rows of a part of the weights' gradient: enough parts to fill the device,
+// and no more, since every part of a group past its first is a copy of the
+// weight to write and add.
+uint32_t rows_per_part(int64_t n, int64_t k, int64_t m) {
+  const int64_t even = ceil_div(n * weight_tiles(k, m), 768);
+  return static_cast<uint32_t>(
+      std::min<int64_t>(std::max<int64_t>(align_up(even, 64), 256), 4096));
 }
 
 // Blocks of the weights' gradient along the rows, at most.
 int64_t part_slots(int64_t n, int64_t k, int64_t m, int64_t groups) {
-  return ceil_div(n, rows_per_part(k, m)) + groups;
+  return ceil_div(n, rows_per_part(n, k, m)) + groups;
 }
 
 struct GradSpace {
@@ -334,61 +695,108 @@ int check_grouped(const char *what, int type, const int32_t *offsets, int64_t n,
   return R2S_OK;
 }
 
+template <typename T, bool kBack, bool kVec, int kCols>
+int rows_launch(const T *in, int64_t stride, const T *weight, const T *bias, Groups g,
+                const int32_t *rows, int64_t k, int64_t m, T *out, hipStream_t stream) {
+  const int64_t inner = kBack ? m : k, outer = kBack ? k : m;
+  const int64_t col_tiles = ceil_div(outer, kCols);
+  const int64_t blocks = (ceil_div(g.n, kRows) + g.count + 1) * col_tiles;
+  if (blocks > kInt32Max) {
+    set_error("grouped_matmul: too many tiles");
+    return R2S_ERANGE;
+  }
+  const int64_t steps = ceil_div(inner * static_cast<int64_t>(sizeof(T)), kSlabBytes);
+  const int stages = static_cast<int>(std::min<int64_t>(std::max<int64_t>(steps, 1), kStages));
+  const bool vector_out = outer % 4 == 0 && address(out) % 16 == 0;
+  rows_kernel<T, kBack, kVec, kCols>
+      <<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads),
+         stages * (kCols + kRows) * kSlabBytes, stream>>>(
+          in, stride, weight, bias, g, rows, k, m, static_cast<uint32_t>(col_tiles),
+          vector_out ? 1u : 0u, out);
+  return check_launch("grouped_matmul");
+}
+
 template <typename T, bool kBack>
 int rows_product(const void *in, int64_t stride, const void *weight, const void *bias, Groups g,
                  const int32_t *rows, int64_t k, int64_t m, void *out, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(ceil_div(g.n, kTile) + g.count + 1),
-                  static_cast<uint32_t>(ceil_div(kBack ? k : m, kTile)));
   const bool vec = address(in) % 16 == 0 && address(weight) % 16 == 0 &&
-                   stride * sizeof(T) % 16 == 0 && k * sizeof(T) % 16 == 0;
+                   stride * sizeof(T) % 16 == 0 && k * sizeof(T) % 16 == 0 &&
+                   (!kBack || m * sizeof(T) % 16 == 0);
   const T *ti = static_cast<const T *>(in), *tw = static_cast<const T *>(weight);
   const T *tb = static_cast<const T *>(bias);
-  if (vec)
-    rows_kernel<T, kBack, true><<<grid, dim3(kThreads), 0, stream>>>(ti, stride, tw, tb, g, rows,
-                                                                     k, m, static_cast<T *>(out));
+  T *to = static_cast<T *>(out);
+  const bool narrow = (kBack ? k : m) <= 64;
+#define R2S_ROWS(VEC, COLS) \
+  return (rows_launch<T, kBack, VEC, COLS>(ti, stride, tw, tb, g, rows, k, m, to, stream))
+  if (vec) {
+    if (narrow) R2S_ROWS(true, 64);
+    R2S_ROWS(true, 128);
+  }
+  if (narrow) R2S_ROWS(false, 64);
+  R2S_ROWS(false, 128);
+#undef R2S_ROWS
+}
+
+template <typename T, bool kVec, int kCols>
+int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride, Groups g,
+                   const int32_t *rows, int64_t k, int64_t m, T *v_weight, T *v_bias,
+                   const GradSpace &s, hipStream_t stream) {
+  const uint32_t per = rows_per_part(g.n, k, m);
+  const int64_t slots = part_slots(g.n, k, m, g.count);
+  const int64_t m_tiles = ceil_div(m, kRows), k_tiles = ceil_div(std::max<int64_t>(k, 1), kCols);
+  if (slots * m_tiles * k_tiles > kInt32Max) {
+    set_error("grouped_matmul_bwd: too many tiles");
+    return R2S_ERANGE;
+  }
+  const bool vector_out = k % 4 == 0 && address(v_weight) % 16 == 0;
+  if (g.n > 0) {
+    weights_kernel<T, kVec, kCols>
+        <<<dim3(static_cast<uint32_t>(slots * m_tiles * k_tiles)), dim3(kThreads),
+           kStages * (kCols + kRows) * kSlabBytes, stream>>>(
+            x, x_stride, v_y, v_stride, g, rows, k, m, per, static_cast<uint32_t>(m_tiles),
+            static_cast<uint32_t>(k_tiles), vector_out ? 1u : 0u, s.parts, s.bias_parts, v_weight,
+            v_bias);
+    R2S_RETURN_IF(check_launch("grouped_matmul_bwd weights"));
+  }
+  // At most 1024 blocks a group: most groups of large weights have one part, and
+  // their blocks only find that out.
+  const bool small = m * k <= 1 << 15;
+  const int64_t elements = small ? kThreads / 8 : kThreads;
+  const int64_t weight_blocks =
+      v_weight != nullptr ? std::min<int64_t>(ceil_div(m * k, elements), 1024) : 0;
+  const int64_t bias_blocks = v_bias != nullptr ? ceil_div(m, elements) : 0;
+  if (weight_blocks + bias_blocks == 0) return R2S_OK;
+  const dim3 grid(static_cast<uint32_t>(weight_blocks + bias_blocks), g.count);
+#define R2S_ADD_PARTS(SHARE)                                                                    \
+  add_parts_kernel<T, SHARE><<<grid, dim3(kThreads), 0, stream>>>(                              \
+      s.parts, s.bias_parts, g, per, static_cast<uint32_t>(slots), m * k, m,                    \
+      static_cast<uint32_t>(weight_blocks), static_cast<uint32_t>(bias_blocks), v_weight, v_bias)
+  if (small)
+    R2S_ADD_PARTS(8);
   else
-    rows_kernel<T, kBack, false><<<grid, dim3(kThreads), 0, stream>>>(ti, stride, tw, tb, g, rows,
-                                                                      k, m, static_cast<T *>(out));
-  return check_launch("grouped_matmul");
+    R2S_ADD_PARTS(1);
+#undef R2S_ADD_PARTS
+  return check_launch("grouped_matmul_bwd weights");
 }
 
 template <typename T>
 int weights_product(const void *x, int64_t x_stride, const void *v_y, int64_t v_stride, Groups g,
                     const int32_t *rows, int64_t k, int64_t m, void *v_weight, void *v_bias,
                     const GradSpace &s, hipStream_t stream) {
-  const uint32_t per = rows_per_part(k, m);
-  const uint32_t slots = static_cast<uint32_t>(part_slots(g.n, k, m, g.count));
-  float *bias_parts = v_bias != nullptr ? s.bias_parts : nullptr;
-  if (g.n > 0) {
-    const dim3 grid(slots,
-                    static_cast<uint32_t>(ceil_div(m, kTile)),
-                    static_cast<uint32_t>(max(ceil_div(k, kTile), int64_t{1})));
-    const bool vec = address(x) % 16 == 0 && address(v_y) % 16 == 0 &&
-                     x_stride * sizeof(T) % 16 == 0 && v_stride * sizeof(T) % 16 == 0;
-    const T *tx = static_cast<const T *>(x), *tv = static_cast<const T *>(v_y);
-    if (vec)
-      weights_kernel<T, true><<<grid, dim3(kThreads), 0, stream>>>(tx, x_stride, tv, v_stride, g,
-                                                                   rows, k, m, per, s.parts,
-                                                                   bias_parts);
-    else
-      weights_kernel<T, false><<<grid, dim3(kThreads), 0, stream>>>(tx, x_stride, tv, v_stride, g,
-                                                                    rows, k, m, per, s.parts,
-                                                                    bias_parts);
-    R2S_RETURN_IF(check_launch("grouped_matmul_bwd weights"));
+  const bool vec = k > 0 && address(x) % 16 == 0 && address(v_y) % 16 == 0 &&
+                   x_stride * sizeof(T) % 16 == 0 && v_stride * sizeof(T) % 16 == 0 &&
+                   k * sizeof(T) % 16 == 0 && m * sizeof(T) % 16 == 0;
+  const T *tx = static_cast<const T *>(x), *tv = static_cast<const T *>(v_y);
+  T *vw = static_cast<T *>(v_weight), *vb = static_cast<T *>(v_bias);
+#define R2S_WEIGHTS(VEC, COLS) \
+  return (weights_launch<T, VEC, COLS>(tx, x_stride, tv, v_stride, g, rows, k, m, vw, vb, s, stream))
+  if (vec) {
+    if (k <= 64) R2S_WEIGHTS(true, 64);
+    R2S_WEIGHTS(true, 128);
   }
-  if (v_weight != nullptr && m * k > 0) {
-    add_parts_kernel<T><<<dim3(static_cast<uint32_t>(ceil_div(m * k, kThreads)), g.count),
-                          dim3(kThreads), 0, stream>>>(s.parts, g, per, slots, m * k,
-                                                       static_cast<T *>(v_weight));
-    R2S_RETURN_IF(check_launch("grouped_matmul_bwd weights"));
-  }
-  if (v_bias != nullptr) {
-    add_parts_kernel<T><<<dim3(static_cast<uint32_t>(ceil_div(m, kThreads)), g.count),
-                          dim3(kThreads), 0, stream>>>(s.bias_parts, g, per, slots, m,
-                                                       static_cast<T *>(v_bias));
-    R2S_RETURN_IF(check_launch("grouped_matmul_bwd bias"));
-  }
-  return R2S_OK;
+  if (k <= 64) R2S_WEIGHTS(false, 64);
+  R2S_WEIGHTS(false, 128);
+#undef R2S_WEIGHTS
 }
 
 }  // namespace
