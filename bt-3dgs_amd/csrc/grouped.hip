@@ -36,7 +36,6 @@ constexpr int kSlabBytes = 128;  // of the summed index per stage
 constexpr int kSlots = kSlabBytes / 16;
 constexpr int kHalves = kSlabBytes / 64;  // what one matrix instruction, or four, sum over
 constexpr int kWindow = 512;     // row numbers of a weights' gradient block in LDS, twice
-constexpr int kStages = 2;       // in LDS: one is multiplied, the other is on its way
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
@@ -107,27 +106,32 @@ __device__ __forceinline__ bool find_part(const Groups &g, bool rest, uint32_t p
 
 // ------------------------------------------------------------- staging ---
 
-// Waits until all but the wave's last `kLeft` loads have arrived, then for the
-// block's other waves: the stage before those is in LDS, and the one that was
-// multiplied last is free.
-template <int kLeft>
+// The wave's loads to LDS have arrived, and so have the other waves': the next
+// stage is in LDS, and the one that was multiplied last is free.
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // An operand's stage is R x 128 bytes of LDS in 16-byte slots:
 //   along   [R rows][kSlots], slot s of row r at s ^ swizzle(r);
 //   across  [kSlab summed][R sizeof(T) / 16 slots], slot s of index c at
 //           s ^ swizzle(c),
-// so that the lanes that read together (8 rows of one slot; 4 or 2 summed
-// indices of 32 or 64 bytes) hit different banks although LDS is filled in
-// order by loads that go straight there.
+// so that the lanes that read together hit different ones of the 64 banks
+// although LDS is filled in order by loads that go straight there.
 __device__ __forceinline__ int along_swizzle(int r) {
   return kSlots == 8 ? r & 7 : (r >> 1) & 3;
 }
-template <typename T>
+template <typename T, int R>
 __device__ __forceinline__ int across_swizzle(int c) {
-  return sizeof(T) == 4 ? ((c >> 2) & 1) << 2 : (c & 3) << 1;
+  // f32: four runs of 64 bytes, 4 indices apart.  16 bits: eight runs of 32
+  // bytes, indices c to c + 3 and c + 8 to c + 11; rows of 128 bytes put every
+  // other index in the other half of the banks by themselves.
+  if constexpr (sizeof(T) == 4)
+    return ((c >> 2) & 3) << 2;
+  else if constexpr (R == 128)
+    return ((c & 3) | ((c >> 3) & 1) << 2) << 1;
+  else
+    return (((c >> 1) & 1) | ((c >> 3) & 1) << 1) << 1;
 }
 
 // The slots that a thread fills: q = i kThreads + threadIdx.x.
@@ -142,7 +146,7 @@ struct Slot {
     if constexpr (kAcross) {
       constexpr int kRow = R * static_cast<int>(sizeof(T)) / 16;
       index = q / kRow;
-      offset = ((q % kRow) ^ across_swizzle<T>(index)) * kPer;
+      offset = ((q % kRow) ^ across_swizzle<T, R>(index)) * kPer;
     } else {
       index = q / kSlots;
       offset = ((q % kSlots) ^ along_swizzle(index)) * kPer;
@@ -165,14 +169,24 @@ __device__ __forceinline__ void fill_slot(char *lds, int i, const void *p, bool 
     *reinterpret_cast<u32x4 *>(lds + (i * kThreads + threadIdx.x) * 16) = u32x4{0, 0, 0, 0};
   }
 }
-// The same from single elements, of which the first `count` exist.
+// 16 bytes at p of which the first `count` elements exist, zeros for the rest;
+// p at any element.
 template <typename T>
-__device__ __forceinline__ void fill_slot_by_elements(char *lds, int i, const T *p, int64_t count) {
+struct __attribute__((packed)) Unaligned {
+  T v[16 / sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ u32x4 load_elements(const T *p, int64_t count) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  if (count >= kPer)
+    return __builtin_bit_cast(u32x4, *reinterpret_cast<const Unaligned<T> *>(p));
   Pack<T, kPer> x;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) x.v[j] = j < count ? p[j] : static_cast<T>(0.0f);
-  *reinterpret_cast<Pack<T, kPer> *>(lds + (i * kThreads + threadIdx.x) * 16) = x;
+  return __builtin_bit_cast(u32x4, x);
+}
+__device__ __forceinline__ void put_slot(char *lds, int i, u32x4 x) {
+  *reinterpret_cast<u32x4 *>(lds + (i * kThreads + threadIdx.x) * 16) = x;
 }
 
 // Where this lane reads its 16 bytes of the summed index in a staged operand,
@@ -196,10 +210,10 @@ struct Fragments {
           // Sixteen lanes read 4 summed indices of 16 neighbours, 8 bytes each,
           // and get 4 indices of one neighbour each.
           const int c = q * 8 + i / 4, slot = (first + n * 16) / 8 + i % 4 / 2;
-          at[n] = c * (R * 2) + (slot ^ across_swizzle<T>(c)) * 16 + i % 2 * 8;
+          at[n] = c * (R * 2) + (slot ^ across_swizzle<T, R>(c)) * 16 + i % 2 * 8;
         } else {
           const int c = q * 4, r = first + n * 16 + i;
-          at[n] = c * (R * 4) + ((r / 4) ^ across_swizzle<T>(c)) * 16 + r % 4 * 4;
+          at[n] = c * (R * 4) + ((r / 4) ^ across_swizzle<T, R>(c)) * 16 + r % 4 * 4;
         }
       }
     }
@@ -284,46 +298,43 @@ __device__ __forceinline__ void multiply_stage(const char *lds, const ColFragmen
   }
 }
 
-// The product over `steps` stages, each put on its way by stage(lds, step), the
-// steps in order: kLoads of them per thread, fewer in the last step.  Step i's
-// stage is at lds + i % kStages * kStageBytes.
-template <int kLoads, int kStageBytes, typename Stage, typename Multiply>
-__device__ __forceinline__ void pipeline(char *lds, int steps, Stage stage, Multiply multiply) {
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i)
-    if (i < steps) stage(lds + i * kStageBytes, i);
-  // Step i, whose stage is the s-th in LDS; more: the step kStages - 1 ahead is
-  // none past the end.
+// The product over `steps` stages.  Step i's stage is at lds + i % 2 *
+// kStageBytes.  stage(lds, step), the steps in order, puts a stage on its way
+// to LDS, or reads it (with null) for commit(lds) to write it there.
+template <bool kDirect, int kStageBytes, typename Stage, typename Commit, typename Multiply>
+__device__ __forceinline__ void pipeline(char *lds, int steps, Stage stage, Commit commit,
+                                         Multiply multiply) {
+  // Step i, whose stage is the s-th in LDS; more: there is a step after it.
   auto turn = [&](int i, int s, bool more) {
-    // Behind step i are kStages - 2 steps' loads, as long as none is the last.
-    if (kStages > 2 && i + kStages - 2 < steps - 1)
-      stage_barrier<(kStages - 2) * kLoads>();
-    else
-      stage_barrier<0>();
-    if (more) stage(lds + (s + kStages - 1) % kStages * kStageBytes, i + kStages - 1);
+    char *next = lds + (s ^ 1) * kStageBytes;
+    stage_barrier();
+    if (more) stage(next, i + 1);
     multiply(lds + s * kStageBytes);
+    if (!kDirect && more) commit(next);
   };
-  int i0 = 0;
-  for (; i0 + 2 * kStages - 2 < steps; i0 += kStages) {
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) turn(i0 + s, s, true);
+  stage(lds, 0);
+  if (!kDirect) commit(lds);
+  int i = 0;
+  for (; i + 2 < steps; i += 2) {
+    turn(i, 0, true);
+    turn(i + 1, 1, true);
   }
-  // At most 2 kStages - 2 steps more.
-#pragma unroll
-  for (int s = 0; s < 2 * kStages - 2; ++s)
-    if (i0 + s < steps) turn(i0 + s, s % kStages, i0 + s + kStages - 1 < steps);
+  if (i < steps) turn(i, 0, i + 1 < steps);
+  if (i + 1 < steps) turn(i + 1, 1, false);
 }
 
-// Four neighbouring columns of an output row of `width`: one store where the
-// row's vectors allow.
+// Four neighbouring columns of an output row of `width`, at any element.
 template <typename T>
-__device__ __forceinline__ void store_four(T *row, int64_t col, int64_t width, bool vector,
-                                           const f32x4 &v) {
-  if (vector && col + 4 <= width) {
-    Pack<T, 4> x;
+struct __attribute__((packed)) UnalignedFour {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ void store_four(T *row, int64_t col, int64_t width, const f32x4 &v) {
+  if (col + 4 <= width) {
+    UnalignedFour<T> x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) x.v[j] = static_cast<T>(v[j]);
-    store_pack<T, 4>(row + col, x);
+    *reinterpret_cast<UnalignedFour<T> *>(row + col) = x;
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -338,14 +349,13 @@ __device__ __forceinline__ void store_four(T *row, int64_t col, int64_t width, b
 // over m).  Blocks of one row tile are neighbours, and neighbours share an XCD:
 // they read the same rows and weight.
 template <typename T, bool kBack, bool kVec, int kCols>
-__global__ __launch_bounds__(kThreads) void rows_kernel(const T *__restrict__ in, int64_t stride,
+__global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void rows_kernel(const T *__restrict__ in, int64_t stride,
                                                         const T *__restrict__ weight,
                                                         const T *__restrict__ bias, Groups g,
                                                         const int32_t *__restrict__ rows,
                                                         int64_t k, int64_t m, uint32_t col_tiles,
-                                                        uint32_t vector_out,
                                                         T *__restrict__ out) {
-  extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [stages][cols, rows]
+  extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [1 or 2][cols, rows]
   __shared__ int32_t s_row[kRows];
   constexpr int kSlab = kSlabBytes / static_cast<int>(sizeof(T));
   constexpr int kColBytes = kCols * kSlabBytes, kStage = (kCols + kRows) * kSlabBytes;
@@ -388,9 +398,22 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const T *__restrict__ in
         col_at[i] = w + min(j0 + s.index, m - 1) * k + s.offset;
     }
     const int64_t col_step = kBack ? kSlab * k : kSlab;
+    u32x4 col_held[kVec ? 1 : ColSlot::kCount], row_held[kVec ? 1 : RowSlot::kCount];
     auto stage = [&](char *lds, int step) {
       const int64_t c0 = static_cast<int64_t>(step) * kSlab;
-      if (kVec && c0 + kSlab <= inner) {
+      if constexpr (!kVec) {
+#pragma unroll
+        for (int i = 0; i < ColSlot::kCount; ++i) {
+          const ColSlot s(i);
+          const int64_t count = !kBack             ? k - (c0 + s.offset)
+                                : c0 + s.index < m ? k - (j0 + s.offset)
+                                                   : 0;
+          col_held[i] = load_elements<T>(col_at[i], count);
+        }
+#pragma unroll
+        for (int i = 0; i < RowSlot::kCount; ++i)
+          row_held[i] = load_elements<T>(row_at[i], inner - (c0 + RowSlot(i).offset));
+      } else if (c0 + kSlab <= inner) {
 #pragma unroll
         for (int i = 0; i < ColSlot::kCount; ++i) load_slot(lds, i, col_at[i]);
 #pragma unroll
@@ -399,36 +422,33 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const T *__restrict__ in
 #pragma unroll
         for (int i = 0; i < ColSlot::kCount; ++i) {
           const ColSlot s(i);
-          if constexpr (kVec) {
-            fill_slot(lds, i, col_at[i], c0 + (kBack ? s.index : s.offset) < inner);
-          } else {
-            const int64_t count = !kBack            ? k - (c0 + s.offset)
-                                  : c0 + s.index < m ? k - (j0 + s.offset)
-                                                     : 0;
-            fill_slot_by_elements<T>(lds, i, col_at[i], count);
-          }
+          fill_slot(lds, i, col_at[i], c0 + (kBack ? s.index : s.offset) < inner);
         }
 #pragma unroll
-        for (int i = 0; i < RowSlot::kCount; ++i) {
-          const RowSlot s(i);
-          if constexpr (kVec)
-            fill_slot(lds + kColBytes, i, row_at[i], c0 + s.offset < inner);
-          else
-            fill_slot_by_elements<T>(lds + kColBytes, i, row_at[i], inner - (c0 + s.offset));
-        }
+        for (int i = 0; i < RowSlot::kCount; ++i)
+          fill_slot(lds + kColBytes, i, row_at[i], c0 + RowSlot(i).offset < inner);
       }
 #pragma unroll
       for (int i = 0; i < ColSlot::kCount; ++i) col_at[i] += col_step;
 #pragma unroll
       for (int i = 0; i < RowSlot::kCount; ++i) row_at[i] += kSlab;
     };
+    auto commit = [&](char *lds) {
+      if constexpr (!kVec) {
+#pragma unroll
+        for (int i = 0; i < ColSlot::kCount; ++i) put_slot(lds, i, col_held[i]);
+#pragma unroll
+        for (int i = 0; i < RowSlot::kCount; ++i) put_slot(lds + kColBytes, i, row_held[i]);
+      }
+    };
     const Fragments<T, kBack, kCols, Accumulator<kCols>::kA> col_fragments(acc.first_col());
     const Fragments<T, false, kRows, Accumulator<kCols>::kB> row_fragments(acc.first_row());
     float none[Accumulator<kCols>::kB];
-    pipeline<kVec ? RowSlot::kCount + ColSlot::kCount : 0, kStage>(
-        s_stage, static_cast<int>((inner + kSlab - 1) / kSlab), stage, [&](const char *lds) {
-          multiply_stage<T, false>(lds, col_fragments, row_fragments, acc, none);
-        });
+    pipeline<kVec, kStage>(s_stage, static_cast<int>((inner + kSlab - 1) / kSlab), stage, commit,
+                           [&](const char *lds) {
+                             multiply_stage<T, false>(lds, col_fragments, row_fragments, acc,
+                                                      none);
+                           });
   }
   // The biases of the lane's columns.
   f32x4 add[Accumulator<kCols>::kA] = {};
@@ -446,7 +466,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const T *__restrict__ in
     if (at < 0) continue;
 #pragma unroll
     for (int a = 0; a < Accumulator<kCols>::kA; ++a)
-      store_four<T>(out + at * outer, j0 + acc.column(a), outer, vector_out != 0,
+      store_four<T>(out + at * outer, j0 + acc.column(a), outer,
                     acc.v[a][b] + add[a]);
   }
 }
@@ -455,12 +475,12 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const T *__restrict__ in
 // group's only part goes to v_weight and v_bias, others to parts
 // [slots][m][k] and bias_parts [slots][m].
 template <typename T, bool kVec, int kCols>
-__global__ __launch_bounds__(kThreads) void weights_kernel(
+__global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ v_y, int64_t v_stride,
     Groups g, const int32_t *__restrict__ rows, int64_t k, int64_t m, uint32_t per,
-    uint32_t m_tiles, uint32_t k_tiles, uint32_t vector_out, float *__restrict__ parts,
-    float *__restrict__ bias_parts, T *__restrict__ v_weight, T *__restrict__ v_bias) {
-  extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [kStages][cols, rows]
+    uint32_t m_tiles, uint32_t k_tiles, float *__restrict__ parts, float *__restrict__ bias_parts,
+    T *__restrict__ v_weight, T *__restrict__ v_bias) {
+  extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [2][cols, rows]
   // The rows' numbers, two windows by turns.
   __shared__ __attribute__((aligned(16))) int32_t s_row[2][kWindow];
   constexpr int kSlab = kSlabBytes / static_cast<int>(sizeof(T));
@@ -491,7 +511,7 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(
     }
   };
   fetch_rows(0);
-  stage_barrier<0>();
+  stage_barrier();
   Accumulator<kCols> acc;
   float sums[Accumulator<kCols>::kB] = {};
   const bool with_bias = v_bias != nullptr && k0 == 0 && Accumulator<kCols>::first_col() == 0;
@@ -501,58 +521,58 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(
     return min(max(static_cast<int64_t>(s_row[c / kWindow & 1][c % kWindow]), int64_t{0}),
                g.n - 1);
   };
+  u32x4 col_held[kVec ? 1 : ColSlot::kCount], row_held[kVec ? 1 : RowSlot::kCount];
   auto stage = [&](char *lds, int step) {
     const int c0 = step * kSlab;
     // The next window, kWindow / kSlab steps before its first use.
     if (c0 % kWindow == 0) fetch_rows(c0 / kWindow + 1);
-    if (kVec && c0 + kSlab <= count) {
-#pragma unroll
-      for (int i = 0; i < ColSlot::kCount; ++i) {
-        const ColSlot s(i);
-        const int64_t c = k0 + s.offset;
-        load_slot(lds, i, x + row_of(c0 + s.index) * x_stride + (c < k ? c : 0));
-      }
-#pragma unroll
-      for (int i = 0; i < RowSlot::kCount; ++i) {
-        const RowSlot s(i);
-        const int64_t c = m0 + s.offset;
-        load_slot(lds + kColBytes, i, v_y + row_of(c0 + s.index) * v_stride + (c < m ? c : 0));
-      }
-      return;
-    }
+    const bool full = c0 + kSlab <= count;
 #pragma unroll
     for (int i = 0; i < ColSlot::kCount; ++i) {
       const ColSlot s(i);
-      const bool some = c0 + s.index < count;
       const int64_t c = k0 + s.offset;
-      const T *p = x + row_of(min(c0 + s.index, count - 1)) * x_stride;
-      if constexpr (kVec)
-        fill_slot(lds, i, p + (c < k ? c : 0), some);
+      const int at = full ? c0 + s.index : min(c0 + s.index, count - 1);
+      const bool some = full || c0 + s.index < count;
+      const T *p = x + row_of(at) * x_stride;
+      if constexpr (!kVec)
+        col_held[i] = load_elements<T>(p + c, some ? k - c : 0);
+      else if (full)
+        load_slot(lds, i, p + (c < k ? c : 0));
       else
-        fill_slot_by_elements<T>(lds, i, p + c, some ? k - c : 0);
+        fill_slot(lds, i, p + (c < k ? c : 0), some);
     }
 #pragma unroll
     for (int i = 0; i < RowSlot::kCount; ++i) {
       const RowSlot s(i);
-      const bool some = c0 + s.index < count;
       const int64_t c = m0 + s.offset;
-      const T *p = v_y + row_of(min(c0 + s.index, count - 1)) * v_stride;
-      if constexpr (kVec)
-        fill_slot(lds + kColBytes, i, p + (c < m ? c : 0), some);
+      const int at = full ? c0 + s.index : min(c0 + s.index, count - 1);
+      const bool some = full || c0 + s.index < count;
+      const T *p = v_y + row_of(at) * v_stride;
+      if constexpr (!kVec)
+        row_held[i] = load_elements<T>(p + c, some ? m - c : 0);
+      else if (full)
+        load_slot(lds + kColBytes, i, p + (c < m ? c : 0));
       else
-        fill_slot_by_elements<T>(lds + kColBytes, i, p + c, some ? m - c : 0);
+        fill_slot(lds + kColBytes, i, p + (c < m ? c : 0), some);
+    }
+  };
+  auto commit = [&](char *lds) {
+    if constexpr (!kVec) {
+#pragma unroll
+      for (int i = 0; i < ColSlot::kCount; ++i) put_slot(lds, i, col_held[i]);
+#pragma unroll
+      for (int i = 0; i < RowSlot::kCount; ++i) put_slot(lds + kColBytes, i, row_held[i]);
     }
   };
   const Fragments<T, true, kCols, Accumulator<kCols>::kA> col_fragments(acc.first_col());
   const Fragments<T, true, kRows, Accumulator<kCols>::kB> row_fragments(acc.first_row());
-  constexpr int kLoads = kVec ? RowSlot::kCount + ColSlot::kCount : 0;
   const int steps = (count + kSlab - 1) / kSlab;
   if (with_bias)
-    pipeline<kLoads, kStage>(s_stage, steps, stage, [&](const char *lds) {
+    pipeline<kVec, kStage>(s_stage, steps, stage, commit, [&](const char *lds) {
       multiply_stage<T, true>(lds, col_fragments, row_fragments, acc, sums);
     });
   else
-    pipeline<kLoads, kStage>(s_stage, steps, stage, [&](const char *lds) {
+    pipeline<kVec, kStage>(s_stage, steps, stage, commit, [&](const char *lds) {
       multiply_stage<T, false>(lds, col_fragments, row_fragments, acc, sums);
     });
   if (v_weight != nullptr) {
@@ -566,9 +586,9 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(
       for (int a = 0; a < Accumulator<kCols>::kA; ++a) {
         const int64_t c = k0 + acc.column(a);
         if (only)
-          store_four<T>(w + r * k, c, k, vector_out != 0, acc.v[a][b]);
+          store_four<T>(w + r * k, c, k, acc.v[a][b]);
         else
-          store_four<float>(p + r * k, c, k, vector_out != 0, acc.v[a][b]);
+          store_four<float>(p + r * k, c, k, acc.v[a][b]);
       }
     }
   }
@@ -705,14 +725,12 @@ int rows_launch(const T *in, int64_t stride, const T *weight, const T *bias, Gro
     set_error("grouped_matmul: too many tiles");
     return R2S_ERANGE;
   }
-  const int64_t steps = ceil_div(inner * static_cast<int64_t>(sizeof(T)), kSlabBytes);
-  const int stages = static_cast<int>(std::min<int64_t>(std::max<int64_t>(steps, 1), kStages));
-  const bool vector_out = outer % 4 == 0 && address(out) % 16 == 0;
+  const int stages = inner * static_cast<int64_t>(sizeof(T)) > kSlabBytes ? 2 : 1;
   rows_kernel<T, kBack, kVec, kCols>
       <<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads),
          stages * (kCols + kRows) * kSlabBytes, stream>>>(
           in, stride, weight, bias, g, rows, k, m, static_cast<uint32_t>(col_tiles),
-          vector_out ? 1u : 0u, out);
+          out);
   return check_launch("grouped_matmul");
 }
 
@@ -748,14 +766,12 @@ int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride,
     set_error("grouped_matmul_bwd: too many tiles");
     return R2S_ERANGE;
   }
-  const bool vector_out = k % 4 == 0 && address(v_weight) % 16 == 0;
   if (g.n > 0) {
     weights_kernel<T, kVec, kCols>
         <<<dim3(static_cast<uint32_t>(slots * m_tiles * k_tiles)), dim3(kThreads),
-           kStages * (kCols + kRows) * kSlabBytes, stream>>>(
+           2 * (kCols + kRows) * kSlabBytes, stream>>>(
             x, x_stride, v_y, v_stride, g, rows, k, m, per, static_cast<uint32_t>(m_tiles),
-            static_cast<uint32_t>(k_tiles), vector_out ? 1u : 0u, s.parts, s.bias_parts, v_weight,
-            v_bias);
+            static_cast<uint32_t>(k_tiles), s.parts, s.bias_parts, v_weight, v_bias);
     R2S_RETURN_IF(check_launch("grouped_matmul_bwd weights"));
   }
   // At most 1024 blocks a group: most groups of large weights have one part, and
