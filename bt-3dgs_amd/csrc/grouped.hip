@@ -11,8 +11,8 @@
 // groups' rows do not lie together, so no permuted copy is made.
 //
 // A block of four waves makes a tile of 128 output rows by 64 or 128 columns on
-// the matrix cores, each wave half of both, from operands staged in LDS 128
-// bytes of the summed index at a time, the next stage's loads in flight while
+// the matrix cores, each wave half of both, from operands staged in LDS 64 or
+// 128 bytes of the summed index at a time, the next stage's loads in flight while
 // one is multiplied.  An operand whose summed index is innermost in memory
 // ("along": rows of x, of W forward) is staged as it lies; one whose tile
 // index is innermost ("across": W backward, both operands of dW) is staged as
@@ -32,9 +32,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRows = 128;      // output rows of a block's tile
-constexpr int kSlabBytes = 128;  // of the summed index per stage
-constexpr int kSlots = kSlabBytes / 16;
-constexpr int kHalves = kSlabBytes / 64;  // what one matrix instruction, or four, sum over
 constexpr int kWindow = 512;     // row numbers of a weights' gradient block in LDS, twice
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
@@ -112,14 +109,16 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// An operand's stage is R x 128 bytes of LDS in 16-byte slots:
-//   along   [R rows][kSlots], slot s of row r at s ^ swizzle(r);
-//   across  [kSlab summed][R sizeof(T) / 16 slots], slot s of index c at
+// An operand's stage is R x S bytes of LDS (S = 64 or 128 of the summed index) in
+// 16-byte slots:
+//   along   [R rows][S / 16 slots], slot s of row r at s ^ swizzle(r);
+//   across  [S / sizeof(T) summed][R sizeof(T) / 16 slots], slot s of index c at
 //           s ^ swizzle(c),
 // so that the lanes that read together hit different ones of the 64 banks
 // although LDS is filled in order by loads that go straight there.
+template <int S>
 __device__ __forceinline__ int along_swizzle(int r) {
-  return kSlots == 8 ? r & 7 : (r >> 1) & 3;
+  return S == 128 ? r & 7 : (r >> 1) & 3;
 }
 template <typename T, int R>
 __device__ __forceinline__ int across_swizzle(int c) {
@@ -135,8 +134,9 @@ __device__ __forceinline__ int across_swizzle(int c) {
 }
 
 // The slots that a thread fills: q = i kThreads + threadIdx.x.
-template <typename T, bool kAcross, int R>
+template <typename T, bool kAcross, int R, int S>
 struct Slot {
+  static constexpr int kSlots = S / 16;
   static constexpr int kCount = R * kSlots / kThreads;
   static constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements
   int index;   // tile row (along) or summed index (across)
@@ -149,7 +149,7 @@ struct Slot {
       offset = ((q % kRow) ^ across_swizzle<T, R>(index)) * kPer;
     } else {
       index = q / kSlots;
-      offset = ((q % kSlots) ^ along_swizzle(index)) * kPer;
+      offset = ((q % kSlots) ^ along_swizzle<S>(index)) * kPer;
     }
   }
 };
@@ -192,8 +192,9 @@ __device__ __forceinline__ void put_slot(char *lds, int i, u32x4 x) {
 // Where this lane reads its 16 bytes of the summed index in a staged operand,
 // for the N tiles of 16 rows from `first` on (a multiple of 16 N, so that a
 // tile's number only adds to, or moves within, what the swizzle touches).
-template <typename T, bool kAcross, int R, int N>
+template <typename T, bool kAcross, int R, int S, int N>
 struct Fragments {
+  static constexpr int kHalves = S / 64;  // what one matrix instruction (f32: four) sums over
   // along: one place per half; the tiles lie 16 rows apart.  across: one place
   // per tile; the halves lie half a slab apart.
   int at[kAcross ? N : kHalves];
@@ -202,7 +203,7 @@ struct Fragments {
     if constexpr (!kAcross) {
 #pragma unroll
       for (int h = 0; h < kHalves; ++h)
-        at[h] = (first + i) * kSlabBytes + ((h * 4 + q) ^ along_swizzle(i)) * 16;
+        at[h] = (first + i) * S + ((h * 4 + q) ^ along_swizzle<S>(i)) * 16;
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -220,7 +221,7 @@ struct Fragments {
   }
   __device__ __forceinline__ u32x4 load(const char *lds, int n, int half) const {
     if constexpr (!kAcross) {
-      return *reinterpret_cast<const u32x4 *>(lds + at[half] + n * (16 * kSlabBytes));
+      return *reinterpret_cast<const u32x4 *>(lds + at[half] + n * (16 * S));
     } else if constexpr (sizeof(T) == 2) {
       const char *p = lds + at[n] + half * (32 * R * 2);
       const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -270,18 +271,19 @@ struct Accumulator {
 
 // acc += the products of a stage at `lds` (columns, then rows); kSums: sums +=
 // the summed index's total of the row operand's rows, per lane its share.
-template <typename T, bool kSums, int kCols, typename ColFragments, typename RowFragments>
+template <typename T, bool kSums, int kColBytes, int kCols, typename ColFragments,
+          typename RowFragments>
 __device__ __forceinline__ void multiply_stage(const char *lds, const ColFragments &cols,
                                                const RowFragments &rows, Accumulator<kCols> &acc,
                                                float (&sums)[Accumulator<kCols>::kB]) {
   using Acc = Accumulator<kCols>;
 #pragma unroll
-  for (int h = 0; h < kHalves; ++h) {
+  for (int h = 0; h < ColFragments::kHalves; ++h) {
     u32x4 a[Acc::kA], b[Acc::kB];
 #pragma unroll
     for (int i = 0; i < Acc::kA; ++i) a[i] = cols.load(lds, i, h);
 #pragma unroll
-    for (int i = 0; i < Acc::kB; ++i) b[i] = rows.load(lds + kCols * kSlabBytes, i, h);
+    for (int i = 0; i < Acc::kB; ++i) b[i] = rows.load(lds + kColBytes, i, h);
 #pragma unroll
     for (int i = 0; i < Acc::kA; ++i)
 #pragma unroll
@@ -298,29 +300,27 @@ __device__ __forceinline__ void multiply_stage(const char *lds, const ColFragmen
   }
 }
 
-// The product over `steps` stages.  Step i's stage is at lds + i % 2 *
-// kStageBytes.  stage(lds, step), the steps in order, puts a stage on its way
-// to LDS, or reads it (with null) for commit(lds) to write it there.
-template <bool kDirect, int kStageBytes, typename Stage, typename Commit, typename Multiply>
+// The product over `steps` stages, two of them in LDS (one where there is but
+// one).  stage(lds, step), the steps in order, puts a stage on its way to LDS,
+// or reads it for commit(lds) to write it there.  More stages ahead measured
+// slower: 16k x 1024 x 1024 bf16 forward and backward 254 us with two of 64 bytes,
+// 281 with three, 340 with four; blocks that share a CU hide more than depth.
+template <int kStageBytes, typename Stage, typename Commit, typename Multiply>
 __device__ __forceinline__ void pipeline(char *lds, int steps, Stage stage, Commit commit,
                                          Multiply multiply) {
-  // Step i, whose stage is the s-th in LDS; more: there is a step after it.
-  auto turn = [&](int i, int s, bool more) {
-    char *next = lds + (s ^ 1) * kStageBytes;
+  char *now = lds, *next = lds + kStageBytes;
+  stage(now, 0);
+  commit(now);
+  for (int i = 0; i < steps; ++i) {
     stage_barrier();
+    const bool more = i + 1 < steps;
     if (more) stage(next, i + 1);
-    multiply(lds + s * kStageBytes);
-    if (!kDirect && more) commit(next);
-  };
-  stage(lds, 0);
-  if (!kDirect) commit(lds);
-  int i = 0;
-  for (; i + 2 < steps; i += 2) {
-    turn(i, 0, true);
-    turn(i + 1, 1, true);
+    multiply(now);
+    if (more) commit(next);
+    char *t = now;
+    now = next;
+    next = t;
   }
-  if (i < steps) turn(i, 0, i + 1 < steps);
-  if (i + 1 < steps) turn(i + 1, 1, false);
 }
 
 // Four neighbouring columns of an output row of `width`, at any element.
@@ -348,7 +348,7 @@ __device__ __forceinline__ void store_four(T *row, int64_t col, int64_t width, c
 // (weight [m, k], summed over k) or with kBack the input's gradient (summed
 // over m).  Blocks of one row tile are neighbours, and neighbours share an XCD:
 // they read the same rows and weight.
-template <typename T, bool kBack, bool kVec, int kCols>
+template <typename T, bool kBack, bool kVec, int kCols, int S>
 __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void rows_kernel(const T *__restrict__ in, int64_t stride,
                                                         const T *__restrict__ weight,
                                                         const T *__restrict__ bias, Groups g,
@@ -357,10 +357,10 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
                                                         T *__restrict__ out) {
   extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [1 or 2][cols, rows]
   __shared__ int32_t s_row[kRows];
-  constexpr int kSlab = kSlabBytes / static_cast<int>(sizeof(T));
-  constexpr int kColBytes = kCols * kSlabBytes, kStage = (kCols + kRows) * kSlabBytes;
-  using RowSlot = Slot<T, false, kRows>;
-  using ColSlot = Slot<T, kBack, kCols>;
+  constexpr int kSlab = S / static_cast<int>(sizeof(T));
+  constexpr int kColBytes = kCols * S, kStage = (kCols + kRows) * S;
+  using RowSlot = Slot<T, false, kRows, S>;
+  using ColSlot = Slot<T, kBack, kCols, S>;
   const int64_t inner = kBack ? m : k, outer = kBack ? k : m;
   const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
   const int64_t j0 = static_cast<int64_t>(id % col_tiles) * kCols;
@@ -441,14 +441,14 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
         for (int i = 0; i < RowSlot::kCount; ++i) put_slot(lds + kColBytes, i, row_held[i]);
       }
     };
-    const Fragments<T, kBack, kCols, Accumulator<kCols>::kA> col_fragments(acc.first_col());
-    const Fragments<T, false, kRows, Accumulator<kCols>::kB> row_fragments(acc.first_row());
+    const Fragments<T, kBack, kCols, S, Accumulator<kCols>::kA> col_fragments(acc.first_col());
+    const Fragments<T, false, kRows, S, Accumulator<kCols>::kB> row_fragments(acc.first_row());
     float none[Accumulator<kCols>::kB];
-    pipeline<kVec, kStage>(s_stage, static_cast<int>((inner + kSlab - 1) / kSlab), stage, commit,
-                           [&](const char *lds) {
-                             multiply_stage<T, false>(lds, col_fragments, row_fragments, acc,
-                                                      none);
-                           });
+    pipeline<kStage>(
+        s_stage, static_cast<int>((inner + kSlab - 1) / kSlab), stage, commit,
+        [&](const char *lds) {
+          multiply_stage<T, false, kColBytes>(lds, col_fragments, row_fragments, acc, none);
+        });
   }
   // The biases of the lane's columns.
   f32x4 add[Accumulator<kCols>::kA] = {};
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
 // dW[m0 + row][k0 + col] (and db) of part `slot`: `per` rows of one group.  The
 // group's only part goes to v_weight and v_bias, others to parts
 // [slots][m][k] and bias_parts [slots][m].
-template <typename T, bool kVec, int kCols>
+template <typename T, bool kVec, int kCols, int S>
 __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ v_y, int64_t v_stride,
     Groups g, const int32_t *__restrict__ rows, int64_t k, int64_t m, uint32_t per,
@@ -483,11 +483,11 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
   extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [2][cols, rows]
   // The rows' numbers, two windows by turns.
   __shared__ __attribute__((aligned(16))) int32_t s_row[2][kWindow];
-  constexpr int kSlab = kSlabBytes / static_cast<int>(sizeof(T));
-  constexpr int kColBytes = kCols * kSlabBytes, kStage = (kCols + kRows) * kSlabBytes;
+  constexpr int kSlab = S / static_cast<int>(sizeof(T));
+  constexpr int kColBytes = kCols * S, kStage = (kCols + kRows) * S;
   static_assert(kWindow % kSlab == 0 && kWindow % kThreads == 0, "whole slabs and waves");
-  using RowSlot = Slot<T, true, kRows>;
-  using ColSlot = Slot<T, true, kCols>;
+  using RowSlot = Slot<T, true, kRows, S>;
+  using ColSlot = Slot<T, true, kCols, S>;
   const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x), tiles = m_tiles * k_tiles;
   const uint32_t slot = id / tiles, tile = id - slot * tiles;
   const int64_t m0 = static_cast<int64_t>(tile / k_tiles) * kRows;
@@ -564,16 +564,16 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
       for (int i = 0; i < RowSlot::kCount; ++i) put_slot(lds + kColBytes, i, row_held[i]);
     }
   };
-  const Fragments<T, true, kCols, Accumulator<kCols>::kA> col_fragments(acc.first_col());
-  const Fragments<T, true, kRows, Accumulator<kCols>::kB> row_fragments(acc.first_row());
+  const Fragments<T, true, kCols, S, Accumulator<kCols>::kA> col_fragments(acc.first_col());
+  const Fragments<T, true, kRows, S, Accumulator<kCols>::kB> row_fragments(acc.first_row());
   const int steps = (count + kSlab - 1) / kSlab;
   if (with_bias)
-    pipeline<kVec, kStage>(s_stage, steps, stage, commit, [&](const char *lds) {
-      multiply_stage<T, true>(lds, col_fragments, row_fragments, acc, sums);
+    pipeline<kStage>(s_stage, steps, stage, commit, [&](const char *lds) {
+      multiply_stage<T, true, kColBytes>(lds, col_fragments, row_fragments, acc, sums);
     });
   else
-    pipeline<kVec, kStage>(s_stage, steps, stage, commit, [&](const char *lds) {
-      multiply_stage<T, false>(lds, col_fragments, row_fragments, acc, sums);
+    pipeline<kStage>(s_stage, steps, stage, commit, [&](const char *lds) {
+      multiply_stage<T, false, kColBytes>(lds, col_fragments, row_fragments, acc, sums);
     });
   if (v_weight != nullptr) {
     float *p = parts + static_cast<int64_t>(slot) * m * k;
@@ -674,6 +674,13 @@ __global__ __launch_bounds__(kThreads) void add_parts_kernel(
 
 // ---------------------------------------------------------------- host ---
 
+// Bytes of the summed index per stage.  Operands read across and tiles of 128
+// columns take 64: four blocks share a CU instead of two.  16k x 1024 x 1024
+// bf16: forward 56 us with 128 bytes and 60 with 64, input gradient 80 and 70,
+// weights' gradient 142 and XXX; 500k x 64 x 64, where tiles have 64 columns:
+// weights' gradient 32 and 36.
+constexpr int slab_bytes(bool across, int cols) { return across && cols == 128 ? 64 : 128; }
+
 int64_t weight_tiles(int64_t k, int64_t m) {
   return ceil_div(m, kRows) * ceil_div(std::max<int64_t>(k, 1), kRows);
 }
@@ -725,10 +732,11 @@ int rows_launch(const T *in, int64_t stride, const T *weight, const T *bias, Gro
     set_error("grouped_matmul: too many tiles");
     return R2S_ERANGE;
   }
-  const int stages = inner * static_cast<int64_t>(sizeof(T)) > kSlabBytes ? 2 : 1;
-  rows_kernel<T, kBack, kVec, kCols>
+  constexpr int S = slab_bytes(kBack, kCols);
+  const int stages = inner * static_cast<int64_t>(sizeof(T)) > S ? 2 : 1;
+  rows_kernel<T, kBack, kVec, kCols, S>
       <<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads),
-         stages * (kCols + kRows) * kSlabBytes, stream>>>(
+         stages * (kCols + kRows) * S, stream>>>(
           in, stride, weight, bias, g, rows, k, m, static_cast<uint32_t>(col_tiles),
           out);
   return check_launch("grouped_matmul");
@@ -767,9 +775,10 @@ int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride,
     return R2S_ERANGE;
   }
   if (g.n > 0) {
-    weights_kernel<T, kVec, kCols>
+    constexpr int S = slab_bytes(true, kCols);
+    weights_kernel<T, kVec, kCols, S>
         <<<dim3(static_cast<uint32_t>(slots * m_tiles * k_tiles)), dim3(kThreads),
-           2 * (kCols + kRows) * kSlabBytes, stream>>>(
+           2 * (kCols + kRows) * S, stream>>>(
             x, x_stride, v_y, v_stride, g, rows, k, m, per, static_cast<uint32_t>(m_tiles),
             static_cast<uint32_t>(k_tiles), s.parts, s.bias_parts, v_weight, v_bias);
     R2S_RETURN_IF(check_launch("grouped_matmul_bwd weights"));
