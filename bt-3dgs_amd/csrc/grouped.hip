@@ -116,8 +116,12 @@ __device__ __forceinline__ void stage_barrier() {
 //           s ^ swizzle(c),
 // so that the lanes that read together hit different ones of the 64 banks
 // although LDS is filled in order by loads that go straight there.
-template <int S>
+// kRun: the tile's rows are taken kRun apart, four at a time (see Accumulator);
+// 0: in order.
+template <int S, int kRun>
 __device__ __forceinline__ int along_swizzle(int r) {
+  static_assert(kRun == 0 || S == 128, "runs of 128-byte rows");
+  if constexpr (kRun > 0) return (r & 3) | ((r / kRun) & 1) << 2;
   return S == 128 ? r & 7 : (r >> 1) & 3;
 }
 template <typename T, int R>
@@ -134,7 +138,7 @@ __device__ __forceinline__ int across_swizzle(int c) {
 }
 
 // The slots that a thread fills: q = i kThreads + threadIdx.x.
-template <typename T, bool kAcross, int R, int S>
+template <typename T, bool kAcross, int R, int S, int kRun = 0>
 struct Slot {
   static constexpr int kSlots = S / 16;
   static constexpr int kCount = R * kSlots / kThreads;
@@ -149,7 +153,7 @@ struct Slot {
       offset = ((q % kRow) ^ across_swizzle<T, R>(index)) * kPer;
     } else {
       index = q / kSlots;
-      offset = ((q % kSlots) ^ along_swizzle<S>(index)) * kPer;
+      offset = ((q % kSlots) ^ along_swizzle<S, kRun>(index)) * kPer;
     }
   }
 };
@@ -190,30 +194,35 @@ __device__ __forceinline__ void put_slot(char *lds, int i, u32x4 x) {
 }
 
 // Where this lane reads its 16 bytes of the summed index in a staged operand,
-// for the N tiles of 16 rows from `first` on (a multiple of 16 N, so that a
-// tile's number only adds to, or moves within, what the swizzle touches).
-template <typename T, bool kAcross, int R, int S, int N>
+// for N tiles of 16 rows from `first` on: row n 16 + i of lane i (mod 16), or
+// with kRun = 4 N row (i / 4) kRun + 4 n + i % 4.
+template <typename T, bool kAcross, int R, int S, int N, int kRun = 0>
 struct Fragments {
+  static_assert(kRun == 0 || kRun == 4 * N, "a run per four lanes");
   static constexpr int kHalves = S / 64;  // what one matrix instruction (f32: four) sums over
-  // along: one place per half; the tiles lie 16 rows apart.  across: one place
-  // per tile; the halves lie half a slab apart.
+  // along: one place per half; the tiles lie 16 (or 4) rows apart, which no
+  // swizzle notices.  across: one place per tile; the halves lie half a slab
+  // apart.
   int at[kAcross ? N : kHalves];
   __device__ __forceinline__ explicit Fragments(int first) {
     const int lane = static_cast<int>(lane_id()), i = lane % 16, q = lane / 16;
     if constexpr (!kAcross) {
+      const int r = first + (kRun > 0 ? i / 4 * kRun + i % 4 : i);
 #pragma unroll
       for (int h = 0; h < kHalves; ++h)
-        at[h] = (first + i) * S + ((h * 4 + q) ^ along_swizzle<S>(i)) * 16;
+        at[h] = r * S + ((h * 4 + q) ^ along_swizzle<S, kRun>(r)) * 16;
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         if constexpr (sizeof(T) == 2) {
-          // Sixteen lanes read 4 summed indices of 16 neighbours, 8 bytes each,
-          // and get 4 indices of one neighbour each.
-          const int c = q * 8 + i / 4, slot = (first + n * 16) / 8 + i % 4 / 2;
-          at[n] = c * (R * 2) + (slot ^ across_swizzle<T, R>(c)) * 16 + i % 2 * 8;
+          // Sixteen lanes read 4 summed indices of 4 times 4 neighbours, 8
+          // bytes each, and get 4 indices of one row each.
+          const int c = q * 8 + i / 4;
+          const int r = first + (kRun > 0 ? i % 4 * kRun + n * 4 : n * 16 + i % 4 * 4);
+          at[n] = c * (R * 2) + ((r / 8) ^ across_swizzle<T, R>(c)) * 16 + r / 4 % 2 * 8;
         } else {
-          const int c = q * 4, r = first + n * 16 + i;
+          const int c = q * 4;
+          const int r = first + (kRun > 0 ? i / 4 * kRun + n * 4 + i % 4 : n * 16 + i);
           at[n] = c * (R * 4) + ((r / 4) ^ across_swizzle<T, R>(c)) * 16 + r % 4 * 4;
         }
       }
@@ -221,7 +230,7 @@ struct Fragments {
   }
   __device__ __forceinline__ u32x4 load(const char *lds, int n, int half) const {
     if constexpr (!kAcross) {
-      return *reinterpret_cast<const u32x4 *>(lds + at[half] + n * (16 * S));
+      return *reinterpret_cast<const u32x4 *>(lds + at[half] + n * ((kRun > 0 ? 4 : 16) * S));
     } else if constexpr (sizeof(T) == 2) {
       const char *p = lds + at[n] + half * (32 * R * 2);
       const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -243,10 +252,13 @@ struct Fragments {
   }
 };
 
-// A wave's part of the tile: 64 rows by kCols / 2 columns.
-template <int kCols>
+// A wave's part of the tile: 64 rows by kCols / 2 columns, as tiles of 16 x 16
+// of which a lane has four neighbouring columns of one row.  With kRuns its
+// tiles' columns are neighbours too, kRun in all, so that it stores them by 16
+// bytes: 500k x 64 x 64 bf16 forward XXX us, and 40 us with 8 bytes per tile.
+template <int kCols, bool kRuns>
 struct Accumulator {
-  static constexpr int kA = kCols / 32, kB = kRows / 32;
+  static constexpr int kA = kCols / 32, kB = kRows / 32, kRun = kRuns ? 4 * kA : 0;
   f32x4 v[kA][kB];
   __device__ __forceinline__ Accumulator() {
 #pragma unroll
@@ -260,23 +272,23 @@ struct Accumulator {
   static __device__ __forceinline__ int first_row() {
     return static_cast<int>(wave_index()) / 2 * (kRows / 2);
   }
-  // The tile row, and the first of the four columns, that a lane has of v[a][b].
+  // The tile's row, and the first of its four columns, that a lane has in v[a][b].
   static __device__ __forceinline__ int row(int b) {
     return first_row() + b * 16 + static_cast<int>(lane_id()) % 16;
   }
   static __device__ __forceinline__ int column(int a) {
-    return first_col() + a * 16 + static_cast<int>(lane_id()) / 16 * 4;
+    const int q = static_cast<int>(lane_id()) / 16;
+    return first_col() + (kRuns ? q * kRun + a * 4 : a * 16 + q * 4);
   }
 };
 
 // acc += the products of a stage at `lds` (columns, then rows); kSums: sums +=
 // the summed index's total of the row operand's rows, per lane its share.
-template <typename T, bool kSums, int kColBytes, int kCols, typename ColFragments,
+template <typename T, bool kSums, int kColBytes, typename Acc, typename ColFragments,
           typename RowFragments>
 __device__ __forceinline__ void multiply_stage(const char *lds, const ColFragments &cols,
-                                               const RowFragments &rows, Accumulator<kCols> &acc,
-                                               float (&sums)[Accumulator<kCols>::kB]) {
-  using Acc = Accumulator<kCols>;
+                                               const RowFragments &rows, Acc &acc,
+                                               float (&sums)[Acc::kB]) {
 #pragma unroll
   for (int h = 0; h < ColFragments::kHalves; ++h) {
     u32x4 a[Acc::kA], b[Acc::kB];
@@ -323,22 +335,27 @@ __device__ __forceinline__ void pipeline(char *lds, int steps, Stage stage, Comm
   }
 }
 
-// Four neighbouring columns of an output row of `width`, at any element.
-template <typename T>
-struct __attribute__((packed)) UnalignedFour {
-  T v[4];
+// N neighbouring columns of an output row of `width`, at any element.
+template <typename T, int N>
+struct __attribute__((packed)) UnalignedRun {
+  T v[N];
 };
-template <typename T>
-__device__ __forceinline__ void store_four(T *row, int64_t col, int64_t width, const f32x4 &v) {
-  if (col + 4 <= width) {
-    UnalignedFour<T> x;
+template <typename T, int N>
+__device__ __forceinline__ void store_run(T *row, int64_t col, int64_t width,
+                                          const f32x4 (&v)[N / 4]) {
+  if (col + N <= width) {
+    constexpr int kMost = 16 / static_cast<int>(sizeof(T)), kStore = N < kMost ? N : kMost;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x.v[j] = static_cast<T>(v[j]);
-    *reinterpret_cast<UnalignedFour<T> *>(row + col) = x;
+    for (int i = 0; i < N; i += kStore) {
+      UnalignedRun<T, kStore> x;
+#pragma unroll
+      for (int j = 0; j < kStore; ++j) x.v[j] = static_cast<T>(v[(i + j) / 4][(i + j) % 4]);
+      *reinterpret_cast<UnalignedRun<T, kStore> *>(row + col + i) = x;
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j < width) row[col + j] = static_cast<T>(v[j]);
+    for (int j = 0; j < N; ++j)
+      if (col + j < width) row[col + j] = static_cast<T>(v[j / 4][j % 4]);
   }
 }
 
@@ -359,8 +376,9 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
   __shared__ int32_t s_row[kRows];
   constexpr int kSlab = S / static_cast<int>(sizeof(T));
   constexpr int kColBytes = kCols * S, kStage = (kCols + kRows) * S;
+  using Acc = Accumulator<kCols, true>;
   using RowSlot = Slot<T, false, kRows, S>;
-  using ColSlot = Slot<T, kBack, kCols, S>;
+  using ColSlot = Slot<T, kBack, kCols, S, kBack ? 0 : Acc::kRun>;
   const int64_t inner = kBack ? m : k, outer = kBack ? k : m;
   const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
   const int64_t j0 = static_cast<int64_t>(id % col_tiles) * kCols;
@@ -378,7 +396,7 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
     s_row[threadIdx.x] = static_cast<int32_t>(r);
   }
   __syncthreads();
-  Accumulator<kCols> acc;
+  Acc acc;
   if (e < g.count && inner > 0) {
     const T *w = weight + static_cast<int64_t>(e) * m * k;
     // Addresses of the thread's slots in the next stage.  Rows and columns past
@@ -441,9 +459,9 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
         for (int i = 0; i < RowSlot::kCount; ++i) put_slot(lds + kColBytes, i, row_held[i]);
       }
     };
-    const Fragments<T, kBack, kCols, S, Accumulator<kCols>::kA> col_fragments(acc.first_col());
-    const Fragments<T, false, kRows, S, Accumulator<kCols>::kB> row_fragments(acc.first_row());
-    float none[Accumulator<kCols>::kB];
+    const Fragments<T, kBack, kCols, S, Acc::kA, Acc::kRun> col_fragments(acc.first_col());
+    const Fragments<T, false, kRows, S, Acc::kB> row_fragments(acc.first_row());
+    float none[Acc::kB];
     pipeline<kStage>(
         s_stage, static_cast<int>((inner + kSlab - 1) / kSlab), stage, commit,
         [&](const char *lds) {
@@ -451,23 +469,23 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
         });
   }
   // The biases of the lane's columns.
-  f32x4 add[Accumulator<kCols>::kA] = {};
+  f32x4 add[Acc::kA] = {};
   if (!kBack && bias != nullptr && e < g.count) {
     const T *b = bias + static_cast<int64_t>(e) * m;
 #pragma unroll
-    for (int a = 0; a < Accumulator<kCols>::kA; ++a)
+    for (int a = 0; a < Acc::kA; ++a)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         add[a][i] = static_cast<float>(b[min(j0 + acc.column(a) + i, m - 1)]);
   }
 #pragma unroll
-  for (int b = 0; b < Accumulator<kCols>::kB; ++b) {
+  for (int b = 0; b < Acc::kB; ++b) {
     const int64_t at = s_row[acc.row(b)];
     if (at < 0) continue;
+    f32x4 run[Acc::kA];
 #pragma unroll
-    for (int a = 0; a < Accumulator<kCols>::kA; ++a)
-      store_four<T>(out + at * outer, j0 + acc.column(a), outer,
-                    acc.v[a][b] + add[a]);
+    for (int a = 0; a < Acc::kA; ++a) run[a] = acc.v[a][b] + add[a];
+    store_run<T, Acc::kRun>(out + at * outer, j0 + acc.column(0), outer, run);
   }
 }
 
@@ -486,6 +504,7 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
   constexpr int kSlab = S / static_cast<int>(sizeof(T));
   constexpr int kColBytes = kCols * S, kStage = (kCols + kRows) * S;
   static_assert(kWindow % kSlab == 0 && kWindow % kThreads == 0, "whole slabs and waves");
+  using Acc = Accumulator<kCols, false>;
   using RowSlot = Slot<T, true, kRows, S>;
   using ColSlot = Slot<T, true, kCols, S>;
   const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x), tiles = m_tiles * k_tiles;
@@ -512,9 +531,9 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
   };
   fetch_rows(0);
   stage_barrier();
-  Accumulator<kCols> acc;
-  float sums[Accumulator<kCols>::kB] = {};
-  const bool with_bias = v_bias != nullptr && k0 == 0 && Accumulator<kCols>::first_col() == 0;
+  Acc acc;
+  float sums[Acc::kB] = {};
+  const bool with_bias = v_bias != nullptr && k0 == 0 && Acc::first_col() == 0;
   // The row of the part's place c < count.
   auto row_of = [&](int c) -> int64_t {
     if (rows == nullptr) return r0 + c;
@@ -564,8 +583,8 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
       for (int i = 0; i < RowSlot::kCount; ++i) put_slot(lds + kColBytes, i, row_held[i]);
     }
   };
-  const Fragments<T, true, kCols, S, Accumulator<kCols>::kA> col_fragments(acc.first_col());
-  const Fragments<T, true, kRows, S, Accumulator<kCols>::kB> row_fragments(acc.first_row());
+  const Fragments<T, true, kCols, S, Acc::kA> col_fragments(acc.first_col());
+  const Fragments<T, true, kRows, S, Acc::kB> row_fragments(acc.first_row());
   const int steps = (count + kSlab - 1) / kSlab;
   if (with_bias)
     pipeline<kStage>(s_stage, steps, stage, commit, [&](const char *lds) {
@@ -579,28 +598,28 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
     float *p = parts + static_cast<int64_t>(slot) * m * k;
     T *w = v_weight + static_cast<int64_t>(e) * m * k;
 #pragma unroll
-    for (int b = 0; b < Accumulator<kCols>::kB; ++b) {
+    for (int b = 0; b < Acc::kB; ++b) {
       const int64_t r = m0 + acc.row(b);
       if (r >= m) continue;
 #pragma unroll
-      for (int a = 0; a < Accumulator<kCols>::kA; ++a) {
+      for (int a = 0; a < Acc::kA; ++a) {
         const int64_t c = k0 + acc.column(a);
         if (only)
-          store_four<T>(w + r * k, c, k, acc.v[a][b]);
+          store_run<T, 4>(w + r * k, c, k, {acc.v[a][b]});
         else
-          store_four<float>(p + r * k, c, k, acc.v[a][b]);
+          store_run<float, 4>(p + r * k, c, k, {acc.v[a][b]});
       }
     }
   }
   if (with_bias) {
     const int lane = static_cast<int>(lane_id());
 #pragma unroll
-    for (int j = 0; j < Accumulator<kCols>::kB; ++j) {
+    for (int j = 0; j < Acc::kB; ++j) {
       // The four lanes of a row hold the slab's quarters.
       float sum = sums[j];
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      const int64_t r = m0 + Accumulator<kCols>::first_row() + j * 16 + lane % 16;
+      const int64_t r = m0 + Acc::first_row() + j * 16 + lane % 16;
       if (lane < 16 && r < m) {
         if (only)
           v_bias[static_cast<int64_t>(e) * m + r] = static_cast<T>(sum);
@@ -689,9 +708,10 @@ int64_t weight_tiles(int64_t k, int64_t m) {
 // and no more, since every part of a group past its first is a copy of the
 // weight to write and add.
 uint32_t rows_per_part(int64_t n, int64_t k, int64_t m) {
-  const int64_t even = ceil_div(n * weight_tiles(k, m), 768);
+  const int64_t tiles = weight_tiles(k, m);
+  const int64_t even = ceil_div(n * tiles, tiles > 8 ? 1152 : 768);
   return static_cast<uint32_t>(
-      std::min<int64_t>(std::max<int64_t>(align_up(even, 64), 256), 4096));
+      std::min<int64_t>(std::max<int64_t>(align_up(even, 64), 128), 4096));
 }
 
 // Blocks of the weights' gradient along the rows, at most.
