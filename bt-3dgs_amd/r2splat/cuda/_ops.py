@@ -2016,7 +2016,7 @@ def _scan_input(t: Tensor, name: str, x: Tensor, n: int):
     d = x.shape[-1]
     # Rows of 16-bit elements of an even width are read in pairs.
     align = 4 if x.element_size() == 2 and d % 2 == 0 else 1
-    return _rows_2d(t.reshape(n, d), align)
+    return _rows_2d(t if t.dim() == 2 else t.reshape(n, d), align)
 
 
 def _scan_state(t: Optional[Tensor], name: str, x: Tensor, sequences: int) -> Optional[Tensor]:
@@ -2059,6 +2059,29 @@ def gated_scan_fwd(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
               sequences, length, n, d, code, bool(reverse), _ptr(y), _ptr(final), _ptr(kept),
               _ptr(ws), need, _stream(dev))
     return y, final, kept
+
+
+def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tuple[Tensor, Tensor]:
+    """(y, next state) after one more token of each of B sequences: x, gate
+    [B, D], state [B, D] float32.  gated_scan_fwd of [B, 1, D] with less around
+    it: this call is bound by its host time."""
+    _check_latent(x, "x")
+    code = _latent_type(x, "gated_scan_step")
+    if x.dim() != 2:
+        _fail("x must be [B, D], got shape ", tuple(x.shape))
+    b, d = x.shape
+    xr, xs = _scan_input(x, "x", x, b)
+    gr, gs = _scan_input(gate, "gate", x, b)
+    state = _scan_state(state, "state", x, b)
+    if state is None:
+        _fail("state must be given")
+    dev = x.device
+    with _on(dev):
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        final = torch.empty_like(state)
+        _call("r2s_gated_scan_fwd", _ptr(xr), xs, _ptr(gr), gs, _ptr(state), None, b, 1, b, d,
+              code, 0, _ptr(y), _ptr(final), None, None, 0, _stream(dev))
+    return y, final
 
 
 def gated_scan_bwd(x: Tensor, gate: Tensor, initial: Optional[Tensor],

@@ -61,6 +61,7 @@ group_rows = _make_cuda_func("group_rows")
 embedding_fwd = _make_cuda_func("embedding_fwd")
 embedding_bwd = _make_cuda_func("embedding_bwd")
 gated_scan_fwd = _make_cuda_func("gated_scan_fwd")
+gated_scan_step = _make_cuda_func("gated_scan_step")
 gated_scan_bwd = _make_cuda_func("gated_scan_bwd")
 grouped_matmul_fwd = _make_cuda_func("grouped_matmul_fwd")
 grouped_matmul_bwd = _make_cuda_func("grouped_matmul_bwd")
