@@ -633,3 +633,67 @@ def test_refusals():
     for call, message in bad:
         with pytest.raises(RuntimeError, match=message):
             call()
+
+
+# ------------------------------------------------------------ the decoder --
+
+
+def test_decoder_fits_a_projection():
+    """Operators, rasterizer, explicit backward and Adam in one loop: a decoder
+    at its start leaves its base alone, and training brings its image closer to
+    another scene's."""
+    from r2splat import geometry, optim, scenes
+    from r2splat.latent import LatentDecoder
+    from r2splat.ops import explicit
+
+    n, levels, width = 1500, 5, 24
+    g = _gen(0)
+    base = scenes.random_gaussians(n, g, -3.4, 0.3, extent=0.6).to(DEV)
+    other = scenes.random_gaussians(n, g, -3.2, 0.3, extent=0.6).to(DEV)
+    views, Ks = (t.to(DEV) for t in geometry.cone_beam_views([0.4], 48))
+    codes = torch.randint(-1, 64, (n,), generator=g).to(DEV)
+    rows, offsets = latent.group_rows(torch.randint(0, levels, (n,), generator=g).to(DEV), levels)
+    decoder = LatentDecoder(64, levels, width, g).to(DEV)
+    optimizer = optim.Adam(decoder.parameters(), lr=1e-2)
+
+    def render(means, quats, scales, opacities):
+        state = explicit.prepare_explicit_gaussians(quats, scales, opacities, scale_min=5e-4,
+                                                    scale_max=1.0)
+        return state, explicit.explicit_rasterize(state, means, views, Ks, img_w=48, img_h=48,
+                                                  tile_size=16, eps2d=1e-8, radius_clip=3.0,
+                                                  absgrad=True).image
+
+    target = render(other.means, other.quats, other.raw_scales, other.raw_opacities)[1].detach()
+    losses = []
+    for _ in range(12):
+        optimizer.zero_grad()
+        raw = decoder(codes, rows, offsets)
+        if not losses:
+            assert raw.abs().max() == 0  # zero weights: the base itself
+        leaves = decoder.leaves(base, raw)
+        state, image = render(*leaves)
+        loss = (image - target).square().mean()
+        loss.backward()
+        explicit.explicit_backward(state, *leaves)
+        decoder.backward(raw, *leaves)
+        optimizer.step()
+        losses.append(loss.item())
+    assert all(torch.isfinite(p).all() for p in decoder.parameters())
+    assert losses[-1] < 0.9 * losses[0], losses
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scan_step_equals_its_general_form(dtype):
+    g = _gen(3)
+    x, gate = (_randn(g, 37, 50, dtype=dtype).to(DEV) for _ in range(2))
+    state = _randn(g, 37, 50).to(DEV)
+    wide = torch.cat([x, gate], 1)
+    y, final = latent.gated_scan_step(wide[:, :50], wide[:, 50:], state)
+    e_y, e_final, _ = W.gated_scan_fwd(x[:, None], gate[:, None], state)
+    assert torch.equal(y, e_y[:, 0]) and torch.equal(final, e_final)
+    x.requires_grad_(True)
+    latent.gated_scan_step(x, gate, state)[1].sum().backward()
+    assert torch.allclose(x.grad.float(), torch.sigmoid(-gate.float()).to(dtype).float(),
+                          rtol=2 * ROUND[dtype], atol=1e-6)
+    with pytest.raises(RuntimeError, match="state must be"):
+        W.gated_scan_step(x.detach(), gate, state[:3])
