@@ -17,11 +17,12 @@
 // strip's map, then, with the state that enters the strip, to write the
 // states.  No step of either walk waits for another lane.
 //
-//   resident   a block's strips hold whole sequences (one equal sequence, or
-//              everything there is): the maps meet in LDS and both walks are
-//              one launch; the second finds its tokens in cache.
+//   rounds     a block holds whole sequences (one equal sequence, or
+//              everything there is) and walks them 8 tokens per group at a
+//              time: tokens are read once, everything is one launch.
 //   packed     a launch composes the strips' maps, one adds them up along the
-//              axis, one walks again: for few long sequences and ragged ones.
+//              axis, one walks again: for few long sequences and ragged ones,
+//              whose lengths only the device knows.
 //   own        short equal sequences: a strip is a sequence, one walk.
 //
 // The gradient runs the other way.  With F_t the gradient that reaches the
@@ -44,8 +45,8 @@
 namespace r2s {
 namespace {
 
-constexpr int kThreads = 256;    // of a packed block
-constexpr int kResident = 1024;  // of a resident block, at most
+constexpr int kThreads = 256;  // of a block of strips
+constexpr int kRoundThreads = 512;  // of a block that walks in rounds, at most
 constexpr int kChunk = 8;        // tokens loaded together, and between kept states
 
 // What every kernel of a call needs to know of its tokens.  Tokens and
@@ -560,7 +561,7 @@ __device__ __forceinline__ void walk_backward(const Rows<T, V> &xr, const Rows<T
         for (int v = 0; v < V; ++v) {
           float a, b;
           gate_pair(R::value(g[k], v), a, b);
-          s_before[(k * V + v) * blockDim.x + threadIdx.x] = h[v];
+          s_before[(k * V + v) * kThreads + threadIdx.x] = h[v];
           h[v] = applied<true>(a, h[v], scaled<true>(b, R::value(x[k], v)));
         }
       }
@@ -576,7 +577,7 @@ __device__ __forceinline__ void walk_backward(const Rows<T, V> &xr, const Rows<T
           float a, b;
           gate_pair(R::value(g[k], v), a, b);
           const float gk = R::value(d[k], v) + f[v], vx = scaled<true>(b, gk);
-          const float before = s_before[(k * V + v) * blockDim.x + threadIdx.x];
+          const float before = s_before[(k * V + v) * kThreads + threadIdx.x];
           const float vg = a * (vx * (before - R::value(x[k], v)));
           dx.v[v] = static_cast<T>(vx);
           dg.v[v] = static_cast<T>(a == 0.0f || b == 0.0f ? 0.0f : vg);
@@ -605,19 +606,6 @@ __device__ __forceinline__ void put_map(float *s_map, const float (&p)[V], const
   for (int v = 0; v < V; ++v) {
     s_map[(threadIdx.x * V + v) * 2] = p[v];
     s_map[(threadIdx.x * V + v) * 2 + 1] = u[v];
-  }
-}
-
-// h through the maps of the strips before this one (after it with kDown).
-template <int V, bool kDown>
-__device__ __forceinline__ void through_maps(const float *s_map, const Tokens &c, const Place &at,
-                                             int groups, float (&h)[V]) {
-  const int count = kDown ? groups - 1 - at.group : at.group;
-  for (int i = 0; i < count; ++i) {
-    const int q = kDown ? groups - 1 - i : i;
-    const float *m = s_map + ((q << c.lane_bits) + static_cast<int>(at.lane)) * V * 2;
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = applied<true>(m[v * 2], h[v], m[v * 2 + 1]);
   }
 }
 
@@ -775,33 +763,26 @@ __device__ __forceinline__ void enter_strip(const float *strips, const float *ca
 }
 
 // How a walk gets the state that enters its strip.
-enum Mode { kPacked, kResidentMode, kOwn };
+enum Mode { kPacked, kRounds, kOwn };
 
 // kept [strips][steps / kChunk][width].
-template <typename T, int V, int kMode, int kBlock>
-__global__ __launch_bounds__(kBlock) void scan_fwd_kernel(
+template <typename T, int V, int kMode>
+__global__ __launch_bounds__(kThreads) void scan_fwd_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
     const float *__restrict__ initial, Tokens c, uint32_t slices,
     const float *__restrict__ strips, const float *__restrict__ carries, float *__restrict__ kept,
     T *__restrict__ y, float *__restrict__ final) {
-  extern __shared__ float s_map[];
   int64_t block;
   uint32_t slice;
   block_and_slice(slices, block, slice);
-  const int groups = static_cast<int>(blockDim.x >> c.lane_bits);
+  const int groups = kThreads >> c.lane_bits;
   const Place at(c, V, block, slice);
   const Rows<T, V> xr(x, x_stride, c, at, block), gr(gate, g_stride, c, at, block);
   const Rows<T, V> yr(y, c.width, c, at, block);
   float h[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = 0.0f;
-  if constexpr (kMode == kResidentMode) {
-    float p[V], u[V];
-    compose_forward<T, V>(xr, gr, initial, c, at, p, u);
-    put_map<V>(s_map, p, u);
-    __syncthreads();
-    through_maps<V, false>(s_map, c, at, groups, h);
-  } else if constexpr (kMode == kPacked) {
+  if constexpr (kMode == kPacked) {
     enter_strip<V, false>(strips, carries, c, at, groups, block, h);
   }
   if (kept != nullptr)
@@ -809,19 +790,19 @@ __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(
   walk_forward<T, V>(xr, gr, yr, initial, c, at, kept, final, h);
 }
 
-template <typename T, int V, int kMode, int kBlock>
-__global__ __launch_bounds__(kBlock) void scan_bwd_kernel(
+template <typename T, int V, int kMode>
+__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
     const float *__restrict__ initial, const T *__restrict__ v_y, int64_t v_stride,
     const float *__restrict__ v_final, Tokens c, uint32_t slices,
     const float *__restrict__ strips, const float *__restrict__ carries,
     const float *__restrict__ kept, T *__restrict__ v_x, T *__restrict__ v_gate,
     float *__restrict__ v_initial) {
-  extern __shared__ float s_map[];
+  __shared__ float s_before[kThreads * V * kChunk];
   int64_t block;
   uint32_t slice;
   block_and_slice(slices, block, slice);
-  const int groups = static_cast<int>(blockDim.x >> c.lane_bits);
+  const int groups = kThreads >> c.lane_bits;
   const Place at(c, V, block, slice);
   const Rows<T, V> xr(x, x_stride, c, at, block), gr(gate, g_stride, c, at, block);
   const Rows<T, V> vr(v_y, v_stride, c, at, block);
@@ -829,18 +810,437 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(
   float f[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) f[v] = 0.0f;
-  if constexpr (kMode == kResidentMode) {
-    float p[V], u[V];
-    compose_backward<T, V>(gr, vr, v_final, c, at, p, u);
-    put_map<V>(s_map, p, u);
-    __syncthreads();
-    through_maps<V, true>(s_map, c, at, groups, f);
-  } else if constexpr (kMode == kPacked) {
+  if constexpr (kMode == kPacked) {
     enter_strip<V, true>(strips, carries, c, at, groups, block, f);
   }
   kept += (block * groups + at.group) * (c.steps / kChunk) * c.width + at.col;
-  walk_backward<T, V>(xr, gr, vr, dxr, dgr, initial, v_final, c, at, kept, v_initial,
-                      s_map + (kMode == kResidentMode ? blockDim.x * V * 2 : 0), f);
+  walk_backward<T, V>(xr, gr, vr, dxr, dgr, initial, v_final, c, at, kept, v_initial, s_before,
+                      f);
+}
+
+// ------------------------------------------------- whole sequences at once ---
+
+// A block whose tokens are whole sequences walks them in rounds: its groups
+// take kChunk tokens each, side by side, and the state that leaves the last one
+// enters the next round.  So x and gate are read once, and a round's words are
+// on their way while the one before is worked on.  32 x 1024 x 1024 bf16 takes
+// 55 us forward (201 MB, 3.7 TB/s) and 77 us back (344 MB, 4.5 TB/s); with one
+// block of 8 waves per CU and 64 bytes of a row (8 x 4096 x 1024) 70 and 96 us,
+// where a round's chain of waits bounds it: the vector units are busy a third
+// of the time.  The packed form takes 185 us for the latter, its second reading
+// of the tokens included.
+
+// What a block's round leaves in LDS: the maps of its waves' tokens.
+template <int V>
+struct Rounds {
+  float map[2][kRoundThreads / 64][32][2 * V];
+};
+
+// Chunks of a block of whole sequences.
+__device__ __forceinline__ int64_t block_chunks(const Tokens &c) {
+  return (c.block + kChunk - 1) / kChunk;
+}
+
+// The lane's place reaches to the block's end; the block's tokens.
+__device__ __forceinline__ int32_t round_place(const Tokens &c, int64_t block, Place &at) {
+  const int64_t end = min((block + 1) * c.block, c.n);
+  at.hi = static_cast<int32_t>(end);
+  return static_cast<int32_t>(end - block * c.block);
+}
+
+// A round's words on their way to LDS, each lane's to a place of its own: held
+// in registers until the next round, the compiler waits for them where paths
+// meet.  words [k][threads] from `at` on; a lane without a token keeps what is
+// there.
+template <typename R>
+__device__ __forceinline__ void fetch_chunk(const R &r, int32_t j, int32_t count,
+                                            uint32_t *words) {
+  typename R::Global s = r.step(j);
+  const uint32_t o = r.lane_offset();
+  words += wave_index() * 64;
+  const bool all = __all(j + kChunk <= count);
+#pragma unroll
+  for (int k = 0; k < kChunk; ++k) {
+    if (all || j + k < count) {
+      const auto *from = (const __attribute__((address_space(1))) void *)(s + o);
+      auto *to = (__attribute__((address_space(3))) void *)(words + k * kRoundThreads);
+      if constexpr (sizeof(typename R::Word) == 4)
+        __builtin_amdgcn_global_load_lds(from, to, 4, 0, 0);
+      else
+        __builtin_amdgcn_global_load_lds(from, to, 2, 0, 0);
+    }
+    s += r.pitch;
+    asm("" : "+s"(s));
+  }
+}
+template <typename Word>
+__device__ __forceinline__ void take_chunk(const uint32_t *words, Word (&x)[kChunk]) {
+#pragma unroll
+  for (int k = 0; k < kChunk; ++k) x[k] = static_cast<Word>(words[k * kRoundThreads + threadIdx.x]);
+}
+// The words fetched for this round have arrived; those taken may be replaced.
+__device__ __forceinline__ void words_arrived() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ void words_taken() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// From the maps of the lanes' chunks to the state that enters each: through
+// the wave's groups by lane shifts and through the waves in LDS, from `carry`,
+// the state that enters the round, which becomes the one that leaves it.
+// Backwards with kDown.
+template <int V, bool kDown>
+__device__ __forceinline__ void enter_chunk(Rounds<V> &s, int turn, const Tokens &c,
+                                            const Place &at, float (&p)[V], float (&u)[V],
+                                            float (&carry)[V], float (&h)[V]) {
+  const int lanes = 1 << c.lane_bits, id = static_cast<int>(lane_id());
+  const int ahead = kDown ? 63 - id : id;  // lanes before this one
+  for (int off = lanes; off < 64; off *= 2) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float pb = kDown ? __shfl_down(p[v], off, 64) : __shfl_up(p[v], off, 64);
+      const float ub = kDown ? __shfl_down(u[v], off, 64) : __shfl_up(u[v], off, 64);
+      if (ahead >= off) {
+        u[v] = applied<true>(p[v], ub, u[v]);
+        p[v] *= pb;
+      }
+    }
+  }
+  const int wave = static_cast<int>(wave_index()), waves = static_cast<int>(blockDim.x / 64);
+  if (ahead >= 64 - lanes) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      s.map[turn][wave][at.lane][2 * v] = p[v];
+      s.map[turn][wave][at.lane][2 * v + 1] = u[v];
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    p[v] = kDown ? __shfl_down(p[v], lanes, 64) : __shfl_up(p[v], lanes, 64);
+    u[v] = kDown ? __shfl_down(u[v], lanes, 64) : __shfl_up(u[v], lanes, 64);
+    if (ahead < lanes) p[v] = 1.0f, u[v] = 0.0f;
+  }
+  // Not __syncthreads, which would also wait for the words on their way.
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll 4
+  for (int i = 0; i < waves; ++i) {
+    const int w = kDown ? waves - 1 - i : i;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (w == wave) h[v] = carry[v];
+      carry[v] = applied<true>(s.map[turn][w][at.lane][2 * v], carry[v],
+                               s.map[turn][w][at.lane][2 * v + 1]);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = applied<true>(p[v], h[v], u[v]);
+}
+
+// kept [blocks][chunks of a block][width].
+template <typename T, int V>
+__global__ __launch_bounds__(kRoundThreads) void scan_fwd_rounds_kernel(
+    const T *__restrict__ tokens, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
+    const float *__restrict__ initial, Tokens c, uint32_t slices, float *__restrict__ kept,
+    T *__restrict__ y, float *__restrict__ final) {
+  __shared__ Rounds<V> s_rounds;
+  __shared__ uint32_t s_words[2 * kChunk * kRoundThreads];  // x, gate
+  int64_t block;
+  uint32_t slice;
+  block_and_slice(slices, block, slice);
+  Place at(c, V, block, slice);
+  const int32_t total = round_place(c, block, at), count = at.hi - at.lo;
+  const int32_t span = static_cast<int32_t>(blockDim.x >> c.lane_bits) * kChunk;
+  using R = Rows<T, V>;
+  const R xr(tokens, x_stride, c, at, block), gr(gate, g_stride, c, at, block);
+  const R yr(y, c.width, c, at, block);
+  if (kept != nullptr)
+    kept += (block * block_chunks(c) + at.group) * c.width + at.col;
+  Cursor q;
+  q.seek(c, at.lo, at.lo < at.hi);
+  float carry[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) carry[v] = 0.0f;
+  fetch_chunk(xr, 0, count, s_words);
+  fetch_chunk(gr, 0, count, s_words + kChunk * kRoundThreads);
+  int turn = 0;
+  for (int32_t j = 0; j < total; j += span, turn ^= 1) {
+    const int32_t t = at.lo + j;
+    typename R::Word x[kChunk], g[kChunk];
+    words_arrived();
+    take_chunk(s_words, x);
+    take_chunk(s_words + kChunk * kRoundThreads, g);
+    if (j + span < total) {
+      words_taken();
+      fetch_chunk(xr, j + span, count, s_words);
+      fetch_chunk(gr, j + span, count, s_words + kChunk * kRoundThreads);
+    }
+    float a[kChunk][V], fresh[kChunk][V], p[V], u[V], h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float b;
+        gate_pair(R::value(g[k], v), a[k][v], b);
+        fresh[k][v] = scaled<true>(b, R::value(x[k], v));
+      }
+    const bool plain = plain_backward(q, t, at.hi);
+    bool fine = plain;
+    if (plain) {
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          u[v] = fmaf(a[k][v], u[v], fresh[k][v]);
+          p[v] *= a[k][v];
+        }
+#pragma unroll
+      for (int v = 0; v < V; ++v) fine = fine && finite(u[v]) && finite(p[v]);
+      fine = __all(fine);
+    }
+    if (!fine) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
+      Cursor w = q;
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) {
+        if (j + k < count) {
+          if (t + k > w.last) w.next(c, t + k);
+          const bool first = t + k == w.first;
+          float h0[V];
+          if (first) load_state<V>(initial, c, at, w.s, h0);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            u[v] = applied<true>(a[k][v], first ? h0[v] : u[v], fresh[k][v]);
+            p[v] = first ? 0.0f : p[v] * a[k][v];
+          }
+        }
+      }
+    }
+    enter_chunk<V, false>(s_rounds, turn, c, at, p, u, carry, h);
+    if (kept != nullptr && j < count && at.inside) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) kept[static_cast<int64_t>(j / kChunk) * c.width + v] = h[v];
+    }
+    if (fine) {
+      float h1[V];
+      Pack<T, V> out[kChunk];
+#pragma unroll
+      for (int v = 0; v < V; ++v) h1[v] = h[v];
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          h1[v] = fmaf(a[k][v], h1[v], fresh[k][v]);
+          out[k].v[v] = static_cast<T>(h1[v]);
+        }
+#pragma unroll
+      for (int v = 0; v < V; ++v) fine = fine && finite(h1[v]);
+      if (__all(fine)) {
+        if (at.inside) store_chunk(yr, j, out);
+        continue;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+      if (j + k < count) {
+        if (t + k > q.last) q.next(c, t + k);
+        if (t + k == q.first) load_state<V>(initial, c, at, q.s, h);
+        Pack<T, V> out;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          h[v] = applied<true>(a[k][v], h[v], fresh[k][v]);
+          out.v[v] = static_cast<T>(h[v]);
+        }
+        if (at.inside) {
+          yr.store(j + k, __builtin_bit_cast(typename R::Word, out));
+          if (t + k == q.last) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) final[c.state_row(q.s) * c.width + at.col + v] = h[v];
+          }
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kRoundThreads) void scan_bwd_rounds_kernel(
+    const T *__restrict__ tokens, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
+    const float *__restrict__ initial, const T *__restrict__ v_y, int64_t v_stride,
+    const float *__restrict__ v_final, Tokens c, uint32_t slices,
+    const float *__restrict__ kept, T *__restrict__ v_x, T *__restrict__ v_gate,
+    float *__restrict__ v_initial) {
+  __shared__ Rounds<V> s_rounds;
+  __shared__ uint32_t s_words[(3 * kChunk + V) * kRoundThreads];  // x, gate, v_y, kept
+  int64_t block;
+  uint32_t slice;
+  block_and_slice(slices, block, slice);
+  Place at(c, V, block, slice);
+  const int32_t total = round_place(c, block, at), count = at.hi - at.lo;
+  const int32_t span = static_cast<int32_t>(blockDim.x >> c.lane_bits) * kChunk;
+  using R = Rows<T, V>;
+  const R xr(tokens, x_stride, c, at, block), gr(gate, g_stride, c, at, block);
+  const R vr(v_y, v_stride, c, at, block);
+  const R dxr(v_x, c.width, c, at, block), dgr(v_gate, c.width, c, at, block);
+  kept += block * block_chunks(c) * c.width + min(at.col, c.width - V);
+  const int32_t last_chunk = (total - 1) / kChunk;
+  Cursor q;
+  q.seek(c, at.hi - 1, total > 0);
+  float carry[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) carry[v] = 0.0f;
+  auto fetch = [&](int32_t j) {
+    fetch_chunk(xr, j, count, s_words);
+    fetch_chunk(gr, j, count, s_words + kChunk * kRoundThreads);
+    fetch_chunk(vr, j, count, s_words + 2 * kChunk * kRoundThreads);
+    // Some row of the block where the lane has no token.
+    const float *p = kept + static_cast<int64_t>(min(at.group + j / kChunk, last_chunk)) * c.width;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)(p + v),
+          (__attribute__((address_space(3))) void *)(s_words + (3 * kChunk + v) * kRoundThreads +
+                                                     wave_index() * 64),
+          4, 0, 0);
+  };
+  int32_t j = (total - 1) / span * span;
+  fetch(j);
+  int turn = 0;
+  for (; j >= 0; j -= span, turn ^= 1) {
+    const int32_t t = at.lo + j;
+    typename R::Word x[kChunk], g[kChunk], d[kChunk];
+    float h[V];
+    words_arrived();
+    take_chunk(s_words, x);
+    take_chunk(s_words + kChunk * kRoundThreads, g);
+    take_chunk(s_words + 2 * kChunk * kRoundThreads, d);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      h[v] = __uint_as_float(s_words[(3 * kChunk + v) * kRoundThreads + threadIdx.x]);
+    if (j >= span) {
+      words_taken();
+      fetch(j - span);
+    }
+    // prior: the state before a token, less its x.
+    float a[kChunk][V], b[kChunk][V], prior[kChunk][V], p[V], u[V], f[V];
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) gate_pair(R::value(g[k], v), a[k][v], b[k][v]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
+    const bool plain = plain_backward(q, t, at.hi);
+    bool fine = plain;
+    if (plain) {
+      float h1[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) h1[v] = h[v];
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float xv = R::value(x[k], v);
+          prior[k][v] = h1[v] - xv;
+          h1[v] = fmaf(a[k][v], h1[v], b[k][v] * xv);
+        }
+#pragma unroll
+      for (int k = kChunk - 1; k >= 0; --k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          u[v] = a[k][v] * (R::value(d[k], v) + u[v]);
+          p[v] *= a[k][v];
+        }
+#pragma unroll
+      for (int v = 0; v < V; ++v) fine = fine && finite(u[v]) && finite(p[v]) && finite(h1[v]);
+      fine = __all(fine);
+    }
+    if (!fine) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[v] = 1.0f, u[v] = 0.0f;
+      Cursor w = q;
+      if (j < count && t < w.first) w.previous(c, t);
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) {
+        if (j + k < count) {
+          if (t + k > w.last) w.next(c, t + k);
+          if (t + k == w.first) load_state<V>(initial, c, at, w.s, h);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float xv = R::value(x[k], v);
+            prior[k][v] = h[v] - xv;
+            h[v] = applied<true>(a[k][v], h[v], scaled<true>(b[k][v], xv));
+          }
+        }
+      }
+      w = q;
+#pragma unroll
+      for (int k = kChunk - 1; k >= 0; --k) {
+        if (j + k < count) {
+          if (t + k < w.first) w.previous(c, t + k);
+          const bool last = t + k == w.last;
+          float f0[V];
+          if (last) load_state<V>(v_final, c, at, w.s, f0);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            u[v] = scaled<true>(a[k][v], R::value(d[k], v) + (last ? f0[v] : u[v]));
+            p[v] = last ? 0.0f : p[v] * a[k][v];
+          }
+        }
+      }
+    }
+    enter_chunk<V, true>(s_rounds, turn, c, at, p, u, carry, f);
+    if (fine) {
+      float f1[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) f1[v] = f[v];
+#pragma unroll
+      for (int k = kChunk - 1; k >= 0; --k) {
+        Pack<T, V> dx, dg;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float gk = R::value(d[k], v) + f1[v], vx = b[k][v] * gk;
+          f1[v] = a[k][v] * gk;
+          dx.v[v] = static_cast<T>(vx);
+          dg.v[v] = static_cast<T>(a[k][v] * (vx * prior[k][v]));
+        }
+        if (at.inside) {
+          dxr.store(j + k, __builtin_bit_cast(typename R::Word, dx));
+          dgr.store(j + k, __builtin_bit_cast(typename R::Word, dg));
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) fine = fine && finite(f1[v]);
+      if (__all(fine)) continue;
+    }
+#pragma unroll
+    for (int k = kChunk - 1; k >= 0; --k) {
+      if (j + k < count) {
+        if (t + k < q.first) q.previous(c, t + k);
+        if (t + k == q.last) load_state<V>(v_final, c, at, q.s, f);
+        Pack<T, V> dx, dg;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float gk = R::value(d[k], v) + f[v], vx = scaled<true>(b[k][v], gk);
+          const float vg = a[k][v] * (vx * prior[k][v]);
+          dx.v[v] = static_cast<T>(vx);
+          dg.v[v] = static_cast<T>(a[k][v] == 0.0f || b[k][v] == 0.0f ? 0.0f : vg);
+          f[v] = scaled<true>(a[k][v], gk);
+        }
+        if (at.inside) {
+          dxr.store(j + k, __builtin_bit_cast(typename R::Word, dx));
+          dgr.store(j + k, __builtin_bit_cast(typename R::Word, dg));
+          if (t + k == q.first && v_initial != nullptr) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+              v_initial[c.state_row(q.s) * c.width + at.col + v] = f[v];
+          }
+        }
+      }
+    }
+  }
 }
 
 __global__ __launch_bounds__(kThreads) void scan_empty_kernel(Tokens c,
@@ -892,7 +1292,9 @@ struct Plan {
   Tokens c;
   int64_t groups() const { return threads >> c.lane_bits; }
   int64_t strips() const { return blocks * groups(); }
-  int64_t kept_rows() const { return strips() * (c.steps / kChunk); }
+  int64_t kept_rows() const {
+    return mode == kRounds ? blocks * ceil_div(c.block, kChunk) : strips() * (c.steps / kChunk);
+  }
 };
 
 // The plan depends on sizes and types alone, so a backward call finds its
@@ -922,12 +1324,23 @@ Plan plan_of(int type, const int32_t *offsets, int64_t n, int64_t sequences, int
     p.threads = kThreads;
     c.strip = static_cast<int32_t>(length);
     c.block = p.groups() * length;
-  } else if ((!ragged && sequences * p.slices >= 192) || n * lanes <= kResident * 32) {
-    p.mode = kResidentMode;
-    c.block = ragged || sequences * p.slices < 192 ? n : length;
+  } else if ((!ragged && sequences * p.slices >= 192) || n * lanes <= 32768) {
+    // Against the packed form, forward and back: 8 x 4096 x 1024 bf16 161 and
+    // 185 us, 64 x 512 x 128 bf16 39 and 54, 200 x 1000 x 128 f32 199 and 278;
+    // 6 x 2000 x 1024 bf16, 192 blocks, 82 and 84.  128 bytes of a row and not
+    // 64 where that leaves a block for each CU: 8 x 4096 x 1024 f32 238 and 327
+    // us, 1000 x 200 x 128 bf16 134 and 173; with 128 blocks (8 x 4096 x 1024
+    // bf16) 262 and 161.
+    p.mode = kRounds;
+    const bool whole = ragged || sequences * p.slices < 192;
+    c.block = whole ? n : length;
+    if (!whole && sequences * ceil_div(vpr, 32) >= 256) set_lanes(5);
+    // At least two rounds, for the overlap: 1000 x 200 x 128 bf16 took 192 us
+    // with one of 512 threads and 146 with two of 256; 1024 threads where they
+    // fit, 179 us against 134 for 32 x 1024 x 1024 bf16.
     p.threads = 64;
-    while (p.threads < kResident && p.groups() * 16 < c.block) p.threads *= 2;
-    c.strip = static_cast<int32_t>(align_up(ceil_div(c.block, p.groups()), kChunk));
+    while (p.threads < kRoundThreads && p.groups() * 2 * kChunk < c.block) p.threads *= 2;
+    c.strip = kChunk;
   } else {
     p.mode = kPacked;
     p.threads = kThreads;
@@ -1037,15 +1450,14 @@ int scan_fwd(const Plan &p, const void *x, int64_t xs, const void *g, int64_t gs
   const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices)), block(p.threads);
   if (p.mode == kPacked) {
     R2S_RETURN_IF((packed_maps<T, V, false>(p, xt, xs, gt, gs, initial, initial, final, s, stream)));
-    scan_fwd_kernel<T, V, kPacked, kThreads><<<grid, block, 0, stream>>>(
+    scan_fwd_kernel<T, V, kPacked><<<grid, block, 0, stream>>>(
         xt, xs, gt, gs, initial, c, p.slices, s.strips, s.carries, kept, y, final);
   } else if (p.mode == kOwn) {
-    scan_fwd_kernel<T, V, kOwn, kThreads><<<grid, block, 0, stream>>>(
+    scan_fwd_kernel<T, V, kOwn><<<grid, block, 0, stream>>>(
         xt, xs, gt, gs, initial, c, p.slices, nullptr, nullptr, kept, y, final);
   } else {
-    scan_fwd_kernel<T, V, kResidentMode, kResident>
-        <<<grid, block, p.threads * V * 2 * sizeof(float), stream>>>(
-            xt, xs, gt, gs, initial, c, p.slices, nullptr, nullptr, kept, y, final);
+    scan_fwd_rounds_kernel<T, V><<<grid, block, 0, stream>>>(xt, xs, gt, gs, initial, c, p.slices,
+                                                             kept, y, final);
   }
   return check_launch("gated_scan_fwd");
 }
@@ -1060,21 +1472,18 @@ int scan_bwd(const Plan &p, const void *x, int64_t xs, const void *g, int64_t gs
   const T *vt = static_cast<const T *>(v_y);
   T *dx = static_cast<T *>(v_x), *dg = static_cast<T *>(v_gate);
   const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices)), block(p.threads);
-  const size_t priors = static_cast<size_t>(p.threads) * V * kChunk * sizeof(float);
   if (p.mode == kPacked) {
     R2S_RETURN_IF((packed_maps<T, V, true>(p, gt, gs, vt, vs, v_final, v_final, v_initial, s, stream)));
-    scan_bwd_kernel<T, V, kPacked, kThreads><<<grid, block, priors, stream>>>(
+    scan_bwd_kernel<T, V, kPacked><<<grid, block, 0, stream>>>(
         xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, s.strips, s.carries, kept, dx, dg,
         v_initial);
   } else if (p.mode == kOwn) {
-    scan_bwd_kernel<T, V, kOwn, kThreads><<<grid, block, priors, stream>>>(
+    scan_bwd_kernel<T, V, kOwn><<<grid, block, 0, stream>>>(
         xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, nullptr, nullptr, kept, dx, dg,
         v_initial);
   } else {
-    scan_bwd_kernel<T, V, kResidentMode, kResident>
-        <<<grid, block, priors + p.threads * V * 2 * sizeof(float), stream>>>(
-            xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, nullptr, nullptr, kept, dx, dg,
-            v_initial);
+    scan_bwd_rounds_kernel<T, V><<<grid, block, 0, stream>>>(
+        xt, xs, gt, gs, initial, vt, vs, v_final, c, p.slices, kept, dx, dg, v_initial);
   }
   return check_launch("gated_scan_bwd");
 }
