@@ -255,7 +255,7 @@ struct Fragments {
 // A wave's part of the tile: 64 rows by kCols / 2 columns, as tiles of 16 x 16
 // of which a lane has four neighbouring columns of one row.  With kRuns its
 // tiles' columns are neighbours too, kRun in all, so that it stores them by 16
-// bytes: 500k x 64 x 64 bf16 forward XXX us, and 40 us with 8 bytes per tile.
+// bytes: 500k x 64 x 64 bf16 forward 35 us, and 40 us with 8 bytes per tile.
 template <int kCols, bool kRuns>
 struct Accumulator {
   static constexpr int kA = kCols / 32, kB = kRows / 32, kRun = kRuns ? 4 * kA : 0;
@@ -315,8 +315,9 @@ __device__ __forceinline__ void multiply_stage(const char *lds, const ColFragmen
 // The product over `steps` stages, two of them in LDS (one where there is but
 // one).  stage(lds, step), the steps in order, puts a stage on its way to LDS,
 // or reads it for commit(lds) to write it there.  More stages ahead measured
-// slower: 16k x 1024 x 1024 bf16 forward and backward 254 us with two of 64 bytes,
-// 281 with three, 340 with four; blocks that share a CU hide more than depth.
+// slower: 16k x 1024 x 1024 bf16 forward and backward 254 us (229 now) with two of
+// 64 bytes, 281 with three, 340 with four; blocks that share a CU hide more than
+// depth.
 template <int kStageBytes, typename Stage, typename Commit, typename Multiply>
 __device__ __forceinline__ void pipeline(char *lds, int steps, Stage stage, Commit commit,
                                          Multiply multiply) {
@@ -365,13 +366,18 @@ __device__ __forceinline__ void store_run(T *row, int64_t col, int64_t width,
 // (weight [m, k], summed over k) or with kBack the input's gradient (summed
 // over m).  Blocks of one row tile are neighbours, and neighbours share an XCD:
 // they read the same rows and weight.
+//
+// 16k x 1024 x 1024 bf16 in 16 groups: 65 us forward (530 TFLOP/s; 930 for one
+// library product of these sizes), 68 us back, bound by a stage's wait, by its
+// LDS reads, which take as long as its products, and by 1160 blocks, of which
+// the last run alone; at 32k x 2048 x 2048, 790 TFLOP/s.  500k x 64 x 64 bf16:
+// 35 us forward, 128 MB at 3.7 TB/s, bound by the writes.  50k x 45 x 11 f32:
+// 13 us, bound by the launch and a block's chain of offsets, rows, tile, store.
 template <typename T, bool kBack, bool kVec, int kCols, int S>
-__global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void rows_kernel(const T *__restrict__ in, int64_t stride,
-                                                        const T *__restrict__ weight,
-                                                        const T *__restrict__ bias, Groups g,
-                                                        const int32_t *__restrict__ rows,
-                                                        int64_t k, int64_t m, uint32_t col_tiles,
-                                                        T *__restrict__ out) {
+__global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void rows_kernel(
+    const T *__restrict__ in, int64_t stride, const T *__restrict__ weight,
+    const T *__restrict__ bias, Groups g, const int32_t *__restrict__ rows, int64_t k, int64_t m,
+    uint32_t col_tiles, T *__restrict__ out) {
   extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [1 or 2][cols, rows]
   __shared__ int32_t s_row[kRows];
   constexpr int kSlab = S / static_cast<int>(sizeof(T));
@@ -492,6 +498,11 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
 // dW[m0 + row][k0 + col] (and db) of part `slot`: `per` rows of one group.  The
 // group's only part goes to v_weight and v_bias, others to parts
 // [slots][m][k] and bias_parts [slots][m].
+//
+// 16k x 1024 x 1024 bf16: 95 us, 360 TFLOP/s; both operands are read across, at
+// half the LDS rate of operands read along, and a group of 4096 rows leaves 20 MB
+// of parts.  Parts of equal length within a group were no faster (99 us).
+// 500k x 64 x 64 bf16: 33 us, 128 MB read at 3.9 TB/s.
 template <typename T, bool kVec, int kCols, int S>
 __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ v_y, int64_t v_stride,
@@ -631,16 +642,20 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
 }
 
 // The weights' (blocks below weight_blocks) and biases' gradient of the groups
-// that have no part or more than one: zeros, or the parts' sum.  kShare threads
-// per element each add every kShare-th part, in row order, and meet in LDS:
-// eight for small weights, whose parts are many, one for large ones.
+// that have no part or more than one: zeros, or the parts' sum, in row order.
+// Many parts of small weights: kShare threads per element each add every
+// kShare-th part and meet in LDS.  Few parts of large ones (kShare 1): a thread
+// adds kRun neighbouring elements, 16 bytes of each part at a time.  16k x 1024
+// x 1024 bf16: 12.6 us, and 20 us element by element.
 template <typename T, int kShare>
 __global__ __launch_bounds__(kThreads) void add_parts_kernel(
     const float *__restrict__ parts, const float *__restrict__ bias_parts, Groups g, uint32_t per,
     uint32_t slots, int64_t weight_size, int64_t bias_size, uint32_t weight_blocks,
     uint32_t bias_blocks, T *__restrict__ v_weight, T *__restrict__ v_bias) {
-  constexpr int kElements = kThreads / kShare;
-  __shared__ float s_sum[kShare][kElements];
+  constexpr int kRun = kShare == 1 ? 4 : 1, kLanes = kThreads / kShare;
+  constexpr int kElements = kLanes * kRun;
+  using Run = UnalignedRun<float, kRun>;
+  __shared__ float s_sum[kShare][kLanes];
   const int32_t e = static_cast<int32_t>(blockIdx.y);
   const bool is_bias = blockIdx.x >= weight_blocks;
   const int64_t size = is_bias ? bias_size : weight_size;
@@ -660,34 +675,45 @@ __global__ __launch_bounds__(kThreads) void add_parts_kernel(
   // Offsets that do not ascend could name more parts than there are.
   const uint32_t first = min(before - mine, slots);
   mine = min(mine, slots - first);
-  const uint32_t share = threadIdx.x / kElements, lane = threadIdx.x % kElements;
+  const uint32_t share = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const uint32_t block = blockIdx.x - (is_bias ? weight_blocks : 0);
   const int64_t stride = static_cast<int64_t>(is_bias ? bias_blocks : weight_blocks) * kElements;
+  T *out = (is_bias ? v_bias : v_weight) + static_cast<int64_t>(e) * size;
   for (int64_t i0 = static_cast<int64_t>(block) * kElements; i0 < size; i0 += stride) {
-    const int64_t i = i0 + lane;
-    float sum = 0.0f;
-    if (i < size) {
-      const float *p = (is_bias ? bias_parts : parts) + static_cast<int64_t>(first) * size + i;
-      for (uint32_t s = share; s < mine; s += kShare * 8) {
-        float v[8];
+    const int64_t i = i0 + lane * kRun;
+    const float *p = (is_bias ? bias_parts : parts) + static_cast<int64_t>(first) * size + i;
+    constexpr uint32_t kBatch = 8 / kRun;  // loads before their sums
+    float sum[kRun] = {};
+    if (i + kRun <= size) {
+      for (uint32_t s = share; s < mine; s += kShare * kBatch) {
+        Run v[kBatch];
 #pragma unroll
-        for (uint32_t q = 0; q < 8; ++q)
-          v[q] = p[static_cast<int64_t>(min(s + q * kShare, mine - 1)) * size];
+        for (uint32_t q = 0; q < kBatch; ++q)
+          v[q] = *reinterpret_cast<const Run *>(
+              p + static_cast<int64_t>(min(s + q * kShare, mine - 1)) * size);
 #pragma unroll
-        for (uint32_t q = 0; q < 8; ++q) sum += s + q * kShare < mine ? v[q] : 0.0f;
+        for (uint32_t q = 0; q < kBatch; ++q)
+#pragma unroll
+          for (int r = 0; r < kRun; ++r) sum[r] += s + q * kShare < mine ? v[q].v[r] : 0.0f;
       }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kRun; ++r)
+        for (uint32_t s = share; s < mine && i + r < size; s += kShare)
+          sum[r] += p[static_cast<int64_t>(s) * size + r];
     }
     if constexpr (kShare > 1) {
-      s_sum[share][lane] = sum;
+      s_sum[share][lane] = sum[0];
       __syncthreads();
       if (share == 0) {
 #pragma unroll
-        for (int q = 1; q < kShare; ++q) sum += s_sum[q][lane];
+        for (int q = 1; q < kShare; ++q) sum[0] += s_sum[q][lane];
       }
       __syncthreads();
+      if (share == 0 && i < size) out[i] = static_cast<T>(sum[0]);
+    } else {
+      store_run<T, kRun>(out, i, size, {f32x4{sum[0], sum[1], sum[2], sum[3]}});
     }
-    if (share == 0 && i < size)
-      (is_bias ? v_bias : v_weight)[static_cast<int64_t>(e) * size + i] = static_cast<T>(sum);
   }
 }
 
@@ -696,7 +722,7 @@ __global__ __launch_bounds__(kThreads) void add_parts_kernel(
 // Bytes of the summed index per stage.  Operands read across and tiles of 128
 // columns take 64: four blocks share a CU instead of two.  16k x 1024 x 1024
 // bf16: forward 56 us with 128 bytes and 60 with 64, input gradient 80 and 70,
-// weights' gradient 142 and XXX; 500k x 64 x 64, where tiles have 64 columns:
+// weights' gradient 142 and 95; 500k x 64 x 64, where tiles have 64 columns:
 // weights' gradient 32 and 36.
 constexpr int slab_bytes(bool across, int cols) { return across && cols == 128 ? 64 : 128; }
 
@@ -803,12 +829,12 @@ int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride,
             static_cast<uint32_t>(k_tiles), s.parts, s.bias_parts, v_weight, v_bias);
     R2S_RETURN_IF(check_launch("grouped_matmul_bwd weights"));
   }
-  // At most 1024 blocks a group: most groups of large weights have one part, and
+  // At most 256 blocks a group: most groups of large weights have one part, and
   // their blocks only find that out.
   const bool small = m * k <= 1 << 15;
-  const int64_t elements = small ? kThreads / 8 : kThreads;
+  const int64_t elements = small ? kThreads / 8 : kThreads * 4;
   const int64_t weight_blocks =
-      v_weight != nullptr ? std::min<int64_t>(ceil_div(m * k, elements), 1024) : 0;
+      v_weight != nullptr ? std::min<int64_t>(ceil_div(m * k, elements), 256) : 0;
   const int64_t bias_blocks = v_bias != nullptr ? ceil_div(m, elements) : 0;
   if (weight_blocks + bias_blocks == 0) return R2S_OK;
   const dim3 grid(static_cast<uint32_t>(weight_blocks + bias_blocks), g.count);

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
 
 // Threads of the second kernel's blocks: a long row of narrow vectors needs the
 // more lane groups (45 f32 columns: 15.4 us with 1024 threads, 19.8 with 512),
-// wide vectors the less LDS (64 bf16 columns: 7.1 us with 512, 13.9 with 1024).
+// wide vectors the less LDS (64 bf16 columns: 9 us with 512, 16 with 1024).
 constexpr int row_threads(int V) { return V <= 2 ? 1024 : 512; }
 constexpr int kLongRow = 32;       // chunks: longer rows are added by a whole block
 constexpr int64_t kSpread = 1 << 18;  // lanes that the chunks are spread over
@@ -93,7 +93,8 @@ struct Sorted {
 // 2^lane_bits lanes hold one row's columns [c0, c0 + lanes V) and walk one
 // chunk; partial [chunks][2][width]: slot 0 the chunk's part of a run that began
 // in an earlier chunk, slot 1 its part of one that goes on into the next (a run
-// that does both is in slot 0).
+// that does both is in slot 0).  500k x 64 bf16: 20 us, 64 MB of gathered rows at
+// 3.2 TB/s, bound by the chain of a chunk: its ids, its positions, its rows.
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void lookup_bwd_chunks_kernel(
     const T *__restrict__ v_out, int64_t stride, Sorted list, float scale, uint32_t n_rows,
@@ -185,7 +186,9 @@ __device__ __forceinline__ void add_parts(const float *__restrict__ partial, uin
 // the sum of its parts if it crosses a chunk end, nothing to do otherwise.
 // Blocks before: block b looks at the row that holds the first entry of chunk
 // (b + 1) kLongRow and adds its parts if it spans more than kLongRow chunks
-// and no smaller b sees it.
+// and no smaller b sees it.  200k x 256 bf16 rows, most of them zeros: 29 us, 100
+// MB written at 3.6 TB/s; 18 x 45 f32 rows of 300k entries: 15 us, bound by the
+// parts of the longest row.
 template <typename T, int V>
 __global__ __launch_bounds__(row_threads(V)) void lookup_bwd_rows_kernel(
     Sorted list, float scale, uint32_t n_rows, uint32_t width, uint32_t lane_bits,
