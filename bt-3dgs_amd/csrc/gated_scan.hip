@@ -295,7 +295,7 @@ __device__ __forceinline__ void find_marks(const Tokens &c, Cursor &q, int32_t t
                                            Marks &m) {
   const uint32_t lanes = 1u << c.lane_bits, lane = lane_id() & (lanes - 1u);
   const uint32_t shift = lane_id() & ~(lanes - 1u);
-  const uint64_t mask = (1ull << lanes) - 1ull;
+  const uint64_t mask = lanes == 64u ? ~0ull : (1ull << lanes) - 1ull;
   constexpr int32_t kNone = kDown ? INT32_MIN : INT32_MAX;
   m.first = m.last = 0;
 #pragma unroll
@@ -711,8 +711,7 @@ __device__ __forceinline__ void block_and_slice(uint32_t slices, int64_t &block,
 }
 
 // The maps of the strips and of each block of them.  500k x 64 bf16: 35 us, the
-// tokens' 128 MB at 3.7 TB/s; 200k x 99 f32: 58 us forward and 47 back for 158 MB,
-// whose rows of odd width start at any 4 bytes.
+// tokens' 128 MB at 3.7 TB/s; 200k x 99 f32: 57 us forward and 37 back for 158 MB.
 template <typename T, int V, bool kBack>
 __global__ __launch_bounds__(kThreads) void scan_maps_kernel(
     const T *__restrict__ a, int64_t a_stride, const T *__restrict__ b, int64_t b_stride,
@@ -874,7 +873,7 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(
   walk_forward<T, V>(xr, gr, yr, initial, c, at, kept, final, h);
 }
 
-// The gradients, likewise.  200k x 99 f32: 129 us, 416 MB at 3.2 TB/s, bound by a
+// The gradients, likewise.  200k x 99 f32: 106 us, 406 MB at 3.8 TB/s, bound by a
 // chunk's chain: three loads, the states, then the gradients token by token.
 template <typename T, int V, int kMode>
 __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(
@@ -1367,7 +1366,7 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(
 // The threads that a packed call spreads the tokens over, in waves per CU.  A
 // lane of 16-bit rows holds two channels, so half the waves have as much in
 // flight: 500k x 64 bf16 74.6 us with 16 and 82.8 us with 32, 200k x 99 f32
-// (forward and backward) 328 and 315 us (309 now).
+// (forward and backward) 328 and 315 us (270 now).
 constexpr int64_t kSpread16 = 256 * 16 * 64, kSpread32 = 256 * 32 * 64;
 
 struct Plan {
@@ -1407,7 +1406,15 @@ Plan plan_of(int type, const int32_t *offsets, int64_t n, int64_t sequences, int
   set_lanes(4);
   const int64_t lanes = int64_t{1} << c.lane_bits;
   if (!ragged && length <= 128) {
+    // As many bytes of a row as leave no more lanes idle than 64 bytes do:
+    // 500 x 100 x 512 f32, forward and back, 185 us with 256 bytes, 204 with 128,
+    // 257 with 64; 3000 x 100 x 64 f32 forward 54, 55 and 61.
     p.mode = kOwn;
+    for (uint32_t bits = 6; bits > 4; --bits)
+      if (align_up(vpr, int64_t{1} << bits) <= align_up(vpr, 16)) {
+        set_lanes(bits);
+        break;
+      }
     p.threads = kThreads;
     c.strip = static_cast<int32_t>(length);
     c.block = p.groups() * length;
@@ -1433,7 +1440,10 @@ Plan plan_of(int type, const int32_t *offsets, int64_t n, int64_t sequences, int
   } else {
     p.mode = kPacked;
     p.threads = kThreads;
-    set_lanes(5);
+    // 256 bytes of a row where that leaves no more lanes idle than 128: 200k x 99
+    // f32, forward and back, 268 and 310 us, 30k x 1024 bf16 of 30 sequences 179
+    // and 208; 200k x 70 f32, 128 lanes for 96, 211 and 188.
+    set_lanes(align_up(vpr, 64) <= align_up(vpr, 32) ? 6 : 5);
     const int64_t even = ceil_div(n * (int64_t{p.slices} << c.lane_bits),
                                   p.V == 2 ? kSpread16 : kSpread32);
     c.strip = static_cast<int32_t>(
