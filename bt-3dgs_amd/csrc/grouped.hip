@@ -732,24 +732,29 @@ int64_t weight_tiles(int64_t k, int64_t m) {
 
 // Rows of a part of the weights' gradient: enough parts to fill the device,
 // and no more, since every part of a group past its first is a copy of the
-// weight to write and add.
-uint32_t rows_per_part(int64_t n, int64_t k, int64_t m) {
+// weight to write and add.  At least 512 rows where 16-bit products of many
+// tiles take less time than that: 4000 x 1024 x 1024 bf16, forward and back,
+// 73 us and 84 with 128, 28k x 256 x 1024 133 and 136; 32-bit products are slower
+// and need the parts: 8000 x 512 x 512 188 us, and 208 with 512.
+uint32_t rows_per_part(int64_t n, int64_t k, int64_t m, size_t element) {
   const int64_t tiles = weight_tiles(k, m);
   const int64_t even = ceil_div(n * tiles, tiles > 8 ? 1152 : 768);
+  const int64_t least = tiles > 8 && element == 2 ? 512 : 128;
   return static_cast<uint32_t>(
-      std::min<int64_t>(std::max<int64_t>(align_up(even, 64), 128), 4096));
+      std::min<int64_t>(std::max<int64_t>(align_up(even, 64), least), 4096));
 }
 
-// Blocks of the weights' gradient along the rows, at most.
-int64_t part_slots(int64_t n, int64_t k, int64_t m, int64_t groups) {
-  return ceil_div(n, rows_per_part(n, k, m)) + groups;
+// Blocks of the weights' gradient along the rows, at most; those of 4-byte
+// elements are the most, which the workspace has to hold.
+int64_t part_slots(int64_t n, int64_t k, int64_t m, int64_t groups, size_t element) {
+  return ceil_div(n, rows_per_part(n, k, m, element)) + groups;
 }
 
 struct GradSpace {
   float *parts, *bias_parts;
 };
 GradSpace carve_grad(Carver &cv, int64_t n, int64_t k, int64_t m, int64_t groups) {
-  const int64_t slots = part_slots(n, k, m, groups);
+  const int64_t slots = part_slots(n, k, m, groups, 4);
   GradSpace s;
   s.parts = cv.take<float>(slots * m * k);
   s.bias_parts = cv.take<float>(slots * m);
@@ -797,7 +802,12 @@ int rows_product(const void *in, int64_t stride, const void *weight, const void 
   const T *ti = static_cast<const T *>(in), *tw = static_cast<const T *>(weight);
   const T *tb = static_cast<const T *>(bias);
   T *to = static_cast<T *>(out);
-  const bool narrow = (kBack ? k : m) <= 64;
+  // 64 columns to a tile, too, where 128 give less than one and a half blocks per
+  // CU.  Forward and back: 3000 x 128 x 256 f32 49 us and 65, 4000 x 1024 x 1024
+  // bf16 86 and 98; with 458 blocks (28k x 1024 x 256 bf16) 142 and 134.
+  const int64_t outer = kBack ? k : m;
+  const bool narrow = outer <= 64 ||
+                      (ceil_div(g.n, kRows) + g.count) * ceil_div(outer, 128) <= 384;
 #define R2S_ROWS(VEC, COLS) \
   return (rows_launch<T, kBack, VEC, COLS>(ti, stride, tw, tb, g, rows, k, m, to, stream))
   if (vec) {
@@ -813,8 +823,8 @@ template <typename T, bool kVec, int kCols>
 int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride, Groups g,
                    const int32_t *rows, int64_t k, int64_t m, T *v_weight, T *v_bias,
                    const GradSpace &s, hipStream_t stream) {
-  const uint32_t per = rows_per_part(g.n, k, m);
-  const int64_t slots = part_slots(g.n, k, m, g.count);
+  const uint32_t per = rows_per_part(g.n, k, m, sizeof(T));
+  const int64_t slots = part_slots(g.n, k, m, g.count, sizeof(T));
   const int64_t m_tiles = ceil_div(m, kRows), k_tiles = ceil_div(std::max<int64_t>(k, 1), kCols);
   if (slots * m_tiles * k_tiles > kInt32Max) {
     set_error("grouped_matmul_bwd: too many tiles");
