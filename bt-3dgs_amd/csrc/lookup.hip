@@ -1,7 +1,7 @@
 // Rows of a table by id, scaled, and the table's gradient.
 //
-//   forward   out_i = s T[id_i]: each thread moves one vector (16 bytes where
-//             addresses and strides allow).  Ids outside the table give zero
+//   forward   out_i = s T[id_i]: each thread moves vectors of 16 bytes, at any
+//             element.  Ids outside the table give zero
 //             rows, so no id reads out of range.
 //   backward  dT_v = s sum_{id_i = v} dy_i, without atomics: the positions are
 //             sorted by id (stable, group.hip), the sorted list is cut into
@@ -21,6 +21,24 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// V consecutive elements at any element, as one load or store.  Rows are taken
+// in vectors of at most 16 bytes, the last of which ends with the row and may
+// overlap the one before: both then hold and write the same values.  300k x 45
+// f32, forward and back: 54 us, and 64 us with the vectors that divide a row;
+// 200k x 99 bf16 53 and 68.
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Run {
+  T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Run<T, V> load_run(const T *p) {
+  return *reinterpret_cast<const Run<T, V> *>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_run(T *p, const Run<T, V> &x) {
+  *reinterpret_cast<Run<T, V> *>(p) = x;
+}
+
 // ------------------------------------------------------------- forward ---
 
 // Vectors per thread: as many bytes of the narrow ones.
@@ -34,28 +52,29 @@ constexpr int fwd_vectors(int bytes) { return bytes <= 4 ? 8 : 4; }
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
     const T *__restrict__ table, int64_t stride, const I *__restrict__ ids, float scale,
-    int64_t n, int64_t n_rows, uint32_t vpr, uint32_t rows, uint32_t magic,
+    int64_t n, int64_t n_rows, uint32_t width, uint32_t vpr, uint32_t rows, uint32_t magic,
     T *__restrict__ out) {
   constexpr int kVectors = fwd_vectors(V * sizeof(T));
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows;
   const uint32_t vec0 = blockIdx.y * (kThreads * kVectors);
   const uint32_t count = static_cast<uint32_t>(min(static_cast<int64_t>(rows), n - row0));
   int64_t id[kVectors], at[kVectors];
-  uint32_t vec[kVectors];
+  uint32_t col[kVectors];
 #pragma unroll
   for (int k = 0; k < kVectors; ++k) {
     const uint32_t q = k * kThreads + threadIdx.x;
     const uint32_t r = rows > 1 ? __umulhi(q, magic) : 0u;
-    vec[k] = vec0 + q - r * vpr;
-    const bool inside = r < count && vec[k] < vpr;
-    at[k] = inside ? (row0 + r) * vpr + vec[k] : -1;
+    const uint32_t vec = vec0 + q - r * vpr;
+    const bool inside = r < count && vec < vpr;
+    col[k] = min(vec * V, width - V);
+    at[k] = inside ? (row0 + r) * width + col[k] : -1;
     id[k] = inside ? static_cast<int64_t>(ids[row0 + r]) : -1;
   }
-  Pack<T, V> x[kVectors];
+  Run<T, V> x[kVectors];
 #pragma unroll
   for (int k = 0; k < kVectors; ++k) {
     if (id[k] >= 0 && id[k] < n_rows) {
-      x[k] = load_pack<T, V>(table + id[k] * stride + static_cast<int64_t>(vec[k]) * V);
+      x[k] = load_run<T, V>(table + id[k] * stride + col[k]);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) x[k].v[j] = static_cast<T>(0.0f);
@@ -67,7 +86,7 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
 #pragma unroll
       for (int j = 0; j < V; ++j)
         x[k].v[j] = static_cast<T>(static_cast<float>(x[k].v[j]) * scale);
-      store_pack<T, V>(out + at[k] * V, x[k]);
+      store_run<T, V>(out + at[k], x[k]);
     }
   }
 }
@@ -75,11 +94,14 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
 // ------------------------------------------------------------ backward ---
 
 // Threads of the second kernel's blocks: a long row of narrow vectors needs the
-// more lane groups (45 f32 columns: 15.4 us with 1024 threads, 19.8 with 512),
-// wide vectors the less LDS (64 bf16 columns: 9 us with 512, 16 with 1024).
-constexpr int row_threads(int V) { return V <= 2 ? 1024 : 512; }
+// more lane groups (300k ids of 18 rows of 45 f32, forward and back: 59 us with
+// 1024 threads, 67 with 512), wide vectors the less LDS (64 bf16 columns: 7 us
+// with 512, 14 with 1024).
+constexpr int row_threads(int V) { return V <= 4 ? 1024 : 512; }
 constexpr int kLongRow = 32;       // chunks: longer rows are added by a whole block
-constexpr int64_t kSpread = 1 << 18;  // lanes that the chunks are spread over
+// Lanes that the chunks are spread over: the same call 54 us, and 59 with twice
+// as many, whose parts are twice as many too; 50k x 297 f32 73 and 70.
+constexpr int64_t kSpread = 1 << 17;
 
 // The sorted ids (n_rows for those outside the table), their positions and each
 // row's first entry.
@@ -99,11 +121,12 @@ template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void lookup_bwd_chunks_kernel(
     const T *__restrict__ v_out, int64_t stride, Sorted list, float scale, uint32_t n_rows,
     uint32_t width, uint32_t lane_bits, T *__restrict__ v_table, float *__restrict__ partial) {
-  const uint32_t col = (blockIdx.y << lane_bits) * V + (threadIdx.x & ((1u << lane_bits) - 1u)) * V;
+  const uint32_t vec = (blockIdx.y << lane_bits) + (threadIdx.x & ((1u << lane_bits) - 1u));
+  const uint32_t col = min(vec * V, width - V);
   const uint64_t chunk = (static_cast<uint64_t>(blockIdx.x) << (8 - lane_bits)) +
                          (threadIdx.x >> lane_bits);
   const uint64_t begin = chunk * list.chunk;
-  if (begin >= list.n || col >= width) return;
+  if (begin >= list.n || vec * V >= width) return;
   const uint32_t j0 = static_cast<uint32_t>(begin);
   const uint32_t j1 = static_cast<uint32_t>(min(begin + list.chunk, uint64_t{list.n}));
   // No id is n_rows + 1: nothing runs past the list's ends.
@@ -122,22 +145,22 @@ __global__ __launch_bounds__(kThreads) void lookup_bwd_chunks_kernel(
 #pragma unroll
       for (int v = 0; v < V; ++v) p[v] = acc[v];
     } else {
-      Pack<T, V> r;
+      Run<T, V> r;
 #pragma unroll
       for (int v = 0; v < V; ++v) r.v[v] = static_cast<T>(acc[v] * scale);
-      store_pack<T, V>(v_table + static_cast<int64_t>(run) * width + col, r);
+      store_run<T, V>(v_table + static_cast<int64_t>(run) * width + col, r);
     }
   };
   // Rows loaded before their first use: as many bytes of the narrow vectors.
   constexpr int kInFlight = sizeof(T) * V <= 4 ? 16 : 8;
   for (uint32_t j = j0; j < j1; j += kInFlight) {
     uint32_t id[kInFlight];
-    Pack<T, V> x[kInFlight];
+    Run<T, V> x[kInFlight];
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
       const uint32_t i = min(j + k, j1 - 1);
       id[k] = list.keys[i];
-      x[k] = load_pack<T, V>(v_out + static_cast<int64_t>(list.order[i]) * stride + col);
+      x[k] = load_run<T, V>(v_out + static_cast<int64_t>(list.order[i]) * stride + col);
     }
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
@@ -196,8 +219,9 @@ __global__ __launch_bounds__(row_threads(V)) void lookup_bwd_rows_kernel(
   const uint32_t lane = threadIdx.x & ((1u << lane_bits) - 1u), group = threadIdx.x >> lane_bits;
   constexpr int kRowThreads = row_threads(V);
   const uint32_t groups = kRowThreads >> lane_bits;
-  const uint32_t col = (blockIdx.y << lane_bits) * V + lane * V;
-  const bool inside = col < width;
+  const uint32_t vec = (blockIdx.y << lane_bits) + lane;
+  const uint32_t col = min(vec * V, width - V);
+  const bool inside = vec * V < width;
   __shared__ float sums[kRowThreads * V];
   const bool whole = blockIdx.x < n_long;
   uint32_t row;
@@ -234,10 +258,10 @@ __global__ __launch_bounds__(row_threads(V)) void lookup_bwd_rows_kernel(
     if (inside && o1 > o0) add_parts<V>(partial, width, col, c0, c0, c1, 1, acc);
   }
   if (!inside) return;
-  Pack<T, V> r;
+  Run<T, V> r;
 #pragma unroll
   for (int v = 0; v < V; ++v) r.v[v] = static_cast<T>(acc[v] * scale);
-  store_pack<T, V>(v_table + static_cast<int64_t>(row) * width + col, r);
+  store_run<T, V>(v_table + static_cast<int64_t>(row) * width + col, r);
 }
 
 // ---------------------------------------------------------------- host ---
@@ -290,7 +314,7 @@ int lookup_fwd(const void *table, int64_t stride, const void *ids, float scale, 
                int64_t n_rows, int64_t width, void *out, hipStream_t stream) {
   constexpr int64_t per_block = kThreads * fwd_vectors(V * static_cast<int>(sizeof(T)));
   static_assert(per_block <= 4096, "vector numbers of a block below 2^13");
-  const int64_t vpr = width / V;
+  const int64_t vpr = ceil_div(width, V);
   const int64_t rows = std::max<int64_t>(per_block / vpr, 1), slices = ceil_div(vpr, per_block);
   if (ceil_div(n, rows) > kInt32Max || slices > 65535) {
     set_error("embedding_fwd: output too large");
@@ -304,8 +328,8 @@ int lookup_fwd(const void *table, int64_t stride, const void *ids, float scale, 
       <<<dim3(static_cast<uint32_t>(ceil_div(n, rows)), static_cast<uint32_t>(slices)),
          dim3(kThreads), 0, stream>>>(static_cast<const T *>(table), stride,
                                       static_cast<const I *>(ids), scale, n, n_rows,
-                                      static_cast<uint32_t>(vpr), static_cast<uint32_t>(rows),
-                                      magic, static_cast<T *>(out));
+                                      static_cast<uint32_t>(width), static_cast<uint32_t>(vpr),
+                                      static_cast<uint32_t>(rows), magic, static_cast<T *>(out));
   return check_launch("embedding_fwd");
 }
 
@@ -313,7 +337,7 @@ template <typename T, int V>
 int lookup_bwd(const void *v_out, int64_t stride, float scale, int64_t n, int64_t n_rows,
                int64_t width_, void *v_table_, const BwdSpace &s, hipStream_t stream) {
   T *v_table = static_cast<T *>(v_table_);
-  const uint32_t width = static_cast<uint32_t>(width_), vpr = width / V;
+  const uint32_t width = static_cast<uint32_t>(width_), vpr = (width + V - 1) / V;
   uint32_t bits = 0;
   while (bits < 6 && (1u << bits) < vpr) ++bits;
   const uint32_t slices = static_cast<uint32_t>(ceil_div(vpr, 1 << bits));
@@ -337,6 +361,13 @@ int lookup_bwd(const void *v_out, int64_t stride, float scale, int64_t n, int64_
          dim3(row_threads(V)), 0, stream>>>(list, scale, static_cast<uint32_t>(n_rows), width, bits,
                                          static_cast<uint32_t>(n_long), s.partial, v_table);
   return check_launch("embedding_bwd rows");
+}
+
+// Bytes of the vectors of a row: 16, or the power of two that a shorter row has.
+int run_bytes(int64_t width, int size) {
+  int bytes = 16;
+  while (bytes > width * size) bytes /= 2;
+  return bytes;
 }
 
 // `call` with V bound to the elements of a vector of `bytes` bytes.
@@ -371,9 +402,7 @@ int r2s_embedding_fwd(const void *table, int64_t table_stride, const void *ids,
   if (n == 0 || width == 0) return R2S_OK;
   R2S_REQUIRE((table != nullptr || n_rows == 0) && out != nullptr,
               "embedding_fwd: null table or output");
-  const uint64_t size = type_size(type);
-  const int bytes = vector_bytes({address(table), address(out), table_stride * size, width * size},
-                                 static_cast<int>(size));
+  const int bytes = run_bytes(width, type_size(type));
   hipStream_t stream = as_stream(st);
   R2S_BY_TYPE(type, R2S_BY_VECTOR(T, bytes, {
     return ids_are_64 ? (lookup_fwd<T, V, int64_t>(table, table_stride, ids, scale, n, n_rows,
@@ -410,10 +439,12 @@ int r2s_embedding_bwd(const void *v_out, int64_t v_out_stride, const void *ids,
   hipStream_t stream = as_stream(st);
   R2S_RETURN_IF(
       sort_ids(ids, ids_are_64 != 0, n, n_rows, s.order, s.offsets, s.keys, s.sort, stream));
-  const uint64_t size = type_size(type);
-  const int bytes = vector_bytes({address(v_out), address(v_table), v_out_stride * size,
-                                  width * size},
-                                 static_cast<int>(size));
+  // Eight vectors to a row where it has them: 300k x 16 bf16 of 3000 rows, forward
+  // and back, 45 us with vectors of 4 bytes and 52 with 16, 400k x 3 f32 45 with
+  // 4 bytes and 52 with 8.
+  const int size = type_size(type);
+  int bytes = run_bytes(width, size);
+  while (bytes > size && ceil_div(width * size, bytes) < 8) bytes /= 2;
   R2S_BY_TYPE(type, R2S_BY_VECTOR(T, bytes, {
     return (lookup_bwd<T, V>(v_out, v_out_stride, scale, n, n_rows, width, v_table, s, stream));
   }));

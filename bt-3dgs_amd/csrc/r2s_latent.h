@@ -34,15 +34,6 @@ inline bool known_type(int type) {
   return type == R2S_TYPE_F32 || type == R2S_TYPE_BF16 || type == R2S_TYPE_F16;
 }
 
-// The widest vector, at most 16 bytes, that divides every given byte count
-// (addresses, row strides, row lengths), in bytes.
-inline int vector_bytes(std::initializer_list<uint64_t> all, int least) {
-  uint64_t any = 16;
-  for (uint64_t v : all) any |= v;
-  int w = 16;
-  while (w > least && any % w != 0) w /= 2;
-  return w;
-}
 inline uint64_t address(const void *p) { return reinterpret_cast<uint64_t>(p); }
 
 // Stable grouping of n ids by value (group.hip): order [n] receives the
