@@ -1913,6 +1913,9 @@ def _rows_2d(t: Tensor, align: int = 1):
     consecutive; a copy where they are not, where rows overlap or lie very far
     apart, or where a row does not start at a multiple of ``align`` bytes."""
     n, d = t.shape
+    if t.is_contiguous() and (
+            align == 1 or not (t.data_ptr() % align or d * t.element_size() % align)):
+        return t, d
     stride = t.stride(0) if n > 1 else d
     if (d > 1 and t.stride(1) != 1) or stride < d or stride > 4 * max(d, 4096) or \
             (align > 1 and (t.data_ptr() % align or (stride * t.element_size()) % align)):
