@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void group_offsets_kernel(const uint32_t *__re
 // A short list in one launch: every item counts the items that go before it, and
 // every group those of the groups before it, over the keys in LDS.  kShare lanes
 // take a part of the keys each: with one, 2000 items took 43 us.
-constexpr int kShortThreads = 256, kShortList = 2048, kShare = 8;
+constexpr int kShortThreads = 256, kShortList = 4096, kShare = 8;
 constexpr int kShortItems = kShortThreads / kShare;  // of a block
 template <typename I>
 __global__ __launch_bounds__(kShortThreads) void short_list_kernel(
@@ -238,9 +238,10 @@ __global__ __launch_bounds__(kShortThreads) void short_list_kernel(
 // ---------------------------------------------------------------- host ---
 
 // Whether a list goes through short_list_kernel, whose work is n (n + groups).
-// A lookup and its gradient, 64 columns: 2000 ids of 4096 rows 27 us and 38 in
-// passes, of 100 rows (one pass) 27 and 29, 264 ids of 108k rows 28 and 56; with
-// four times the work of this limit, 2000 of 120k, 53 and 41.
+// A lookup and its gradient, 64 columns: 4000 ids of 4096 rows 28 us and 36 in
+// passes, of 500 rows (one pass) 28 and 29, 264 ids of 108k rows 28 and 56; 8000
+// ids of 100 rows 38 and 29, and with four times the work of this limit, 2000 ids
+// of 120k rows, 53 and 41.
 bool is_short(int64_t n, int64_t n_groups) {
   return n <= kShortList && n * (n + n_groups) <= (1 << 26);
 }

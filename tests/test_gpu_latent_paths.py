@@ -122,7 +122,8 @@ def test_grouped_tiles_and_parts(n, k, m, e, routed, dtype):
 
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("n,groups", [(2048, 5), (2049, 5), (2047, 30_000), (2000, 40_000),
-                                      (31, 200_000), (32, 0), (33, 1)])
+                                      (31, 200_000), (32, 0), (33, 1), (4096, 4000),
+                                      (4097, 4000), (4000, 20_000)])
 def test_group_rows_of_short_lists(n, groups, wide):
     ids = torch.randint(-2, max(groups + 2, 1), (n,), generator=_gen(n + groups))
     ids[n // 2:] = ids[:n - n // 2].flip(0)  # equal ids far apart
