@@ -47,8 +47,9 @@ constexpr int fwd_vectors(int bytes) { return bytes <= 4 ? 8 : 4; }
 // A block takes `rows` whole rows (of at most kThreads fwd_vectors vectors
 // together), or in a longer row one run of that many.  vpr: vectors per row;
 // magic: 2^32 / vpr rounded up, the quotient of every vector number of a block
-// (below 2^13, so exact) by one multiplication.  Bound by the writes: 64 MB of
-// 500k x 64 bf16 rows in 16 us, 3.9 TB/s.
+// (below 2^13, so exact) by one multiplication; a row of one vector, whose magic
+// would be 2^32, needs none.  Bound by the writes: 64 MB of 500k x 64 bf16 rows
+// in 16 us, 3.9 TB/s.
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
     const T *__restrict__ table, int64_t stride, const I *__restrict__ ids, float scale,
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
 #pragma unroll
   for (int k = 0; k < kVectors; ++k) {
     const uint32_t q = k * kThreads + threadIdx.x;
-    const uint32_t r = rows > 1 ? __umulhi(q, magic) : 0u;
+    const uint32_t r = vpr == 1 ? q : rows > 1 ? __umulhi(q, magic) : 0u;
     const uint32_t vec = vec0 + q - r * vpr;
     const bool inside = r < count && vec < vpr;
     col[k] = min(vec * V, width - V);
@@ -321,9 +322,7 @@ int lookup_fwd(const void *table, int64_t stride, const void *ids, float scale, 
     return R2S_ERANGE;
   }
   const uint32_t magic =
-      rows > 1 ? static_cast<uint32_t>(std::min<uint64_t>(((uint64_t{1} << 32) + vpr - 1) / vpr,
-                                                          0xffffffffull))
-               : 0u;
+      rows > 1 && vpr > 1 ? static_cast<uint32_t>(((uint64_t{1} << 32) + vpr - 1) / vpr) : 0u;
   lookup_fwd_kernel<T, V, I>
       <<<dim3(static_cast<uint32_t>(ceil_div(n, rows)), static_cast<uint32_t>(slices)),
          dim3(kThreads), 0, stream>>>(static_cast<const T *>(table), stride,
