@@ -22,7 +22,8 @@
 //
 // dW sums over rows: its blocks take a fixed number of rows of one group each.
 // A group of one such part is stored at once; the others leave float32 parts,
-// which a second kernel adds in row order.
+// which a second kernel adds in row order.  Only those parts have a place in the
+// workspace, so its size does not grow with the groups.
 #include <algorithm>
 
 #include "r2s_latent.h"
@@ -69,13 +70,25 @@ struct Groups {
   }
 };
 
-// Part `slot` of the groups cut into parts of `per` rows each: its group, rows
-// [r0, r1), and whether it is the group's only part.  With `rest` the rows past
-// the last group follow as group `count`.  False past the last part.  Called by
-// whole waves.
+// A group's parts that have a place in the workspace: all of several, but not an
+// only one.
+__device__ __forceinline__ uint32_t kept_parts(uint32_t parts) { return parts > 1u ? parts : 0u; }
+
+// A part of a group: its rows [r0, r1), whether it is the group's only one, and
+// else its place among the parts of all groups that have several.
+struct Part {
+  int32_t group;
+  int64_t r0, r1;
+  bool only;
+  uint32_t place;
+};
+
+// Part `slot` of the groups cut into parts of `per` rows each.  With `rest` the
+// rows past the last group follow as group `count`.  False past the last part.
+// Called by whole waves.
 __device__ __forceinline__ bool find_part(const Groups &g, bool rest, uint32_t per, uint32_t slot,
-                                          int32_t &group, int64_t &r0, int64_t &r1, bool &only) {
-  uint32_t before = 0;
+                                          Part &part) {
+  uint32_t before = 0, kept_before = 0;
   const int32_t total = g.count + (rest ? 1 : 0);
   for (int32_t e0 = 0; e0 < total; e0 += 64) {
     const int32_t e = e0 + static_cast<int32_t>(lane_id());
@@ -86,17 +99,20 @@ __device__ __forceinline__ bool find_part(const Groups &g, bool rest, uint32_t p
       lo = g.bound(e), hi = g.n;
     const uint32_t parts = hi > lo ? static_cast<uint32_t>((hi - lo + per - 1) / per) : 0u;
     const uint32_t end = before + wave_inclusive_scan(parts);
+    const uint32_t kept_end = kept_before + wave_inclusive_scan(kept_parts(parts));
     const uint64_t past = ballot(end > slot);
     if (past != 0) {
       const uint32_t src = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(past))) - 1u;
-      group = static_cast<int32_t>(readlane_u32(static_cast<uint32_t>(e), src));
+      part.group = static_cast<int32_t>(readlane_u32(static_cast<uint32_t>(e), src));
       const uint32_t count = readlane_u32(parts, src), first = readlane_u32(end, src) - count;
-      r0 = readlane_i64(lo, src) + static_cast<int64_t>(slot - first) * per;
-      r1 = min(readlane_i64(hi, src), r0 + per);
-      only = count == 1;
+      part.r0 = readlane_i64(lo, src) + static_cast<int64_t>(slot - first) * per;
+      part.r1 = min(readlane_i64(hi, src), part.r0 + per);
+      part.only = count == 1;
+      part.place = readlane_u32(kept_end, src) - kept_parts(count) + (slot - first);
       return true;
     }
     before = readlane_u32(end, 63);
+    kept_before = readlane_u32(kept_end, 63);
   }
   return false;
 }
@@ -388,10 +404,10 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
   const int64_t inner = kBack ? m : k, outer = kBack ? k : m;
   const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
   const int64_t j0 = static_cast<int64_t>(id % col_tiles) * kCols;
-  int32_t e;
-  int64_t r0, r1;
-  bool only;
-  if (!find_part(g, true, kRows, id / col_tiles, e, r0, r1, only)) return;
+  Part part;
+  if (!find_part(g, true, kRows, id / col_tiles, part)) return;
+  const int32_t e = part.group;
+  const int64_t r0 = part.r0, r1 = part.r1;
   if (threadIdx.x < kRows) {
     const int64_t i = r0 + threadIdx.x;
     int64_t r = -1;
@@ -495,9 +511,9 @@ __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void ro
   }
 }
 
-// dW[m0 + row][k0 + col] (and db) of part `slot`: `per` rows of one group.  The
-// group's only part goes to v_weight and v_bias, others to parts
-// [slots][m][k] and bias_parts [slots][m].
+// dW[m0 + row][k0 + col] (and db) of one part: `per` rows of one group.  The
+// group's only part goes to v_weight and v_bias, others to their place in parts
+// [places][m][k] and bias_parts [places][m].
 //
 // 16k x 1024 x 1024 bf16: 95 us, 360 TFLOP/s; both operands are read across, at
 // half the LDS rate of operands read along, and a group of 4096 rows leaves 20 MB
@@ -507,8 +523,8 @@ template <typename T, bool kVec, int kCols, int S>
 __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ v_y, int64_t v_stride,
     Groups g, const int32_t *__restrict__ rows, int64_t k, int64_t m, uint32_t per,
-    uint32_t m_tiles, uint32_t k_tiles, float *__restrict__ parts, float *__restrict__ bias_parts,
-    T *__restrict__ v_weight, T *__restrict__ v_bias) {
+    uint32_t m_tiles, uint32_t k_tiles, uint32_t places, float *__restrict__ parts,
+    float *__restrict__ bias_parts, T *__restrict__ v_weight, T *__restrict__ v_bias) {
   extern __shared__ __attribute__((aligned(16))) char s_stage[];  // [2][cols, rows]
   // The rows' numbers, two windows by turns.
   __shared__ __attribute__((aligned(16))) int32_t s_row[2][kWindow];
@@ -522,10 +538,13 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
   const uint32_t slot = id / tiles, tile = id - slot * tiles;
   const int64_t m0 = static_cast<int64_t>(tile / k_tiles) * kRows;
   const int64_t k0 = static_cast<int64_t>(tile % k_tiles) * kCols;
-  int32_t e;
-  int64_t r0, r1;
-  bool only;
-  if (!find_part(g, false, per, slot, e, r0, r1, only)) return;
+  Part part;
+  if (!find_part(g, false, per, slot, part)) return;
+  // Offsets that do not ascend could name more parts than there are places.
+  if (!part.only && part.place >= places) return;
+  const int32_t e = part.group;
+  const int64_t r0 = part.r0, r1 = part.r1;
+  const bool only = part.only;
   const int count = static_cast<int>(r1 - r0);
   // Window w's numbers on their way to LDS; past the part's end the last one's.
   auto fetch_rows = [&](int w) {
@@ -606,7 +625,7 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
       multiply_stage<T, false, kColBytes>(lds, col_fragments, row_fragments, acc, sums);
     });
   if (v_weight != nullptr) {
-    float *p = parts + static_cast<int64_t>(slot) * m * k;
+    float *p = parts + static_cast<int64_t>(part.place) * m * k;
     T *w = v_weight + static_cast<int64_t>(e) * m * k;
 #pragma unroll
     for (int b = 0; b < Acc::kB; ++b) {
@@ -635,7 +654,7 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
         if (only)
           v_bias[static_cast<int64_t>(e) * m + r] = static_cast<T>(sum);
         else
-          bias_parts[static_cast<int64_t>(slot) * m + r] = sum;
+          bias_parts[static_cast<int64_t>(part.place) * m + r] = sum;
       }
     }
   }
@@ -650,7 +669,7 @@ __global__ __launch_bounds__(kThreads, kCols == 64 && kVec ? 3 : 2) void weights
 template <typename T, int kShare>
 __global__ __launch_bounds__(kThreads) void add_parts_kernel(
     const float *__restrict__ parts, const float *__restrict__ bias_parts, Groups g, uint32_t per,
-    uint32_t slots, int64_t weight_size, int64_t bias_size, uint32_t weight_blocks,
+    uint32_t places, int64_t weight_size, int64_t bias_size, uint32_t weight_blocks,
     uint32_t bias_blocks, T *__restrict__ v_weight, T *__restrict__ v_bias) {
   constexpr int kRun = kShare == 1 ? 4 : 1, kLanes = kThreads / kShare;
   constexpr int kElements = kLanes * kRun;
@@ -667,14 +686,14 @@ __global__ __launch_bounds__(kThreads) void add_parts_kernel(
       const int64_t rows = g.bound(q + 1) - g.bound(q);
       n = rows > 0 ? static_cast<uint32_t>((rows + per - 1) / per) : 0u;
     }
-    const uint32_t end = before + wave_inclusive_scan(n);
+    const uint32_t end = before + wave_inclusive_scan(kept_parts(n));
     mine = readlane_u32(n, static_cast<uint32_t>(min(e - e0, 63)));
     before = readlane_u32(end, 63);
   }
   if (mine == 1) return;
-  // Offsets that do not ascend could name more parts than there are.
-  const uint32_t first = min(before - mine, slots);
-  mine = min(mine, slots - first);
+  // Offsets that do not ascend could name more parts than there are places.
+  const uint32_t first = min(before - mine, places);
+  mine = min(mine, places - first);
   const uint32_t share = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const uint32_t block = blockIdx.x - (is_bias ? weight_blocks : 0);
   const int64_t stride = static_cast<int64_t>(is_bias ? bias_blocks : weight_blocks) * kElements;
@@ -744,20 +763,28 @@ uint32_t rows_per_part(int64_t n, int64_t k, int64_t m, size_t element) {
       std::min<int64_t>(std::max<int64_t>(align_up(even, 64), least), 4096));
 }
 
-// Blocks of the weights' gradient along the rows, at most; those of 4-byte
-// elements are the most, which the workspace has to hold.
+// Blocks of the weights' gradient along the rows, at most.
 int64_t part_slots(int64_t n, int64_t k, int64_t m, int64_t groups, size_t element) {
   return ceil_div(n, rows_per_part(n, k, m, element)) + groups;
+}
+
+// Parts of groups that have several, at most: such a group of r rows has more
+// than `per` of them, so fewer than 2 r / per parts, and fewer than r / per + 1.
+int64_t part_places(int64_t n, int64_t k, int64_t m, int64_t groups, size_t element) {
+  const int64_t per = rows_per_part(n, k, m, element);
+  return n <= per ? 0 : std::min(2 * n / per, n / per + groups);
 }
 
 struct GradSpace {
   float *parts, *bias_parts;
 };
-GradSpace carve_grad(Carver &cv, int64_t n, int64_t k, int64_t m, int64_t groups) {
-  const int64_t slots = part_slots(n, k, m, groups, 4);
+// parts only where the weights' gradient is wanted.
+GradSpace carve_grad(Carver &cv, int64_t n, int64_t k, int64_t m, int64_t groups, size_t element,
+                     bool with_weight) {
+  const int64_t places = part_places(n, k, m, groups, element);
   GradSpace s;
-  s.parts = cv.take<float>(slots * m * k);
-  s.bias_parts = cv.take<float>(slots * m);
+  s.parts = cv.take<float>(with_weight ? places * m * k : 0);
+  s.bias_parts = cv.take<float>(std::max<int64_t>(places, 1) * m);
   return s;
 }
 
@@ -825,6 +852,7 @@ int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride,
                    const GradSpace &s, hipStream_t stream) {
   const uint32_t per = rows_per_part(g.n, k, m, sizeof(T));
   const int64_t slots = part_slots(g.n, k, m, g.count, sizeof(T));
+  const uint32_t places = static_cast<uint32_t>(part_places(g.n, k, m, g.count, sizeof(T)));
   const int64_t m_tiles = ceil_div(m, kRows), k_tiles = ceil_div(std::max<int64_t>(k, 1), kCols);
   if (slots * m_tiles * k_tiles > kInt32Max) {
     set_error("grouped_matmul_bwd: too many tiles");
@@ -836,7 +864,7 @@ int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride,
         <<<dim3(static_cast<uint32_t>(slots * m_tiles * k_tiles)), dim3(kThreads),
            2 * (kCols + kRows) * S, stream>>>(
             x, x_stride, v_y, v_stride, g, rows, k, m, per, static_cast<uint32_t>(m_tiles),
-            static_cast<uint32_t>(k_tiles), s.parts, s.bias_parts, v_weight, v_bias);
+            static_cast<uint32_t>(k_tiles), places, s.parts, s.bias_parts, v_weight, v_bias);
     R2S_RETURN_IF(check_launch("grouped_matmul_bwd weights"));
   }
   // At most 256 blocks a group: most groups of large weights have one part, and
@@ -850,7 +878,7 @@ int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride,
   const dim3 grid(static_cast<uint32_t>(weight_blocks + bias_blocks), g.count);
 #define R2S_ADD_PARTS(SHARE)                                                                    \
   add_parts_kernel<T, SHARE><<<grid, dim3(kThreads), 0, stream>>>(                              \
-      s.parts, s.bias_parts, g, per, static_cast<uint32_t>(slots), m * k, m,                    \
+      s.parts, s.bias_parts, g, per, places, m * k, m,                                          \
       static_cast<uint32_t>(weight_blocks), static_cast<uint32_t>(bias_blocks), v_weight, v_bias)
   if (small)
     R2S_ADD_PARTS(8);
@@ -902,10 +930,11 @@ int r2s_grouped_matmul_fwd(const void *x, int64_t x_stride, const void *weight, 
   return R2S_OK;
 }
 
-int64_t r2s_grouped_matmul_bwd_workspace_bytes(int64_t n, int64_t k, int64_t m, int64_t groups) {
-  if (n < 0 || k < 0 || m < 0 || groups < 0) return 0;
+int64_t r2s_grouped_matmul_bwd_workspace_bytes(int64_t n, int64_t k, int64_t m, int64_t groups,
+                                               int32_t type, int32_t with_weight) {
+  if (n < 0 || k < 0 || m < 0 || groups < 0 || !r2s::known_type(type)) return 0;
   r2s::Carver cv(nullptr);
-  r2s::carve_grad(cv, n, k, m, groups);
+  r2s::carve_grad(cv, n, k, m, groups, r2s::type_size(type), with_weight != 0);
   return static_cast<int64_t>(cv.used);
 }
 
@@ -929,14 +958,15 @@ int r2s_grouped_matmul_bwd(const void *x, int64_t x_stride, const void *weight,
   if ((v_weight == nullptr && v_bias == nullptr) || groups == 0 || m == 0) return R2S_OK;
   R2S_REQUIRE(n == 0 || (v_y != nullptr && (x != nullptr || k == 0)),
               "grouped_matmul_bwd: null gradient or input");
-  const int64_t need = r2s_grouped_matmul_bwd_workspace_bytes(n, k, m, groups);
+  const int64_t need =
+      r2s_grouped_matmul_bwd_workspace_bytes(n, k, m, groups, type, v_weight != nullptr);
   if (ws == nullptr || static_cast<int64_t>(ws_bytes) < need) {
     set_error("grouped_matmul_bwd: workspace of %zu bytes, %lld required", ws_bytes,
               (long long)need);
     return R2S_EWORKSPACE;
   }
   Carver cv(ws);
-  const GradSpace s = carve_grad(cv, n, k, m, groups);
+  const GradSpace s = carve_grad(cv, n, k, m, groups, type_size(type), v_weight != nullptr);
   R2S_BY_TYPE(type, return (weights_product<T>(x, x_stride, v_y, v_y_stride, g, rows, k, m,
                                                v_weight, v_bias, s, stream)));
   return R2S_OK;

@@ -139,7 +139,7 @@ _PLAIN = {
                                   _i64, _i32, _i32, _p, _p, _p, _p, _sz, _p]),
     "r2s_grouped_matmul_fwd": (_i32, [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _p,
                                       _p]),
-    "r2s_grouped_matmul_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "r2s_grouped_matmul_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i32, _i32]),
     "r2s_grouped_matmul_bwd": (_i32, [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                                       _i32, _p, _p, _p, _p, _sz, _p]),
 }
@@ -178,7 +178,7 @@ TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
 
 SYMBOLS = sorted(list(_PLAIN) + [f"r2s_{n}_{s}" for n in _FLOAT_OPS for s in ("f32", "f64")])
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 
 def load(path: str = LIB_PATH) -> ctypes.CDLL:

@@ -2182,7 +2182,7 @@ def grouped_matmul_bwd(x: Tensor, weight: Tensor, offsets: Tensor, rows: Optiona
         v_x, v_weight, v_bias = new(with_x, n, k), new(with_weight, e, m, k), new(with_bias, e, m)
         need = 0
         if with_weight or with_bias:
-            need = lib.r2s_grouped_matmul_bwd_workspace_bytes(n, k, m, e)
+            need = lib.r2s_grouped_matmul_bwd_workspace_bytes(n, k, m, e, code, with_weight)
         ws = _workspace(need, dev)
         _call("r2s_grouped_matmul_bwd", _ptr(x), xs, _ptr(weight), _ptr(offsets), _ptr(rows),
               _ptr(v_y), vs, n, k, m, e, code, _ptr(v_x), _ptr(v_weight), _ptr(v_bias), _ptr(ws),

@@ -1206,8 +1206,11 @@ int r2s_grouped_matmul_fwd(const void *x, int64_t x_stride, const void *weight, 
                            const int32_t *offsets, const int32_t *rows, int64_t n, int64_t k,
                            int64_t m, int64_t groups, int32_t type, void *y, r2s_stream_t stream);
 /* Its gradient from v_y [n, m]: v_x [n, k], v_weight [groups, m, k], v_bias
- * [groups, m]; any of them may be NULL (not wanted). */
-int64_t r2s_grouped_matmul_bwd_workspace_bytes(int64_t n, int64_t k, int64_t m, int64_t groups);
+ * [groups, m]; any of them may be NULL (not wanted).  The workspace holds float32
+ * parts of the weights' gradient for groups of many rows, as many as the rows
+ * can fill whatever the number of groups; none without v_weight. */
+int64_t r2s_grouped_matmul_bwd_workspace_bytes(int64_t n, int64_t k, int64_t m, int64_t groups,
+                                               int32_t type, int32_t with_weight);
 int r2s_grouped_matmul_bwd(const void *x, int64_t x_stride, const void *weight,
                            const int32_t *offsets, const int32_t *rows, const void *v_y,
                            int64_t v_y_stride, int64_t n, int64_t k, int64_t m, int64_t groups,

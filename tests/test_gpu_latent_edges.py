@@ -35,3 +35,42 @@ def test_lookup_writes_every_row(d, wide, dtype):
     grad = W.embedding_bwd(v_out.to(DEV), i, v, scale)
     exact, mass, count = ref.lookup_grad(_np(v_out), ids.numpy(), v, scale)
     _close(grad, exact, (count[:, None] + 3) * U * mass, dtype, "v_table")
+
+
+# Groups around the ends of a part of 128 rows: none, one and several parts in
+# one call, and as many groups of two as the rows can fill.  The workspace is
+# exactly as long as the query says; what follows it stays.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("routed", [False, True])
+@pytest.mark.parametrize("want", ["both", "weight", "bias"])
+@pytest.mark.parametrize("sizes", [
+    [0, 1, 127, 128, 129, 0, 255, 256, 257, 385, 2, 0], [129] * 20, [0] * 70 + [300] + [0] * 70,
+    [128] * 9 + [129], [3] * 130])
+def test_grouped_parts_of_ragged_groups(sizes, want, routed, dtype):
+    n, e, k, m = sum(sizes) + 5, len(sizes), 40, 24
+    g = torch.Generator().manual_seed(e)
+    x, v_y = (torch.randn(n, d, generator=g).to(dtype) for d in (k, m))
+    weight = torch.zeros(e, m, k, dtype=dtype)
+    offsets = np.concatenate([[0], np.cumsum(sizes)])
+    rows = torch.randperm(n, generator=g) if routed else None
+    r = None if rows is None else rows.numpy()
+    _, (e_w, m_w), (e_b, m_b), count = ref.grouped_grad(_np(x), _np(weight), offsets, r, _np(v_y))
+    lib, code = _lib.load(), _ops._LATENT_TYPES[dtype]
+    need = lib.r2s_grouped_matmul_bwd_workspace_bytes(n, k, m, e, code, want != "bias")
+    ws = torch.full((need + 4096,), 0xAB, dtype=torch.uint8, device=DEV)
+    v_weight = torch.full((e, m, k), float("nan"), dtype=dtype, device=DEV)
+    v_bias = torch.full((e, m), float("nan"), dtype=dtype, device=DEV)
+    on = [t.to(DEV) for t in (x, v_y, torch.from_numpy(offsets).int())]
+    order = None if rows is None else rows.int().to(DEV)
+    assert lib.r2s_grouped_matmul_bwd(
+        on[0].data_ptr(), k, None, on[2].data_ptr(), None if order is None else order.data_ptr(),
+        on[1].data_ptr(), m, n, k, m, e, code, None,
+        None if want == "bias" else v_weight.data_ptr(),
+        None if want == "weight" else v_bias.data_ptr(), ws.data_ptr(), need,
+        torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert (ws[need:] == 0xAB).all()
+    if want != "bias":
+        _close(v_weight, e_w, (count[:, None, None] + 2) * U * m_w, dtype, "v_weight")
+    if want != "weight":
+        _close(v_bias, e_b, (count[:, None] + 2) * U * m_b, dtype, "v_bias")
