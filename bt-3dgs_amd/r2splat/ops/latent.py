@@ -17,7 +17,7 @@ of them.
 
 Activations, tables and weights are float32, bfloat16 or float16 CUDA
 tensors; sums and states are float32.  Gradients come from HIP kernels; they
-are not differentiable again.
+are not differentiable again, and forward-mode tangents are refused.
 """
 
 from __future__ import annotations
@@ -26,6 +26,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ..cuda import _wrapper as W
 
@@ -33,7 +34,14 @@ __all__ = ["embedding_lookup", "gated_scan", "gated_scan_step", "grouped_matmul"
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether the call goes through its autograd function: for a gradient, and
+    for a forward-mode tangent, which that function refuses (the kernels would
+    drop it)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    # Outside a dual level there is none to look for; looking costs 0.3 us a tensor.
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _index32(t: Optional[Tensor]) -> Optional[Tensor]:
