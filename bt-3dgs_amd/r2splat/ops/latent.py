@@ -114,6 +114,8 @@ def gated_scan(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
 def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tuple[Tensor, Tensor]:
     """(y, next state) after one more token of each of B sequences: x, gate
     [B, D], state [B, D] float32."""
+    if state is None:
+        raise RuntimeError("state must be given")
     if not _wants_grad(x, gate, state):
         return W.gated_scan_step(x, gate, state)
     y, final = gated_scan(x[:, None], gate[:, None], state)

@@ -76,3 +76,13 @@ def test_tangents_are_refused_rather_than_lost(monkeypatch):
         # Inputs without one are taken as ever.
         assert latent.embedding_lookup(t, ids, 2.0).equal(2.0 * t[ids])
         assert latent.grouped_matmul(t, t[None], off).equal(t @ t.T)
+
+
+def test_scan_step_needs_its_state_with_and_without_gradients(monkeypatch):
+    latent = _plain_wrapper(monkeypatch)
+    for wanted in (False, True):
+        x = torch.randn(4, 4, requires_grad=wanted)
+        with pytest.raises(RuntimeError, match="state must be given"):
+            latent.gated_scan_step(x, x, None)
+        y, _ = latent.gated_scan_step(x, x, torch.zeros(4, 4))
+        assert y.shape == (4, 4)
