@@ -102,9 +102,10 @@ def gated_scan(x: Tensor, gate: Tensor, initial: Optional[Tensor] = None,
     sequences).  ``initial`` [B or S, D] float32 is each sequence's history
     (zeros by default), ``final`` float32 its last state, y the states in x's
     type.  ``reverse`` runs each sequence from its last token.  A gate of +inf
-    holds the state whatever x is; one of -inf forgets it.  A NaN or infinity
-    elsewhere reaches the later states of its channel and sequence, until a
-    gate of -inf or until the gates' product leaves float32's range."""
+    holds the state whatever x is; one of -inf forgets it; finite gates beyond
+    87.3, whose smaller factor leaves float32's normal range, do the same.  A
+    NaN or infinity elsewhere reaches the later states of its channel and
+    sequence until a gate forgets it."""
     offsets = _index32(offsets)
     if not _wants_grad(x, gate, initial):
         return W.gated_scan_fwd(x, gate, initial, offsets, reverse, keep=False)[:2]

@@ -10,7 +10,9 @@ from oracle import latent as ref
 from r2splat.cuda import _lib, _ops
 from r2splat.cuda import _wrapper as W
 from r2splat.ops import latent
-from test_gpu_latent import DEV, TYPES, U, _close, _lookup_case, _np
+from test_gpu_latent import (DEV, TYPES, U, _check_scan, _close, _lookup_case, _np, _run_scan,
+                             _scan_case)
+from test_gpu_latent_paths import _check_equal, _equal_case, _run_equal
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +76,48 @@ def test_grouped_parts_of_ragged_groups(sizes, want, routed, dtype):
         _close(v_weight, e_w, (count[:, None, None] + 2) * U * m_w, dtype, "v_weight")
     if want != "weight":
         _close(v_bias, e_b, (count[:, None] + 2) * U * m_b, dtype, "v_bias")
+
+
+# A state that is not finite stays so to its sequence's end, however small the
+# product of the gates after it gets, whatever form the launch takes, until a
+# gate forgets it; its gradient, the other way, likewise.
+def _spoil(x, gate, v_y, seed):
+    g = torch.Generator().manual_seed(seed)
+    n, d = x.shape
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for t in (x, v_y):
+            t[torch.randint(0, n, (3,), generator=g), torch.randint(0, d, (3,), generator=g)] = bad
+    gate[torch.rand(n, d, generator=g) < 1.0 / 900.0] = -float("inf")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("n,d,kind", [(6000, 10, "one"), (9000, 64, "one"), (7000, 33, "ragged"),
+                                      (5000, 130, "one")])
+def test_scan_keeps_what_is_not_finite(n, d, kind, reverse, dtype):
+    x, gate, offsets, initial, v_y, v_final = _scan_case(n, d, kind, dtype, n + d)
+    _spoil(x, gate, v_y, d)
+    case = (x, gate, offsets, initial, v_y, v_final)
+    _check_scan(*case, reverse, _run_scan(*case, reverse))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("b,l,d", [(192, 600, 6), (1, 3000, 5), (2, 5000, 70)])
+def test_scan_of_equal_sequences_keeps_what_is_not_finite(b, l, d, reverse, dtype):
+    x, gate, initial, v_y, v_final = _equal_case(b, l, d, dtype, b + l + d)
+    _spoil(x.view(b * l, d), gate.view(b * l, d), v_y.view(b * l, d), l)
+    case = (x, gate, initial, v_y, v_final)
+    _check_equal(case, reverse, _run_equal(*case, reverse))
+
+
+def test_scan_ends_as_its_steps_do_after_a_nan():
+    x, gate = torch.ones(3, 900, 8, device=DEV), torch.full((3, 900, 8), -1.0, device=DEV)
+    x[1, 4], x[2, 4] = float("nan"), float("inf")
+    _, final = latent.gated_scan(x, gate)
+    state = torch.zeros(3, 8, device=DEV)
+    for t in range(900):
+        _, state = latent.gated_scan_step(x[:, t], gate[:, t], state)
+    assert torch.isnan(final[1]).all() and torch.isinf(final[2]).all()
+    assert torch.isnan(state[1]).all() and torch.isinf(state[2]).all()
+    assert torch.isfinite(final[0]).all()
