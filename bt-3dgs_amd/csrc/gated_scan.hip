@@ -6,7 +6,8 @@
 // the other; a sequence's first token has its initial state as history.
 // 1 - a is computed as sigmoid(-g), so neither factor cancels.  g = +inf
 // holds the state whatever x is (a term whose factor is 0 is dropped, not
-// multiplied); g = -inf forgets whatever the state was.
+// multiplied); g = -inf forgets whatever the state was.  So do finite gates
+// beyond 87.3, whose smaller factor is below float32's normal range: it is 0.
 //
 // A step is the affine map h -> p h + u with p = a, u = (1 - a) x, and maps
 // compose: (p2, u2) after (p1, u1) is (p2 p1, p2 u1 + u2).  A sequence's first
@@ -78,7 +79,9 @@ struct Tokens {
   }
 };
 
-// sigmoid(g) and sigmoid(-g), each to a few units in its own last place.
+// sigmoid(g) and sigmoid(-g).  The exponent is rounded before exp2, so the smaller
+// one is good to 2 |g| + 6 units of 2^-24 (|g| below 87.3; 0 beyond, where exp2
+// returns no subnormal numbers), the larger to a few.
 __device__ __forceinline__ void gate_pair(float g, float &a, float &b) {
   const float e = __builtin_amdgcn_exp2f(fabsf(g) * -1.44269504088896341f);
   const float r = __builtin_amdgcn_rcpf(1.0f + e), q = e * r;
@@ -748,7 +751,8 @@ __device__ __forceinline__ void block_and_slice(uint32_t slices, int64_t &block,
 }
 
 // The maps of the strips and of each block of them.  500k x 64 bf16: 35 us, the
-// tokens' 128 MB at 3.7 TB/s; 200k x 99 f32: 57 us forward and 37 back for 158 MB.
+// tokens' 128 MB at 3.7 TB/s; 200k x 99 f32: 58 us forward and 37 back for 158 MB,
+// of which 184 and 189 MB are read (see scan_bwd_kernel).
 template <typename T, int V, bool kBack>
 __global__ __launch_bounds__(kThreads) void scan_maps_kernel(
     const T *__restrict__ a, int64_t a_stride, const T *__restrict__ b, int64_t b_stride,
@@ -910,8 +914,10 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(
   walk_forward<T, V>(xr, gr, yr, initial, c, at, kept, final, h);
 }
 
-// The gradients, likewise.  200k x 99 f32: 106 us, 406 MB at 3.8 TB/s, bound by a
-// chunk's chain: three loads, the states, then the gradients token by token.
+// The gradients, likewise.  200k x 99 f32: 105 us, 535 MB at 5.1 TB/s, bound by
+// bytes, a quarter of which nobody needs: a row of 396 bytes is two blocks' slices,
+// and both fetch (and write parts of) the cache lines between them, 351 MB for
+// the 248 of operands and kept states and 184 for the 158 of gradients.
 template <typename T, int V, int kMode>
 __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t g_stride,
@@ -947,10 +953,11 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(
 // enters the next round.  So x and gate are read once, and a round's words are
 // on their way while the one before is worked on.  32 x 1024 x 1024 bf16 takes
 // 55 us forward (201 MB, 3.7 TB/s) and 77 us back (344 MB, 4.5 TB/s); with one
-// block of 8 waves per CU and 64 bytes of a row (8 x 4096 x 1024) 70 and 96 us,
-// where a round's chain of waits bounds it: the vector units are busy a third
-// of the time.  The packed form takes 185 us for the latter, its second reading
-// of the tokens included.
+// block of 8 waves per CU and 64 bytes of a row (8 x 4096 x 1024) 70 and 98 us,
+// where a round's chain of waits bounds it (for words, for the stores of the round
+// before, which the same counter holds, and for the other waves' maps): the
+// vector units are busy a third of the time.  The packed form takes 185 us for
+// the latter, its second reading of the tokens included.
 
 // What a block's round leaves in LDS: the maps of its waves' tokens.
 template <int V>
@@ -1000,7 +1007,8 @@ __device__ __forceinline__ void take_chunk(const uint32_t *words, Word (&x)[kChu
 #pragma unroll
   for (int k = 0; k < kChunk; ++k) x[k] = static_cast<Word>(words[k * kRoundThreads + threadIdx.x]);
 }
-// The words fetched for this round have arrived; those taken may be replaced.
+// The words fetched for this round have arrived (and the stores of the round before
+// are done: one counter holds both); those taken may be replaced.
 __device__ __forceinline__ void words_arrived() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }

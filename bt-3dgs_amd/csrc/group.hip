@@ -2,9 +2,10 @@
 // the row lookup's gradient and for the groups of a grouped product.
 //
 // The ids lie in [0, n_groups); any other sorts behind them.  Short lists take
-// one launch (short_list_kernel), others passes of at most 9 bits (one for up to 511 groups, two for up to 2^18 - 1).  A pass cuts
-// the list into at most kMaxTiles tiles of equal length and is two launches: the
-// digit counts of every tile, then the scatter, whose blocks each add up the
+// one launch (short_list_kernel), others passes of at most 9 bits (one for up to
+// 511 groups, two for up to 2^18 - 1) and, after more than one, a launch for the
+// offsets.  A pass cuts the list into at most kMaxTiles tiles of equal length and
+// is two launches: the digit counts of every tile, then the scatter, whose blocks each add up the
 // counts table themselves (at most kTableWords words, every thread a few
 // dozen loads in parallel) instead of a scan between the two.  Lists this short
 // are bound by launches and waits, not by bytes: 500k ids of 4096 groups,

@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRows = 128;      // output rows of a block's tile
-constexpr int kWindow = 512;     // row numbers of a weights' gradient block in LDS, twice
+constexpr int kWindow = 512;    // row numbers of a weights' gradient block in LDS, twice
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
@@ -131,7 +131,10 @@ __device__ __forceinline__ void stage_barrier() {
 //   across  [S / sizeof(T) summed][R sizeof(T) / 16 slots], slot s of index c at
 //           s ^ swizzle(c),
 // so that the lanes that read together hit different ones of the 64 banks
-// although LDS is filled in order by loads that go straight there.
+// although LDS is filled in order by loads that go straight there.  The across
+// order is made for tiles whose rows are in order (the weights' gradient).  Read
+// in runs (the input's gradient) its lanes lie 16 columns apart and meet in
+// banks, four at a time in tiles of 128 columns and two in those of 64.
 // kRun: the tile's rows are taken kRun apart, four at a time (see Accumulator);
 // 0: in order.
 template <int S, int kRun>
@@ -383,12 +386,13 @@ __device__ __forceinline__ void store_run(T *row, int64_t col, int64_t width,
 // over m).  Blocks of one row tile are neighbours, and neighbours share an XCD:
 // they read the same rows and weight.
 //
-// 16k x 1024 x 1024 bf16 in 16 groups: 65 us forward (530 TFLOP/s; 930 for one
-// library product of these sizes), 68 us back, bound by a stage's wait, by its
-// LDS reads, which take as long as its products, and by 1160 blocks, of which
-// the last run alone; at 32k x 2048 x 2048, 790 TFLOP/s.  500k x 64 x 64 bf16:
-// 35 us forward, 128 MB at 3.7 TB/s, bound by the writes.  50k x 45 x 11 f32:
-// 13 us, bound by the launch and a block's chain of offsets, rows, tile, store.
+// 16k x 1024 x 1024 bf16 in 16 groups: 66 us forward (520 TFLOP/s; 930 for one
+// library product of these sizes), 69 us back (6.7e6 cycles of bank conflicts on
+// 1.7e6 LDS instructions; none forward), bound by a stage's wait, by its LDS
+// reads, which take as long as its products, and by 1160 blocks, of which the
+// last run alone; at 32k x 2048 x 2048, 790 TFLOP/s.  500k x 64 x 64 bf16: 35 us
+// forward, 128 MB at 3.7 TB/s, bound by the writes.  50k x 45 x 11 f32: 13 us,
+// bound by the launch and a block's chain of offsets, rows, tile, store.
 template <typename T, bool kBack, bool kVec, int kCols, int S>
 __global__ __launch_bounds__(kThreads, kCols == 64 ? (kVec ? 4 : 3) : 2) void rows_kernel(
     const T *__restrict__ in, int64_t stride, const T *__restrict__ weight,
@@ -740,9 +744,10 @@ __global__ __launch_bounds__(kThreads) void add_parts_kernel(
 
 // Bytes of the summed index per stage.  Operands read across and tiles of 128
 // columns take 64: four blocks share a CU instead of two.  16k x 1024 x 1024
-// bf16: forward 56 us with 128 bytes and 60 with 64, input gradient 80 and 70,
-// weights' gradient 142 and 95; 500k x 64 x 64, where tiles have 64 columns:
-// weights' gradient 32 and 36.
+// bf16: input gradient 78 us with 128 bytes and 69 with 64, weights' gradient 119
+// and 97; 500k x 64 x 64, where tiles have 64 columns: weights' gradient 33 and
+// 37, input gradient 31 both ways.  Operands read along take 128, as runs of
+// columns need (along_swizzle).
 constexpr int slab_bytes(bool across, int cols) { return across && cols == 128 ? 64 : 128; }
 
 int64_t weight_tiles(int64_t k, int64_t m) {
@@ -751,7 +756,10 @@ int64_t weight_tiles(int64_t k, int64_t m) {
 
 // Rows of a part of the weights' gradient: enough parts to fill the device,
 // and no more, since every part of a group past its first is a copy of the
-// weight to write and add.  At least 512 rows where 16-bit products of many
+// weight to write and add.  Blocks in all, weights' kernel and the parts' sum:
+// 500k x 64 x 64 bf16 (1 tile) 39 us with 768 and 47 with 1152, 100k x 256 x 256
+// (4) 54 and 66, 8000 x 512 x 512 f32 (16) 75 and 75, 28k x 256 x 1024 bf16 (16)
+// 54 and 61, 16k x 1024 x 1024 (64) 120 and 110.  At least 512 rows where 16-bit products of many
 // tiles take less time than that: 4000 x 1024 x 1024 bf16, forward and back,
 // 73 us and 84 with 128, 28k x 256 x 1024 133 and 136; 32-bit products are slower
 // and need the parts: 8000 x 512 x 512 188 us, and 208 with 512.

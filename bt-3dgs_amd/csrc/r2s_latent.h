@@ -1,6 +1,6 @@
 // Shared pieces of the latent decoder's operators (lookup.hip,
 // gated_scan.hip, grouped.hip): element types, vectors of them, and the
-// stable sort of ids that binning.hip provides.
+// stable sort of ids that group.hip provides.
 #pragma once
 
 #include <initializer_list>

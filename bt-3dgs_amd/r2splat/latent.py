@@ -2,8 +2,10 @@
 
 The reference trains 11 free numbers per Gaussian.  ``LatentDecoder`` gives
 each Gaussian a code instead: a row of a shared codebook, mixed along the
-table's order (a tree grown by splits keeps relatives together) by a gated
-recurrence both ways, and mapped to 11 numbers by one weight per tree level.
+table's order by a gated recurrence both ways, and mapped to 11 numbers by one
+weight per tree level.  A split appends its children in their parents' order,
+first all of one side, then all of the other, so the recurrence mixes each
+generation in the order of the one before; siblings lie far apart.
 Its output is added to a base table, so a decoder at its initial weights
 leaves the base as it is.  No reference counterpart.
 

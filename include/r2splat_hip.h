@@ -1171,7 +1171,8 @@ int r2s_embedding_bwd(const void *v_out, int64_t v_out_stride, const void *ids,
  * zeros) is the history of each sequence's first token, final_state
  * [sequences, width] the state after its last (its initial one if it is
  * empty); y [n, width] contiguous.  A gate of +inf holds the state whatever x
- * is, one of -inf forgets it whatever it was.
+ * is, one of -inf forgets it whatever it was, and finite ones beyond 87.3 do the
+ * same (their smaller factor is below float32's normal range).
  * kept [r2s_gated_scan_kept_rows(...), width] (may be NULL: no backward
  * follows) receives the states that the backward starts from; the decode form
  * (offsets NULL, length 1) leaves it alone.  ragged: offsets are given.  Rows
