@@ -38,6 +38,9 @@ SOURCES = [
     "lookup.hip",
     "gated_scan.hip",
     "grouped.hip",
+    "rotary.hip",
+    "residual_norm.hip",
+    "adamw.hip",
 ]
 
 ARCH = os.environ.get("R2S_OFFLOAD_ARCH", "gfx950")

@@ -1,5 +1,5 @@
-// Shared pieces of the latent decoder's operators (lookup.hip,
-// gated_scan.hip, grouped.hip): element types, vectors of them, and the
+// Shared pieces of the latent decoder's operators (lookup.hip, gated_scan.hip,
+// grouped.hip, rotary.hip, residual_norm.hip) and of adamw.hip: element types, vectors of them, and the
 // stable sort of ids that group.hip provides.
 #pragma once
 
@@ -34,7 +34,7 @@ inline bool known_type(int type) {
   return type == R2S_TYPE_F32 || type == R2S_TYPE_BF16 || type == R2S_TYPE_F16;
 }
 
-inline uint64_t address(const void *p) { return reinterpret_cast<uint64_t>(p); }
+__host__ __device__ inline uint64_t address(const void *p) { return reinterpret_cast<uint64_t>(p); }
 
 // Stable grouping of n ids by value (group.hip): order [n] receives the
 // positions sorted by (id, position), ids outside [0, n_groups) last; keys [n]

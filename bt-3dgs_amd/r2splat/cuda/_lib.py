@@ -142,6 +142,15 @@ _PLAIN = {
     "r2s_grouped_matmul_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i32, _i32]),
     "r2s_grouped_matmul_bwd": (_i32, [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                                       _i32, _p, _p, _p, _p, _sz, _p]),
+    "r2s_adamw_step": (_i32, [_p, _i32, _p]),
+    "r2s_rotary_axes": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i32, _p, _i32,
+                               _i32, _f64, _i32, _i32, _i32, _i64, _i64, _p, _p, _p]),
+    "r2s_residual_norm_fwd": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _f32, _f32, _i32,
+                                     _i32, _i64, _i64, _p, _p, _p]),
+    "r2s_residual_norm_bwd_workspace_bytes": (_i64, [_i32, _i64, _i64]),
+    "r2s_residual_norm_bwd": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _i64, _p,
+                                     _i64, _f32, _f32, _i32, _i32, _i64, _i64, _p, _p, _p, _p, _p,
+                                     _p, _sz, _p]),
 }
 
 
@@ -169,16 +178,29 @@ class AdamTensor(ctypes.Structure):
                 ("step_size", _f32)]
 
 
+class AdamwTensor(ctypes.Structure):
+    """r2s_adamw_tensor_t: one parameter tensor of an AdamW step."""
+
+    _fields_ = [("param", _p), ("grad", _p), ("master", _p), ("exp_avg", _p), ("second", _p),
+                ("exp_avg_scale", _p), ("second_scale", _p), ("n", _i64), ("beta1", _f32),
+                ("lerp_weight", _f32), ("beta2", _f32), ("one_minus_beta2", _f32),
+                ("keep", _f32), ("bias_correction2_sqrt", _f32), ("eps", _f32),
+                ("step_size", _f32), ("type", ctypes.c_int32), ("step", _u32)]
+
+
 # Column roles (R2S_COL_* in include/r2splat_hip.h).
 COL_COPY, COL_ZERO_NEW, COL_MEANS, COL_RAW_SCALES, COL_RAW_OPACITIES, COL_PARENT, COL_LEVEL, \
     COL_HISTORY = range(8)
 DENSIFY_MAX_WIDTH = 16
 # Element types of the latent decoder's operators (R2S_TYPE_*).
 TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
+# Types of rotary positions (R2S_POSITION_*) and the most axes of them.
+POSITION_F32, POSITION_I32, POSITION_I64 = range(3)
+ROTARY_MAX_AXES = 8
 
 SYMBOLS = sorted(list(_PLAIN) + [f"r2s_{n}_{s}" for n in _FLOAT_OPS for s in ("f32", "f64")])
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 
 def load(path: str = LIB_PATH) -> ctypes.CDLL:

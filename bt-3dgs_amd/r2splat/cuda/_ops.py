@@ -2188,3 +2188,157 @@ def grouped_matmul_bwd(x: Tensor, weight: Tensor, offsets: Tensor, rows: Optiona
               _ptr(v_y), vs, n, k, m, e, code, _ptr(v_x), _ptr(v_weight), _ptr(v_bias), _ptr(ws),
               need, _stream(dev))
     return v_x, v_weight, v_bias
+
+
+# -- rotary positions
+
+
+_POSITION_TYPES = {torch.float32: L.POSITION_F32, torch.int32: L.POSITION_I32,
+                   torch.int64: L.POSITION_I64}
+
+
+def _heads_3d(t: Tensor, name: str, n: int):
+    """(tensor, token stride, head stride, heads) of [..., H, D] as [n, H, D]; a
+    copy where a head's elements are not consecutive or the tokens have no one
+    stride."""
+    heads, d = t.shape[-2:]
+    if t.dim() != 3:
+        t = t.reshape(n, heads, d)
+    if d > 1 and t.stride(2) != 1:
+        t = t.contiguous()
+    return t, t.stride(0), t.stride(1), heads
+
+
+def rotary_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, sections, base: float = 1e4,
+                interleaved: bool = False, shared: bool = False, inverse: bool = False
+                ) -> Tuple[Tensor, Optional[Tensor]]:
+    """(q', k') with every head's pairs of channels turned by positions times
+    frequencies; ``inverse`` turns back (the gradient).  q [..., H, D], k
+    [..., Hk, D] or None, positions [..., A] int32, int64 or float32, sections A
+    numbers of pairs."""
+    _check_latent(q, "q")
+    code = _latent_type(q, "rotary_axes")
+    if q.dim() < 2:
+        _fail("q must be [..., H, D], got shape ", tuple(q.shape))
+    lead, d = q.shape[:-2], q.shape[-1]
+    if k is not None:
+        _check_latent(k, "k", q, q.dtype)
+        if k.dim() < 2 or k.shape[:-2] != lead or k.shape[-1] != d:
+            _fail("k must be [..., Hk, D] beside q ", tuple(q.shape), ", got shape ",
+                  tuple(k.shape))
+    _check_latent(positions, "positions", q)
+    kind = _POSITION_TYPES.get(positions.dtype)
+    if kind is None:
+        _fail("positions must be float32, int32 or int64, got ", positions.dtype)
+    sections = tuple(int(s) for s in sections)
+    axes = len(sections)
+    if not 1 <= axes <= L.ROTARY_MAX_AXES:
+        _fail("sections must name 1 to ", L.ROTARY_MAX_AXES, " axes, got ", axes)
+    if positions.shape != (*lead, axes):
+        _fail("positions must be ", (*lead, axes), ", got shape ", tuple(positions.shape))
+    if min(sections) < 0 or 2 * sum(sections) > d:
+        _fail("sections ", sections, " are not pairs of ", d, " channels")
+    n = math.prod(lead)
+    qr, qt, qh, hq = _heads_3d(q, "q", n)
+    kr, kt, kh, hk = (None, 0, 0, 0) if k is None else _heads_3d(k, "k", n)
+    positions = positions.contiguous()
+    dev = q.device
+    with _on(dev):
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+        _call("r2s_rotary_axes", _ptr(qr), qt, qh, hq, _ptr(kr), kt, kh, hk, _ptr(positions), kind,
+              (ctypes.c_int32 * axes)(*sections), axes, bool(shared), float(base),
+              bool(interleaved), bool(inverse), code, n, d, _ptr(q_out), _ptr(k_out), _stream(dev))
+    return q_out, k_out
+
+
+# -- norms around a block
+
+
+def _norm_rows(t: Optional[Tensor], name: str, x: Tensor):
+    """(tensor of rows, row stride) of an input of x's shape, or (None, 0)."""
+    if t is None:
+        return None, 0
+    if t is not x:
+        _check_latent(t, name, x, x.dtype)
+        if t.shape != x.shape:
+            _fail(name, " must have the shape of x ", tuple(x.shape), ", got ", tuple(t.shape))
+    d = t.shape[-1]
+    return _rows_2d(t if t.dim() == 2 else t.reshape(-1, d) if t.numel() else t.new_empty(0, d))
+
+
+def _norm_weight(t: Optional[Tensor], name: str, x: Tensor) -> Optional[Tensor]:
+    if t is None:
+        return None
+    _check_latent(t, name, x, x.dtype)
+    if t.shape != x.shape[-1:]:
+        _fail(name, " must be [", x.shape[-1], "], got shape ", tuple(t.shape))
+    return t.contiguous()
+
+
+def _norm_inputs(x, update, gate, update_weight, weight, op):
+    """The checked inputs as the C entries take them, and (n, d)."""
+    _check_latent(x, "x")
+    code = _latent_type(x, op)
+    if x.dim() < 1:
+        _fail("x must be [..., D], got a scalar")
+    d = x.shape[-1]
+    if update is None and (gate is not None or update_weight is not None):
+        _fail("a gate or an update's weight needs an update")
+    xr, xs = _norm_rows(x, "x", x)
+    ur, us = _norm_rows(update, "update", x)
+    kind, gr, gs = 0, None, 0
+    if gate is not None:
+        if isinstance(gate, Tensor) and gate.shape == (d,) and x.dim() > 1:
+            kind, gr = 2, _norm_weight(gate, "gate", x)
+        else:
+            kind, (gr, gs) = 1, _norm_rows(gate, "gate", x)
+    w1 = _norm_weight(update_weight, "update_weight", x)
+    w2 = _norm_weight(weight, "weight", x)
+    n = math.prod(x.shape[:-1])
+    return (xr, xs, ur, us, gr, gs, kind, w1, w2), code, n, d
+
+
+def residual_norm_fwd(x: Tensor, update: Optional[Tensor], gate: Optional[Tensor],
+                      update_weight: Optional[Tensor], weight: Optional[Tensor],
+                      scale: float = 1.0, eps: float = 1e-6, centered: bool = False
+                      ) -> Tuple[Tensor, Optional[Tensor]]:
+    """(y, u) with y = x + scale sigmoid(gate) norm(update) update_weight and
+    u = norm(y) weight (None without a weight).  y is x itself without an update;
+    the update is not normalised without its weight.  gate: x's shape, or [D] for
+    all rows."""
+    (xr, xs, ur, us, gr, gs, kind, w1, w2), code, n, d = _norm_inputs(
+        x, update, gate, update_weight, weight, "residual_norm_fwd")
+    dev = x.device
+    with _on(dev):
+        y = x if update is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        u = None if weight is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        _call("r2s_residual_norm_fwd", _ptr(xr), xs, _ptr(ur), us, _ptr(gr), gs, kind, _ptr(w1),
+              _ptr(w2), float(scale), float(eps), bool(centered), code, n, d,
+              None if update is None else _ptr(y), _ptr(u), _stream(dev))
+    return y, u
+
+
+def residual_norm_bwd(x: Tensor, update: Optional[Tensor], gate: Optional[Tensor],
+                      update_weight: Optional[Tensor], weight: Optional[Tensor],
+                      v_y: Optional[Tensor], v_u: Optional[Tensor], scale: float = 1.0,
+                      eps: float = 1e-6, centered: bool = False, want=(True,) * 5):
+    """(v_x, v_update, v_gate, v_update_weight, v_weight) of residual_norm_fwd
+    from v_y and v_u; None for inputs that are not there or not wanted."""
+    (xr, xs, ur, us, gr, gs, kind, w1, w2), code, n, d = _norm_inputs(
+        x, update, gate, update_weight, weight, "residual_norm_bwd")
+    if v_u is not None and weight is None:
+        _fail("v_u needs the weight of u")
+    yr, ys = _norm_rows(v_y, "v_y", x)
+    vr, vs = _norm_rows(v_u, "v_u", x)
+    dev = x.device
+    lib = _lib()
+    with _on(dev):
+        grads = [torch.empty(t.shape, dtype=x.dtype, device=dev) if w and t is not None else None
+                 for w, t in zip(want, (x, update, gate, update_weight, weight))]
+        need = lib.r2s_residual_norm_bwd_workspace_bytes(code, n, d)
+        ws = _workspace(need, dev)
+        _call("r2s_residual_norm_bwd", _ptr(xr), xs, _ptr(ur), us, _ptr(gr), gs, kind, _ptr(w1),
+              _ptr(w2), _ptr(yr), ys, _ptr(vr), vs, float(scale), float(eps), bool(centered), code,
+              n, d, *(_ptr(g) for g in grads), _ptr(ws), need, _stream(dev))
+    return tuple(grads)

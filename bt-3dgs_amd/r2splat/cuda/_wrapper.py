@@ -65,6 +65,9 @@ gated_scan_step = _make_cuda_func("gated_scan_step")
 gated_scan_bwd = _make_cuda_func("gated_scan_bwd")
 grouped_matmul_fwd = _make_cuda_func("grouped_matmul_fwd")
 grouped_matmul_bwd = _make_cuda_func("grouped_matmul_bwd")
+rotary_axes = _make_cuda_func("rotary_axes")
+residual_norm_fwd = _make_cuda_func("residual_norm_fwd")
+residual_norm_bwd = _make_cuda_func("residual_norm_bwd")
 
 
 def is_cuda_extension_available() -> bool:

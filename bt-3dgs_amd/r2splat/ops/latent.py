@@ -13,7 +13,11 @@ of them.
   a_t = sigmoid(gate_t), over equal or ragged sequences of any length, and
   ``gated_scan_step`` for one more token of running sequences;
 * ``grouped_matmul``    one weight per group of rows, groups of any size, the
-  groups' rows anywhere in the table; ``group_rows`` finds them.
+  groups' rows anywhere in the table; ``group_rows`` finds them;
+* ``rotary_axes``       queries and keys turned by their positions along several
+  axes;
+* ``pre_norm``, ``residual_norm``  the norms before and after a block, with its
+  gate and the residual stream between them.
 
 Activations, tables and weights are float32, bfloat16 or float16 CUDA
 tensors; sums and states are float32.  Gradients come from HIP kernels; they
@@ -22,7 +26,7 @@ are not differentiable again, and forward-mode tangents are refused.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -30,7 +34,8 @@ from torch.autograd import forward_ad
 
 from ..cuda import _wrapper as W
 
-__all__ = ["embedding_lookup", "gated_scan", "gated_scan_step", "grouped_matmul", "group_rows"]
+__all__ = ["embedding_lookup", "gated_scan", "gated_scan_step", "grouped_matmul", "group_rows",
+           "rotary_axes", "pre_norm", "residual_norm"]
 
 
 def _wants_grad(*tensors) -> bool:
@@ -156,3 +161,104 @@ def group_rows(ids: Tensor, n_groups: int) -> Tuple[Tensor, Tensor]:
     """(rows [N], offsets [n_groups + 1]), int32: the positions of ids [N] in
     stable order of their id, those of ids outside [0, n_groups) last."""
     return W.group_rows(ids, n_groups)
+
+
+def _refuse_grad(t, name: str) -> None:
+    """For an input that the kernels give no derivative for."""
+    if t is not None and _wants_grad(t):
+        raise NotImplementedError(f"{name} must not require a gradient")
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, plan):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.plan = plan
+        return W.rotary_axes(q, k, positions, *plan)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, v_q, v_k):
+        (positions,) = ctx.saved_tensors
+        if v_q is None:  # alone, the keys' gradient takes the queries' place
+            v_k, _ = (None, None) if v_k is None else W.rotary_axes(
+                v_k, None, positions, *ctx.plan, inverse=True)
+            return None, v_k, None, None
+        return (*W.rotary_axes(v_q, v_k, positions, *ctx.plan, inverse=True), None, None)
+
+
+def rotary_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, sections: Sequence[int],
+                base: float = 1e4, interleaved: bool = False, shared: bool = False
+                ) -> Tuple[Tensor, Optional[Tensor]]:
+    """(q', k'): pairs (a, b) of each head's channels turned to
+    ``(a cos t - b sin t, b cos t + a sin t)``, so that the product of a query and
+    a key depends on where they are to each other along each axis.
+
+    q [..., H, D], k [..., Hk, D] (or None), positions [..., A] int32, int64 or
+    float32, the tokens' places on A axes.  ``sections[a]`` pairs belong to axis
+    a; pair i of its m has ``t = position[a] base^(-i / m)``, or with ``shared``
+    i and m count all pairs of all axes.  With R pairs in all, pair j is channels
+    j and R + j, or with ``interleaved`` 2j and 2j + 1; channels from 2R on stay
+    as they are.  Angles are exact to a float32 turn for positions up to 2^31.
+    Positions have no gradient."""
+    _refuse_grad(positions, "positions")
+    plan = (tuple(sections), float(base), bool(interleaved), bool(shared))
+    if not _wants_grad(q, k):
+        return W.rotary_axes(q, k, positions, *plan)
+    return _Rotary.apply(q, k, positions, plan)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, update, gate, update_weight, weight, plan):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, update, gate, update_weight, weight)
+        ctx.plan = plan
+        y, u = W.residual_norm_fwd(x, update, gate, update_weight, weight, *plan)
+        return (u,) if update is None else (y,) if weight is None else (y, u)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        x, update, gate, update_weight, weight = ctx.saved_tensors
+        v_y, v_u = (None, *grads) if update is None else (*grads, None)[:2]
+        if v_y is None and v_u is None:
+            return (None,) * 6
+        return (*W.residual_norm_bwd(x, update, gate, update_weight, weight, v_y, v_u, *ctx.plan,
+                                     want=ctx.needs_input_grad[:5]), None)
+
+
+def pre_norm(x: Tensor, weight: Tensor, eps: float = 1e-6, centered: bool = False) -> Tensor:
+    """``norm(x) * weight`` over the last dimension (at most 8192 channels):
+    ``norm(x) = x / sqrt(mean(x^2) + eps)``, with ``centered`` of x less its mean.
+    x [..., D], weight [D]."""
+    if weight is None:
+        raise RuntimeError("weight must be given")
+    plan = (1.0, float(eps), bool(centered))
+    if not _wants_grad(x, weight):
+        return W.residual_norm_fwd(x, None, None, None, weight, *plan)[1]
+    return _ResidualNorm.apply(x, None, None, None, weight, plan)[0]
+
+
+def residual_norm(x: Tensor, update: Tensor, gate: Optional[Tensor] = None,
+                  update_weight: Optional[Tensor] = None, weight: Optional[Tensor] = None,
+                  scale: float = 1.0, eps: float = 1e-6, centered: bool = False
+                  ) -> Tuple[Tensor, Optional[Tensor]]:
+    """(y, u): a block's output joined to the stream, and the norm before the
+    next block, in one pass::
+
+        y = x + scale * sigmoid(gate) * norm(update) * update_weight
+        u = norm(y) * weight
+
+    x, update [..., D]; gate of their shape or [D] for all rows (none: 1); without
+    ``update_weight`` the update is not normalised, without ``weight`` u is None.
+    ``norm`` is that of ``pre_norm``; u is made from y before y is rounded to its
+    type."""
+    if update is None:
+        raise RuntimeError("update must be given")
+    plan = (float(scale), float(eps), bool(centered))
+    if not _wants_grad(x, update, gate, update_weight, weight):
+        return W.residual_norm_fwd(x, update, gate, update_weight, weight, *plan)
+    out = _ResidualNorm.apply(x, update, gate, update_weight, weight, plan)
+    return out if weight is not None else (out[0], None)

@@ -1,4 +1,5 @@
-"""Adam for the Gaussian parameter groups, stepped by one HIP launch.
+"""Adam for the Gaussian parameter groups, stepped by one HIP launch, and
+AdamW for a latent decoder's.
 
 The binary-tree trainer builds one ``torch.optim.Adam`` per parameter group
 (``src/models/gaussian_model.py:514-530``) and steps them one after another
@@ -15,6 +16,9 @@ The binary-tree trainer builds one ``torch.optim.Adam`` per parameter group
 Supported: float32 CUDA parameters, dense gradients, coupled weight decay;
 not amsgrad, maximize, capturable, differentiable or fused -- those raise
 ``NotImplementedError`` (the reference uses none of them).
+
+``AdamW`` (no reference counterpart) steps float32, bfloat16 and float16
+parameters with decoupled weight decay; its states are float32 or 8 bits.
 """
 
 from __future__ import annotations
@@ -28,12 +32,16 @@ from torch.optim.optimizer import _get_scalar_dtype
 from .cuda import _backend
 from .cuda import _lib as L
 
-__all__ = ["Adam", "step_all"]
+__all__ = ["Adam", "AdamW", "step_all"]
 
 
 def _check_group(group: dict) -> None:
-    for key in ("amsgrad", "maximize", "capturable", "differentiable", "fused",
-                "decoupled_weight_decay"):
+    _check_options(group, ("amsgrad", "maximize", "capturable", "differentiable", "fused",
+                           "decoupled_weight_decay"))
+
+
+def _check_options(group: dict, refused) -> None:
+    for key in refused:
         if group.get(key):
             raise NotImplementedError(f"the fused Adam step does not support {key}=True")
     for key in ("lr", "eps", "weight_decay"):
@@ -139,3 +147,159 @@ class Adam(torch.optim.Adam):
         _entries(self, entries, keep)
         _launch(entries, _device_of([self]))
         return loss
+
+
+# Elements that share a scale of 8-bit states, and the fewest that a tensor has
+# whose states are kept in 8 bits: below, the scales' and the launch's share is
+# larger than what is saved.
+_RUN = 256
+_FEWEST_8BIT = 4096
+_PARAM_TYPES = {torch.float32: L.TYPE_F32, torch.bfloat16: L.TYPE_BF16,
+                torch.float16: L.TYPE_F16}
+# State tensors of an element each, and of a run each.
+_STATE_32 = ("exp_avg", "exp_avg_sq")
+_STATE_8 = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` over float32, bfloat16 and float16 CUDA parameters
+    (gradients of their type), one launch for every 32 tensors of a device.
+
+    The step is made in float32.  A 16-bit parameter keeps a float32 copy in its
+    state (``master``), taken at its first step, and is that copy's rounding
+    after every step: what is written to the parameter in between is lost.  With
+    ``state_bits=32`` the states are torch's (``exp_avg``, ``exp_avg_sq``) and so
+    is the arithmetic, bit for bit in float32.  With ``state_bits=8`` tensors of
+    at least 4096 elements keep float8 codes of the average (``exp_avg``) and of
+    the root of the average of squares (``exp_avg_sq_root``) with a float32 scale
+    for every 256 elements (``exp_avg_scale``, ``exp_avg_sq_root_scale``): a code
+    times its scale is the value.  Codes are rounded up by chance, the chances a
+    function of the element's index and the step, so that a run can be repeated
+    bit for bit.  A gradient that is not finite makes its own element NaN.
+
+    The step's scalars come from the host: ``step()`` refuses to be captured into
+    a graph, where they would stay those of the capture."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 state_bits=32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not isinstance(lr, torch.Tensor) and lr < 0.0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not isinstance(eps, torch.Tensor) and eps < 0.0:
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        for i, beta in enumerate(betas):
+            if not isinstance(beta, torch.Tensor) and not 0.0 <= beta < 1.0:
+                raise ValueError(f"Invalid beta parameter at index {i}: {beta}")
+        if not isinstance(weight_decay, torch.Tensor) and weight_decay < 0.0:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits))
+        for group in self.param_groups:
+            _check_options(group, ())
+
+    def _new_state(self, p: torch.Tensor, bits: int) -> None:
+        state = self.state[p]
+        state["step"] = 0
+        if p.dtype != torch.float32:
+            state["master"] = p.detach().float()
+        if bits == 8 and p.numel() >= _FEWEST_8BIT:
+            runs = -(-p.numel() // _RUN)
+            for name in _STATE_8[::2]:
+                state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
+                state[name + "_scale"] = torch.zeros(runs, dtype=torch.float32, device=p.device)
+        else:
+            for name in _STATE_32:
+                state[name] = torch.zeros_like(p, dtype=torch.float32)
+
+    @staticmethod
+    def _state_tensors(p: torch.Tensor, state: dict) -> tuple:
+        """(master, average, second, their scales), None for those that are not
+        there, checked: the kernel takes their addresses."""
+        runs, n = (-(-p.numel() // _RUN),), p.shape
+        master = (n, torch.float32) if p.dtype != torch.float32 else None
+        if "exp_avg_sq_root" in state:
+            names = ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
+            wanted = ((n, torch.float8_e4m3fn),) * 2 + ((runs, torch.float32),) * 2
+        else:
+            names = ("exp_avg", "exp_avg_sq", None, None)
+            wanted = ((n, torch.float32),) * 2 + (None, None)
+        out = []
+        for name, want in zip(("master", *names), (master, *wanted)):
+            t = state.get(name)
+            if want is None:
+                out.append(None)
+                continue
+            if not isinstance(t, torch.Tensor) or t.shape != want[0] or t.dtype != want[1] \
+                    or t.device != p.device or not t.is_contiguous():
+                raise RuntimeError(f"AdamW state {name!r} does not match its parameter")
+            out.append(t)
+        return tuple(out)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work: dict = {}  # device -> (entries, tensors kept until the launch)
+        for group in self.param_groups:
+            _check_options(group, ())
+            lr, (beta1, beta2) = group["lr"], group["betas"]
+            fixed = beta1, 1 - beta1, beta2, 1 - beta2, 1 - lr * group["weight_decay"]
+            eps = group["eps"]
+            for p in group["params"]:
+                grad = p.grad
+                if grad is None:
+                    continue
+                if grad.is_sparse:
+                    raise RuntimeError("AdamW does not support sparse gradients")
+                kind = _PARAM_TYPES.get(p.dtype)
+                if kind is None or not p.is_cuda:
+                    raise NotImplementedError("the fused AdamW step needs float32, bfloat16 or "
+                                              "float16 CUDA parameters")
+                if not p.is_contiguous():
+                    raise NotImplementedError("the fused AdamW step needs contiguous parameters")
+                if grad.dtype != p.dtype or grad.device != p.device or grad.shape != p.shape:
+                    raise RuntimeError("AdamW gradient does not match its parameter")
+                if p.device not in work:
+                    with torch.cuda.device(p.device):
+                        if torch.cuda.is_current_stream_capturing():
+                            raise RuntimeError("AdamW.step cannot be captured into a graph")
+                    work[p.device] = [], []
+                entries, kept = work[p.device]
+                state = self.state[p]
+                if not state:
+                    self._new_state(p, group["state_bits"])
+                tensors = self._state_tensors(p, state)
+                grad = grad.contiguous()
+                state["step"] = step = int(state["step"]) + 1
+                entries.append(L.AdamwTensor(
+                    p.data_ptr(), grad.data_ptr(),
+                    *[None if t is None else t.data_ptr() for t in tensors], p.numel(), *fixed,
+                    (1 - beta2 ** step) ** 0.5, eps, -lr / (1 - beta1 ** step), kind,
+                    step & 0xFFFFFFFF))
+                kept.append(grad)
+        lib = _backend.library() if work else None
+        for device, (entries, _) in work.items():
+            table = (L.AdamwTensor * len(entries))(*entries)
+            with torch.cuda.device(device):
+                rc = lib.r2s_adamw_step(ctypes.cast(table, ctypes.c_void_p), len(entries),
+                                        torch.cuda.current_stream(device).cuda_stream)
+            if rc != 0:
+                raise RuntimeError(f"r2s_adamw_step failed ({rc}): "
+                                   f"{lib.r2s_last_error().decode(errors='replace')}")
+        return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """torch's, with the states in the types that they were saved in (torch
+        casts them to their parameters')."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            for name, t in saved.get(i, {}).items():
+                if name != "step" and isinstance(t, torch.Tensor):
+                    self.state[p][name] = t.detach().to(p.device, copy=True).contiguous()

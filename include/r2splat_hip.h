@@ -1127,6 +1127,41 @@ typedef struct r2s_adam_tensor {
 int r2s_adam_step_f32(const r2s_adam_tensor_t *tensors, int32_t n_tensors,
                       r2s_stream_t stream);
 
+/* One tensor of an AdamW step.  param and grad are of the element type;
+ * master (float32) goes with a 16-bit param, which becomes its rounding, and is
+ * NULL for a float32 one.  exp_avg and second are either float32 (the second the
+ * average of squares) with both scales NULL, or float8 e4m3 codes (the second
+ * those of the square root of that average) with a float32 scale for every 256
+ * elements: ceil(n / 256) each.  The step's scalars are the caller's:
+ *   beta1, lerp_weight = 1 - beta1, beta2, one_minus_beta2 = 1 - beta2,
+ *   keep = 1 - lr weight_decay, bias_correction2_sqrt = (1 - beta2^t)^0.5,
+ *   step_size = -lr / (1 - beta1^t), step = t modulo 2^32 (8-bit states round up
+ * with chances that depend on the element's index and it). */
+typedef struct r2s_adamw_tensor {
+  void *param;
+  const void *grad;
+  float *master;
+  void *exp_avg;
+  void *second;
+  float *exp_avg_scale;
+  float *second_scale;
+  int64_t n;
+  float beta1;
+  float lerp_weight;
+  float beta2;
+  float one_minus_beta2;
+  float keep;
+  float bias_correction2_sqrt;
+  float eps;
+  float step_size;
+  int32_t type;
+  uint32_t step;
+} r2s_adamw_tensor_t;
+
+/* AdamW for every tensor of the list, 32 to a launch, in place.  float32 states:
+ * the arithmetic of torch.optim.AdamW. */
+int r2s_adamw_step(const r2s_adamw_tensor_t *tensors, int32_t n_tensors, r2s_stream_t stream);
+
 /* ---------------------------------------------------------------------- */
 /* Latent decoder: row lookup, gated scan, products per group              */
 /* ---------------------------------------------------------------------- */
@@ -1217,6 +1252,52 @@ int r2s_grouped_matmul_bwd(const void *x, int64_t x_stride, const void *weight,
                            int64_t v_y_stride, int64_t n, int64_t k, int64_t m, int64_t groups,
                            int32_t type, void *v_x, void *v_weight, void *v_bias,
                            void *workspace, size_t workspace_bytes, r2s_stream_t stream);
+
+/* Rotary positions along axes: in each head the pairs (a, b) of channels become
+ * (a cos t - b sin t, b cos t + a sin t), t = position[axis] base^(-i / m).  The
+ * pairs are dealt to the axes in order, sections[a] to axis a; i is a pair's number
+ * within its axis and m that axis' pairs, or with `shared` its number among all R
+ * pairs and m = R.  Pair j is channels j and R + j, or with `interleaved` 2j and
+ * 2j + 1; channels from 2R on are copied.  inverse: the turn by -t (the gradient).
+ * q [n, q_heads, head] and k [n, k_heads, head] (either may have no heads) by the
+ * strides of their tokens and heads, in elements; positions [n, axes]; q_out and
+ * k_out dense. */
+#define R2S_POSITION_F32 0
+#define R2S_POSITION_I32 1
+#define R2S_POSITION_I64 2
+#define R2S_ROTARY_MAX_AXES 8
+int r2s_rotary_axes(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                    int64_t q_heads, const void *k, int64_t k_token_stride,
+                    int64_t k_head_stride, int64_t k_heads, const void *positions,
+                    int32_t position_type, const int32_t *sections, int32_t axes,
+                    int32_t shared, double base, int32_t interleaved, int32_t inverse,
+                    int32_t type, int64_t n, int64_t head, void *q_out, void *k_out,
+                    r2s_stream_t stream);
+
+/* y = x + scale sigmoid(gate) h with h = norm(update) update_weight (update
+ * itself without that weight), u = norm(y) weight; norm(z) = (z - c) /
+ * sqrt(mean((z - c)^2) + eps), c = 0 or with `centered` the row's mean.  Rows of
+ * `width` (at most 8192) by strides; gate_kind 0: no gate, 1: gate [n, width], 2:
+ * gate [width] for all rows.  update NULL: y = x, which is not stored (y NULL).
+ * weight NULL: no u (u NULL).  y and u dense. */
+int r2s_residual_norm_fwd(const void *x, int64_t x_stride, const void *update,
+                          int64_t update_stride, const void *gate, int64_t gate_stride,
+                          int32_t gate_kind, const void *update_weight, const void *weight,
+                          float scale, float eps, int32_t centered, int32_t type, int64_t n,
+                          int64_t width, void *y, void *u, r2s_stream_t stream);
+/* Its gradient from v_y and v_u [n, width] (either may be NULL: zeros): v_x,
+ * v_update [n, width], v_gate of the gate's shape, v_update_weight and v_weight
+ * [width]; any may be NULL (not wanted).  The workspace holds float32 parts of the
+ * sums over rows. */
+int64_t r2s_residual_norm_bwd_workspace_bytes(int32_t type, int64_t n, int64_t width);
+int r2s_residual_norm_bwd(const void *x, int64_t x_stride, const void *update,
+                          int64_t update_stride, const void *gate, int64_t gate_stride,
+                          int32_t gate_kind, const void *update_weight, const void *weight,
+                          const void *v_y, int64_t v_y_stride, const void *v_u,
+                          int64_t v_u_stride, float scale, float eps, int32_t centered,
+                          int32_t type, int64_t n, int64_t width, void *v_x, void *v_update,
+                          void *v_gate, void *v_update_weight, void *v_weight, void *workspace,
+                          size_t workspace_bytes, r2s_stream_t stream);
 
 #ifdef __cplusplus
 }
