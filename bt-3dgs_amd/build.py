@@ -41,6 +41,7 @@ SOURCES = [
     "rotary.hip",
     "residual_norm.hip",
     "adamw.hip",
+    "decay_attention.hip",
 ]
 
 ARCH = os.environ.get("R2S_OFFLOAD_ARCH", "gfx950")

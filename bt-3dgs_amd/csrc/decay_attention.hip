@@ -1,0 +1,1129 @@
+// Linear attention with a decay for each head, over sequences of tokens:
+//
+//   S_t = g S_{t-1} + k_t v_t^T,   y_t = s S_t^T q_t,   g = exp(log_decay).
+//
+// A sequence is walked in chunks of C tokens.  With i, j the tokens of a chunk and S
+// the state before it,
+//
+//   y_i = s (g^(i+1) S^T q_i + sum_{j <= i} g^(i-j) (q_i k_j) v_j),
+//   S' = g^C S + sum_j g^(C-1-j) k_j v_j^T,
+//
+// four products on the matrix cores.  No power is negative: the weights g^(i-j) are
+// made for the pairs, so a strong decay underflows to the zeros it means.
+//
+// The backward is the same walk three times, of other inputs:
+//
+//   dq: S (as its transpose) from dy, v, k in the forward's order,
+//   dv: R_t = g R_{t+1} + s q_t dy_t^T from k, q, dy from the other end,
+//   dk: R (as its transpose) from v, dy, q from the other end,
+//
+// where R begins with the last state's gradient before any decay: "early" roles
+// decay a state behind its token, g^i and g^(C-j) above.  g R after the last token is
+// the first state's gradient.
+//
+// A block is one head and up to 16 NT W columns of v of one span of a sequence.
+// The state stays in registers: each of its W waves holds all rows of 16 NT columns,
+// as accumulators that turn into operands without moving between lanes.  For
+// that the products are made transposed (scores as k q^T, outputs as v^T p), so a
+// lane has one token's scores and neighbouring columns of its output.  Every wave
+// makes the chunk's scores for itself, which costs it less than sharing them.
+//
+// Precision: the scores, the state and the decayed v are float32 values.  As
+// operands of 16-bit products they are split into a rounded part and a rounded
+// rest (two products instead of one), so that nothing is rounded to 16 bits but
+// the outputs; float16 inputs beside them, whose range does not hold those values,
+// are split without loss into bfloat16 parts.
+//
+// A zero weight times a NaN or an infinity is a NaN: a chunk with such a v would
+// reach back to its earlier tokens.  Its tokens are walked one by one.
+//
+// Few sequences are cut into spans: their own states first (k and v alone), one
+// pass along each sequence over those, and then all spans at once from the states
+// before them.
+#include <algorithm>
+
+#include "r2s_latent.h"
+
+namespace r2s {
+namespace {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using i16x4 = __attribute__((ext_vector_type(4))) short;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+constexpr int kMostChannels = 256;
+
+// One input: sequence s (of equal ones), its token and head by strides.
+struct View {
+  const void *p;
+  int64_t sequence, token, head;
+};
+
+// One walk: the names are those of the forward's.
+struct Role {
+  View q, k, v;
+  const float *initial;  // [sequences][heads][state], may be null: zeros
+  float *carried;        // [cuts][heads][state]: the state behind each span but the last
+  int32_t dk, dv;
+  int32_t transposed;    // initial and carried are stored [dv][dk]
+  int32_t early, backwards;
+  float scale_in, scale_out;  // of k v^T, and of everything that is read
+  void *y;                    // [n][heads][dv]
+  float *final_state;         // [sequences][heads][dk][dv], may be null
+};
+
+constexpr int kRoles = 3;
+
+// How the sequences are cut.
+struct Cut {
+  const int32_t *offsets;  // ragged
+  const int32_t *owner;    // ragged, several spans: each item's sequence
+  const int32_t *first;    // and each sequence's first item
+  int64_t n, sequences, length, span;
+  int64_t carried;  // places for states between spans
+  int32_t spans;    // of an equal sequence
+};
+
+struct Walk {
+  Role role[kRoles];
+  const float *log_decay;
+  Cut cut;
+  int32_t heads, column_blocks;
+};
+
+// A block's span of its sequence: tokens [at, at + count) of the walk's order.
+struct Span {
+  int64_t sequence, lo, length;  // the sequence's first token and tokens
+  int64_t at, count;
+  int64_t place;  // among the carried states
+  bool first, last;
+};
+
+__device__ __forceinline__ int64_t bound(const Cut &c, int64_t s) {
+  return min(max(static_cast<int64_t>(c.offsets[s]), int64_t{0}), c.n);
+}
+
+// False for an item that there is not.  Sequence `sequences` stands for the
+// tokens behind the last one.
+__device__ __forceinline__ bool find_span(const Cut &c, int64_t item, Span &x) {
+  int64_t index = 0, items = 1;
+  if (c.offsets == nullptr) {
+    x.sequence = item / c.spans;
+    index = item - x.sequence * c.spans;
+    items = c.spans;
+    x.lo = x.sequence * c.length;
+    x.length = c.length;
+    x.place = x.sequence * (c.spans - 1) + index;
+  } else {
+    x.sequence = item;
+    if (c.owner != nullptr) {
+      x.sequence = c.owner[item];
+      if (x.sequence < 0) return false;
+      index = item - c.first[x.sequence];
+      items = c.first[x.sequence + 1] - c.first[x.sequence];
+    }
+    x.lo = bound(c, x.sequence);
+    const int64_t hi = x.sequence < c.sequences ? bound(c, x.sequence + 1) : c.n;
+    x.length = max(hi - x.lo, int64_t{0});
+    x.place = item - x.sequence;  // each sequence before has an item without a place
+  }
+  x.at = index * c.span;
+  x.count = max(min(x.length - x.at, c.span), int64_t{0});
+  x.first = index == 0;
+  x.last = index + 1 >= items;
+  // Offsets that do not ascend may ask for more places than there are.
+  return x.place >= 0 && (x.last || x.place < c.carried) &&
+         (x.first || (x.place > 0 && x.place <= c.carried));
+}
+
+// The items of ragged sequences: each sequence's spans, at least one; those of
+// the tokens behind the last; -1 for the others.
+__global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
+                                                           int32_t *__restrict__ owner,
+                                                           int32_t *__restrict__ first) {
+  __shared__ int64_t s_total[16];
+  int64_t before = 0;
+  for (int64_t s0 = 0; s0 <= c.sequences; s0 += 1024) {
+    const int64_t s = s0 + threadIdx.x;
+    int64_t items = 0;
+    if (s <= c.sequences) {
+      const int64_t hi = s < c.sequences ? bound(c, s + 1) : c.n;
+      const int64_t tokens = max(hi - bound(c, s), int64_t{0});
+      items = (tokens + c.span - 1) / c.span;
+      if (s < c.sequences) items = max(items, int64_t{1});
+    }
+    const int64_t inside = wave_inclusive_scan(items);
+    if (lane_id() == 63) s_total[wave_index()] = inside;
+    __syncthreads();
+    int64_t at = before + inside - items;
+    for (uint32_t w = 0; w < 16; ++w) {
+      if (w < wave_index()) at += s_total[w];
+      before += s_total[w];
+    }
+    // Offsets that do not ascend may name more items than there is room for.
+    at = min(at, most);
+    before = min(before, most);
+    if (s <= c.sequences) first[s] = static_cast<int32_t>(at);
+    for (int64_t i = at; i < min(at + items, most); ++i) owner[i] = static_cast<int32_t>(s);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) first[c.sequences + 1] = static_cast<int32_t>(before);
+  for (int64_t i = before + threadIdx.x; i < most; i += 1024) owner[i] = -1;
+}
+
+// The states behind the spans from each span's own, along every sequence.
+__global__ __launch_bounds__(256) void decay_carry_kernel(Walk w, int64_t total) {
+  const Role &r = w.role[0];
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t size = static_cast<int64_t>(r.dk) * r.dv;
+  const int64_t sequence = i / (w.heads * size), inside = i - sequence * w.heads * size;
+  const int32_t head = static_cast<int32_t>(inside / size);
+  int64_t place = sequence * (w.cut.spans - 1), count = w.cut.spans - 1;
+  if (w.cut.offsets != nullptr) {
+    place = w.cut.first[sequence] - sequence;
+    count = w.cut.first[sequence + 1] - w.cut.first[sequence] - 1;
+    count = min(count, w.cut.carried - place);
+  }
+  if (count <= 0) return;
+  const float keep = expf(w.log_decay[head] * static_cast<float>(w.cut.span));
+  float now = r.initial != nullptr ? r.initial[i] : 0.0f;
+  float *p = r.carried + place * w.heads * size + inside;
+  const int64_t step = w.heads * size;
+  constexpr int kAhead = 8;
+  for (int64_t c = 0; c < count; c += kAhead) {
+    float own[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) own[a] = c + a < count ? p[(c + a) * step] : 0.0f;
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      now = fmaf(keep, now, own[a]);
+      if (c + a < count) p[(c + a) * step] = now;
+    }
+  }
+}
+
+// ------------------------------------------------------------ operands ---
+
+template <typename T>
+__device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 acc) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], acc, 0, 0, 0);
+    return acc;
+  } else if constexpr (std::is_same<T, bf16_t>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+  }
+}
+
+// Float values of an operand's 16 bytes as a rounded part and the rounded rest;
+// float32 as they are.
+template <typename T>
+struct Parts {
+  u32x4 high, rest;
+};
+template <typename T>
+__device__ __forceinline__ Parts<T> split(const float (&x)[16 / sizeof(T)]) {
+  Parts<T> out;
+  if constexpr (sizeof(T) == 4) {
+    out.high = __builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]});
+  } else {
+    Pack<T, 8> high, rest;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      high.v[i] = static_cast<T>(x[i]);
+      rest.v[i] = static_cast<T>(x[i] - static_cast<float>(high.v[i]));
+    }
+    out.high = __builtin_bit_cast(u32x4, high);
+    out.rest = __builtin_bit_cast(u32x4, rest);
+  }
+  return out;
+}
+template <typename T>
+__device__ __forceinline__ void widen(u32x4 raw, float (&x)[16 / sizeof(T)]) {
+  const Pack<T, 16 / sizeof(T)> p = __builtin_bit_cast(Pack<T, 16 / sizeof(T)>, raw);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) x[i] = static_cast<float>(p.v[i]);
+}
+
+// The type that values are split in: float16's range does not hold scores and
+// states, and the rests of decayed v's would be below its normal numbers.
+template <typename T>
+struct Wide {
+  using type = T;
+};
+template <>
+struct Wide<f16_t> {
+  using type = bf16_t;
+};
+
+// An input beside them: float16's in two bfloat16 parts, which hold it exactly.
+template <typename T>
+__device__ __forceinline__ Parts<typename Wide<T>::type> beside(u32x4 raw) {
+  if constexpr (std::is_same<T, f16_t>::value) {
+    float x[8];
+    widen<T>(raw, x);
+    return split<bf16_t>(x);
+  } else {
+    return {raw, raw};
+  }
+}
+
+// acc += a b of an input and split values, as rows and columns or the other way
+// round.  T is the inputs' type.
+template <typename T, bool kInputRows>
+__device__ __forceinline__ f32x4 multiply_split(const Parts<typename Wide<T>::type> &input,
+                                                const Parts<typename Wide<T>::type> &values,
+                                                f32x4 acc) {
+  using U = typename Wide<T>::type;
+  auto go = [&](u32x4 a, u32x4 b) {
+    acc = kInputRows ? multiply<U>(a, b, acc) : multiply<U>(b, a, acc);
+  };
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (std::is_same<T, f16_t>::value) go(input.rest, values.high);
+    go(input.high, values.rest);
+  }
+  go(input.high, values.high);
+  return acc;
+}
+
+// g^x for a whole number x of tokens.
+__device__ __forceinline__ float power(float log2_decay, int x) {
+  return x == 0 ? 1.0f : exp2f(log2_decay * static_cast<float>(x));
+}
+
+// --------------------------------------------------------------- walk ----
+
+// Rows of D elements in LDS, 16 bytes apart from a power of two so that rows side by
+// side start in different banks.
+template <typename T, int D>
+struct Tile {
+  static constexpr int kPitch = D * static_cast<int>(sizeof(T)) + 16;
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+};
+
+// 16 bytes of the summed index along a row, from LDS.
+template <typename T, int D>
+__device__ __forceinline__ u32x4 along(const char *tile, int row, int piece) {
+  return *reinterpret_cast<const u32x4 *>(tile + row * Tile<T, D>::kPitch + piece * 16);
+}
+// 16 bytes of the summed index across rows: 16 bits: rows 4 g to 4 g + 3 and 16
+// on, g the lane's group of 16, of the lane's column; float32: rows 4 g to 4 g + 3.
+// The lane's column is (i / 4) run + first + i % 4, i = lane % 16.
+template <typename T, int D, int kRun>
+__device__ __forceinline__ u32x4 across(const char *tile, int row, int first) {
+  const int lane = static_cast<int>(lane_id()), i = lane % 16, g = lane / 16;
+  if constexpr (sizeof(T) == 2) {
+    // Sixteen lanes read 4 rows of 4 times 4 neighbours, 8 bytes each, and get 4
+    // rows of one column each.
+    const char *p = tile + (row + g * 4 + i / 4) * Tile<T, D>::kPitch +
+                    (i % 4 * kRun + first) * 2;
+    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4 *)p);
+    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4 *)(p + 16 * Tile<T, D>::kPitch));
+    u32x4 out;
+    __builtin_memcpy(&out, &x, 8);
+    __builtin_memcpy(reinterpret_cast<char *>(&out) + 8, &y, 8);
+    return out;
+  } else {
+    const char *p = tile + (row + g * 4) * Tile<T, D>::kPitch + (i / 4 * kRun + first + i % 4) * 4;
+    u32x4 out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      out[j] = *reinterpret_cast<const uint32_t *>(p + j * Tile<T, D>::kPitch);
+    return out;
+  }
+}
+
+template <typename T, int V>
+struct __attribute__((packed)) Loose {
+  T v[V];
+};
+
+// A chunk's rows on their way to LDS: N pieces of 16 bytes a thread.
+template <typename T, int D, int C, int kThreads>
+struct Stage {
+  static constexpr int kPieces = D * static_cast<int>(sizeof(T)) / 16;
+  static constexpr int kCount = (C * kPieces + kThreads - 1) / kThreads;
+  static constexpr int kPer = Tile<T, D>::kPer;
+  u32x4 raw[kCount];
+  // Rows pos.. of the walk, `left` of them; zeros for those past them and for
+  // columns past `width`.
+  __device__ __forceinline__ void load(const T *base, int64_t stride, int64_t pos, int64_t left,
+                                       int width) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int q = i * kThreads + static_cast<int>(threadIdx.x);
+      const int row = q / kPieces, column = q % kPieces * kPer;
+      u32x4 x{0, 0, 0, 0};
+      if (row < C && row < left && column < width) {
+        const T *p = base + (pos + row) * stride + column;
+        if (column + kPer <= width) {
+          x = __builtin_bit_cast(u32x4, *reinterpret_cast<const Loose<T, kPer> *>(p));
+        } else {
+          Pack<T, kPer> e;
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            e.v[j] = column + j < width ? p[j] : static_cast<T>(0.0f);
+          x = __builtin_bit_cast(u32x4, e);
+        }
+      }
+      raw[i] = x;
+    }
+  }
+  __device__ __forceinline__ void put(char *tile) const {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int q = i * kThreads + static_cast<int>(threadIdx.x);
+      if (C * kPieces % kThreads == 0 || q < C * kPieces)
+        *reinterpret_cast<u32x4 *>(tile + q / kPieces * Tile<T, D>::kPitch + q % kPieces * 16) =
+            raw[i];
+    }
+  }
+  // Whether an element is not finite.
+  __device__ __forceinline__ bool bad() const {
+    constexpr uint32_t kMask = sizeof(T) == 4 ? 0x7F800000u
+                               : std::is_same<T, bf16_t>::value ? 0x7F80u : 0x7C00u;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        found |= (raw[i][j] & kMask) == kMask;
+        if constexpr (sizeof(T) == 2) found |= (raw[i][j] >> 16 & kMask) == kMask;
+      }
+    return found;
+  }
+};
+
+// Zeros in the rows of a tile from the second on.
+template <typename T, int D, int C, int kThreads>
+__device__ __forceinline__ void clear_rows(char *tile) {
+  constexpr int kPieces = D * static_cast<int>(sizeof(T)) / 16;
+  for (int q = kPieces + static_cast<int>(threadIdx.x); q < C * kPieces; q += kThreads)
+    *reinterpret_cast<u32x4 *>(tile + q / kPieces * Tile<T, D>::kPitch + q % kPieces * 16) =
+        u32x4{0, 0, 0, 0};
+}
+
+// KD: channels of q and k that LDS and registers have room for; the block's W waves
+// have 16 NT columns of v each.  kStates: the spans' own states, no outputs.
+template <typename T, int KD, int NT, int W, bool kStates>
+struct Shape {
+  static constexpr int C = sizeof(T) == 4 ? 32 : 64;    // tokens of a chunk
+  static constexpr int kThreads = 64 * W;
+  static constexpr int kColumns = 16 * NT * W;
+  static constexpr int kFragment = 64 / static_cast<int>(sizeof(T));  // summed by 16 bytes a lane
+  static constexpr int kTiles = kFragment / 16;         // tiles of 16 to a fragment
+  static constexpr int KB = KD / kFragment, JB = C / kFragment;
+  static constexpr int kQ = kStates ? 0 : C * Tile<T, KD>::kPitch;
+  static constexpr int kK = C * Tile<T, KD>::kPitch, kV = C * Tile<T, kColumns>::kPitch;
+  static constexpr int kLds = kQ + kK + kV;
+};
+
+template <typename T, int KD, int NT, int W, bool kStates>
+__global__ __launch_bounds__(64 * W) void decay_walk_kernel(Walk w) {
+  using S = Shape<T, KD, NT, W, kStates>;
+  constexpr int C = S::C, kThreads = S::kThreads, KB = S::KB, JB = S::JB, kTiles = S::kTiles;
+  constexpr int kFragment = S::kFragment, kPer = Tile<T, KD>::kPer;
+  constexpr int kRun = 4 * NT;        // neighbouring columns of v in a lane's outputs
+  constexpr int kRows = 4 * kTiles;   // neighbouring rows of the state in a lane
+  using U = typename Wide<T>::type;
+  extern __shared__ __attribute__((aligned(16))) char s_tile[];
+  __shared__ int s_bad[2];
+  char *s_q = s_tile, *s_k = s_tile + S::kQ, *s_v = s_k + S::kK;
+
+  const Role &r = w.role[blockIdx.y];
+  const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const uint32_t per_item = static_cast<uint32_t>(w.heads) * w.column_blocks;
+  const int64_t item = id / per_item;
+  const int head = static_cast<int>(id % per_item) / w.column_blocks;
+  const int block_column = static_cast<int>(id % per_item) % w.column_blocks * S::kColumns;
+  const int dk = r.dk, dv = r.dv;
+  if (block_column >= dv) return;
+  Span x;
+  if (!find_span(w.cut, item, x)) return;
+  const int width = min(dv - block_column, S::kColumns);
+  T *y = static_cast<T *>(r.y);
+  if (x.sequence >= w.cut.sequences) {  // behind the last sequence
+    if constexpr (!kStates) {
+      for (int64_t i = threadIdx.x; i < x.count * width; i += kThreads)
+        y[((x.lo + x.at + i / width) * w.heads + head) * dv + block_column + i % width] =
+            static_cast<T>(0.0f);
+    }
+    return;
+  }
+  if (kStates && x.last) return;
+
+  const int lane = static_cast<int>(lane_id()), i = lane % 16, g = lane / 16;
+  const int wave_column = static_cast<int>(wave_index()) * 16 * NT;  // in the block's
+  const int column0 = block_column + wave_column;
+  const bool idle = column0 >= dv;
+  // The lane's column of v as an operand, and the first of its outputs'.
+  auto column_of = [&](int nt) { return column0 + i / 4 * kRun + nt * 4 + i % 4; };
+
+  const int64_t size = static_cast<int64_t>(dk) * dv;
+  auto state_at = [&](const float *base, int64_t which, bool transposed, int row, int column) {
+    return base + (which * w.heads + head) * size +
+           (transposed ? static_cast<int64_t>(column) * dk + row
+                       : static_cast<int64_t>(row) * dv + column);
+  };
+  // state[kb][t][nt][e]: row kb kFragment + g kRows + 4 t + e, column_of(nt).
+  f32x4 state[KB][kTiles][NT];
+  const float *begin = kStates ? nullptr : x.first ? r.initial : r.carried;
+  const int64_t which = x.first ? x.sequence : x.place - 1;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = kb * kFragment + g * kRows + t * 4 + e, column = column_of(nt);
+          state[kb][t][nt][e] = begin != nullptr && row < dk && column < dv
+                                    ? *state_at(begin, which, r.transposed != 0, row, column)
+                                    : 0.0f;
+        }
+
+  const float log2_decay = w.log_decay[head] * 1.44269504088896341f;
+  const int early = r.early;
+  // Weights of the pairs (i, j) of two tiles of 16 tokens depend on how many tiles
+  // they lie apart alone.  Scores' rows are j, their columns i.
+  constexpr int kApart = C / 16;
+  float weight[kApart][4], reach[kApart];
+  if constexpr (!kStates) {
+#pragma unroll
+    for (int a = 0; a < kApart; ++a) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int apart = a * 16 + i - (g * 4 + e);
+        weight[a][e] = apart >= 0 ? r.scale_in * power(log2_decay, apart) : 0.0f;
+      }
+      reach[a] = power(log2_decay, a * 16 + i + 1 - early);
+    }
+  }
+  // What is left at the chunk's end of the fragments' tokens.
+  float left[JB][kPer];
+  auto set_left = [&](int count) {
+#pragma unroll
+    for (int b = 0; b < JB; ++b)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int j = b * kFragment + e / 4 * 16 + g * 4 + e % 4;
+        left[b][e] = j < count ? r.scale_in * power(log2_decay, count - 1 - j + early) : 0.0f;
+      }
+  };
+  set_left(C);
+  float keep = power(log2_decay, C);
+
+  // Token `t` of the walk is row lo + t of the inputs, or hi - 1 - t.
+  const int64_t way = r.backwards != 0 ? -1 : 1;
+  auto base_of = [&](const View &v) {
+    const T *p = static_cast<const T *>(v.p) + head * v.head;
+    p += w.cut.offsets == nullptr ? x.sequence * v.sequence : x.lo * v.token;
+    return r.backwards != 0 ? p + (x.length - 1) * v.token : p;
+  };
+  const T *q_base = kStates ? nullptr : base_of(r.q), *k_base = base_of(r.k),
+          *v_base = base_of(r.v) + block_column;
+  const int64_t q_step = way * r.q.token, k_step = way * r.k.token, v_step = way * r.v.token;
+  Stage<T, KD, C, kThreads> q_stage, k_stage;
+  Stage<T, S::kColumns, C, kThreads> v_stage;
+  auto load = [&](int64_t pos) {
+    const int64_t rows = x.count - pos;
+    if constexpr (!kStates) q_stage.load(q_base, q_step, x.at + pos, rows, dk);
+    k_stage.load(k_base, k_step, x.at + pos, rows, dk);
+    v_stage.load(v_base, v_step, x.at + pos, rows, width);
+  };
+
+  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+  __syncthreads();
+  load(0);
+  int turn = 0;
+  for (int64_t pos = 0; pos < x.count; turn ^= 1) {
+    if constexpr (!kStates) q_stage.put(s_q);
+    k_stage.put(s_k);
+    v_stage.put(s_v);
+    if constexpr (!kStates) {
+      if (v_stage.bad()) s_bad[turn] = 1;
+    }
+    __syncthreads();
+    int count = static_cast<int>(min(x.count - pos, static_cast<int64_t>(C)));
+    if constexpr (!kStates) {
+      if (s_bad[turn] != 0 && count > 1) {
+        count = 1;
+        clear_rows<T, KD, C, kThreads>(s_k);
+        clear_rows<T, S::kColumns, C, kThreads>(s_v);
+        __syncthreads();
+      }
+    }
+    load(pos + count);
+    if (count < C) {
+      set_left(count);
+      keep = power(log2_decay, count);
+    }
+    if (!idle) {
+      u32x4 v_raw[JB][NT];
+#pragma unroll
+      for (int b = 0; b < JB; ++b)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          v_raw[b][nt] = across<T, S::kColumns, kRun>(s_v, b * kFragment, wave_column + nt * 4);
+      if constexpr (!kStates) {
+        Parts<U> v_parts[JB][NT], s_parts[KB][NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int b = 0; b < JB; ++b) v_parts[b][nt] = beside<T>(v_raw[b][nt]);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            float z[kPer];
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) z[e] = state[kb][e / 4][nt][e % 4];
+            s_parts[kb][nt] = split<U>(z);
+          }
+        }
+#pragma unroll
+        for (int it = 0; it < C / 16; ++it) {
+          if (it * 16 >= count) break;
+          u32x4 q_raw[KB];
+          f32x4 out[NT] = {};
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            q_raw[kb] = along<T, KD>(s_q, it * 16 + i, kb * 4 + g);
+            const Parts<U> q_parts = beside<T>(q_raw[kb]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              out[nt] = multiply_split<T, false>(q_parts, s_parts[kb][nt], out[nt]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) out[nt] *= reach[it];
+#pragma unroll
+          for (int b = 0; b < JB; ++b) {
+            if (b * kFragment > it * 16 + 15) continue;
+            const int apart = it - b * kTiles;
+            float p[kPer];
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+              if (t > apart) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[t * 4 + e] = 0.0f;
+                continue;
+              }
+              f32x4 score{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+              for (int kb = 0; kb < KB; ++kb)
+                score = multiply<T>(along<T, KD>(s_k, b * kFragment + t * 16 + i, kb * 4 + g),
+                                    q_raw[kb], score);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                p[t * 4 + e] = score[e] * weight[apart - t][e];
+                // A later token's score may be anything.
+                if (t == apart && i < g * 4 + e) p[t * 4 + e] = 0.0f;
+              }
+            }
+            const Parts<U> p_parts = split<U>(p);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              out[nt] = multiply_split<T, true>(v_parts[b][nt], p_parts, out[nt]);
+          }
+          const int64_t t = x.at + pos + it * 16 + i;
+          if (it * 16 + i < count) {
+            const int64_t token = x.lo + (r.backwards != 0 ? x.length - 1 - t : t);
+            const int column = column0 + g * kRun;
+            T *p = y + (token * w.heads + head) * dv + column;
+            Loose<T, kRun> z;
+#pragma unroll
+            for (int e = 0; e < kRun; ++e)
+              z.v[e] = static_cast<T>(out[e / 4][e % 4] * r.scale_out);
+            if (column + kRun <= dv) {
+              *reinterpret_cast<Loose<T, kRun> *>(p) = z;
+            } else {
+#pragma unroll
+              for (int e = 0; e < kRun; ++e)
+                if (column + e < dv) p[e] = z.v[e];
+            }
+          }
+        }
+      }
+      Parts<U> fresh[JB][NT];
+#pragma unroll
+      for (int b = 0; b < JB; ++b)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float z[kPer];
+          widen<T>(v_raw[b][nt], z);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) z[e] *= left[b][e];
+          fresh[b][nt] = split<U>(z);
+        }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) state[kb][t][nt] *= keep;
+#pragma unroll
+          for (int b = 0; b < JB; ++b) {
+            const Parts<U> k_parts = beside<T>(
+                across<T, KD, kRows>(s_k, b * kFragment, kb * kFragment + t * 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              state[kb][t][nt] =
+                  multiply_split<T, true>(k_parts, fresh[b][nt], state[kb][t][nt]);
+          }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s_bad[turn] = 0;
+    if (count < C) {
+      set_left(C);
+      keep = power(log2_decay, C);
+    }
+    pos += count;
+  }
+
+  float *end = kStates ? r.carried : x.last ? r.final_state : nullptr;
+  if (end == nullptr || idle) return;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = kb * kFragment + g * kRows + t * 4 + e, column = column_of(nt);
+          if (row < dk && column < dv)
+            *const_cast<float *>(state_at(end, kStates ? x.place : x.sequence, false, row,
+                                          column)) = state[kb][t][nt][e];
+        }
+}
+
+// One token of every sequence: the state is read, decayed, added to, stored and
+// multiplied in one pass.  A block has one head of one sequence; its threads lie
+// along the rows of the state, V columns each.  Bound by the state's bytes.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void decay_step_kernel(
+    View q, View k, View v, const float *__restrict__ log_decay, const float *__restrict__ state,
+    int heads, int dk, int dv, float scale, T *__restrict__ y, float *__restrict__ next) {
+  __shared__ float s_q[kMostChannels], s_k[kMostChannels];
+  __shared__ float s_sum[256 * V];
+  const int64_t which = blockIdx.x, sequence = which / heads;
+  const int head = static_cast<int>(which - sequence * heads);
+  const T *qp = static_cast<const T *>(q.p) + sequence * q.token + head * q.head;
+  const T *kp = static_cast<const T *>(k.p) + sequence * k.token + head * k.head;
+  const T *vp = static_cast<const T *>(v.p) + sequence * v.token + head * v.head;
+  if (static_cast<int>(threadIdx.x) < dk) {
+    s_q[threadIdx.x] = static_cast<float>(qp[threadIdx.x]);
+    s_k[threadIdx.x] = static_cast<float>(kp[threadIdx.x]);
+  }
+  const int across = (dv + V - 1) / V, rows = 256 / across;
+  const int row0 = static_cast<int>(threadIdx.x) / across;
+  const int column = (static_cast<int>(threadIdx.x) - row0 * across) * V;
+  const float decay = expf(log_decay[head]);
+  float fresh[V], sum[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    fresh[e] = row0 < rows ? static_cast<float>(vp[column + e]) : 0.0f;
+    sum[e] = 0.0f;
+  }
+  __syncthreads();
+  if (row0 < rows) {
+    const int64_t base = which * dk * dv + column;
+#pragma unroll 4
+    for (int row = row0; row < dk; row += rows) {
+      const int64_t at = base + static_cast<int64_t>(row) * dv;
+      Pack<float, V> z = load_pack<float, V>(state + at);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        z.v[e] = fmaf(s_k[row], fresh[e], decay * z.v[e]);
+        sum[e] = fmaf(s_q[row], z.v[e], sum[e]);
+      }
+      store_pack<float, V>(next + at, z);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_sum[row0 * dv + column + e] = sum[e];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < dv; c += 256) {
+    float total = 0.0f;
+    for (int i = 0; i < min(rows, dk); ++i) total += s_sum[i * dv + c];
+    y[which * dv + c] = static_cast<T>(total * scale);
+  }
+}
+
+// ---------------------------------------------------------------- host ----
+
+struct Sizes {
+  int type;
+  bool ragged;
+  int64_t sequences, length, n, heads, dk, dv;
+};
+
+// Columns of v that a block takes, for the wider of both heads' sides (the
+// backward's roles swap them).
+struct Form {
+  int kd, nt, waves;
+  int columns() const { return 16 * nt * waves; }
+};
+Form form_of(const Sizes &z) {
+  const int64_t wide = std::max(z.dk, z.dv);
+  const int kd = wide <= 32 ? 32 : wide <= 64 ? 64 : wide <= 128 ? 128 : 256;
+  if (kd <= 64) return {kd, 1, wide <= 16 ? 1 : 4};
+  return {kd, kd == 128 ? 2 : 1, 4};
+}
+
+// Tokens of a span: as many as leave a block for each of 1024 places, but at least
+// 256, so that a span's own tokens outweigh its states.
+int64_t span_of(const Sizes &z) {
+  const Form f = form_of(z);
+  const int64_t blocks = std::max<int64_t>(1, z.heads * ceil_div(std::max(z.dk, z.dv), f.columns()));
+  const int64_t longest = z.ragged ? z.n : z.length;
+  const int64_t sequences = z.ragged ? 1 : std::max<int64_t>(1, z.sequences);
+  const int64_t spans = std::max<int64_t>(1, 1024 / (blocks * sequences));
+  const int64_t span = ceil_div(ceil_div(std::max<int64_t>(longest, 1), spans), 64) * 64;
+  return std::max<int64_t>(256, span);
+}
+
+// Whether any sequence may have several spans, the number of states that they
+// carry at most, and of items.
+struct Plan {
+  int64_t span, carried, items;
+  int32_t spans;
+  bool cut;
+};
+Plan plan_of(const Sizes &z) {
+  Plan p{};
+  p.span = span_of(z);
+  if (z.ragged) {
+    p.cut = z.n > p.span;
+    p.carried = p.cut ? z.n / p.span : 0;
+    p.items = z.sequences + 1 + (p.cut ? z.n / p.span + 1 : 0);
+    p.spans = 1;
+  } else {
+    p.spans = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(z.length, p.span)));
+    p.cut = p.spans > 1;
+    p.carried = z.sequences * (p.spans - 1);
+    p.items = z.sequences * p.spans;
+  }
+  return p;
+}
+
+int64_t table_bytes(const Sizes &z, const Plan &p) {
+  if (!z.ragged || !p.cut) return 0;
+  Carver c(nullptr);
+  c.take<int32_t>(p.items);
+  c.take<int32_t>(z.sequences + 2);
+  return static_cast<int64_t>(align_up(c.used, 256));
+}
+
+template <typename T, int KD, int NT, int W, bool kStates>
+int launch_walk(const Walk &w, int64_t blocks, int roles, hipStream_t stream) {
+  using S = Shape<T, KD, NT, W, kStates>;
+  static_assert(S::kLds + 16 <= 160 * 1024, "LDS of a CU");
+  if (S::kLds > 64 * 1024) {
+    const hipError_t err = hipFuncSetAttribute(
+        reinterpret_cast<const void *>(&decay_walk_kernel<T, KD, NT, W, kStates>),
+        hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
+    if (err != hipSuccess) {
+      set_error("decay_attention: %d bytes of LDS refused: %s", S::kLds, hipGetErrorString(err));
+      return R2S_EHIP;
+    }
+  }
+  decay_walk_kernel<T, KD, NT, W, kStates>
+      <<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(roles)), dim3(64 * W), S::kLds,
+         stream>>>(w);
+  return check_launch("decay_attention");
+}
+
+template <bool kStates>
+int walk(const Sizes &z, const Plan &p, Walk &w, int roles, hipStream_t stream) {
+  const Form f = form_of(z);
+  int64_t columns = 0;
+  for (int i = 0; i < roles; ++i)
+    columns = std::max<int64_t>(columns, ceil_div(w.role[i].dv, f.columns()));
+  w.column_blocks = static_cast<int32_t>(columns);
+  const int64_t blocks = p.items * z.heads * columns;
+  if (blocks > kInt32Max) {
+    set_error("decay_attention: %lld blocks exceed 2^31 - 1", static_cast<long long>(blocks));
+    return R2S_ERANGE;
+  }
+  if (blocks == 0) return R2S_OK;
+  R2S_BY_TYPE(z.type, {
+    if (f.kd == 32)
+      return f.waves == 1 ? launch_walk<T, 32, 1, 1, kStates>(w, blocks, roles, stream)
+                          : launch_walk<T, 32, 1, 4, kStates>(w, blocks, roles, stream);
+    if (f.kd == 64) return launch_walk<T, 64, 1, 4, kStates>(w, blocks, roles, stream);
+    if (f.kd == 128) return launch_walk<T, 128, 2, 4, kStates>(w, blocks, roles, stream);
+    return launch_walk<T, 256, 1, 4, kStates>(w, blocks, roles, stream);
+  });
+}
+
+int carry(const Sizes &z, const Plan &p, const Walk &w, hipStream_t stream) {
+  const int64_t total = z.sequences * z.heads * z.dk * z.dv;
+  const int64_t blocks = ceil_div(total, 256);
+  if (blocks > kInt32Max) {
+    set_error("decay_attention: too many states");
+    return R2S_ERANGE;
+  }
+  if (blocks == 0) return R2S_OK;
+  decay_carry_kernel<<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(w, total);
+  return check_launch("decay_attention carry");
+}
+
+int check_sizes(const char *op, const Sizes &z) {
+  R2S_REQUIRE(known_type(z.type), "%s: unknown element type %d", op, z.type);
+  R2S_REQUIRE(z.sequences >= 0 && z.length >= 0 && z.n >= 0 && z.heads >= 0 && z.dk >= 0 &&
+                  z.dv >= 0,
+              "%s: negative size", op);
+  if (z.dk > kMostChannels || z.dv > kMostChannels) {
+    set_error("%s: at most %d channels of a head", op, kMostChannels);
+    return R2S_ERANGE;
+  }
+  if (z.n > kInt32Max || z.sequences > kInt32Max - 2 || z.heads > 65535 || z.length > kInt32Max) {
+    set_error("%s: at most 2^31 - 1 tokens and 65535 heads", op);
+    return R2S_ERANGE;
+  }
+  if (z.ragged) {
+    R2S_REQUIRE(z.sequences > 0 || z.n == 0, "%s: tokens without a sequence", op);
+  } else {
+    R2S_REQUIRE(z.sequences * z.length == z.n, "%s: %lld tokens are not %lld sequences of %lld",
+                op, static_cast<long long>(z.n), static_cast<long long>(z.sequences),
+                static_cast<long long>(z.length));
+  }
+  return R2S_OK;
+}
+
+bool bad_view(const Sizes &z, const View &v) {
+  const __int128 reach = static_cast<__int128>(z.sequences) * v.sequence +
+                         static_cast<__int128>(z.n) * v.token +
+                         static_cast<__int128>(z.heads) * v.head;
+  return v.sequence < 0 || v.token < 0 || v.head < 0 || reach >= (static_cast<__int128>(1) << 60);
+}
+
+// The table of ragged items where sequences may have several spans.
+int make_items(const Sizes &z, const Plan &p, Cut &cut, void *workspace, size_t bytes,
+               hipStream_t stream) {
+  const int64_t need = table_bytes(z, p);
+  if (need == 0) return R2S_OK;
+  if (workspace == nullptr || bytes < static_cast<size_t>(need)) {
+    set_error("decay_attention: workspace of %zu bytes, %lld needed", bytes,
+              static_cast<long long>(need));
+    return R2S_EWORKSPACE;
+  }
+  Carver c(workspace);
+  int32_t *owner = c.take<int32_t>(p.items), *first = c.take<int32_t>(z.sequences + 2);
+  decay_items_kernel<<<dim3(1), dim3(1024), 0, stream>>>(cut, p.items, owner, first);
+  cut.owner = owner;
+  cut.first = first;
+  return check_launch("decay_attention items");
+}
+
+Cut cut_of(const Sizes &z, const Plan &p, const int32_t *offsets) {
+  Cut c{};
+  c.offsets = offsets;
+  c.n = z.n;
+  c.sequences = z.sequences;
+  c.length = z.length;
+  c.span = p.span;
+  c.carried = p.carried;
+  c.spans = p.spans;
+  return c;
+}
+
+}  // namespace
+}  // namespace r2s
+
+extern "C" {
+
+int64_t r2s_decay_attention_kept_states(int32_t type, int32_t ragged, int64_t sequences,
+                                        int64_t length, int64_t n, int64_t heads, int64_t dk,
+                                        int64_t dv) {
+  const r2s::Sizes z{type, ragged != 0, sequences, length, n, heads, dk, dv};
+  if (r2s::check_sizes("decay_attention", z) != R2S_OK) return 0;
+  return r2s::plan_of(z).carried;
+}
+
+int64_t r2s_decay_attention_workspace_bytes(int32_t type, int32_t ragged, int64_t sequences,
+                                            int64_t length, int64_t n, int64_t heads, int64_t dk,
+                                            int64_t dv, int32_t backward) {
+  const r2s::Sizes z{type, ragged != 0, sequences, length, n, heads, dk, dv};
+  if (r2s::check_sizes("decay_attention", z) != R2S_OK) return 0;
+  const r2s::Plan p = r2s::plan_of(z);
+  const int64_t states = backward != 0 ? p.carried * heads * dk * dv * 4 : 0;
+  return r2s::table_bytes(z, p) + states;
+}
+
+int r2s_decay_attention_fwd(const void *q, int64_t q_sequence, int64_t q_token, int64_t q_head,
+                            const void *k, int64_t k_sequence, int64_t k_token, int64_t k_head,
+                            const void *v, int64_t v_sequence, int64_t v_token, int64_t v_head,
+                            const float *log_decay, const float *initial, const int32_t *offsets,
+                            int64_t sequences, int64_t length, int64_t n, int64_t heads,
+                            int64_t dk, int64_t dv, float scale, int32_t type, int32_t reverse,
+                            void *y, float *final_state, float *kept, void *workspace,
+                            size_t workspace_bytes, r2s_stream_t st) {
+  r2s::clear_error();
+  const r2s::Sizes z{type, offsets != nullptr, sequences, length, n, heads, dk, dv};
+  R2S_RETURN_IF(r2s::check_sizes("decay_attention_fwd", z));
+  if (sequences == 0 || heads == 0 || (n == 0 && dk * dv == 0) || dv == 0) return R2S_OK;
+  R2S_REQUIRE(log_decay != nullptr, "decay_attention_fwd: null decays");
+  R2S_REQUIRE(dk == 0 || final_state != nullptr, "decay_attention_fwd: null final state");
+  R2S_REQUIRE(n == 0 || (y != nullptr && (dk == 0 || (q != nullptr && k != nullptr)) &&
+                         v != nullptr),
+              "decay_attention_fwd: null tokens");
+  r2s::Walk w{};
+  r2s::Role &r = w.role[0];
+  r.q = {q, q_sequence, q_token, q_head};
+  r.k = {k, k_sequence, k_token, k_head};
+  r.v = {v, v_sequence, v_token, v_head};
+  R2S_REQUIRE(!r2s::bad_view(z, r.q) && !r2s::bad_view(z, r.k) && !r2s::bad_view(z, r.v),
+              "decay_attention_fwd: bad stride");
+  const r2s::Plan p = r2s::plan_of(z);
+  R2S_REQUIRE(p.carried == 0 || dk == 0 || kept != nullptr,
+              "decay_attention_fwd: null kept states");
+  hipStream_t stream = r2s::as_stream(st);
+  w.log_decay = log_decay;
+  w.heads = static_cast<int32_t>(heads);
+  w.cut = r2s::cut_of(z, p, offsets);
+  R2S_RETURN_IF(r2s::make_items(z, p, w.cut, workspace, workspace_bytes, stream));
+  r.initial = initial;
+  r.carried = kept;
+  r.dk = static_cast<int32_t>(dk);
+  r.dv = static_cast<int32_t>(dv);
+  r.backwards = reverse != 0;
+  r.scale_in = 1.0f;
+  r.scale_out = scale;
+  r.y = y;
+  r.final_state = final_state;
+  if (p.cut && dk > 0) {
+    R2S_RETURN_IF(r2s::walk<true>(z, p, w, 1, stream));
+    R2S_RETURN_IF(r2s::carry(z, p, w, stream));
+  }
+  return r2s::walk<false>(z, p, w, 1, stream);
+}
+
+int r2s_decay_attention_bwd(const void *q, int64_t q_sequence, int64_t q_token, int64_t q_head,
+                            const void *k, int64_t k_sequence, int64_t k_token, int64_t k_head,
+                            const void *v, int64_t v_sequence, int64_t v_token, int64_t v_head,
+                            const float *log_decay, const float *initial, const int32_t *offsets,
+                            const float *kept, const void *v_y, int64_t vy_sequence,
+                            int64_t vy_token, int64_t vy_head, const float *v_final,
+                            int64_t sequences, int64_t length, int64_t n, int64_t heads,
+                            int64_t dk, int64_t dv, float scale, int32_t type, int32_t reverse,
+                            void *v_q, void *v_k, void *v_v, float *v_initial, void *workspace,
+                            size_t workspace_bytes, r2s_stream_t st) {
+  r2s::clear_error();
+  const r2s::Sizes z{type, offsets != nullptr, sequences, length, n, heads, dk, dv};
+  R2S_RETURN_IF(r2s::check_sizes("decay_attention_bwd", z));
+  if (sequences == 0 || heads == 0 || dk == 0 || dv == 0) return R2S_OK;
+  R2S_REQUIRE(log_decay != nullptr, "decay_attention_bwd: null decays");
+  R2S_REQUIRE(n == 0 || (q && k && v && v_y && v_q && v_k && v_v),
+              "decay_attention_bwd: null tokens");
+  const r2s::View vq{q, q_sequence, q_token, q_head}, vk{k, k_sequence, k_token, k_head},
+      vv{v, v_sequence, v_token, v_head}, vg{v_y, vy_sequence, vy_token, vy_head};
+  R2S_REQUIRE(!r2s::bad_view(z, vq) && !r2s::bad_view(z, vk) && !r2s::bad_view(z, vv) &&
+                  !r2s::bad_view(z, vg),
+              "decay_attention_bwd: bad stride");
+  const r2s::Plan p = r2s::plan_of(z);
+  R2S_REQUIRE(p.carried == 0 || kept != nullptr, "decay_attention_bwd: null kept states");
+  const int64_t table = r2s::table_bytes(z, p);
+  const int64_t need = table + p.carried * heads * dk * dv * 4;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(need))) {
+    r2s::set_error("decay_attention_bwd: workspace of %zu bytes, %lld needed", workspace_bytes,
+                   static_cast<long long>(need));
+    return R2S_EWORKSPACE;
+  }
+  hipStream_t stream = r2s::as_stream(st);
+  r2s::Walk w{};
+  w.log_decay = log_decay;
+  w.heads = static_cast<int32_t>(heads);
+  w.cut = r2s::cut_of(z, p, offsets);
+  R2S_RETURN_IF(r2s::make_items(z, p, w.cut, workspace, workspace_bytes, stream));
+  float *carried = reinterpret_cast<float *>(static_cast<char *>(workspace) + table);
+  r2s::Role from_end{};  // R: what dk and dv have alike
+  from_end.initial = v_final;
+  from_end.carried = carried;
+  from_end.backwards = reverse == 0;
+  from_end.early = 1;
+  from_end.scale_in = scale;
+  from_end.scale_out = 1.0f;
+  r2s::Role dv_role = from_end, dk_role = from_end, dq_role{};
+  dv_role.q = vk;
+  dv_role.k = vq;
+  dv_role.v = vg;
+  dv_role.dk = static_cast<int32_t>(dk);
+  dv_role.dv = static_cast<int32_t>(dv);
+  dv_role.y = v_v;
+  dv_role.final_state = v_initial;
+  dk_role.q = vv;
+  dk_role.k = vg;
+  dk_role.v = vq;
+  dk_role.dk = static_cast<int32_t>(dv);
+  dk_role.dv = static_cast<int32_t>(dk);
+  dk_role.transposed = 1;
+  dk_role.y = v_k;
+  dq_role.q = vg;
+  dq_role.k = vv;
+  dq_role.v = vk;
+  dq_role.initial = initial;
+  dq_role.carried = const_cast<float *>(kept);  // read only: no states are made here
+  dq_role.dk = static_cast<int32_t>(dv);
+  dq_role.dv = static_cast<int32_t>(dk);
+  dq_role.transposed = 1;
+  dq_role.backwards = reverse != 0;
+  dq_role.scale_in = 1.0f;
+  dq_role.scale_out = scale;
+  dq_role.y = v_q;
+  w.role[0] = dv_role;
+  if (p.cut) {
+    R2S_RETURN_IF(r2s::walk<true>(z, p, w, 1, stream));
+    R2S_RETURN_IF(r2s::carry(z, p, w, stream));
+  }
+  w.role[1] = dk_role;
+  w.role[2] = dq_role;
+  return r2s::walk<false>(z, p, w, 3, stream);
+}
+
+int r2s_decay_attention_step(const void *q, int64_t q_token, int64_t q_head, const void *k,
+                             int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
+                             int64_t v_head, const float *log_decay, const float *state,
+                             int64_t sequences, int64_t heads, int64_t dk, int64_t dv, float scale,
+                             int32_t type, void *y, float *next, r2s_stream_t st) {
+  r2s::clear_error();
+  const r2s::Sizes z{type, false, sequences, 1, sequences, heads, dk, dv};
+  R2S_RETURN_IF(r2s::check_sizes("decay_attention_step", z));
+  if (sequences == 0 || heads == 0 || dv == 0) return R2S_OK;
+  R2S_REQUIRE(log_decay && v && y && (dk == 0 || (q && k && state && next)),
+              "decay_attention_step: null pointer");
+  const r2s::View vq{q, 0, q_token, q_head}, vk{k, 0, k_token, k_head}, vv{v, 0, v_token, v_head};
+  R2S_REQUIRE(!r2s::bad_view(z, vq) && !r2s::bad_view(z, vk) && !r2s::bad_view(z, vv),
+              "decay_attention_step: bad stride");
+  if (sequences * heads > r2s::kInt32Max) {
+    r2s::set_error("decay_attention_step: more than 2^31 - 1 states");
+    return R2S_ERANGE;
+  }
+  const bool wide = dv % 4 == 0 && (r2s::address(state) | r2s::address(next)) % 16 == 0;
+  const dim3 grid(static_cast<uint32_t>(sequences * heads));
+  hipStream_t stream = r2s::as_stream(st);
+  const int h = static_cast<int>(heads), a = static_cast<int>(dk), b = static_cast<int>(dv);
+  R2S_BY_TYPE(type, {
+    if (wide)
+      r2s::decay_step_kernel<T, 4><<<grid, dim3(256), 0, stream>>>(
+          vq, vk, vv, log_decay, state, h, a, b, scale, static_cast<T *>(y), next);
+    else
+      r2s::decay_step_kernel<T, 1><<<grid, dim3(256), 0, stream>>>(
+          vq, vk, vv, log_decay, state, h, a, b, scale, static_cast<T *>(y), next);
+  });
+  return r2s::check_launch("decay_attention_step");
+}
+
+}  // extern "C"

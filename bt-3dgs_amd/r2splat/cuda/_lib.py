@@ -151,6 +151,17 @@ _PLAIN = {
     "r2s_residual_norm_bwd": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _i64, _p,
                                      _i64, _f32, _f32, _i32, _i32, _i64, _i64, _p, _p, _p, _p, _p,
                                      _p, _sz, _p]),
+    "r2s_decay_attention_kept_states": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "r2s_decay_attention_workspace_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
+                                                   _i32]),
+    "r2s_decay_attention_fwd": (_i32, [_p, _i64, _i64, _i64] * 3 + [
+        _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _p, _p, _p, _p, _sz,
+        _p]),
+    "r2s_decay_attention_bwd": (_i32, [_p, _i64, _i64, _i64] * 3 + [
+        _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32,
+        _i32, _p, _p, _p, _p, _p, _sz, _p]),
+    "r2s_decay_attention_step": (_i32, [_p, _i64, _i64] * 3 + [
+        _p, _p, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p, _p]),
 }
 
 
@@ -200,7 +211,7 @@ ROTARY_MAX_AXES = 8
 
 SYMBOLS = sorted(list(_PLAIN) + [f"r2s_{n}_{s}" for n in _FLOAT_OPS for s in ("f32", "f64")])
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 
 def load(path: str = LIB_PATH) -> ctypes.CDLL:

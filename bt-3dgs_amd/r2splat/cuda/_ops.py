@@ -2342,3 +2342,151 @@ def residual_norm_bwd(x: Tensor, update: Optional[Tensor], gate: Optional[Tensor
               _ptr(w2), _ptr(yr), ys, _ptr(vr), vs, float(scale), float(eps), bool(centered), code,
               n, d, *(_ptr(g) for g in grads), _ptr(ws), need, _stream(dev))
     return tuple(grads)
+
+
+# -- linear attention with a decay for each head
+
+
+def _attention_input(t: Tensor, name: str, like: Tensor, shape):
+    """(tensor, (sequence, token, head) strides) of [B, L, H, D] or [N, H, D]; a
+    copy where a head's elements are not consecutive."""
+    _check_latent(t, name, like, like.dtype)
+    if t.shape != shape:
+        _fail(name, " must be ", tuple(shape), ", got shape ", tuple(t.shape))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return (t, *t.stride()[:-1]) if t.dim() == 4 else (t, 0, *t.stride()[:-1])
+
+
+def _attention_state(t: Optional[Tensor], name: str, like: Tensor, shape) -> Optional[Tensor]:
+    if t is None:
+        return None
+    _check_latent(t, name, like, torch.float32)
+    if t.shape != shape:
+        _fail(name, " must be ", tuple(shape), ", got shape ", tuple(t.shape))
+    return t.contiguous()
+
+
+def _attention_inputs(q, k, v, log_decay, offsets, op):
+    """(type code, the inputs with their strides, decays, sizes as the C entries
+    take them, the states' shape)."""
+    _check_latent(q, "q")
+    code = _latent_type(q, op)
+    dims = 4 if offsets is None else 3
+    if q.dim() != dims:
+        _fail("q must be ", "[B, L, H, Dk] without" if dims == 4 else "[N, H, Dk] with",
+              " offsets, got shape ", tuple(q.shape))
+    lead, heads, dk = q.shape[:-2], q.shape[-2], q.shape[-1]
+    qr = _attention_input(q, "q", q, q.shape)
+    kr = _attention_input(k, "k", q, q.shape)
+    _check_latent(v, "v", q, q.dtype)
+    vr = _attention_input(v, "v", q, (*lead, heads, v.shape[-1] if v.dim() else 0))
+    _check_latent(log_decay, "log_decay", q, torch.float32)
+    if log_decay.shape != (heads,):
+        _fail("log_decay must be [", heads, "], got shape ", tuple(log_decay.shape))
+    if offsets is None:
+        sequences, length = lead
+    else:
+        _check_latent(offsets, "offsets", q, torch.int32)
+        if offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
+            _fail("offsets must be a contiguous [S + 1], got shape ", tuple(offsets.shape))
+        sequences, length = offsets.numel() - 1, 0
+        if sequences == 0 and lead[0] > 0:
+            _fail("offsets name no sequence for ", lead[0], " tokens")
+    sizes = (sequences, length, math.prod(lead), heads, dk, v.shape[-1])
+    return code, (*qr, *kr, *vr), log_decay.contiguous(), sizes, (sequences, heads, dk, v.shape[-1])
+
+
+def _with_ptrs(inputs):
+    """Inputs and their strides with addresses in the tensors' places."""
+    return [t.data_ptr() if isinstance(t, Tensor) else t for t in inputs]
+
+
+def decay_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor,
+                        initial: Optional[Tensor] = None, offsets: Optional[Tensor] = None,
+                        reverse: bool = False, scale: float = 1.0, keep: bool = True
+                        ) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
+    """(y, final, kept) of S_t = exp(log_decay) S_{t-1} + k_t v_t^T and
+    y_t = scale S_t^T q_t: y in v's shape, final [S, H, Dk, Dv] float32 each
+    sequence's last state, kept what decay_attention_bwd takes (None without
+    ``keep``).  q, k [B, L, H, Dk], v [B, L, H, Dv], or [N, H, D] with offsets
+    [S + 1] (int32, from 0 to at most N); log_decay [H], initial like final."""
+    code, inputs, log_decay, sizes, shape = _attention_inputs(q, k, v, log_decay, offsets,
+                                                              "decay_attention_fwd")
+    initial = _attention_state(initial, "initial", q, shape)
+    dev = q.device
+    lib = _lib()
+    ragged = offsets is not None
+    with _on(dev):
+        y = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        final = torch.empty(shape, dtype=torch.float32, device=dev)
+        kept = torch.empty((lib.r2s_decay_attention_kept_states(code, ragged, *sizes), *shape[1:]),
+                           dtype=torch.float32, device=dev)
+        need = lib.r2s_decay_attention_workspace_bytes(code, ragged, *sizes, 0)
+        ws = _workspace(need, dev) if need else None
+        _call("r2s_decay_attention_fwd", *_with_ptrs(inputs), _ptr(log_decay), _ptr(initial),
+              _ptr(offsets), *sizes, float(scale), code, bool(reverse), _ptr(y), _ptr(final),
+              _ptr(kept), _ptr(ws), need, _stream(dev))
+    return y, final, kept if keep else None
+
+
+def decay_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor,
+                        initial: Optional[Tensor], offsets: Optional[Tensor], kept: Tensor,
+                        v_y: Tensor, v_final: Optional[Tensor] = None, reverse: bool = False,
+                        scale: float = 1.0) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(v_q, v_k, v_v, v_initial) of decay_attention_fwd with the same inputs,
+    whose ``kept`` this is, from v_y (v's shape and type) and v_final."""
+    code, inputs, log_decay, sizes, shape = _attention_inputs(q, k, v, log_decay, offsets,
+                                                              "decay_attention_bwd")
+    grad = _attention_input(v_y, "v_y", q, v.shape)
+    initial = _attention_state(initial, "initial", q, shape)
+    v_final = _attention_state(v_final, "v_final", q, shape)
+    dev = q.device
+    lib = _lib()
+    ragged = offsets is not None
+    _check_latent(kept, "kept", q, torch.float32)
+    if kept.shape != (lib.r2s_decay_attention_kept_states(code, ragged, *sizes), *shape[1:]) \
+            or not kept.is_contiguous():
+        _fail("kept is not that of the forward of these inputs: shape ", tuple(kept.shape))
+    with _on(dev):
+        # Heads of no channels leave nothing to be written.
+        new = torch.empty if shape[2] and shape[3] else torch.zeros
+        v_q, v_k, v_v = (new(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
+        v_initial = torch.empty(shape, dtype=torch.float32, device=dev)
+        need = lib.r2s_decay_attention_workspace_bytes(code, ragged, *sizes, 1)
+        ws = _workspace(need, dev) if need else None
+        _call("r2s_decay_attention_bwd", *_with_ptrs(inputs), _ptr(log_decay), _ptr(initial),
+              _ptr(offsets), _ptr(kept), *_with_ptrs(grad), _ptr(v_final), *sizes, float(scale),
+              code, bool(reverse), _ptr(v_q), _ptr(v_k), _ptr(v_v), _ptr(v_initial), _ptr(ws), need,
+              _stream(dev))
+    return v_q, v_k, v_v, v_initial
+
+
+def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor,
+                         scale: float = 1.0) -> Tuple[Tensor, Tensor]:
+    """(y, next state) after one more token of each of B sequences: q, k
+    [B, H, Dk], v [B, H, Dv], state [B, H, Dk, Dv] float32."""
+    _check_latent(q, "q")
+    code = _latent_type(q, "decay_attention_step")
+    if q.dim() != 3:
+        _fail("q must be [B, H, Dk], got shape ", tuple(q.shape))
+    b, heads, dk = q.shape
+    _check_latent(v, "v", q, q.dtype)
+    dv = v.shape[-1] if v.dim() else 0
+    qr, _, *qs = _attention_input(q, "q", q, q.shape)
+    kr, _, *ks = _attention_input(k, "k", q, q.shape)
+    vr, _, *vs = _attention_input(v, "v", q, (b, heads, dv))
+    _check_latent(log_decay, "log_decay", q, torch.float32)
+    if log_decay.shape != (heads,):
+        _fail("log_decay must be [", heads, "], got shape ", tuple(log_decay.shape))
+    state = _attention_state(state, "state", q, (b, heads, dk, dv))
+    if state is None:
+        _fail("state must be given")
+    dev = q.device
+    with _on(dev):
+        y = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        final = torch.empty(state.shape, dtype=torch.float32, device=dev)
+        _call("r2s_decay_attention_step", _ptr(qr), *qs, _ptr(kr), *ks, _ptr(vr), *vs,
+              _ptr(log_decay.contiguous()), _ptr(state), b, heads, dk, dv, float(scale), code,
+              _ptr(y), _ptr(final), _stream(dev))
+    return y, final

@@ -68,6 +68,9 @@ grouped_matmul_bwd = _make_cuda_func("grouped_matmul_bwd")
 rotary_axes = _make_cuda_func("rotary_axes")
 residual_norm_fwd = _make_cuda_func("residual_norm_fwd")
 residual_norm_bwd = _make_cuda_func("residual_norm_bwd")
+decay_attention_fwd = _make_cuda_func("decay_attention_fwd")
+decay_attention_step = _make_cuda_func("decay_attention_step")
+decay_attention_bwd = _make_cuda_func("decay_attention_bwd")
 
 
 def is_cuda_extension_available() -> bool:

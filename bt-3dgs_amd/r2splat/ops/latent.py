@@ -14,6 +14,9 @@ of them.
   ``gated_scan_step`` for one more token of running sequences;
 * ``grouped_matmul``    one weight per group of rows, groups of any size, the
   groups' rows anywhere in the table; ``group_rows`` finds them;
+* ``decay_attention``   linear attention whose state every head forgets at its
+  own rate, over equal or ragged sequences of any length, and
+  ``decay_attention_step`` for one more token of running sequences;
 * ``rotary_axes``       queries and keys turned by their positions along several
   axes;
 * ``pre_norm``, ``residual_norm``  the norms before and after a block, with its
@@ -35,7 +38,7 @@ from torch.autograd import forward_ad
 from ..cuda import _wrapper as W
 
 __all__ = ["embedding_lookup", "gated_scan", "gated_scan_step", "grouped_matmul", "group_rows",
-           "rotary_axes", "pre_norm", "residual_norm"]
+           "decay_attention", "decay_attention_step", "rotary_axes", "pre_norm", "residual_norm"]
 
 
 def _wants_grad(*tensors) -> bool:
@@ -262,3 +265,66 @@ def residual_norm(x: Tensor, update: Tensor, gate: Optional[Tensor] = None,
         return W.residual_norm_fwd(x, update, gate, update_weight, weight, *plan)
     out = _ResidualNorm.apply(x, update, gate, update_weight, weight, plan)
     return out if weight is not None else (out[0], None)
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial, offsets, reverse, scale):
+        ctx.set_materialize_grads(False)
+        y, final, kept = W.decay_attention_fwd(q, k, v, log_decay, initial, offsets, reverse, scale)
+        ctx.save_for_backward(q, k, v, log_decay, initial, offsets, kept)
+        ctx.reverse, ctx.scale = reverse, scale
+        return y, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, v_y, v_final):
+        q, k, v, log_decay, initial, offsets, kept = ctx.saved_tensors
+        if v_y is None:
+            v_y = torch.zeros_like(v)
+        v_q, v_k, v_v, v_initial = W.decay_attention_bwd(q, k, v, log_decay, initial, offsets, kept,
+                                                         v_y, v_final, ctx.reverse, ctx.scale)
+        return (v_q, v_k, v_v, None, v_initial if ctx.needs_input_grad[4] else None, None, None,
+                None)
+
+
+def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor,
+                    initial: Optional[Tensor] = None, offsets: Optional[Tensor] = None,
+                    reverse: bool = False, scale: Optional[float] = None
+                    ) -> Tuple[Tensor, Tensor]:
+    """(y, final) of linear attention with a decay for each head::
+
+        S_t = exp(log_decay) S_{t-1} + k_t v_t^T,    y_t = scale S_t^T q_t
+
+    q, k: [B, L, H, Dk], v: [B, L, H, Dv], or ragged sequences one behind the
+    other, [N, H, D] with ``offsets`` [S + 1] (integers that ascend from 0 to at
+    most N; equal ones are empty sequences; tokens behind the last give zeros).
+    Dk and Dv up to 256.  ``log_decay`` [H] float32 holds the natural logarithms
+    of the decays, at most 0 (-inf: every token alone); it has no gradient.
+    ``initial`` [B or S, H, Dk, Dv] float32 is each sequence's first state (zeros
+    by default), ``final`` its last.  ``scale`` is Dk^-0.5 by default; ``reverse``
+    runs each sequence from its last token.  A NaN or infinity reaches later
+    tokens of its head and sequence, never earlier ones."""
+    _refuse_grad(log_decay, "log_decay")
+    offsets = _index32(offsets)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
+    if not _wants_grad(q, k, v, initial):
+        return W.decay_attention_fwd(q, k, v, log_decay, initial, offsets, bool(reverse),
+                                     float(scale), keep=False)[:2]
+    return _DecayAttention.apply(q, k, v, log_decay, initial, offsets, bool(reverse), float(scale))
+
+
+def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor,
+                         scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
+    """(y, next state) after one more token of each of B sequences: q, k
+    [B, H, Dk], v [B, H, Dv], state [B, H, Dk, Dv] float32."""
+    if state is None:
+        raise RuntimeError("state must be given")
+    _refuse_grad(log_decay, "log_decay")
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
+    if not _wants_grad(q, k, v, state):
+        return W.decay_attention_step(q, k, v, log_decay, state, float(scale))
+    y, final = decay_attention(q[:, None], k[:, None], v[:, None], log_decay, state, scale=scale)
+    return y[:, 0], final

@@ -1299,6 +1299,53 @@ int r2s_residual_norm_bwd(const void *x, int64_t x_stride, const void *update,
                           void *v_gate, void *v_update_weight, void *v_weight, void *workspace,
                           size_t workspace_bytes, r2s_stream_t stream);
 
+/* Linear attention with a decay for each head: S_t = exp(log_decay) S_{t-1} +
+ * k_t v_t^T, y_t = scale S_t^T q_t, for `sequences` sequences of `length` tokens
+ * (n in all) or (offsets [sequences + 1] given, ascending from 0 to at most n)
+ * ragged ones, empty ones among them; tokens behind the last give zeros.
+ * reverse: each sequence from its last token to its first.  A token's row of q, k
+ * [heads, dk] and v [heads, dv] is found by the strides of its sequence (equal ones
+ * alone; ragged tokens are counted from 0), its place in it and its head, in
+ * elements; a head's elements are consecutive.  dk, dv at most 256.  log_decay
+ * [heads]; initial [sequences, heads, dk, dv] (may be NULL: zeros); final_state
+ * likewise; y [n, heads, dv] dense.  kept [r2s_decay_attention_kept_states(...),
+ * heads, dk, dv] receives states that the backward starts from (NULL where that
+ * is 0). */
+int64_t r2s_decay_attention_kept_states(int32_t type, int32_t ragged, int64_t sequences,
+                                        int64_t length, int64_t n, int64_t heads, int64_t dk,
+                                        int64_t dv);
+int64_t r2s_decay_attention_workspace_bytes(int32_t type, int32_t ragged, int64_t sequences,
+                                            int64_t length, int64_t n, int64_t heads, int64_t dk,
+                                            int64_t dv, int32_t backward);
+int r2s_decay_attention_fwd(const void *q, int64_t q_sequence, int64_t q_token, int64_t q_head,
+                            const void *k, int64_t k_sequence, int64_t k_token, int64_t k_head,
+                            const void *v, int64_t v_sequence, int64_t v_token, int64_t v_head,
+                            const float *log_decay, const float *initial, const int32_t *offsets,
+                            int64_t sequences, int64_t length, int64_t n, int64_t heads,
+                            int64_t dk, int64_t dv, float scale, int32_t type, int32_t reverse,
+                            void *y, float *final_state, float *kept, void *workspace,
+                            size_t workspace_bytes, r2s_stream_t stream);
+/* Its gradient from v_y (by strides) and v_final [sequences, heads, dk, dv] (may
+ * be NULL): v_q, v_k [n, heads, dk] and v_v [n, heads, dv] dense, v_initial (may be
+ * NULL: not wanted).  kept as the forward of the same inputs left it. */
+int r2s_decay_attention_bwd(const void *q, int64_t q_sequence, int64_t q_token, int64_t q_head,
+                            const void *k, int64_t k_sequence, int64_t k_token, int64_t k_head,
+                            const void *v, int64_t v_sequence, int64_t v_token, int64_t v_head,
+                            const float *log_decay, const float *initial, const int32_t *offsets,
+                            const float *kept, const void *v_y, int64_t vy_sequence,
+                            int64_t vy_token, int64_t vy_head, const float *v_final,
+                            int64_t sequences, int64_t length, int64_t n, int64_t heads,
+                            int64_t dk, int64_t dv, float scale, int32_t type, int32_t reverse,
+                            void *v_q, void *v_k, void *v_v, float *v_initial, void *workspace,
+                            size_t workspace_bytes, r2s_stream_t stream);
+/* One token of each of `sequences` sequences: y [sequences, heads, dv] and the next
+ * states from state [sequences, heads, dk, dv]. */
+int r2s_decay_attention_step(const void *q, int64_t q_token, int64_t q_head, const void *k,
+                             int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
+                             int64_t v_head, const float *log_decay, const float *state,
+                             int64_t sequences, int64_t heads, int64_t dk, int64_t dv, float scale,
+                             int32_t type, void *y, float *next, r2s_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -191,3 +191,61 @@ def quantize(x, r, root):
     if root:
         code = np.where((x > 0) & (code == 0), LEAST, code)
     return np.where(np.isfinite(x), np.copysign(code, x), np.nan), scale
+
+
+# ------------------------------------------------------- decay attention --
+
+
+class DecayAttention:
+    """S_t = g S_{t-1} + k_t v_t^T, y_t = scale S_t^T q_t over q, k [N, H, Dk],
+    v [N, H, Dv], sequences [bounds[s], bounds[s + 1]), token after token.
+
+    Beside y, the final states and the gradients it keeps the same sums of absolute
+    terms (``*_mass``): an evaluation by products of c-token chunks in float32 makes
+    sums of at most dk + dv + c terms and powers of g off by a few units, and walks
+    length / c steps, each of which rounds the state once more."""
+
+    def __init__(self, q, k, v, log_decay, bounds, initial=None, reverse=False, scale=1.0):
+        self.q, self.k, self.v, self.scale = q, k, v, scale
+        self.g = np.exp(log_decay)[:, None, None]
+        self.bounds, self.reverse = bounds, reverse
+        s, h = len(bounds) - 1, q.shape[1]
+        zeros = np.zeros((s, h, q.shape[2], v.shape[2]))
+        self.initial = zeros if initial is None else initial
+
+    def _walk(self, q, k, v, start, early, reverse):
+        """y and last states of the recurrence that all the outputs are."""
+        y, last = np.zeros(v.shape), start.copy()
+        with np.errstate(invalid="ignore"):
+            for s in range(len(self.bounds) - 1):
+                state = start[s].copy()
+                order = range(self.bounds[s], self.bounds[s + 1])
+                for t in reversed(order) if reverse else order:
+                    if not early:
+                        state = self.g * state
+                    state = state + k[t][:, :, None] * v[t][:, None, :]
+                    y[t] = (q[t][:, :, None] * state).sum(1)
+                    if early:
+                        state = self.g * state
+                last[s] = state
+        return y, last
+
+    def _both(self, q, k, v, start, early, reverse):
+        exact = self._walk(q, k, v, start, early, reverse)
+        mass = self._walk(*(np.abs(a) for a in (q, k, v, start)), early, reverse)
+        return (*exact, *mass)
+
+    def forward(self):
+        """(y, final, y_mass, final_mass)."""
+        y, final, ym, fm = self._both(self.q, self.k, self.v, self.initial, False, self.reverse)
+        return self.scale * y, final, abs(self.scale) * ym, fm
+
+    def backward(self, v_y, v_final=None):
+        """{name: (gradient, mass)}."""
+        turn = lambda a: a.swapaxes(-1, -2)  # noqa: E731
+        last = np.zeros_like(self.initial) if v_final is None else v_final
+        g = self.scale * v_y
+        v_q, _, qm, _ = self._both(g, self.v, self.k, turn(self.initial), False, self.reverse)
+        v_v, start, vm, sm = self._both(self.k, self.q, g, last, True, not self.reverse)
+        v_k, _, km, _ = self._both(self.v, g, self.q, turn(last), True, not self.reverse)
+        return dict(v_q=(v_q, qm), v_k=(v_k, km), v_v=(v_v, vm), v_initial=(start, sm))

@@ -225,3 +225,71 @@ def test_tangents_are_refused_rather_than_lost(monkeypatch):
                 call()
         with pytest.raises(NotImplementedError, match="positions"):
             latent.rotary_axes(t, None, forward_ad.make_dual(p, torch.ones_like(p)), (3,))
+
+
+def test_decay_attention_arguments(lib):
+    def fwd(q=FAKE, qs=(80, 16, 8), offsets=None, s=2, length=5, n=10, h=2, dk=8, dv=8, type_=0,
+            final=FAKE, kept=FAKE, decay=FAKE):
+        return lib.r2s_decay_attention_fwd(q, *qs, FAKE, 80, 16, 8, FAKE, 80, 16, 8, decay, None,
+                                           offsets, s, length, n, h, dk, dv, 1.0, type_, 0, FAKE,
+                                           final, kept, None, 0, None)
+
+    _refused(lib, fwd(type_=9), 1001, b"element type")
+    _refused(lib, fwd(h=-1), 1001, b"negative")
+    _refused(lib, fwd(dk=257), 1002, b"256 channels")
+    _refused(lib, fwd(n=1 << 31), 1002, b"tokens")
+    _refused(lib, fwd(n=11), 1001, b"11 tokens are not 2 sequences of 5")
+    _refused(lib, fwd(offsets=FAKE, s=0), 1001, b"without a sequence")
+    _refused(lib, fwd(decay=None), 1001, b"null decays")
+    _refused(lib, fwd(final=None), 1001, b"null final")
+    _refused(lib, fwd(q=None), 1001, b"null tokens")
+    _refused(lib, fwd(qs=(-1, 16, 8)), 1001, b"bad stride")
+    _refused(lib, fwd(qs=(80, 1 << 58, 8)), 1001, b"bad stride")
+    _refused(lib, fwd(s=1, length=100_000, n=100_000, kept=None), 1001, b"null kept")
+    _refused(lib, fwd(offsets=FAKE, n=100_000), 1004, b"workspace")
+    assert fwd(s=0, n=0) == 0 and fwd(h=0) == 0 and fwd(dv=0) == 0
+    kept, room = lib.r2s_decay_attention_kept_states, lib.r2s_decay_attention_workspace_bytes
+    # Short sequences carry nothing; a long one's states are few beside its tokens.
+    assert kept(0, 0, 8, 200, 1600, 4, 16, 16) == 0 and room(0, 0, 8, 200, 1600, 4, 16, 16, 1) == 0
+    states = kept(1, 0, 1, 500_000, 500_000, 4, 16, 16)
+    assert 0 < states <= 500_000 // 256
+    assert room(1, 0, 1, 500_000, 500_000, 4, 16, 16, 0) == 0
+    assert room(1, 0, 1, 500_000, 500_000, 4, 16, 16, 1) == states * 4 * 16 * 16 * 4
+    # Ragged calls have a table of their spans, and no state for each sequence.
+    assert kept(0, 1, 100_000, 0, 100_000, 4, 16, 16) <= 100_000 // 256
+    assert 4 * 100_000 < room(0, 1, 100_000, 0, 100_000, 4, 16, 16, 0) < 1 << 20
+    assert kept(7, 0, 1, 9, 9, 1, 1, 1) == 0 and room(0, 0, 1, 9, 8, 1, 1, 1, 1) == 0
+    rc = lib.r2s_decay_attention_bwd(FAKE, 80, 16, 8, FAKE, 80, 16, 8, FAKE, 80, 16, 8, FAKE, None,
+                                     None, None, FAKE, 80, 16, 8, None, 2, 5, 10, 2, 8, 8, 1.0, 0,
+                                     0, None, FAKE, FAKE, None, None, 0, None)
+    _refused(lib, rc, 1001, b"null tokens")
+    rc = lib.r2s_decay_attention_step(FAKE, 16, 8, FAKE, 16, 8, FAKE, 16, 8, FAKE, None, 2, 2, 8, 8,
+                                      1.0, 0, FAKE, FAKE, None)
+    _refused(lib, rc, 1001, b"null pointer")
+
+
+def test_decay_attention_restatement_against_autograd():
+    g = torch.Generator().manual_seed(3)
+    draw = lambda *s: torch.randn(s, generator=g, dtype=torch.float64)  # noqa: E731
+    bounds = [0, 7, 7, 20]
+    for reverse in (False, True):
+        q, k, v, state = draw(20, 2, 4), draw(20, 2, 4), draw(20, 2, 3), draw(3, 2, 4, 3)
+        v_y, v_final, log_decay = draw(20, 2, 3), draw(3, 2, 4, 3), -draw(2).abs()
+        leaves = [t.requires_grad_(True) for t in (q, k, v, state)]
+        gamma, ys, finals = log_decay.exp()[:, None, None], [None] * 20, []
+        for s in range(3):
+            now = state[s]
+            order = range(bounds[s], bounds[s + 1])
+            for t in reversed(order) if reverse else order:
+                now = gamma * now + k[t][:, :, None] * v[t][:, None]
+                ys[t] = 0.4 * (q[t][:, :, None] * now).sum(1)
+            finals.append(now)
+        y, final = torch.stack(ys), torch.stack(finals)
+        want = torch.autograd.grad((y * v_y).sum() + (final * v_final).sum(), leaves)
+        exact = ref.DecayAttention(*(t.detach().numpy() for t in (q, k, v, log_decay)), bounds,
+                                   state.detach().numpy(), reverse, 0.4)
+        ey, ef, _, _ = exact.forward()
+        assert np.allclose(ey, y.detach()) and np.allclose(ef, final.detach())
+        found = exact.backward(v_y.numpy(), v_final.numpy())
+        for name, grad in zip(("v_q", "v_k", "v_v", "v_initial"), want):
+            assert np.allclose(found[name][0], grad), name
