@@ -21,18 +21,20 @@
 // decay a state behind its token, g^i and g^(C-j) above.  g R after the last token is
 // the first state's gradient.
 //
-// A block is one head and up to 16 NT W columns of v of one span of a sequence.
-// The state stays in registers: each of its W waves holds all rows of 16 NT columns,
-// as accumulators that turn into operands without moving between lanes.  For
-// that the products are made transposed (scores as k q^T, outputs as v^T p), so a
-// lane has one token's scores and neighbouring columns of its output.  Every wave
-// makes the chunk's scores for itself, which costs it less than sharing them.
+// A block is one head and up to 16 W columns of v of one span of a sequence.  Each of
+// its W waves keeps the state's rows of 16 columns in registers and brings them up to
+// date; the outputs are shared out by tokens instead, so that each score is made
+// once, and every wave reads the state of all columns, as operands, from LDS.  The
+// products are made transposed (scores as k q^T, outputs as v^T p): then an
+// accumulator's values are, lane by lane, the next product's operand, and a lane
+// ends with neighbouring columns of one token.
 //
 // Precision: the scores, the state and the decayed v are float32 values.  As
 // operands of 16-bit products they are split into a rounded part and a rounded
-// rest (two products instead of one), so that nothing is rounded to 16 bits but
-// the outputs; float16 inputs beside them, whose range does not hold those values,
-// are split without loss into bfloat16 parts.
+// rest (the decayed v, which adds up in the state, into three), a product for
+// each, so that nothing is rounded to 16 bits but the outputs; float16 inputs
+// beside them, whose range does not hold those values, are split without loss into
+// bfloat16 parts.
 //
 // A zero weight times a NaN or an infinity is a NaN: a chunk with such a v would
 // reach back to its earlier tokens.  Its tokens are walked one by one.
@@ -54,6 +56,7 @@ using i16x4 = __attribute__((ext_vector_type(4))) short;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 constexpr int kMostChannels = 256;
+constexpr int64_t kMostStep = 1 << 24;  // elements between tokens: a chunk is within 2^31 bytes
 
 // One input: sequence s (of equal ones), its token and head by strides.
 struct View {
@@ -110,8 +113,9 @@ __device__ __forceinline__ int64_t bound(const Cut &c, int64_t s) {
 __device__ __forceinline__ bool find_span(const Cut &c, int64_t item, Span &x) {
   int64_t index = 0, items = 1;
   if (c.offsets == nullptr) {
-    x.sequence = item / c.spans;
-    index = item - x.sequence * c.spans;
+    const uint32_t which = static_cast<uint32_t>(item), spans = static_cast<uint32_t>(c.spans);
+    x.sequence = which / spans;
+    index = which % spans;
     items = c.spans;
     x.lo = x.sequence * c.length;
     x.length = c.length;
@@ -173,25 +177,11 @@ __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
   for (int64_t i = before + threadIdx.x; i < most; i += 1024) owner[i] = -1;
 }
 
-// The states behind the spans from each span's own, along every sequence.
-__global__ __launch_bounds__(256) void decay_carry_kernel(Walk w, int64_t total) {
-  const Role &r = w.role[0];
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int64_t size = static_cast<int64_t>(r.dk) * r.dv;
-  const int64_t sequence = i / (w.heads * size), inside = i - sequence * w.heads * size;
-  const int32_t head = static_cast<int32_t>(inside / size);
-  int64_t place = sequence * (w.cut.spans - 1), count = w.cut.spans - 1;
-  if (w.cut.offsets != nullptr) {
-    place = w.cut.first[sequence] - sequence;
-    count = w.cut.first[sequence + 1] - w.cut.first[sequence] - 1;
-    count = min(count, w.cut.carried - place);
-  }
-  if (count <= 0) return;
-  const float keep = expf(w.log_decay[head] * static_cast<float>(w.cut.span));
-  float now = r.initial != nullptr ? r.initial[i] : 0.0f;
-  float *p = r.carried + place * w.heads * size + inside;
-  const int64_t step = w.heads * size;
+// The states behind `count` spans of a sequence from each span's own, from `now` on:
+// p [count] of one element, `step` apart.  Returns the last; stores them with kStore.
+template <bool kStore>
+__device__ __forceinline__ float carry_along(float *p, int64_t step, int64_t count, float keep,
+                                             float now) {
   constexpr int kAhead = 8;
   for (int64_t c = 0; c < count; c += kAhead) {
     float own[kAhead];
@@ -199,8 +189,67 @@ __global__ __launch_bounds__(256) void decay_carry_kernel(Walk w, int64_t total)
     for (int a = 0; a < kAhead; ++a) own[a] = c + a < count ? p[(c + a) * step] : 0.0f;
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
-      now = fmaf(keep, now, own[a]);
-      if (c + a < count) p[(c + a) * step] = now;
+      if (c + a < count) {
+        now = fmaf(keep, now, own[a]);
+        if constexpr (kStore) p[(c + a) * step] = now;
+      }
+    }
+  }
+  return now;
+}
+
+// Equal sequences of few spans: a thread to an element of their states.
+__global__ __launch_bounds__(256) void decay_carry_few_kernel(Walk w, int64_t total) {
+  const Role &r = w.role[0];
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t size = static_cast<int64_t>(r.dk) * r.dv, step = w.heads * size;
+  const int64_t sequence = i / step, e = i - sequence * step, count = w.cut.spans - 1;
+  const float keep = expf(w.log_decay[e / size] * static_cast<float>(w.cut.span));
+  carry_along<true>(r.carried + sequence * count * step + e, step, count, keep,
+                    r.initial != nullptr ? r.initial[i] : 0.0f);
+}
+
+// Any sequences: a block takes 64 elements of the states of one after another.  Its
+// 16 waves take a run of a long sequence's spans each, add it up, and go over it
+// again from what the waves before them leave, so that hundreds of spans are not a
+// chain of as many loads (four heads of 16 x 16: 600 spans in 11 us; a chain took 12
+// for 252).  `per` sequences are looked at together: ragged ones mostly have one span.
+__global__ __launch_bounds__(1024) void decay_carry_kernel(Walk w, int per) {
+  __shared__ float s_sum[16][64];
+  const Role &r = w.role[0];
+  const int64_t size = static_cast<int64_t>(r.dk) * r.dv, step = w.heads * size;
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 64 + lane_id();
+  const bool some = e < step;
+  const int wave = static_cast<int>(wave_index());
+  const float log_span = some ? w.log_decay[e / size] * static_cast<float>(w.cut.span) : 0.0f;
+  const float keep = expf(log_span);
+  for (int64_t s0 = static_cast<int64_t>(blockIdx.y) * per; s0 < w.cut.sequences;
+       s0 += static_cast<int64_t>(gridDim.y) * per) {
+    const int64_t mine = s0 + lane_id();
+    int64_t place = 0, count = 0;
+    if (static_cast<int>(lane_id()) < per && mine < w.cut.sequences) {
+      place = mine * (w.cut.spans - 1);
+      count = w.cut.spans - 1;
+      if (w.cut.offsets != nullptr) {
+        place = w.cut.first[mine] - mine;
+        count = w.cut.first[mine + 1] - w.cut.first[mine] - 1;
+        count = min(count, w.cut.carried - place);
+      }
+    }
+    for (uint64_t left = ballot(count > 0); left != 0; left &= left - 1) {
+      const uint32_t from = static_cast<uint32_t>(__builtin_ctzll(left));
+      const int64_t spans = readlane_i64(count, from);
+      const int64_t each = spans <= 16 ? spans : (spans + 15) / 16;
+      const int64_t lo = min(wave * each, spans), run = some ? min(each, spans - lo) : 0;
+      float *p = r.carried + (readlane_i64(place, from) + lo) * step + e;
+      if (spans > each) s_sum[wave][lane_id()] = carry_along<false>(p, step, run, keep, 0.0f);
+      __syncthreads();
+      float now = r.initial != nullptr && some ? r.initial[(s0 + from) * step + e] : 0.0f;
+      const float whole = expf(log_span * static_cast<float>(each));
+      for (int i = 0; i < wave && run > 0; ++i) now = fmaf(whole, now, s_sum[i][lane_id()]);
+      carry_along<true>(p, step, run, keep, now);
+      __syncthreads();  // the sums have been read
     }
   }
 }
@@ -224,26 +273,29 @@ __device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 acc) {
   }
 }
 
-// Float values of an operand's 16 bytes as a rounded part and the rounded rest;
-// float32 as they are.
+// Float values of an operand's 16 bytes as a rounded part and the rounded rest, and
+// with kThree what that leaves; float32 as they are.
 template <typename T>
 struct Parts {
-  u32x4 high, rest;
+  u32x4 high, rest, last;
 };
-template <typename T>
+template <typename T, bool kThree = false>
 __device__ __forceinline__ Parts<T> split(const float (&x)[16 / sizeof(T)]) {
   Parts<T> out;
   if constexpr (sizeof(T) == 4) {
     out.high = __builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]});
   } else {
-    Pack<T, 8> high, rest;
+    Pack<T, 8> high, rest, last;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       high.v[i] = static_cast<T>(x[i]);
-      rest.v[i] = static_cast<T>(x[i] - static_cast<float>(high.v[i]));
+      const float left = x[i] - static_cast<float>(high.v[i]);
+      rest.v[i] = static_cast<T>(left);
+      if constexpr (kThree) last.v[i] = static_cast<T>(left - static_cast<float>(rest.v[i]));
     }
     out.high = __builtin_bit_cast(u32x4, high);
     out.rest = __builtin_bit_cast(u32x4, rest);
+    if constexpr (kThree) out.last = __builtin_bit_cast(u32x4, last);
   }
   return out;
 }
@@ -278,8 +330,8 @@ __device__ __forceinline__ Parts<typename Wide<T>::type> beside(u32x4 raw) {
 }
 
 // acc += a b of an input and split values, as rows and columns or the other way
-// round.  T is the inputs' type.
-template <typename T, bool kInputRows>
+// round.  T is the inputs' type; smaller products first.
+template <typename T, bool kInputRows, bool kThree = false>
 __device__ __forceinline__ f32x4 multiply_split(const Parts<typename Wide<T>::type> &input,
                                                 const Parts<typename Wide<T>::type> &values,
                                                 f32x4 acc) {
@@ -288,6 +340,8 @@ __device__ __forceinline__ f32x4 multiply_split(const Parts<typename Wide<T>::ty
     acc = kInputRows ? multiply<U>(a, b, acc) : multiply<U>(b, a, acc);
   };
   if constexpr (sizeof(T) == 2) {
+    if constexpr (kThree) go(input.high, values.last);
+    if constexpr (kThree && std::is_same<T, f16_t>::value) go(input.rest, values.rest);
     if constexpr (std::is_same<T, f16_t>::value) go(input.rest, values.high);
     go(input.high, values.rest);
   }
@@ -295,9 +349,9 @@ __device__ __forceinline__ f32x4 multiply_split(const Parts<typename Wide<T>::ty
   return acc;
 }
 
-// g^x for a whole number x of tokens.
+// g^x for a whole number x of tokens; what is below float32's normal range is 0.
 __device__ __forceinline__ float power(float log2_decay, int x) {
-  return x == 0 ? 1.0f : exp2f(log2_decay * static_cast<float>(x));
+  return x == 0 ? 1.0f : __builtin_amdgcn_exp2f(log2_decay * static_cast<float>(x));
 }
 
 // --------------------------------------------------------------- walk ----
@@ -349,31 +403,44 @@ struct __attribute__((packed)) Loose {
   T v[V];
 };
 
-// A chunk's rows on their way to LDS: N pieces of 16 bytes a thread.
-template <typename T, int D, int C, int kThreads>
+// A chunk's rows on their way to LDS: kCount pieces of 16 bytes a thread, of one
+// column and rows kStep apart.  The addresses are a scalar one for each piece and an
+// unsigned 32-bit offset of the thread's own, which is all that stays in vector
+// registers.  kWhole: the width is a multiple of a piece.
+template <typename T, int D, int C, int kThreads, bool kWhole>
 struct Stage {
   static constexpr int kPieces = D * static_cast<int>(sizeof(T)) / 16;
-  static constexpr int kCount = (C * kPieces + kThreads - 1) / kThreads;
+  static constexpr int kStep = kThreads / kPieces;
+  static constexpr int kCount = C / kStep;
   static constexpr int kPer = Tile<T, D>::kPer;
+  static_assert(kThreads % kPieces == 0 && C % kStep == 0, "whole rows of pieces");
   u32x4 raw[kCount];
-  // Rows pos.. of the walk, `left` of them; zeros for those past them and for
-  // columns past `width`.
-  __device__ __forceinline__ void load(const T *base, int64_t stride, int64_t pos, int64_t left,
-                                       int width) {
+  uint32_t offset;
+  int row, there;  // the first piece's row; elements of the width in the column's piece
+  // `step` elements between rows, at most 2^24 of either sign.
+  __device__ __forceinline__ Stage(int64_t step, int width) {
+    row = static_cast<int>(threadIdx.x) / kPieces;
+    const int column = static_cast<int>(threadIdx.x) % kPieces * kPer;
+    const int64_t rows = step >= 0 ? row * step : (kStep - 1 - row) * -step;
+    offset = static_cast<uint32_t>(rows + column) * static_cast<uint32_t>(sizeof(T));
+    there = width - column;
+  }
+  // Rows from `first` on, `left` of them; zeros for those past them and for columns
+  // past the width.
+  __device__ __forceinline__ void load(const T *first, int64_t step, int64_t left) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      const int q = i * kThreads + static_cast<int>(threadIdx.x);
-      const int row = q / kPieces, column = q % kPieces * kPer;
+      const char *base = reinterpret_cast<const char *>(
+          first + (i * kStep + (step < 0 ? kStep - 1 : 0)) * step);
       u32x4 x{0, 0, 0, 0};
-      if (row < C && row < left && column < width) {
-        const T *p = base + (pos + row) * stride + column;
-        if (column + kPer <= width) {
+      if (row + i * kStep < left && there > 0) {
+        const T *p = reinterpret_cast<const T *>(base + offset);
+        if (kWhole || there >= kPer) {
           x = __builtin_bit_cast(u32x4, *reinterpret_cast<const Loose<T, kPer> *>(p));
         } else {
           Pack<T, kPer> e;
 #pragma unroll
-          for (int j = 0; j < kPer; ++j)
-            e.v[j] = column + j < width ? p[j] : static_cast<T>(0.0f);
+          for (int j = 0; j < kPer; ++j) e.v[j] = j < there ? p[j] : static_cast<T>(0.0f);
           x = __builtin_bit_cast(u32x4, e);
         }
       }
@@ -381,13 +448,10 @@ struct Stage {
     }
   }
   __device__ __forceinline__ void put(char *tile) const {
+    char *p = tile + row * Tile<T, D>::kPitch + static_cast<int>(threadIdx.x) % kPieces * 16;
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const int q = i * kThreads + static_cast<int>(threadIdx.x);
-      if (C * kPieces % kThreads == 0 || q < C * kPieces)
-        *reinterpret_cast<u32x4 *>(tile + q / kPieces * Tile<T, D>::kPitch + q % kPieces * 16) =
-            raw[i];
-    }
+    for (int i = 0; i < kCount; ++i)
+      *reinterpret_cast<u32x4 *>(p + i * kStep * Tile<T, D>::kPitch) = raw[i];
   }
   // Whether an element is not finite.
   __device__ __forceinline__ bool bad() const {
@@ -414,43 +478,56 @@ __device__ __forceinline__ void clear_rows(char *tile) {
         u32x4{0, 0, 0, 0};
 }
 
-// KD: channels of q and k that LDS and registers have room for; the block's W waves
-// have 16 NT columns of v each.  kStates: the spans' own states, no outputs.
-template <typename T, int KD, int NT, int W, bool kStates>
+// KD: channels of q and k that LDS and registers have room for; W waves.  kStates: the
+// spans' own states, no outputs.
+template <typename T, int KD, int W, bool kStates>
 struct Shape {
-  static constexpr int C = sizeof(T) == 4 ? 32 : 64;    // tokens of a chunk
-  static constexpr int kThreads = 64 * W;
-  static constexpr int kColumns = 16 * NT * W;
+  static constexpr int C = sizeof(T) == 4 || KD == 256 ? 32 : 64;  // tokens of a chunk
+  static constexpr int kThreads = 64 * W, kColumns = 16 * W;
   static constexpr int kFragment = 64 / static_cast<int>(sizeof(T));  // summed by 16 bytes a lane
-  static constexpr int kTiles = kFragment / 16;         // tiles of 16 to a fragment
+  static constexpr int kTiles = kFragment / 16;                       // tiles of 16 to a fragment
   static constexpr int KB = KD / kFragment, JB = C / kFragment;
+  // Outputs: tiles of 16 tokens for each wave, or tokens by parts of the columns.
+  static constexpr int IT = C / 16, kOwn = IT > W ? IT / W : 1, kPartsOfColumns = W > IT ? W / IT : 1;
+  static constexpr int NT = W / kPartsOfColumns;  // column tiles of a wave's outputs
+  static constexpr int kRun = 4 * NT;             // neighbouring columns of a lane's outputs
+  static constexpr int kOperands = sizeof(T) == 4 ? 1 : 2;
   static constexpr int kQ = kStates ? 0 : C * Tile<T, KD>::kPitch;
   static constexpr int kK = C * Tile<T, KD>::kPitch, kV = C * Tile<T, kColumns>::kPitch;
-  static constexpr int kLds = kQ + kK + kV;
+  static constexpr int kS = kStates ? 0 : KB * W * kOperands * 1024;
+  static constexpr int kLds = kQ + kK + kV + kS;
 };
 
-template <typename T, int KD, int NT, int W, bool kStates>
-__global__ __launch_bounds__(64 * W) void decay_walk_kernel(Walk w) {
-  using S = Shape<T, KD, NT, W, kStates>;
+template <typename T, int KD, int W, bool kStates, bool kWhole>
+__global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void decay_walk_kernel(
+    Walk w) {
+  using S = Shape<T, KD, W, kStates>;
   constexpr int C = S::C, kThreads = S::kThreads, KB = S::KB, JB = S::JB, kTiles = S::kTiles;
-  constexpr int kFragment = S::kFragment, kPer = Tile<T, KD>::kPer;
-  constexpr int kRun = 4 * NT;        // neighbouring columns of v in a lane's outputs
-  constexpr int kRows = 4 * kTiles;   // neighbouring rows of the state in a lane
+  constexpr int kFragment = S::kFragment, kPer = Tile<T, KD>::kPer, NT = S::NT, kRun = S::kRun;
+  constexpr int kRows = 4 * kTiles;  // neighbouring rows of the state in a lane
   using U = typename Wide<T>::type;
   extern __shared__ __attribute__((aligned(16))) char s_tile[];
   __shared__ int s_bad[2];
-  char *s_q = s_tile, *s_k = s_tile + S::kQ, *s_v = s_k + S::kK;
+  __shared__ float s_left[2 * C];
+  char *s_q = s_tile, *s_k = s_tile + S::kQ, *s_v = s_k + S::kK, *s_s = s_v + S::kV;
 
   const Role &r = w.role[blockIdx.y];
   const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
   const uint32_t per_item = static_cast<uint32_t>(w.heads) * w.column_blocks;
-  const int64_t item = id / per_item;
-  const int head = static_cast<int>(id % per_item) / w.column_blocks;
-  const int block_column = static_cast<int>(id % per_item) % w.column_blocks * S::kColumns;
+  const uint32_t item = id / per_item, inside = id - item * per_item;
+  const int head = static_cast<int>(inside / static_cast<uint32_t>(w.column_blocks));
+  const int block_column = static_cast<int>(inside % static_cast<uint32_t>(w.column_blocks)) *
+                           S::kColumns;
   const int dk = r.dk, dv = r.dv;
   if (block_column >= dv) return;
   Span x;
   if (!find_span(w.cut, item, x)) return;
+  x.sequence = uniform_value(x.sequence);
+  x.lo = uniform_value(x.lo);
+  x.length = uniform_value(x.length);
+  x.at = uniform_value(x.at);
+  x.count = uniform_value(x.count);
+  x.place = uniform_value(x.place);
   const int width = min(dv - block_column, S::kColumns);
   T *y = static_cast<T *>(r.y);
   if (x.sequence >= w.cut.sequences) {  // behind the last sequence
@@ -464,97 +541,104 @@ __global__ __launch_bounds__(64 * W) void decay_walk_kernel(Walk w) {
   if (kStates && x.last) return;
 
   const int lane = static_cast<int>(lane_id()), i = lane % 16, g = lane / 16;
-  const int wave_column = static_cast<int>(wave_index()) * 16 * NT;  // in the block's
-  const int column0 = block_column + wave_column;
-  const bool idle = column0 >= dv;
-  // The lane's column of v as an operand, and the first of its outputs'.
-  auto column_of = [&](int nt) { return column0 + i / 4 * kRun + nt * 4 + i % 4; };
-
+  const int wave = static_cast<int>(wave_index());
+  // Column tile c of the block holds, of each 16 NT columns, those 4 in every kRun
+  // that make neighbours of a lane's outputs: lane i's is part_of(c) + i / 4 kRun + i % 4.
+  auto part_of = [](int c) { return c / NT * (16 * NT) + c % NT * 4; };
   const int64_t size = static_cast<int64_t>(dk) * dv;
-  auto state_at = [&](const float *base, int64_t which, bool transposed, int row, int column) {
-    return base + (which * w.heads + head) * size +
-           (transposed ? static_cast<int64_t>(column) * dk + row
-                       : static_cast<int64_t>(row) * dv + column);
-  };
-  // state[kb][t][nt][e]: row kb kFragment + g kRows + 4 t + e, column_of(nt).
-  f32x4 state[KB][kTiles][NT];
-  const float *begin = kStates ? nullptr : x.first ? r.initial : r.carried;
-  const int64_t which = x.first ? x.sequence : x.place - 1;
+  // The wave's state, state[kb][t][e]: row kb kFragment + g kRows + 4 t + e and the
+  // lane's column of tile `wave`.  `visit` calls f(element, its address, whether it
+  // exists); the address is a valid one in any case.
+  f32x4 state[KB][kTiles] = {};
+  const int row_of_lane = g * kRows;
+  const int column_of_lane = block_column + part_of(wave) + i / 4 * kRun + i % 4;
+  auto visit = [&](const float *base, int64_t which, bool transposed, auto f) {
+    const char *p = reinterpret_cast<const char *>(base + (which * w.heads + head) * size);
+    const uint32_t down = transposed ? 4 : 4 * dv, over = transposed ? 4 * dk : 4;
+    const uint32_t offset = row_of_lane * down + column_of_lane * over;
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = kb * kFragment + g * kRows + t * 4 + e, column = column_of(nt);
-          state[kb][t][nt][e] = begin != nullptr && row < dk && column < dv
-                                    ? *state_at(begin, which, r.transposed != 0, row, column)
-                                    : 0.0f;
+          const int row = kb * kFragment + t * 4 + e;  // and the lane's
+          const bool there = row + row_of_lane < dk && column_of_lane < dv;
+          float value = state[kb][t][e];
+          f(value, reinterpret_cast<const float *>(p + (there ? offset + row * down : 0u)), there);
+          state[kb][t][e] = value;
         }
+  };
+  const float *begin = kStates ? nullptr : x.first ? r.initial : r.carried;
+  if (begin != nullptr && dk > 0)
+    visit(begin, x.first ? x.sequence : x.place - 1, r.transposed != 0,
+          [&](float &value, const float *at, bool there) { value = there ? *at : 0.0f; });
 
   const float log2_decay = w.log_decay[head] * 1.44269504088896341f;
   const int early = r.early;
-  // Weights of the pairs (i, j) of two tiles of 16 tokens depend on how many tiles
-  // they lie apart alone.  Scores' rows are j, their columns i.
-  constexpr int kApart = C / 16;
-  float weight[kApart][4], reach[kApart];
+  // Weights of the pairs (i, j) of two tiles of 16 tokens: of the same, and of
+  // neighbours, each tile further apart another g^16.  Scores' rows are j, their
+  // columns i.
+  float same[4], next[4], reach = 0.0f;
   if constexpr (!kStates) {
 #pragma unroll
-    for (int a = 0; a < kApart; ++a) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int apart = a * 16 + i - (g * 4 + e);
-        weight[a][e] = apart >= 0 ? r.scale_in * power(log2_decay, apart) : 0.0f;
-      }
-      reach[a] = power(log2_decay, a * 16 + i + 1 - early);
+    for (int e = 0; e < 4; ++e) {
+      const int apart = i - (g * 4 + e);
+      same[e] = apart >= 0 ? r.scale_in * power(log2_decay, apart) : 0.0f;
+      next[e] = r.scale_in * power(log2_decay, apart + 16);
     }
+    reach = power(log2_decay, i + 1 - early);
   }
-  // What is left at the chunk's end of the fragments' tokens.
-  float left[JB][kPer];
-  auto set_left = [&](int count) {
-#pragma unroll
-    for (int b = 0; b < JB; ++b)
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int j = b * kFragment + e / 4 * 16 + g * 4 + e % 4;
-        left[b][e] = j < count ? r.scale_in * power(log2_decay, count - 1 - j + early) : 0.0f;
-      }
-  };
-  set_left(C);
-  float keep = power(log2_decay, C);
+  // What is left at the end of a chunk of its tokens, and nothing of those behind
+  // it: token j of `count` is at C - count + j.
+  for (int j = threadIdx.x; j < 2 * C; j += kThreads)
+    s_left[j] = j < C ? r.scale_in * power(log2_decay, C - 1 - j + early) : 0.0f;
+  const float keep_all = power(log2_decay, C);
 
   // Token `t` of the walk is row lo + t of the inputs, or hi - 1 - t.
   const int64_t way = r.backwards != 0 ? -1 : 1;
   auto base_of = [&](const View &v) {
     const T *p = static_cast<const T *>(v.p) + head * v.head;
     p += w.cut.offsets == nullptr ? x.sequence * v.sequence : x.lo * v.token;
-    return r.backwards != 0 ? p + (x.length - 1) * v.token : p;
+    return p + (r.backwards != 0 ? x.length - 1 - x.at : x.at) * v.token;
   };
-  const T *q_base = kStates ? nullptr : base_of(r.q), *k_base = base_of(r.k),
-          *v_base = base_of(r.v) + block_column;
   const int64_t q_step = way * r.q.token, k_step = way * r.k.token, v_step = way * r.v.token;
-  Stage<T, KD, C, kThreads> q_stage, k_stage;
-  Stage<T, S::kColumns, C, kThreads> v_stage;
+  const T *q_first = kStates ? nullptr : base_of(r.q), *k_first = base_of(r.k),
+          *v_first = base_of(r.v) + block_column;
+  Stage<T, KD, C, kThreads, kWhole> q_stage(q_step, dk), k_stage(k_step, dk);
+  Stage<T, S::kColumns, C, kThreads, kWhole> v_stage(v_step, width);
   auto load = [&](int64_t pos) {
     const int64_t rows = x.count - pos;
-    if constexpr (!kStates) q_stage.load(q_base, q_step, x.at + pos, rows, dk);
-    k_stage.load(k_base, k_step, x.at + pos, rows, dk);
-    v_stage.load(v_base, v_step, x.at + pos, rows, width);
+    if constexpr (!kStates) q_stage.load(q_first + pos * q_step, q_step, rows);
+    k_stage.load(k_first + pos * k_step, k_step, rows);
+    v_stage.load(v_first + pos * v_step, v_step, rows);
+  };
+  // The wave's state as operands of its column tile.
+  auto put_state = [&]() {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      float z[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) z[e] = state[kb][e / 4][e % 4];
+      const Parts<U> parts = split<U>(z);
+      char *p = s_s + ((kb * W + wave) * S::kOperands * 64 + lane) * 16;
+      *reinterpret_cast<u32x4 *>(p) = parts.high;
+      if constexpr (S::kOperands == 2) *reinterpret_cast<u32x4 *>(p + 1024) = parts.rest;
+    }
   };
 
   if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
-  __syncthreads();
   load(0);
+  __syncthreads();
   int turn = 0;
   for (int64_t pos = 0; pos < x.count; turn ^= 1) {
-    if constexpr (!kStates) q_stage.put(s_q);
-    k_stage.put(s_k);
-    v_stage.put(s_v);
     if constexpr (!kStates) {
+      q_stage.put(s_q);
+      put_state();
       if (v_stage.bad()) s_bad[turn] = 1;
     }
+    k_stage.put(s_k);
+    v_stage.put(s_v);
     __syncthreads();
     int count = static_cast<int>(min(x.count - pos, static_cast<int64_t>(C)));
     if constexpr (!kStates) {
@@ -566,146 +650,127 @@ __global__ __launch_bounds__(64 * W) void decay_walk_kernel(Walk w) {
       }
     }
     load(pos + count);
-    if (count < C) {
-      set_left(count);
-      keep = power(log2_decay, count);
-    }
-    if (!idle) {
-      u32x4 v_raw[JB][NT];
+    if constexpr (!kStates) {
+      const int part = wave / S::IT;  // of the columns
+#pragma unroll 1
+      for (int own = 0; own < S::kOwn; ++own) {
+        const int it = (W > S::IT ? wave % S::IT : wave) + own * W;
+        if (it * 16 >= count) break;
+        u32x4 q_raw[KB];
+        f32x4 out[NT] = {};
 #pragma unroll
-      for (int b = 0; b < JB; ++b)
+        for (int kb = 0; kb < KB; ++kb) {
+          q_raw[kb] = along<T, KD>(s_q, it * 16 + i, kb * 4 + g);
+          const Parts<U> q_parts = beside<T>(q_raw[kb]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          v_raw[b][nt] = across<T, S::kColumns, kRun>(s_v, b * kFragment, wave_column + nt * 4);
-      if constexpr (!kStates) {
-        Parts<U> v_parts[JB][NT], s_parts[KB][NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int b = 0; b < JB; ++b) v_parts[b][nt] = beside<T>(v_raw[b][nt]);
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            float z[kPer];
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) z[e] = state[kb][e / 4][nt][e % 4];
-            s_parts[kb][nt] = split<U>(z);
+          for (int nt = 0; nt < NT; ++nt) {
+            const char *p = s_s + ((kb * W + part * NT + nt) * S::kOperands * 64 + lane) * 16;
+            Parts<U> s_parts;
+            s_parts.high = *reinterpret_cast<const u32x4 *>(p);
+            if constexpr (S::kOperands == 2)
+              s_parts.rest = *reinterpret_cast<const u32x4 *>(p + 1024);
+            out[nt] = multiply_split<T, false>(q_parts, s_parts, out[nt]);
           }
         }
+        const float far = reach * power(log2_decay, it * 16);
 #pragma unroll
-        for (int it = 0; it < C / 16; ++it) {
-          if (it * 16 >= count) break;
-          u32x4 q_raw[KB];
-          f32x4 out[NT] = {};
+        for (int nt = 0; nt < NT; ++nt) out[nt] *= far;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            q_raw[kb] = along<T, KD>(s_q, it * 16 + i, kb * 4 + g);
-            const Parts<U> q_parts = beside<T>(q_raw[kb]);
+        for (int b = 0; b < JB; ++b) {
+          if (b * kTiles > it) break;
+          float p[kPer];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              out[nt] = multiply_split<T, false>(q_parts, s_parts[kb][nt], out[nt]);
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) out[nt] *= reach[it];
-#pragma unroll
-          for (int b = 0; b < JB; ++b) {
-            if (b * kFragment > it * 16 + 15) continue;
-            const int apart = it - b * kTiles;
-            float p[kPer];
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-              if (t > apart) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) p[t * 4 + e] = 0.0f;
-                continue;
-              }
-              f32x4 score{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int t = 0; t < kTiles; ++t) {
+            const int apart = it - b * kTiles - t;
+            f32x4 score{0.0f, 0.0f, 0.0f, 0.0f};
+            if (apart >= 0) {
 #pragma unroll
               for (int kb = 0; kb < KB; ++kb)
                 score = multiply<T>(along<T, KD>(s_k, b * kFragment + t * 16 + i, kb * 4 + g),
                                     q_raw[kb], score);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                p[t * 4 + e] = score[e] * weight[apart - t][e];
+              if (apart == 0) {
                 // A later token's score may be anything.
-                if (t == apart && i < g * 4 + e) p[t * 4 + e] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) score[e] = i < g * 4 + e ? 0.0f : score[e] * same[e];
+              } else {
+                const float more = power(log2_decay, (apart - 1) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) score[e] *= next[e] * more;
               }
             }
-            const Parts<U> p_parts = split<U>(p);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              out[nt] = multiply_split<T, true>(v_parts[b][nt], p_parts, out[nt]);
+            for (int e = 0; e < 4; ++e) p[t * 4 + e] = score[e];
           }
-          const int64_t t = x.at + pos + it * 16 + i;
-          if (it * 16 + i < count) {
-            const int64_t token = x.lo + (r.backwards != 0 ? x.length - 1 - t : t);
-            const int column = column0 + g * kRun;
-            T *p = y + (token * w.heads + head) * dv + column;
-            Loose<T, kRun> z;
+          const Parts<U> p_parts = split<U>(p);
 #pragma unroll
-            for (int e = 0; e < kRun; ++e)
-              z.v[e] = static_cast<T>(out[e / 4][e % 4] * r.scale_out);
-            if (column + kRun <= dv) {
-              *reinterpret_cast<Loose<T, kRun> *>(p) = z;
-            } else {
+          for (int nt = 0; nt < NT; ++nt) {
+            const Parts<U> v_parts = beside<T>(
+                across<T, S::kColumns, kRun>(s_v, b * kFragment, part_of(part * NT + nt)));
+            out[nt] = multiply_split<T, true>(v_parts, p_parts, out[nt]);
+          }
+        }
+        if (it * 16 + i < count) {
+          // The tile's lowest row of y, and the lane's from there.
+          const int64_t t = x.at + pos + it * 16;
+          const int64_t token = x.lo + (r.backwards != 0 ? x.length - 16 - t : t);
+          const int row = r.backwards != 0 ? 15 - i : i;
+          const int column = block_column + part_of(part * NT) + g * kRun;
+          const uint32_t offset = static_cast<uint32_t>(row * w.heads * dv + column) *
+                                  static_cast<uint32_t>(sizeof(T));
+          T *p = reinterpret_cast<T *>(
+              reinterpret_cast<char *>(y + (token * w.heads + head) * dv) + offset);
+          constexpr int kMost = 16 / static_cast<int>(sizeof(T)), kStore = kRun < kMost ? kRun : kMost;
 #pragma unroll
-              for (int e = 0; e < kRun; ++e)
-                if (column + e < dv) p[e] = z.v[e];
+          for (int c = 0; c < kRun; c += kStore) {
+            Loose<T, kStore> z;
+#pragma unroll
+            for (int e = 0; e < kStore; ++e)
+              z.v[e] = static_cast<T>(out[(c + e) / 4][(c + e) % 4] * r.scale_out);
+            if (column + c + kStore <= dv) {
+              *reinterpret_cast<Loose<T, kStore> *>(p + c) = z;
+            } else if (!kWhole || kRun < kMost) {
+#pragma unroll
+              for (int e = 0; e < kStore; ++e)
+                if (column + c + e < dv) p[c + e] = z.v[e];
             }
           }
         }
       }
-      Parts<U> fresh[JB][NT];
-#pragma unroll
-      for (int b = 0; b < JB; ++b)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float z[kPer];
-          widen<T>(v_raw[b][nt], z);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) z[e] *= left[b][e];
-          fresh[b][nt] = split<U>(z);
-        }
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) state[kb][t][nt] *= keep;
-#pragma unroll
-          for (int b = 0; b < JB; ++b) {
-            const Parts<U> k_parts = beside<T>(
-                across<T, KD, kRows>(s_k, b * kFragment, kb * kFragment + t * 4));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              state[kb][t][nt] =
-                  multiply_split<T, true>(k_parts, fresh[b][nt], state[kb][t][nt]);
-          }
-        }
     }
+    const float keep = count == C ? keep_all : power(log2_decay, count);
+    Parts<U> fresh[JB];
+#pragma unroll
+    for (int b = 0; b < JB; ++b) {
+      float z[kPer];
+      widen<T>(across<T, S::kColumns, kRun>(s_v, b * kFragment, part_of(wave)), z);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        z[e] *= s_left[C - count + b * kFragment + e / 4 * 16 + g * 4 + e % 4];
+      fresh[b] = split<U, true>(z);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        state[kb][t] *= keep;
+#pragma unroll
+        for (int b = 0; b < JB; ++b) {
+          const Parts<U> k_parts =
+              beside<T>(across<T, KD, kRows>(s_k, b * kFragment, kb * kFragment + t * 4));
+          state[kb][t] = multiply_split<T, true, true>(k_parts, fresh[b], state[kb][t]);
+        }
+      }
     __syncthreads();
     if (threadIdx.x == 0) s_bad[turn] = 0;
-    if (count < C) {
-      set_left(C);
-      keep = power(log2_decay, C);
-    }
     pos += count;
   }
 
   float *end = kStates ? r.carried : x.last ? r.final_state : nullptr;
-  if (end == nullptr || idle) return;
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = kb * kFragment + g * kRows + t * 4 + e, column = column_of(nt);
-          if (row < dk && column < dv)
-            *const_cast<float *>(state_at(end, kStates ? x.place : x.sequence, false, row,
-                                          column)) = state[kb][t][nt][e];
-        }
+  if (end == nullptr) return;
+  visit(end, kStates ? x.place : x.sequence, false,
+        [&](float &value, const float *at, bool there) {
+          if (there) *const_cast<float *>(at) = value;
+        });
 }
 
 // One token of every sequence: the state is read, decayed, added to, stored and
@@ -769,27 +834,34 @@ struct Sizes {
   int64_t sequences, length, n, heads, dk, dv;
 };
 
-// Columns of v that a block takes, for the wider of both heads' sides (the
-// backward's roles swap them).
+// KD and W of a walk (see Shape): those of the wider of both heads' sides, which the
+// backward's roles swap.
 struct Form {
-  int kd, nt, waves;
-  int columns() const { return 16 * nt * waves; }
+  int kd, waves;
+  int columns() const { return 16 * waves; }
 };
 Form form_of(const Sizes &z) {
   const int64_t wide = std::max(z.dk, z.dv);
-  const int kd = wide <= 32 ? 32 : wide <= 64 ? 64 : wide <= 128 ? 128 : 256;
-  if (kd <= 64) return {kd, 1, wide <= 16 ? 1 : 4};
-  return {kd, kd == 128 ? 2 : 1, 4};
+  if (wide <= 16) return {32, 1};
+  if (wide <= 32) return {32, 2};
+  return {wide <= 64 ? 64 : wide <= 128 ? 128 : 256, 4};
 }
 
-// Tokens of a span: as many as leave a block for each of 1024 places, but at least
-// 256, so that a span's own tokens outweigh its states.
+// Blocks of a walk that the device holds at once: by their registers and LDS, 10 of
+// one wave, 6 of two and 3, 2 or 1 of four to a CU.  A few blocks more would be a
+// second round.
+int64_t blocks_at_once(const Form &f) {
+  return 256 * (f.waves == 1 ? 10 : f.waves == 2 ? 6 : f.kd == 64 ? 3 : f.kd == 128 ? 2 : 1);
+}
+
+// Tokens of a span: as many as fill the device once, but at least 256, so that a
+// span's own tokens outweigh its states.
 int64_t span_of(const Sizes &z) {
   const Form f = form_of(z);
   const int64_t blocks = std::max<int64_t>(1, z.heads * ceil_div(std::max(z.dk, z.dv), f.columns()));
   const int64_t longest = z.ragged ? z.n : z.length;
   const int64_t sequences = z.ragged ? 1 : std::max<int64_t>(1, z.sequences);
-  const int64_t spans = std::max<int64_t>(1, 1024 / (blocks * sequences));
+  const int64_t spans = std::max<int64_t>(1, blocks_at_once(f) / (blocks * sequences));
   const int64_t span = ceil_div(ceil_div(std::max<int64_t>(longest, 1), spans), 64) * 64;
   return std::max<int64_t>(256, span);
 }
@@ -826,23 +898,30 @@ int64_t table_bytes(const Sizes &z, const Plan &p) {
   return static_cast<int64_t>(align_up(c.used, 256));
 }
 
-template <typename T, int KD, int NT, int W, bool kStates>
-int launch_walk(const Walk &w, int64_t blocks, int roles, hipStream_t stream) {
-  using S = Shape<T, KD, NT, W, kStates>;
-  static_assert(S::kLds + 16 <= 160 * 1024, "LDS of a CU");
-  if (S::kLds > 64 * 1024) {
+template <typename T, int KD, int W, bool kStates, bool kWhole>
+int launch_walk_as(const Walk &w, int64_t blocks, int roles, hipStream_t stream) {
+  using S = Shape<T, KD, W, kStates>;
+  static_assert(S::kLds + 1024 <= 160 * 1024, "LDS of a CU");
+  if (S::kLds > 60 * 1024) {
     const hipError_t err = hipFuncSetAttribute(
-        reinterpret_cast<const void *>(&decay_walk_kernel<T, KD, NT, W, kStates>),
+        reinterpret_cast<const void *>(&decay_walk_kernel<T, KD, W, kStates, kWhole>),
         hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
     if (err != hipSuccess) {
       set_error("decay_attention: %d bytes of LDS refused: %s", S::kLds, hipGetErrorString(err));
       return R2S_EHIP;
     }
   }
-  decay_walk_kernel<T, KD, NT, W, kStates>
+  decay_walk_kernel<T, KD, W, kStates, kWhole>
       <<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(roles)), dim3(64 * W), S::kLds,
          stream>>>(w);
   return check_launch("decay_attention");
+}
+template <typename T, int KD, int W, bool kStates>
+int launch_walk(const Walk &w, int64_t blocks, int roles, hipStream_t stream) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  return w.role[0].dk % kPer == 0 && w.role[0].dv % kPer == 0
+             ? launch_walk_as<T, KD, W, kStates, true>(w, blocks, roles, stream)
+             : launch_walk_as<T, KD, W, kStates, false>(w, blocks, roles, stream);
 }
 
 template <bool kStates>
@@ -859,24 +938,27 @@ int walk(const Sizes &z, const Plan &p, Walk &w, int roles, hipStream_t stream) 
   }
   if (blocks == 0) return R2S_OK;
   R2S_BY_TYPE(z.type, {
-    if (f.kd == 32)
-      return f.waves == 1 ? launch_walk<T, 32, 1, 1, kStates>(w, blocks, roles, stream)
-                          : launch_walk<T, 32, 1, 4, kStates>(w, blocks, roles, stream);
-    if (f.kd == 64) return launch_walk<T, 64, 1, 4, kStates>(w, blocks, roles, stream);
-    if (f.kd == 128) return launch_walk<T, 128, 2, 4, kStates>(w, blocks, roles, stream);
-    return launch_walk<T, 256, 1, 4, kStates>(w, blocks, roles, stream);
+    if (f.waves == 1) return launch_walk<T, 32, 1, kStates>(w, blocks, roles, stream);
+    if (f.waves == 2) return launch_walk<T, 32, 2, kStates>(w, blocks, roles, stream);
+    if (f.kd == 64) return launch_walk<T, 64, 4, kStates>(w, blocks, roles, stream);
+    if (f.kd == 128) return launch_walk<T, 128, 4, kStates>(w, blocks, roles, stream);
+    return launch_walk<T, 256, 4, kStates>(w, blocks, roles, stream);
   });
 }
 
 int carry(const Sizes &z, const Plan &p, const Walk &w, hipStream_t stream) {
-  const int64_t total = z.sequences * z.heads * z.dk * z.dv;
-  const int64_t blocks = ceil_div(total, 256);
-  if (blocks > kInt32Max) {
-    set_error("decay_attention: too many states");
-    return R2S_ERANGE;
+  const int64_t states = z.heads * z.dk * z.dv, total = z.sequences * states;
+  if (total == 0) return R2S_OK;
+  if (!z.ragged && p.spans <= 16 && ceil_div(total, 256) <= kInt32Max) {
+    decay_carry_few_kernel<<<dim3(static_cast<uint32_t>(ceil_div(total, 256))), dim3(256), 0,
+                             stream>>>(w, total);
+  } else {
+    const int per = z.ragged ? 64 : 1;
+    const int64_t rows = std::min<int64_t>(ceil_div(z.sequences, per), 65535);
+    decay_carry_kernel<<<dim3(static_cast<uint32_t>(ceil_div(states, 64)),
+                              static_cast<uint32_t>(rows)),
+                         dim3(1024), 0, stream>>>(w, per);
   }
-  if (blocks == 0) return R2S_OK;
-  decay_carry_kernel<<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(w, total);
   return check_launch("decay_attention carry");
 }
 
@@ -907,7 +989,8 @@ bool bad_view(const Sizes &z, const View &v) {
   const __int128 reach = static_cast<__int128>(z.sequences) * v.sequence +
                          static_cast<__int128>(z.n) * v.token +
                          static_cast<__int128>(z.heads) * v.head;
-  return v.sequence < 0 || v.token < 0 || v.head < 0 || reach >= (static_cast<__int128>(1) << 60);
+  return v.sequence < 0 || v.token < 0 || v.token > kMostStep || v.head < 0 ||
+         reach >= (static_cast<__int128>(1) << 60);
 }
 
 // The table of ragged items where sequences may have several spans.

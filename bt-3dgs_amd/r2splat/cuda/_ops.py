@@ -2349,12 +2349,15 @@ def residual_norm_bwd(x: Tensor, update: Optional[Tensor], gate: Optional[Tensor
 
 def _attention_input(t: Tensor, name: str, like: Tensor, shape):
     """(tensor, (sequence, token, head) strides) of [B, L, H, D] or [N, H, D]; a
-    copy where a head's elements are not consecutive."""
+    copy where a head's elements are not consecutive or tokens lie 2^24 elements
+    apart."""
     _check_latent(t, name, like, like.dtype)
     if t.shape != shape:
         _fail(name, " must be ", tuple(shape), ", got shape ", tuple(t.shape))
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if (t.shape[-1] > 1 and t.stride(-1) != 1) or (t.stride(-3) > 1 << 24 and t.shape[-3] > 1):
         t = t.contiguous()
+    if t.stride(-3) > 1 << 24:  # one token's: it leads nowhere
+        t = t.as_strided(t.shape, (*t.stride()[:-3], 0, *t.stride()[-2:]))
     return (t, *t.stride()[:-1]) if t.dim() == 4 else (t, 0, *t.stride()[:-1])
 
 
