@@ -455,17 +455,70 @@ struct Stage {
   }
   // Whether an element is not finite.
   __device__ __forceinline__ bool bad() const {
-    constexpr uint32_t kMask = sizeof(T) == 4 ? 0x7F800000u
-                               : std::is_same<T, bf16_t>::value ? 0x7F80u : 0x7C00u;
-    bool found = false;
+    using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
+    if constexpr (sizeof(T) == 4) {
+      uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < kCount; ++i)
+      for (int i = 0; i < kCount; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        found |= (raw[i][j] & kMask) == kMask;
-        if constexpr (sizeof(T) == 2) found |= (raw[i][j] >> 16 & kMask) == kMask;
+        for (int j = 0; j < 4; ++j) most = max(most, raw[i][j] & 0x7FFFFFFFu);
+      return most >= 0x7F800000u;
+    } else {
+      u16x2 most{0, 0};
+#pragma unroll
+      for (int i = 0; i < kCount; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          most = __builtin_elementwise_max(
+              most, __builtin_bit_cast(u16x2, raw[i][j] & 0x7FFF7FFFu));
+      const uint16_t least = std::is_same<T, bf16_t>::value ? 0x7F80 : 0x7C00;
+      return most[0] >= least || most[1] >= least;
+    }
+  }
+};
+
+// A wave's rows of q as operands, straight from memory: tile `own` of 16 rows, row i
+// and piece 4 kb + g of 16 bytes to a lane.
+template <typename T, int KB, int kOwn, bool kWhole>
+struct Rows {
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  u32x4 raw[kOwn][KB];
+  uint32_t offset;
+  int row, width;  // elements of a row from the lane's first on
+  __device__ __forceinline__ Rows(int64_t step, int channels) {
+    row = static_cast<int>(lane_id()) % 16;
+    const int column = static_cast<int>(lane_id()) / 16 * kPer;
+    offset = static_cast<uint32_t>((step >= 0 ? row * step : (15 - row) * -step) + column) *
+             static_cast<uint32_t>(sizeof(T));
+    width = channels - column;
+  }
+  // The tiles first + own of `tiles` each; zeros past `left` rows and the width.
+  __device__ __forceinline__ void load(const T *base, int64_t step, int64_t left, int first,
+                                       int tiles) {
+#pragma unroll
+    for (int own = 0; own < kOwn; ++own) {
+      const int it = first + own * tiles;
+      const char *p = reinterpret_cast<const char *>(
+          base + (it * 16 + (step < 0 ? 15 : 0)) * step);
+      const bool some = it * 16 + row < left;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const T *at = reinterpret_cast<const T *>(p + offset) + kb * 4 * kPer;
+        const int there = width - kb * 4 * kPer;
+        u32x4 x{0, 0, 0, 0};
+        if (some && there > 0) {
+          if (kWhole || there >= kPer) {
+            x = __builtin_bit_cast(u32x4, *reinterpret_cast<const Loose<T, kPer> *>(at));
+          } else {
+            Pack<T, kPer> e;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) e.v[j] = j < there ? at[j] : static_cast<T>(0.0f);
+            x = __builtin_bit_cast(u32x4, e);
+          }
+        }
+        raw[own][kb] = x;
       }
-    return found;
+    }
   }
 };
 
@@ -482,7 +535,7 @@ __device__ __forceinline__ void clear_rows(char *tile) {
 // spans' own states, no outputs.
 template <typename T, int KD, int W, bool kStates>
 struct Shape {
-  static constexpr int C = sizeof(T) == 4 || KD == 256 ? 32 : 64;  // tokens of a chunk
+  static constexpr int C = sizeof(T) == 4 || KD == 256 || W < 4 ? 32 : 64;  // tokens of a chunk
   static constexpr int kThreads = 64 * W, kColumns = 16 * W;
   static constexpr int kFragment = 64 / static_cast<int>(sizeof(T));  // summed by 16 bytes a lane
   static constexpr int kTiles = kFragment / 16;                       // tiles of 16 to a fragment
@@ -492,14 +545,13 @@ struct Shape {
   static constexpr int NT = W / kPartsOfColumns;  // column tiles of a wave's outputs
   static constexpr int kRun = 4 * NT;             // neighbouring columns of a lane's outputs
   static constexpr int kOperands = sizeof(T) == 4 ? 1 : 2;
-  static constexpr int kQ = kStates ? 0 : C * Tile<T, KD>::kPitch;
   static constexpr int kK = C * Tile<T, KD>::kPitch, kV = C * Tile<T, kColumns>::kPitch;
   static constexpr int kS = kStates ? 0 : KB * W * kOperands * 1024;
-  static constexpr int kLds = kQ + kK + kV + kS;
+  static constexpr int kLds = kK + kV + kS;
 };
 
 template <typename T, int KD, int W, bool kStates, bool kWhole>
-__global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void decay_walk_kernel(
+__global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2 : 1) void decay_walk_kernel(
     Walk w) {
   using S = Shape<T, KD, W, kStates>;
   constexpr int C = S::C, kThreads = S::kThreads, KB = S::KB, JB = S::JB, kTiles = S::kTiles;
@@ -509,7 +561,7 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
   extern __shared__ __attribute__((aligned(16))) char s_tile[];
   __shared__ int s_bad[2];
   __shared__ float s_left[2 * C];
-  char *s_q = s_tile, *s_k = s_tile + S::kQ, *s_v = s_k + S::kK, *s_s = s_v + S::kV;
+  char *s_k = s_tile, *s_v = s_k + S::kK, *s_s = s_v + S::kV;
 
   const Role &r = w.role[blockIdx.y];
   const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
@@ -576,18 +628,26 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
 
   const float log2_decay = w.log_decay[head] * 1.44269504088896341f;
   const int early = r.early;
-  // Weights of the pairs (i, j) of two tiles of 16 tokens: of the same, and of
-  // neighbours, each tile further apart another g^16.  Scores' rows are j, their
-  // columns i.
-  float same[4], next[4], reach = 0.0f;
+  // A wave's outputs: tiles first + own tiles of 16 tokens, of one part of the columns.
+  constexpr int tiles = W < S::IT ? W : S::IT;
+  const int first_tile = wave % tiles, part = wave / S::IT;
+  // Weights of the pairs (i, j) of these tiles, with the scales; scores' rows are j,
+  // their columns i.
+  float weight[S::kOwn][JB][kPer], reach[S::kOwn];
   if constexpr (!kStates) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int apart = i - (g * 4 + e);
-      same[e] = apart >= 0 ? r.scale_in * power(log2_decay, apart) : 0.0f;
-      next[e] = r.scale_in * power(log2_decay, apart + 16);
+    for (int own = 0; own < S::kOwn; ++own) {
+      const int now = (first_tile + own * tiles) * 16 + i;
+      reach[own] = r.scale_out * power(log2_decay, now + 1 - early);
+#pragma unroll
+      for (int b = 0; b < JB; ++b)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const int apart = now - (b * kFragment + e / 4 * 16 + g * 4 + e % 4);
+          weight[own][b][e] =
+              apart >= 0 ? r.scale_in * r.scale_out * power(log2_decay, apart) : 0.0f;
+        }
     }
-    reach = power(log2_decay, i + 1 - early);
   }
   // What is left at the end of a chunk of its tokens, and nothing of those behind
   // it: token j of `count` is at C - count + j.
@@ -605,13 +665,17 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
   const int64_t q_step = way * r.q.token, k_step = way * r.k.token, v_step = way * r.v.token;
   const T *q_first = kStates ? nullptr : base_of(r.q), *k_first = base_of(r.k),
           *v_first = base_of(r.v) + block_column;
-  Stage<T, KD, C, kThreads, kWhole> q_stage(q_step, dk), k_stage(k_step, dk);
+  Rows<T, KB, S::kOwn, kWhole> q_rows(q_step, dk);
+  Stage<T, KD, C, kThreads, kWhole> k_stage(k_step, dk);
   Stage<T, S::kColumns, C, kThreads, kWhole> v_stage(v_step, width);
   auto load = [&](int64_t pos) {
     const int64_t rows = x.count - pos;
-    if constexpr (!kStates) q_stage.load(q_first + pos * q_step, q_step, rows);
     k_stage.load(k_first + pos * k_step, k_step, rows);
     v_stage.load(v_first + pos * v_step, v_step, rows);
+  };
+  u32x4 q_raw[S::kOwn][KB];  // of the present chunk; q_rows those of the next
+  auto load_q = [&](int64_t pos) {
+    q_rows.load(q_first + pos * q_step, q_step, x.count - pos, first_tile, tiles);
   };
   // The wave's state as operands of its column tile.
   auto put_state = [&]() {
@@ -629,11 +693,11 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
 
   if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
   load(0);
+  if constexpr (!kStates) load_q(0);
   __syncthreads();
   int turn = 0;
   for (int64_t pos = 0; pos < x.count; turn ^= 1) {
     if constexpr (!kStates) {
-      q_stage.put(s_q);
       put_state();
       if (v_stage.bad()) s_bad[turn] = 1;
     }
@@ -651,17 +715,19 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
     }
     load(pos + count);
     if constexpr (!kStates) {
-      const int part = wave / S::IT;  // of the columns
-#pragma unroll 1
+#pragma unroll
+      for (int own = 0; own < S::kOwn; ++own)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) q_raw[own][kb] = q_rows.raw[own][kb];
+      load_q(pos + count);
+#pragma unroll
       for (int own = 0; own < S::kOwn; ++own) {
-        const int it = (W > S::IT ? wave % S::IT : wave) + own * W;
+        const int it = first_tile + own * tiles;
         if (it * 16 >= count) break;
-        u32x4 q_raw[KB];
         f32x4 out[NT] = {};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          q_raw[kb] = along<T, KD>(s_q, it * 16 + i, kb * 4 + g);
-          const Parts<U> q_parts = beside<T>(q_raw[kb]);
+          const Parts<U> q_parts = beside<T>(q_raw[own][kb]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const char *p = s_s + ((kb * W + part * NT + nt) * S::kOperands * 64 + lane) * 16;
@@ -672,9 +738,8 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
             out[nt] = multiply_split<T, false>(q_parts, s_parts, out[nt]);
           }
         }
-        const float far = reach * power(log2_decay, it * 16);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) out[nt] *= far;
+        for (int nt = 0; nt < NT; ++nt) out[nt] *= reach[own];
 #pragma unroll
         for (int b = 0; b < JB; ++b) {
           if (b * kTiles > it) break;
@@ -687,19 +752,14 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
 #pragma unroll
               for (int kb = 0; kb < KB; ++kb)
                 score = multiply<T>(along<T, KD>(s_k, b * kFragment + t * 16 + i, kb * 4 + g),
-                                    q_raw[kb], score);
-              if (apart == 0) {
-                // A later token's score may be anything.
+                                    q_raw[own][kb], score);
+              if (apart == 0) {  // a later token's score may be anything
 #pragma unroll
-                for (int e = 0; e < 4; ++e) score[e] = i < g * 4 + e ? 0.0f : score[e] * same[e];
-              } else {
-                const float more = power(log2_decay, (apart - 1) * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) score[e] *= next[e] * more;
+                for (int e = 0; e < 4; ++e) score[e] = i < g * 4 + e ? 0.0f : score[e];
               }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[t * 4 + e] = score[e];
+            for (int e = 0; e < 4; ++e) p[t * 4 + e] = score[e] * weight[own][b][t * 4 + e];
           }
           const Parts<U> p_parts = split<U>(p);
 #pragma unroll
@@ -725,7 +785,7 @@ __global__ __launch_bounds__(64 * W, KD <= 64 ? 3 : KD == 128 ? 2 : 1) void deca
             Loose<T, kStore> z;
 #pragma unroll
             for (int e = 0; e < kStore; ++e)
-              z.v[e] = static_cast<T>(out[(c + e) / 4][(c + e) % 4] * r.scale_out);
+              z.v[e] = static_cast<T>(out[(c + e) / 4][(c + e) % 4]);
             if (column + c + kStore <= dv) {
               *reinterpret_cast<Loose<T, kStore> *>(p + c) = z;
             } else if (!kWhole || kRun < kMost) {
