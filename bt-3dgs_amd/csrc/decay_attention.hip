@@ -94,6 +94,7 @@ struct Walk {
   const float *log_decay;
   Cut cut;
   int32_t heads, column_blocks;
+  uint32_t roles;
 };
 
 // A block's span of its sequence: tokens [at, at + count) of the walk's order.
@@ -563,8 +564,10 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
   __shared__ float s_left[2 * C];
   char *s_k = s_tile, *s_v = s_k + S::kK, *s_s = s_v + S::kV;
 
-  const Role &r = w.role[blockIdx.y];
-  const uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
+  // Roles of the same tokens are neighbours, and neighbours share an XCD's cache.
+  uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const Role &r = w.role[id % w.roles];
+  id /= w.roles;
   const uint32_t per_item = static_cast<uint32_t>(w.heads) * w.column_blocks;
   const uint32_t item = id / per_item, inside = id - item * per_item;
   const int head = static_cast<int>(inside / static_cast<uint32_t>(w.column_blocks));
@@ -959,7 +962,7 @@ int64_t table_bytes(const Sizes &z, const Plan &p) {
 }
 
 template <typename T, int KD, int W, bool kStates, bool kWhole>
-int launch_walk_as(const Walk &w, int64_t blocks, int roles, hipStream_t stream) {
+int launch_walk_as(const Walk &w, int64_t blocks, hipStream_t stream) {
   using S = Shape<T, KD, W, kStates>;
   static_assert(S::kLds + 1024 <= 160 * 1024, "LDS of a CU");
   if (S::kLds > 60 * 1024) {
@@ -972,16 +975,15 @@ int launch_walk_as(const Walk &w, int64_t blocks, int roles, hipStream_t stream)
     }
   }
   decay_walk_kernel<T, KD, W, kStates, kWhole>
-      <<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(roles)), dim3(64 * W), S::kLds,
-         stream>>>(w);
+      <<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * W), S::kLds, stream>>>(w);
   return check_launch("decay_attention");
 }
 template <typename T, int KD, int W, bool kStates>
-int launch_walk(const Walk &w, int64_t blocks, int roles, hipStream_t stream) {
+int launch_walk(const Walk &w, int64_t blocks, hipStream_t stream) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(T));
   return w.role[0].dk % kPer == 0 && w.role[0].dv % kPer == 0
-             ? launch_walk_as<T, KD, W, kStates, true>(w, blocks, roles, stream)
-             : launch_walk_as<T, KD, W, kStates, false>(w, blocks, roles, stream);
+             ? launch_walk_as<T, KD, W, kStates, true>(w, blocks, stream)
+             : launch_walk_as<T, KD, W, kStates, false>(w, blocks, stream);
 }
 
 template <bool kStates>
@@ -991,18 +993,19 @@ int walk(const Sizes &z, const Plan &p, Walk &w, int roles, hipStream_t stream) 
   for (int i = 0; i < roles; ++i)
     columns = std::max<int64_t>(columns, ceil_div(w.role[i].dv, f.columns()));
   w.column_blocks = static_cast<int32_t>(columns);
-  const int64_t blocks = p.items * z.heads * columns;
+  w.roles = static_cast<uint32_t>(roles);
+  const int64_t blocks = p.items * z.heads * columns * roles;
   if (blocks > kInt32Max) {
     set_error("decay_attention: %lld blocks exceed 2^31 - 1", static_cast<long long>(blocks));
     return R2S_ERANGE;
   }
   if (blocks == 0) return R2S_OK;
   R2S_BY_TYPE(z.type, {
-    if (f.waves == 1) return launch_walk<T, 32, 1, kStates>(w, blocks, roles, stream);
-    if (f.waves == 2) return launch_walk<T, 32, 2, kStates>(w, blocks, roles, stream);
-    if (f.kd == 64) return launch_walk<T, 64, 4, kStates>(w, blocks, roles, stream);
-    if (f.kd == 128) return launch_walk<T, 128, 4, kStates>(w, blocks, roles, stream);
-    return launch_walk<T, 256, 4, kStates>(w, blocks, roles, stream);
+    if (f.waves == 1) return launch_walk<T, 32, 1, kStates>(w, blocks, stream);
+    if (f.waves == 2) return launch_walk<T, 32, 2, kStates>(w, blocks, stream);
+    if (f.kd == 64) return launch_walk<T, 64, 4, kStates>(w, blocks, stream);
+    if (f.kd == 128) return launch_walk<T, 128, 4, kStates>(w, blocks, stream);
+    return launch_walk<T, 256, 4, kStates>(w, blocks, stream);
   });
 }
 
