@@ -8,8 +8,8 @@
 // v = norm(z) w is r (v' - n m(v' n) - c'), v' = v w, n = norm(z), r its factor and
 // c' = m(v') where c is the mean, else 0.
 //
-// A row is held in registers by 8 to 64 lanes, or by a block where it is longer, so
-// each input is read once and each output written once, and the sums of squares are
+// A row is held in registers by 8 to 512 lanes, 16 bytes of each input a lane (more
+// only where a row has over 512 such pieces), so each input is read once and each output written once, and the sums of squares are
 // of differences from the mean that was found first.  The backward makes the
 // forward's values again from its inputs, which costs no bytes.  Weights' gradients
 // are sums over rows: a lane group adds its rows, a block its groups, and a second
@@ -21,8 +21,6 @@
 namespace r2s {
 namespace {
 
-constexpr int kNormThreads = 256;
-constexpr int kNormBlocks = 512;  // of the backward: parts of the weights' gradients
 constexpr int kNormMost = 8192;   // channels
 
 enum : int { kNoGate = 0, kRowGate = 1, kChannelGate = 2 };
@@ -69,59 +67,78 @@ __device__ __forceinline__ void store_row(T *p, int count, const Loose<T, V> &x)
   }
 }
 
-// sigmoid(g) and 1 - sigmoid(g), each to float32's precision.
+// sigmoid(g) and 1 - sigmoid(g), each within a few units of float32's last place: the
+// hardware's exponential and reciprocal are within one, and what rounding the
+// exponential's argument in units of log 2 leaves is put back.  Below 2^-126 it is 0.
 __device__ __forceinline__ float2 sigmoids(float g) {
-  const float e = expf(-fabsf(g)), big = 1.0f / (1.0f + e), small = e * big;
+  constexpr float kLog2e = 1.44269502162933349609f, kRest = 1.92596299e-8f;  // of log2(e)
+  const float x = -fabsf(g), t = x * kLog2e;
+  const float left = fmaf(x, kRest, fmaf(x, kLog2e, -t));
+  const float near = __builtin_amdgcn_exp2f(t);
+  // An infinite x leaves a NaN beside its exponential of 0.
+  const float e = near == 0.0f ? 0.0f : fmaf(near, left * 0.693147180559945f, near);
+  const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
   return g >= 0.0f ? make_float2(big, small) : make_float2(small, big);
 }
 
-// The lanes of a row: 2^bits of a wave, or the block's.
-template <bool kBlock>
+// The sum over the 2^bits lanes (aligned, bits >= 3) that hold a row's part of a wave:
+// lanes 1, 2, 4 and 8 apart by moves within rows of 16 lanes (by then whole quads and
+// halves agree, so mirrors do), 16 and 32 by swaps of such rows.
+__device__ __forceinline__ float lanes_sum(float a, int bits) {
+  a += dpp_take<0xB1, 0xf>(a);   // quad_perm 1 0 3 2
+  a += dpp_take<0x4E, 0xf>(a);   // quad_perm 2 3 0 1
+  a += dpp_take<0x141, 0xf>(a);  // row_half_mirror
+  if (bits > 3) a += dpp_take<0x140, 0xf>(a);  // row_mirror
+  if (bits > 4) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(a), false,
+                                                    false);
+    a = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (bits > 5) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(a), false,
+                                                    false);
+    a = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return a;
+}
+
+// The lanes of a row: 2^bits of a wave, or (kWide, bits > 6) of several waves.
+template <bool kWide, int kThreads>
 struct Lanes {
+  static constexpr int kWaves = kThreads / 64;
   int bits, lane;
-  float *s_sums;  // [2][kNormThreads / 64][2], kBlock
+  float2 *s_sums;  // [2][kWaves], kWide
   int turn = 0;
-  __device__ __forceinline__ Lanes(int b, float *sums) : bits(b), s_sums(sums) {
+  __device__ __forceinline__ Lanes(int b, float2 *sums) : bits(b), s_sums(sums) {
     lane = static_cast<int>(threadIdx.x) & ((1 << bits) - 1);
   }
   __device__ __forceinline__ float2 sum(float a, float b) {
-#pragma unroll
-    for (int s = 0; s < 6; ++s) {
-      if (s < bits) {
-        a += __shfl_xor(a, 1 << s, 64);
-        b += __shfl_xor(b, 1 << s, 64);
-      }
-    }
-    if constexpr (kBlock) {
-      constexpr int kWaves = kNormThreads / 64;
-      float *at = s_sums + turn * kWaves * 2;
-      turn ^= 1;  // the sum before the last one has been read by all
-      if (lane_id() == 0) {
-        at[wave_index() * 2] = a;
-        at[wave_index() * 2 + 1] = b;
-      }
-      __syncthreads();
-      a = b = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) a += at[w * 2], b += at[w * 2 + 1];
-    }
-    return make_float2(a, b);
+    a = lanes_sum(a, kWide ? 6 : bits);
+    b = lanes_sum(b, kWide ? 6 : bits);
+    return across(a, b);
   }
   __device__ __forceinline__ float sum(float a) {
-#pragma unroll
-    for (int s = 0; s < 6; ++s)
-      if (s < bits) a += __shfl_xor(a, 1 << s, 64);
-    if constexpr (kBlock) {
-      constexpr int kWaves = kNormThreads / 64;
-      float *at = s_sums + turn * kWaves * 2;
-      turn ^= 1;
-      if (lane_id() == 0) at[wave_index() * 2] = a;
+    a = lanes_sum(a, kWide ? 6 : bits);
+    return across(a, 0.0f).x;
+  }
+
+ private:
+  // The sums of all the row's waves, the same bits in each.
+  __device__ __forceinline__ float2 across(float a, float b) {
+    float2 total = make_float2(a, b);
+    if constexpr (kWide) {
+      float2 *at = s_sums + turn * kWaves;
+      turn ^= 1;  // the sums before the last ones have been read by all
+      if (lane_id() == 0) at[wave_index()] = make_float2(a, b);
       __syncthreads();
-      a = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) a += at[w * 2];
+      const int waves = 1 << (bits - 6), first = static_cast<int>(wave_index()) & ~(waves - 1);
+      total = at[first];
+      for (int i = 1; i < waves; ++i) {
+        total.x += at[first + i].x;
+        total.y += at[first + i].y;
+      }
     }
-    return a;
+    return total;
   }
 };
 
@@ -132,12 +149,12 @@ struct Row {
   float v[E][V];
 };
 
-template <typename T, int E, bool kBlock>
+template <typename T, int E, bool kWide, int kThreads>
 struct RowOf {
   static constexpr int V = Row<T, E>::V;
   int first[E], count[E];
   float share;  // 1 / d
-  __device__ __forceinline__ RowOf(const Lanes<kBlock> &lanes, int d) : share(1.0f / d) {
+  __device__ __forceinline__ RowOf(const Lanes<kWide, kThreads> &lanes, int d) : share(1.0f / d) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       first[e] = ((e << lanes.bits) + lanes.lane) * V;
@@ -172,7 +189,7 @@ struct RowOf {
     }
   }
   // x <- norm(x); returns the factor.
-  __device__ __forceinline__ float norm(Lanes<kBlock> &lanes, bool centered, float eps,
+  __device__ __forceinline__ float norm(Lanes<kWide, kThreads> &lanes, bool centered, float eps,
                                         Row<T, E> &x) const {
     if (centered) {
       float total = 0.0f;
@@ -209,33 +226,33 @@ __device__ __forceinline__ void widen(const Loose<T, Row<T, E>::V> (&raw)[E], Ro
 }
 
 // 32k x 1024 bf16 and 4k x 64 f32: the figures are those of the backward's comment.
-template <typename T, int E, bool kBlock>
-__global__ __launch_bounds__(kNormThreads) void residual_norm_fwd_kernel(NormArgs a, int bits) {
-  __shared__ float s_sums[2 * (kNormThreads / 64) * 2];
+template <typename T, int E, bool kWide, int kThreads, int kGate>
+__global__ __launch_bounds__(kThreads) void residual_norm_fwd_kernel(NormArgs a, int bits) {
+  __shared__ float2 s_sums[2 * (kThreads / 64)];
   constexpr int V = Row<T, E>::V;
-  Lanes<kBlock> lanes(bits, s_sums);
-  const RowOf<T, E, kBlock> at(lanes, a.d);
+  Lanes<kWide, kThreads> lanes(bits, s_sums);
+  const RowOf<T, E, kWide, kThreads> at(lanes, a.d);
   Row<T, E> w1, w2, all;
   at.load_weight(a.w1, w1);
   at.load_weight(a.w2, w2);
-  if (a.gate_kind == kChannelGate) {
+  if constexpr (kGate == kChannelGate) {
     at.load_weight(a.gate.p, all);
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int i = 0; i < V; ++i) all.v[e][i] = sigmoids(all.v[e][i]).x;
   }
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kNormThreads >> bits);
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (kNormThreads >> bits) + (threadIdx.x >> bits);
-  // A wave's groups stop together: the sums are over whole waves' lanes.
-  const int64_t group0 = row - (threadIdx.x >> bits) + ((threadIdx.x & ~63) >> bits);
-  for (int64_t lead = kBlock ? row : group0; lead < a.n; lead += groups, row += groups) {
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kThreads >> bits);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads >> bits) + (threadIdx.x >> bits);
+  // A wave's groups stop together, and with kWide a block's: they add up together.
+  const int64_t group0 = row - (threadIdx.x >> bits) + (kWide ? 0 : (threadIdx.x & ~63) >> bits);
+  for (int64_t lead = group0; lead < a.n; lead += groups, row += groups) {
     const bool some = row < a.n;
     const int64_t r = some ? row : lead;
     Loose<T, V> rx[E], rf[E], rg[E];
     at.load(a.x, r, rx);
     if (a.update.p != nullptr) at.load(a.update, r, rf);
-    if (a.gate_kind == kRowGate) at.load(a.gate, r, rg);
+    if constexpr (kGate == kRowGate) at.load(a.gate, r, rg);
     Row<T, E> y;
     widen<T, E>(rx, y);
     if (a.update.p != nullptr) {
@@ -247,8 +264,8 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_fwd_kernel(NormArg
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           float s = a.scale;
-          if (a.gate_kind == kRowGate) s *= sigmoids(static_cast<float>(rg[e].v[i])).x;
-          if (a.gate_kind == kChannelGate) s *= all.v[e][i];
+          if constexpr (kGate == kRowGate) s *= sigmoids(static_cast<float>(rg[e].v[i])).x;
+          if constexpr (kGate == kChannelGate) s *= all.v[e][i];
           y.v[e][i] = fmaf(s, h.v[e][i] * w1.v[e][i], y.v[e][i]);
         }
       if (some) at.store(a.y, r, a.d, y);
@@ -265,64 +282,67 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_fwd_kernel(NormArg
 }
 
 // A block's sum of its groups' `sums`, into its part.
-template <typename T, int E, bool kBlock>
-__device__ __forceinline__ void store_part(const RowOf<T, E, kBlock> &at, int bits, int d,
+template <typename T, int E, bool kWide, int kThreads>
+__device__ __forceinline__ void store_part(const RowOf<T, E, kWide, kThreads> &at, int bits, int d,
                                            const Row<T, E> &sums, float *s_row, float *part) {
   constexpr int V = Row<T, E>::V;
-  if constexpr (kBlock) {
+  const int groups = kThreads >> bits;
+  float *mine = groups > 1 ? s_row + (threadIdx.x >> bits) * d : part;
+  __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+  for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < at.count[e]) part[at.first[e] + i] = sums.v[e][i];
-  } else {
-    float *mine = s_row + (threadIdx.x >> bits) * d;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < at.count[e]) mine[at.first[e] + i] = sums.v[e][i];
-    __syncthreads();
-    for (int c = threadIdx.x; c < d; c += kNormThreads) {
-      float total = 0.0f;
-      for (int g = 0; g < (kNormThreads >> bits); ++g) total += s_row[g * d + c];
-      part[c] = total;
-    }
+    for (int i = 0; i < V; ++i)
+      if (i < at.count[e]) mine[at.first[e] + i] = sums.v[e][i];
+  if (groups == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < d; c += kThreads) {
+    float total = 0.0f;
+    for (int g = 0; g < groups; ++g) total += s_row[g * d + c];
+    part[c] = total;
   }
 }
 
-template <typename T, int E, bool kBlock>
-__global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_kernel(NormArgs a, int bits) {
-  __shared__ float s_sums[2 * (kNormThreads / 64) * 2];
-  extern __shared__ float s_row[];  // [groups][d], not kBlock
+template <typename T, int E, bool kWide, int kThreads, int kGate>
+__global__ __launch_bounds__(kThreads, E > 1 ? 2 : sizeof(T) == 2 ? 3 : 4) void
+residual_norm_bwd_kernel(NormArgs a, int bits) {
+  __shared__ float2 s_sums[2 * (kThreads / 64)];
+  extern __shared__ float s_row[];  // [groups][d], of several groups
   constexpr int V = Row<T, E>::V;
-  Lanes<kBlock> lanes(bits, s_sums);
-  const RowOf<T, E, kBlock> at(lanes, a.d);
+  Lanes<kWide, kThreads> lanes(bits, s_sums);
+  const RowOf<T, E, kWide, kThreads> at(lanes, a.d);
   const bool centered = a.centered != 0, update = a.update.p != nullptr;
   Row<T, E> w1, w2, all, v_w1{}, v_w2{}, v_all{};
   at.load_weight(a.w1, w1);
   at.load_weight(a.w2, w2);
-  if (a.gate_kind == kChannelGate) at.load_weight(a.gate.p, all);
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kNormThreads >> bits);
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (kNormThreads >> bits) + (threadIdx.x >> bits);
-  const int64_t group0 = row - (threadIdx.x >> bits) + ((threadIdx.x & ~63) >> bits);
-  for (int64_t lead = kBlock ? row : group0; lead < a.n; lead += groups, row += groups) {
+  if constexpr (kGate == kChannelGate) at.load_weight(a.gate.p, all);
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kThreads >> bits);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads >> bits) + (threadIdx.x >> bits);
+  const int64_t group0 = row - (threadIdx.x >> bits) + (kWide ? 0 : (threadIdx.x & ~63) >> bits);
+  for (int64_t lead = group0; lead < a.n; lead += groups, row += groups) {
     const bool some = row < a.n;
     const int64_t r = some ? row : lead;
     Loose<T, V> rx[E], rf[E], rg[E], ry[E], ru[E];
     at.load(a.x, r, rx);
     if (update) at.load(a.update, r, rf);
-    if (a.gate_kind == kRowGate) at.load(a.gate, r, rg);
+    if constexpr (kGate == kRowGate) at.load(a.gate, r, rg);
     if (a.v_u.p != nullptr) at.load(a.v_u, r, ru);
     if (a.v_y.p != nullptr) at.load(a.v_y, r, ry);
     Row<T, E> z, h;
     widen<T, E>(rx, z);
     float h_factor = 1.0f;
-    auto gate = [&](int e, int i) {
-      if (a.gate_kind == kNoGate) return make_float2(1.0f, 0.0f);
-      return sigmoids(a.gate_kind == kRowGate ? static_cast<float>(rg[e].v[i]) : all.v[e][i]);
-    };
+    // The gate, and its derivative's factor.
+    Row<T, E> up, slope;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float2 g = make_float2(1.0f, 0.0f);
+        if constexpr (kGate == kChannelGate) g = sigmoids(all.v[e][i]);
+        if constexpr (kGate == kRowGate) g = sigmoids(static_cast<float>(rg[e].v[i]));
+        up.v[e][i] = a.scale * g.x;
+        slope.v[e][i] = g.y;
+      }
     if (update) {
       widen<T, E>(rf, h);
       if (a.w1 != nullptr) h_factor = at.norm(lanes, centered, a.eps, h);
@@ -339,7 +359,7 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_kernel(NormArg
         for (int e = 0; e < E; ++e)
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            z.v[e][i] = fmaf(a.scale * gate(e, i).x, h.v[e][i] * w1.v[e][i], z.v[e][i]);
+            z.v[e][i] = fmaf(up.v[e][i], h.v[e][i] * w1.v[e][i], z.v[e][i]);
       }
       const float z_factor = at.norm(lanes, centered, a.eps, z);
       float along = 0.0f, total = 0.0f;
@@ -371,17 +391,15 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_kernel(NormArg
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float2 g = gate(e, i);
-        const float down = a.scale * v.v[e][i];
-        z.v[e][i] = down * (h.v[e][i] * w1.v[e][i]) * (g.x * g.y);
-        v.v[e][i] = down * g.x;
+        v.v[e][i] *= up.v[e][i];
+        z.v[e][i] = v.v[e][i] * slope.v[e][i] * (h.v[e][i] * w1.v[e][i]);
         if (some) {
           v_w1.v[e][i] = fmaf(v.v[e][i], h.v[e][i], v_w1.v[e][i]);
-          if (a.want_gate != 0) v_all.v[e][i] += z.v[e][i];
+          if constexpr (kGate == kChannelGate) v_all.v[e][i] += z.v[e][i];
         }
         v.v[e][i] *= w1.v[e][i];
       }
-    if (some && a.v_gate != nullptr && a.gate_kind == kRowGate) at.store(a.v_gate, r, a.d, z);
+    if (kGate == kRowGate && some && a.v_gate != nullptr) at.store(a.v_gate, r, a.d, z);
     if (a.w1 != nullptr) {
       float along = 0.0f, total = 0.0f;
 #pragma unroll
@@ -405,10 +423,10 @@ __global__ __launch_bounds__(kNormThreads) void residual_norm_bwd_kernel(NormArg
     if (some && a.v_update != nullptr) at.store(a.v_update, r, a.d, v);
   }
   float *part = a.parts + static_cast<int64_t>(blockIdx.x) * 3 * a.d;
-  if (a.want_w1 != 0) store_part<T, E, kBlock>(at, bits, a.d, v_w1, s_row, part);
-  if (a.want_w2 != 0) store_part<T, E, kBlock>(at, bits, a.d, v_w2, s_row, part + a.d);
-  if (a.want_gate != 0)
-    store_part<T, E, kBlock>(at, bits, a.d, v_all, s_row, part + 2 * a.d);
+  if (a.want_w1 != 0) store_part<T, E, kWide, kThreads>(at, bits, a.d, v_w1, s_row, part);
+  if (a.want_w2 != 0) store_part<T, E, kWide, kThreads>(at, bits, a.d, v_w2, s_row, part + a.d);
+  if constexpr (kGate == kChannelGate)
+    if (a.want_gate != 0) store_part<T, E, kWide, kThreads>(at, bits, a.d, v_all, s_row, part + 2 * a.d);
 }
 
 // The blocks' parts of up to three sums, 64 columns of one sum to a block, 16
@@ -435,54 +453,57 @@ __global__ __launch_bounds__(1024) void norm_sums_kernel(const float *__restrict
   out[column] = static_cast<T>(total);
 }
 
-// Lanes to a row (as a power of two; 8 for the block's 256) and vectors per lane.
+// Lanes to a row, as a power of two, and 16-byte pieces of a lane.
 struct NormForm {
-  int bits, vectors;
+  int bits, pieces;
 };
 NormForm norm_form(int64_t d, int type) {
-  const int64_t per = 16 / type_size(type), vectors = ceil_div(d, per);
-  int bits = 3;
-  while (bits < 6 && (1 << bits) < vectors) ++bits;
-  if (vectors <= (1 << bits)) return {bits, 1};
-  if (vectors <= 128) return {6, 2};
-  int e = 1;
-  while (256 * e < vectors) e *= 2;
-  return {8, e};
+  const int64_t pieces = ceil_div(d, 16 / type_size(type));
+  int bits = 3, each = 1;
+  while (bits < 9 && (1 << bits) < pieces) ++bits;
+  while ((each << bits) < pieces) each *= 2;
+  return {bits, each};
 }
+int norm_threads(const NormForm &f) { return f.bits > 8 ? 512 : 256; }
 int64_t norm_blocks(int64_t n, const NormForm &f, int64_t most) {
-  return std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(n, kNormThreads >> f.bits)));
+  return std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(n, norm_threads(f) >> f.bits)));
+}
+// Blocks of the backward: six to a CU while their parts of the sums are few bytes
+// beside the rows, then three, then two.
+int64_t norm_parts(int64_t n, int64_t d, const NormForm &f) {
+  return norm_blocks(n, f, d <= 512 ? 1536 : d <= 1024 ? 768 : 512);
 }
 
+template <typename T, bool kBack, int E, bool kWide, int kThreads, int kGate>
+void launch_norm_gate(const NormArgs &a, const NormForm &f, int64_t blocks, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
+  if constexpr (kBack) {
+    const int groups = kThreads >> f.bits;
+    const size_t lds = groups > 1 ? static_cast<size_t>(groups) * a.d * sizeof(float) : 0;
+    residual_norm_bwd_kernel<T, E, kWide, kThreads, kGate><<<grid, block, lds, stream>>>(a, f.bits);
+  } else {
+    residual_norm_fwd_kernel<T, E, kWide, kThreads, kGate><<<grid, block, 0, stream>>>(a, f.bits);
+  }
+}
+template <typename T, bool kBack, int E, bool kWide, int kThreads>
+int launch_norm_as(const NormArgs &a, const NormForm &f, int64_t blocks, hipStream_t stream) {
+  if (a.gate_kind == kRowGate)
+    launch_norm_gate<T, kBack, E, kWide, kThreads, kRowGate>(a, f, blocks, stream);
+  else if (a.gate_kind == kChannelGate)
+    launch_norm_gate<T, kBack, E, kWide, kThreads, kChannelGate>(a, f, blocks, stream);
+  else
+    launch_norm_gate<T, kBack, E, kWide, kThreads, kNoGate>(a, f, blocks, stream);
+  return check_launch("residual_norm");
+}
 template <typename T, bool kBack>
 int launch_norm(const NormArgs &a, const NormForm &f, int64_t blocks, hipStream_t stream) {
-  const size_t lds = kBack && f.bits < 8
-                         ? static_cast<size_t>(kNormThreads >> f.bits) * a.d * sizeof(float)
-                         : 0;
-#define R2S_NORM_LAUNCH(E, kBlock)                                                        \
-  do {                                                                                    \
-    if constexpr (kBack)                                                                  \
-      residual_norm_bwd_kernel<T, E, kBlock><<<dim3(static_cast<uint32_t>(blocks)),       \
-                                               dim3(kNormThreads), lds, stream>>>(a, f.bits); \
-    else                                                                                  \
-      residual_norm_fwd_kernel<T, E, kBlock><<<dim3(static_cast<uint32_t>(blocks)),       \
-                                               dim3(kNormThreads), 0, stream>>>(a, f.bits); \
-  } while (0)
-  if (f.bits < 8) {
-    if (f.vectors == 1)
-      R2S_NORM_LAUNCH(1, false);
-    else
-      R2S_NORM_LAUNCH(2, false);
-  } else if (f.vectors <= 1) {
-    R2S_NORM_LAUNCH(1, true);
-  } else if (f.vectors == 2) {
-    R2S_NORM_LAUNCH(2, true);
-  } else if (f.vectors == 4) {
-    R2S_NORM_LAUNCH(4, true);
-  } else {
-    if constexpr (sizeof(T) == 4) R2S_NORM_LAUNCH(8, true);
-  }
-#undef R2S_NORM_LAUNCH
-  return check_launch("residual_norm");
+  if (f.bits <= 6) return launch_norm_as<T, kBack, 1, false, 256>(a, f, blocks, stream);
+  if (f.bits <= 8) return launch_norm_as<T, kBack, 1, true, 256>(a, f, blocks, stream);
+  if (f.pieces == 1) return launch_norm_as<T, kBack, 1, true, 512>(a, f, blocks, stream);
+  if (f.pieces == 2) return launch_norm_as<T, kBack, 2, true, 512>(a, f, blocks, stream);
+  if constexpr (sizeof(T) == 4) return launch_norm_as<T, kBack, 4, true, 512>(a, f, blocks, stream);
+  set_error("residual_norm: no form for this width");
+  return R2S_ERANGE;
 }
 
 int check_norm(const char *op, int type, int64_t n, int64_t d, const void *x, int64_t xs,
@@ -546,7 +567,7 @@ int r2s_residual_norm_fwd(const void *x, int64_t x_stride, const void *update,
 int64_t r2s_residual_norm_bwd_workspace_bytes(int32_t type, int64_t n, int64_t width) {
   if (!r2s::known_type(type) || n <= 0 || width <= 0 || width > r2s::kNormMost) return 0;
   const r2s::NormForm f = r2s::norm_form(width, type);
-  return r2s::norm_blocks(n, f, r2s::kNormBlocks) * 3 * width * static_cast<int64_t>(sizeof(float));
+  return r2s::norm_parts(n, width, f) * 3 * width * static_cast<int64_t>(sizeof(float));
 }
 
 int r2s_residual_norm_bwd(const void *x, int64_t x_stride, const void *update,
@@ -605,7 +626,7 @@ int r2s_residual_norm_bwd(const void *x, int64_t x_stride, const void *update,
   a.eps = eps;
   hipStream_t stream = r2s::as_stream(st);
   const r2s::NormForm f = r2s::norm_form(width, type);
-  const int64_t blocks = n > 0 ? r2s::norm_blocks(n, f, r2s::kNormBlocks) : 0;
+  const int64_t blocks = n > 0 ? r2s::norm_parts(n, width, f) : 0;
   R2S_BY_TYPE(type, {
     if (n > 0) R2S_RETURN_IF((r2s::launch_norm<T, true>(a, f, blocks, stream)));
     if (!sums) return R2S_OK;

@@ -24,6 +24,7 @@ parameters with decoupled weight decay; its states are float32 or 8 bits.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Iterable, List
 
 import torch
@@ -31,6 +32,7 @@ from torch.optim.optimizer import _get_scalar_dtype
 
 from .cuda import _backend
 from .cuda import _lib as L
+from .cuda import _ops
 
 __all__ = ["Adam", "AdamW", "step_all"]
 
@@ -156,7 +158,10 @@ _RUN = 256
 _FEWEST_8BIT = 4096
 _PARAM_TYPES = {torch.float32: L.TYPE_F32, torch.bfloat16: L.TYPE_BF16,
                 torch.float16: L.TYPE_F16}
-# State tensors of an element each, and of a run each.
+# r2s_adamw_tensor_t, packed without a ctypes object for each tensor.
+_ENTRY = struct.Struct("<7Qq8fiI")
+assert _ENTRY.size == ctypes.sizeof(L.AdamwTensor)
+# The names of states in 32 bits, and in 8 with the scales of each run.
 _STATE_32 = ("exp_avg", "exp_avg_sq")
 _STATE_8 = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
 
@@ -217,24 +222,50 @@ class AdamW(torch.optim.Optimizer):
         """(master, average, second, their scales), None for those that are not
         there, checked: the kernel takes their addresses."""
         runs, n = (-(-p.numel() // _RUN),), p.shape
-        master = (n, torch.float32) if p.dtype != torch.float32 else None
+        wanted = [("master", n, torch.float32) if p.dtype != torch.float32 else None]
         if "exp_avg_sq_root" in state:
-            names = ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
-            wanted = ((n, torch.float8_e4m3fn),) * 2 + ((runs, torch.float32),) * 2
+            wanted += [(name, n, torch.float8_e4m3fn) for name in _STATE_8[::2]]
+            wanted += [(name, runs, torch.float32) for name in _STATE_8[1::2]]
         else:
-            names = ("exp_avg", "exp_avg_sq", None, None)
-            wanted = ((n, torch.float32),) * 2 + (None, None)
+            wanted += [(name, n, torch.float32) for name in _STATE_32] + [None, None]
         out = []
-        for name, want in zip(("master", *names), (master, *wanted)):
-            t = state.get(name)
-            if want is None:
-                out.append(None)
-                continue
-            if not isinstance(t, torch.Tensor) or t.shape != want[0] or t.dtype != want[1] \
-                    or t.device != p.device or not t.is_contiguous():
-                raise RuntimeError(f"AdamW state {name!r} does not match its parameter")
+        for want in wanted:
+            t = None
+            if want is not None:
+                name, shape, dtype = want
+                t = state.get(name)
+                if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype \
+                        or t.device != p.device or not t.is_contiguous():
+                    raise RuntimeError(f"AdamW state {name!r} does not match its parameter")
             out.append(t)
         return tuple(out)
+
+    def _checked(self, p: torch.Tensor, state: dict, seen: dict) -> tuple:
+        """(element type, the state's tensors) of a parameter that the kernel may
+        step.  What was found for the very same tensor objects at an earlier step is
+        not looked up again but for their sizes: that was most of a step's host time."""
+        before = seen.get(p)
+        if before is not None:
+            kind, names, tensors = before
+            n, runs = p.numel(), -(-p.numel() // _RUN)
+            for name, t, per in zip(names, tensors, (n, n, n, runs, runs)):
+                if t is not None and (state.get(name) is not t or t.numel() != per
+                                      or not t.is_contiguous()):
+                    break
+            else:
+                if p.is_contiguous():
+                    return kind, tensors
+        kind = _PARAM_TYPES.get(p.dtype)
+        if kind is None or not p.is_cuda:
+            raise NotImplementedError("the fused AdamW step needs float32, bfloat16 or float16 "
+                                      "CUDA parameters")
+        if not p.is_contiguous():
+            raise NotImplementedError("the fused AdamW step needs contiguous parameters")
+        second = "exp_avg_sq_root" if "exp_avg_sq_root" in state else "exp_avg_sq"
+        names = ("master", "exp_avg", second, "exp_avg_scale", "exp_avg_sq_root_scale")
+        tensors = self._state_tensors(p, state)
+        seen[p] = kind, names, tensors
+        return kind, tensors
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -242,50 +273,51 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work: dict = {}  # device -> (entries, tensors kept until the launch)
+        seen = self.__dict__.setdefault("_seen", {})
+        work: dict = {}  # device -> (packed entries, gradients kept until the launch)
         for group in self.param_groups:
             _check_options(group, ())
             lr, (beta1, beta2) = group["lr"], group["betas"]
             fixed = beta1, 1 - beta1, beta2, 1 - beta2, 1 - lr * group["weight_decay"]
             eps = group["eps"]
+            last, scalars = None, ()  # those of one step count serve all that share it
             for p in group["params"]:
                 grad = p.grad
                 if grad is None:
                     continue
                 if grad.is_sparse:
                     raise RuntimeError("AdamW does not support sparse gradients")
-                kind = _PARAM_TYPES.get(p.dtype)
-                if kind is None or not p.is_cuda:
-                    raise NotImplementedError("the fused AdamW step needs float32, bfloat16 or "
-                                              "float16 CUDA parameters")
-                if not p.is_contiguous():
-                    raise NotImplementedError("the fused AdamW step needs contiguous parameters")
-                if grad.dtype != p.dtype or grad.device != p.device or grad.shape != p.shape:
+                device = p.device
+                if grad.dtype != p.dtype or grad.device != device or grad.shape != p.shape:
                     raise RuntimeError("AdamW gradient does not match its parameter")
-                if p.device not in work:
-                    with torch.cuda.device(p.device):
-                        if torch.cuda.is_current_stream_capturing():
-                            raise RuntimeError("AdamW.step cannot be captured into a graph")
-                    work[p.device] = [], []
-                entries, kept = work[p.device]
+                if device not in work:
+                    if p.is_cuda:
+                        with _ops._on(device):
+                            if torch.cuda.is_current_stream_capturing():
+                                raise RuntimeError("AdamW.step cannot be captured into a graph")
+                    work[device] = [], []
+                entries, kept = work[device]
                 state = self.state[p]
                 if not state:
                     self._new_state(p, group["state_bits"])
-                tensors = self._state_tensors(p, state)
-                grad = grad.contiguous()
+                kind, (master, mean, second, scale, second_scale) = self._checked(p, state, seen)
+                if not grad.is_contiguous():
+                    grad = grad.contiguous()
                 state["step"] = step = int(state["step"]) + 1
-                entries.append(L.AdamwTensor(
-                    p.data_ptr(), grad.data_ptr(),
-                    *[None if t is None else t.data_ptr() for t in tensors], p.numel(), *fixed,
-                    (1 - beta2 ** step) ** 0.5, eps, -lr / (1 - beta1 ** step), kind,
-                    step & 0xFFFFFFFF))
+                if step != last:
+                    last, scalars = step, ((1 - beta2 ** step) ** 0.5, eps,
+                                           -lr / (1 - beta1 ** step))
+                entries.append(_ENTRY.pack(
+                    p.data_ptr(), grad.data_ptr(), 0 if master is None else master.data_ptr(),
+                    mean.data_ptr(), second.data_ptr(), 0 if scale is None else scale.data_ptr(),
+                    0 if second_scale is None else second_scale.data_ptr(), p.numel(), *fixed,
+                    *scalars, kind, step & 0xFFFFFFFF))
                 kept.append(grad)
         lib = _backend.library() if work else None
         for device, (entries, _) in work.items():
-            table = (L.AdamwTensor * len(entries))(*entries)
-            with torch.cuda.device(device):
-                rc = lib.r2s_adamw_step(ctypes.cast(table, ctypes.c_void_p), len(entries),
-                                        torch.cuda.current_stream(device).cuda_stream)
+            table = b"".join(entries)
+            with _ops._on(device):
+                rc = lib.r2s_adamw_step(table, len(entries), _ops._stream(device))
             if rc != 0:
                 raise RuntimeError(f"r2s_adamw_step failed ({rc}): "
                                    f"{lib.r2s_last_error().decode(errors='replace')}")
@@ -296,6 +328,7 @@ class AdamW(torch.optim.Optimizer):
         """torch's, with the states in the types that they were saved in (torch
         casts them to their parameters')."""
         super().load_state_dict(state_dict)
+        self.__dict__.pop("_seen", None)
         saved = state_dict["state"]
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]

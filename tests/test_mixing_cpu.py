@@ -70,7 +70,7 @@ def test_residual_norm_arguments(lib):
     assert fwd(n=0) == 0 and fwd(d=0) == 0 and fwd(f=None, w2=None, y=None, u=None) == 0
     size = lib.r2s_residual_norm_bwd_workspace_bytes
     assert size(0, 0, 8) == size(7, 5, 8) == size(0, 5, 9000) == 0
-    assert size(1, 1 << 20, 1024) <= 512 * 3 * 4 * 1024
+    assert size(1, 1 << 20, 1024) <= 768 * 3 * 4 * 1024
 
     def bwd(f=FAKE, w1=FAKE, w2=FAKE, kind=0, v_u=FAKE, grads=(FAKE,) * 5, ws=FAKE, room=1 << 20):
         return lib.r2s_residual_norm_bwd(FAKE, 8, f, 8, FAKE, 8, kind, w1, w2, FAKE, 8, v_u, 8, 1.0,
