@@ -404,6 +404,53 @@ struct __attribute__((packed)) Loose {
   T v[V];
 };
 
+// The piece of 16 bytes of a row that holds its last `there` elements, where that is
+// less than a piece: read as the row's last 16 bytes, and moved down.
+template <typename T>
+struct Tail {
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  int back;  // elements that the read begins earlier
+  __device__ __forceinline__ Tail(int there, int width)
+      : back(there > 0 && there < kPer && width >= kPer ? kPer - there : 0) {}
+  __device__ __forceinline__ u32x4 move(u32x4 x) const {
+    constexpr int kWord = sizeof(T) == 4 ? 1 : 2;  // elements
+#pragma unroll
+    for (int step = kPer / 2; step > 0; step /= 2) {
+      if (step >= kWord) {
+        const int words = step / kWord;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t from = j + words < 4 ? x[j + words] : 0u;
+          x[j] = (back & step) != 0 ? from : x[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t from = x[j] >> 16 | (j < 3 ? x[j + 1] << 16 : 0u);
+          x[j] = (back & step) != 0 ? from : x[j];
+        }
+      }
+    }
+    return x;
+  }
+};
+// A piece of a row: 16 bytes at `at` (Tail's place), of a row narrower than that
+// element by element.
+template <typename T, bool kWhole>
+__device__ __forceinline__ u32x4 load_piece(const T *at, int there, const Tail<T> &tail) {
+  constexpr int kPer = Tail<T>::kPer;
+  if constexpr (kWhole) {
+    return __builtin_bit_cast(u32x4, *reinterpret_cast<const Loose<T, kPer> *>(at));
+  } else {
+    if (there >= kPer || tail.back != 0)
+      return tail.move(__builtin_bit_cast(u32x4, *reinterpret_cast<const Loose<T, kPer> *>(at)));
+    Pack<T, kPer> e;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) e.v[j] = j < there ? at[j] : static_cast<T>(0.0f);
+    return __builtin_bit_cast(u32x4, e);
+  }
+}
+
 // A chunk's rows on their way to LDS: kCount pieces of 16 bytes a thread, of one
 // column and rows kStep apart.  The addresses are a scalar one for each piece and an
 // unsigned 32-bit offset of the thread's own, which is all that stays in vector
@@ -418,13 +465,14 @@ struct Stage {
   u32x4 raw[kCount];
   uint32_t offset;
   int row, there;  // the first piece's row; elements of the width in the column's piece
+  Tail<T> tail;
   // `step` elements between rows, at most 2^24 of either sign.
-  __device__ __forceinline__ Stage(int64_t step, int width) {
-    row = static_cast<int>(threadIdx.x) / kPieces;
-    const int column = static_cast<int>(threadIdx.x) % kPieces * kPer;
+  __device__ __forceinline__ Stage(int64_t step, int width)
+      : row(static_cast<int>(threadIdx.x) / kPieces),
+        there(width - static_cast<int>(threadIdx.x) % kPieces * kPer), tail(there, width) {
     const int64_t rows = step >= 0 ? row * step : (kStep - 1 - row) * -step;
-    offset = static_cast<uint32_t>(rows + column) * static_cast<uint32_t>(sizeof(T));
-    there = width - column;
+    offset = static_cast<uint32_t>(rows + (width - there) - (kWhole ? 0 : tail.back)) *
+             static_cast<uint32_t>(sizeof(T));
   }
   // Rows from `first` on, `left` of them; zeros for those past them and for columns
   // past the width.
@@ -435,15 +483,7 @@ struct Stage {
           first + (i * kStep + (step < 0 ? kStep - 1 : 0)) * step);
       u32x4 x{0, 0, 0, 0};
       if (row + i * kStep < left && there > 0) {
-        const T *p = reinterpret_cast<const T *>(base + offset);
-        if (kWhole || there >= kPer) {
-          x = __builtin_bit_cast(u32x4, *reinterpret_cast<const Loose<T, kPer> *>(p));
-        } else {
-          Pack<T, kPer> e;
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) e.v[j] = j < there ? p[j] : static_cast<T>(0.0f);
-          x = __builtin_bit_cast(u32x4, e);
-        }
+        x = load_piece<T, kWhole>(reinterpret_cast<const T *>(base + offset), there, tail);
       }
       raw[i] = x;
     }
@@ -485,8 +525,8 @@ struct Rows {
   static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
   u32x4 raw[kOwn][KB];
   uint32_t offset;
-  int row, width;  // elements of a row from the lane's first on
-  __device__ __forceinline__ Rows(int64_t step, int channels) {
+  int row, width, channels;  // elements of a row from the lane's first on, and in all
+  __device__ __forceinline__ Rows(int64_t step, int c) : channels(c) {
     row = static_cast<int>(lane_id()) % 16;
     const int column = static_cast<int>(lane_id()) / 16 * kPer;
     offset = static_cast<uint32_t>((step >= 0 ? row * step : (15 - row) * -step) + column) *
@@ -506,17 +546,9 @@ struct Rows {
       for (int kb = 0; kb < KB; ++kb) {
         const T *at = reinterpret_cast<const T *>(p + offset) + kb * 4 * kPer;
         const int there = width - kb * 4 * kPer;
+        const Tail<T> tail(kWhole ? 0 : there, channels);
         u32x4 x{0, 0, 0, 0};
-        if (some && there > 0) {
-          if (kWhole || there >= kPer) {
-            x = __builtin_bit_cast(u32x4, *reinterpret_cast<const Loose<T, kPer> *>(at));
-          } else {
-            Pack<T, kPer> e;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) e.v[j] = j < there ? at[j] : static_cast<T>(0.0f);
-            x = __builtin_bit_cast(u32x4, e);
-          }
-        }
+        if (some && there > 0) x = load_piece<T, kWhole>(at - tail.back, there, tail);
         raw[own][kb] = x;
       }
     }
@@ -910,11 +942,10 @@ Form form_of(const Sizes &z) {
   return {wide <= 64 ? 64 : wide <= 128 ? 128 : 256, 4};
 }
 
-// Blocks of a walk that the device holds at once: by their registers and LDS, 10 of
-// one wave, 6 of two and 3, 2 or 1 of four to a CU.  A few blocks more would be a
-// second round.
+// Blocks of a walk that the device holds at once, by their registers and LDS.  A few
+// blocks more would be a second round.
 int64_t blocks_at_once(const Form &f) {
-  return 256 * (f.waves == 1 ? 10 : f.waves == 2 ? 6 : f.kd == 64 ? 3 : f.kd == 128 ? 2 : 1);
+  return 256 * (f.waves == 1 ? 16 : f.waves == 2 ? 8 : f.kd == 64 ? 3 : f.kd == 128 ? 2 : 1);
 }
 
 // Tokens of a span: as many as fill the device once, but at least 256, so that a
