@@ -211,20 +211,24 @@ __global__ __launch_bounds__(256) void decay_carry_few_kernel(Walk w, int64_t to
                     r.initial != nullptr ? r.initial[i] : 0.0f);
 }
 
-// Any sequences: a block takes 64 elements of the states of one after another.  Its
-// 16 waves take a run of a long sequence's spans each, add it up, and go over it
-// again from what the waves before them leave, so that hundreds of spans are not a
-// chain of as many loads (four heads of 16 x 16: 600 spans in 11 us; a chain took 12
-// for 252).  `per` sequences are looked at together: ragged ones mostly have one span.
+// Any sequences: a block takes 64 elements of the states of `per` sequences, of which
+// it looks at all together, as ragged ones mostly have one span.  Its 16 waves take
+// a sequence of few spans each; of many they take a run of spans each, add it up, and
+// go over it again from what the waves before them leave, so that hundreds of spans
+// are not a chain of as many loads (four heads of 16 x 16: 600 spans in 11 us; a
+// chain took 12 for 252).
 __global__ __launch_bounds__(1024) void decay_carry_kernel(Walk w, int per) {
   __shared__ float s_sum[16][64];
   const Role &r = w.role[0];
   const int64_t size = static_cast<int64_t>(r.dk) * r.dv, step = w.heads * size;
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 64 + lane_id();
   const bool some = e < step;
-  const int wave = static_cast<int>(wave_index());
+  const uint32_t wave = wave_index();
   const float log_span = some ? w.log_decay[e / size] * static_cast<float>(w.cut.span) : 0.0f;
   const float keep = expf(log_span);
+  auto begin = [&](int64_t sequence) {
+    return r.initial != nullptr && some ? r.initial[sequence * step + e] : 0.0f;
+  };
   for (int64_t s0 = static_cast<int64_t>(blockIdx.y) * per; s0 < w.cut.sequences;
        s0 += static_cast<int64_t>(gridDim.y) * per) {
     const int64_t mine = s0 + lane_id();
@@ -238,17 +242,23 @@ __global__ __launch_bounds__(1024) void decay_carry_kernel(Walk w, int per) {
         count = min(count, w.cut.carried - place);
       }
     }
-    for (uint64_t left = ballot(count > 0); left != 0; left &= left - 1) {
-      const uint32_t from = static_cast<uint32_t>(__builtin_ctzll(left));
-      const int64_t spans = readlane_i64(count, from);
-      const int64_t each = spans <= 16 ? spans : (spans + 15) / 16;
+    uint32_t turn = 0;
+    for (uint64_t few = ballot(count > 0 && count <= 16); few != 0; few &= few - 1) {
+      if (turn++ % 16 != wave) continue;
+      const uint32_t from = static_cast<uint32_t>(__builtin_ctzll(few));
+      carry_along<true>(r.carried + readlane_i64(place, from) * step + e, step,
+                        some ? readlane_i64(count, from) : 0, keep, begin(s0 + from));
+    }
+    for (uint64_t many = ballot(count > 16); many != 0; many &= many - 1) {
+      const uint32_t from = static_cast<uint32_t>(__builtin_ctzll(many));
+      const int64_t spans = readlane_i64(count, from), each = (spans + 15) / 16;
       const int64_t lo = min(wave * each, spans), run = some ? min(each, spans - lo) : 0;
       float *p = r.carried + (readlane_i64(place, from) + lo) * step + e;
-      if (spans > each) s_sum[wave][lane_id()] = carry_along<false>(p, step, run, keep, 0.0f);
+      s_sum[wave][lane_id()] = carry_along<false>(p, step, run, keep, 0.0f);
       __syncthreads();
-      float now = r.initial != nullptr && some ? r.initial[(s0 + from) * step + e] : 0.0f;
+      float now = begin(s0 + from);
       const float whole = expf(log_span * static_cast<float>(each));
-      for (int i = 0; i < wave && run > 0; ++i) now = fmaf(whole, now, s_sum[i][lane_id()]);
+      for (uint32_t i = 0; i < wave && run > 0; ++i) now = fmaf(whole, now, s_sum[i][lane_id()]);
       carry_along<true>(p, step, run, keep, now);
       __syncthreads();  // the sums have been read
     }
@@ -726,6 +736,10 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
     }
   };
 
+  // float32 products are dear: fragments past the channels of odd heads are left out
+  // (3 heads of 33 x 45: 228 us forward and 247).
+  auto none = [&](int kb) { return !kWhole && sizeof(T) == 4 && kb * kFragment >= dk; };
+
   if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
   load(0);
   if constexpr (!kStates) load_q(0);
@@ -762,6 +776,7 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
         f32x4 out[NT] = {};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
+          if (none(kb)) break;
           const Parts<U> q_parts = beside<T>(q_raw[own][kb]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -785,9 +800,11 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
             f32x4 score{0.0f, 0.0f, 0.0f, 0.0f};
             if (apart >= 0) {
 #pragma unroll
-              for (int kb = 0; kb < KB; ++kb)
+              for (int kb = 0; kb < KB; ++kb) {
+                if (none(kb)) break;
                 score = multiply<T>(along<T, KD>(s_k, b * kFragment + t * 16 + i, kb * 4 + g),
                                     q_raw[own][kb], score);
+              }
               if (apart == 0) {  // a later token's score may be anything
 #pragma unroll
                 for (int e = 0; e < 4; ++e) score[e] = i < g * 4 + e ? 0.0f : score[e];
@@ -847,6 +864,7 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
+        if (none(kb)) break;
         state[kb][t] *= keep;
 #pragma unroll
         for (int b = 0; b < JB; ++b) {
@@ -948,14 +966,17 @@ int64_t blocks_at_once(const Form &f) {
   return 256 * (f.waves == 1 ? 16 : f.waves == 2 ? 8 : f.kd == 64 ? 3 : f.kd == 128 ? 2 : 1);
 }
 
-// Tokens of a span: as many as fill the device once, but at least 256, so that a
-// span's own tokens outweigh its states.
+// Tokens of a span: as many as fill the device once (twice where the sequences'
+// lengths are not known, so that short ones even out the ends: 100k tokens in 512
+// sequences, 3 heads of 33 x 45 float32, 247 us forward and 269), but at least 256, so
+// that a span's own tokens outweigh its states.
 int64_t span_of(const Sizes &z) {
   const Form f = form_of(z);
   const int64_t blocks = std::max<int64_t>(1, z.heads * ceil_div(std::max(z.dk, z.dv), f.columns()));
   const int64_t longest = z.ragged ? z.n : z.length;
   const int64_t sequences = z.ragged ? 1 : std::max<int64_t>(1, z.sequences);
-  const int64_t spans = std::max<int64_t>(1, blocks_at_once(f) / (blocks * sequences));
+  const int64_t spans = std::max<int64_t>(
+      1, (z.ragged ? 2 : 1) * blocks_at_once(f) / (blocks * sequences));
   const int64_t span = ceil_div(ceil_div(std::max<int64_t>(longest, 1), spans), 64) * 64;
   return std::max<int64_t>(256, span);
 }
