@@ -254,7 +254,24 @@ def test_values_that_are_not_finite_reach_later_tokens_alone(d, dtype):
                 assert not bad[204:].any() and torch.isfinite(final).all()
             else:
                 assert bad[204:, 1].any(1).all() and not torch.isfinite(final[0, 1]).all()
-    # Gradients run the other way.
+    # Gradients run the other way, and the queries' on.
+    y, final, kept = W.decay_attention_fwd(q[None], k[None], v[None], log_decay)
+    for which, behind in (("q", ("v_k", "v_v")), ("k", ("v_v",)), ("v", ("v_k",))):
+        t = {"q": q, "k": k, "v": v}[which].clone()
+        t[203, 1, 3] = float("inf")
+        args = [t if which == name else x for name, x in (("q", q), ("k", k), ("v", v))]
+        kept = W.decay_attention_fwd(*(a[None] for a in args), log_decay)[2]
+        grads = dict(zip(("v_q", "v_k", "v_v"), W.decay_attention_bwd(
+            *(a[None] for a in args), log_decay, None, None, kept, v_y[None])))
+        for name, grad in grads.items():
+            bad = ~torch.isfinite(grad[0]).all(-1)
+            assert not bad[:, 0].any(), (which, name)
+            if which == "q":  # reaches the tokens before, not its own gradient
+                assert not bad[204:].any() and bool(bad[:203, 1].all()) == (name != "v_q")
+            else:  # what it was multiplied with: behind it the queries, at it the other
+                assert not bad[:203].any() and bad[203:, 1].any() == (name in (*behind, "v_q"))
+                assert name == "v_q" or not bad[204:].any()
+    y, final, kept = W.decay_attention_fwd(q[None], k[None], v[None], log_decay)
     v_y[203, 0, 2] = float("nan")
     y, final, kept = W.decay_attention_fwd(q[None], k[None], v[None], log_decay)
     v_q, v_k, v_v, _ = W.decay_attention_bwd(q[None], k[None], v[None], log_decay, None, None, kept,
@@ -341,6 +358,28 @@ def test_offsets_that_do_not_ascend_stay_in_bounds():
         grads = W.decay_attention_bwd(q, q, v, log_decay, None, off, kept, v)
         torch.cuda.synchronize()
         assert y.shape == v.shape and grads[0].shape == q.shape
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 128), (torch.bfloat16, 256)])
+def test_large_heads_captured(dtype, d):
+    """More LDS than a launch has without asking."""
+    q, k, v, log_decay, _, v_y, _ = (
+        None if t is None else t.to(DEV) for t in _case(700, 1, d, d, 1, dtype, 11, False))
+    q, k, v, v_y = (t[None] for t in (q, k, v, v_y))
+
+    def work():
+        y, final, kept = W.decay_attention_fwd(q, k, v, log_decay)
+        return (y, final, *W.decay_attention_bwd(q, k, v, log_decay, None, None, kept, v_y))
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work()
+    for seed in range(2):
+        torch.manual_seed(seed)
+        q.copy_(torch.randn_like(q))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, work()))
 
 
 def test_captured_and_on_another_stream():

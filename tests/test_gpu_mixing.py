@@ -107,6 +107,10 @@ def test_rotary_strides_gradients_and_empty(dtype):
     out = latent.rotary_axes(q, k, p, (4, 6))
     (only,) = torch.autograd.grad(out[1], (k,), v[1])
     assert torch.equal(only, grads[1])
+    alone, none = latent.rotary_axes(q, None, p, (4, 6))
+    assert none is None
+    (only,) = torch.autograd.grad(alone, (q,), v[0])
+    assert torch.equal(only, grads[0])
     # Turning is linear: <turn(q), v> = <q, turn back(v)>.
     if dtype == torch.float32:
         left = float((out[0].detach() * v[0]).sum())

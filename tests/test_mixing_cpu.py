@@ -209,6 +209,14 @@ def test_tangents_are_refused_rather_than_lost(monkeypatch):
         def residual_norm_fwd(x, update, gate, w1, w2, *args):
             return x.detach().clone(), x.detach().clone()
 
+        @staticmethod
+        def decay_attention_fwd(q, k, v, *args, **kw):
+            return v.detach().clone(), torch.zeros(1), torch.zeros(1)
+
+        @staticmethod
+        def decay_attention_step(q, k, v, *args):
+            return v.detach().clone(), torch.zeros(1)
+
     monkeypatch.setattr(latent, "W", Plain)
     t, w, p = torch.randn(4, 2, 6), torch.ones(6), torch.zeros(4, 1)
     with forward_ad.dual_level():
@@ -225,6 +233,32 @@ def test_tangents_are_refused_rather_than_lost(monkeypatch):
                 call()
         with pytest.raises(NotImplementedError, match="positions"):
             latent.rotary_axes(t, None, forward_ad.make_dual(p, torch.ones_like(p)), (3,))
+        g = torch.zeros(2)
+        state = torch.zeros(4, 2, 6, 6)
+        for args in ((d, t, t), (t, d, t), (t, t, d)):
+            with pytest.raises(NotImplementedError, match="forward mode AD"):
+                latent.decay_attention(*(a[None] for a in args), g)
+            with pytest.raises(NotImplementedError, match="forward mode AD"):
+                latent.decay_attention_step(*args, g, state)
+        with pytest.raises(NotImplementedError, match="log_decay"):
+            latent.decay_attention(t[None], t[None], t[None],
+                                   forward_ad.make_dual(g, torch.ones(2)))
+
+
+def test_functions_are_there_without_the_library():
+    from r2splat.cuda import _wrapper
+    from r2splat.ops import latent
+
+    for name in ("decay_attention", "decay_attention_step", "rotary_axes", "pre_norm",
+                 "residual_norm"):
+        assert name in latent.__all__ and callable(getattr(latent, name))
+    for name in ("decay_attention_fwd", "decay_attention_bwd", "decay_attention_step",
+                 "rotary_axes", "residual_norm_fwd", "residual_norm_bwd"):
+        assert callable(getattr(_wrapper, name))
+    if not torch.cuda.is_available():
+        q = torch.zeros(1, 1, 1, 2)
+        with pytest.raises(RuntimeError, match="unavailable"):
+            latent.decay_attention(q, q, q, torch.zeros(1))
 
 
 def test_decay_attention_arguments(lib):
