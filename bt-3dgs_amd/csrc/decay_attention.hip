@@ -409,6 +409,24 @@ __device__ __forceinline__ u32x4 across(const char *tile, int row, int first) {
   }
 }
 
+// A thread's number among the kThreads that share a head, and their meeting.  A head of
+// one wave needs no barrier: a wave's LDS accesses are in order, and its heads
+// beside it in the block go their own ways.
+template <int kThreads>
+__device__ __forceinline__ int head_thread() {
+  return static_cast<int>(kThreads == 64 ? lane_id() : threadIdx.x);
+}
+template <int kThreads>
+__device__ __forceinline__ void head_sync() {
+  if constexpr (kThreads == 64) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  } else {
+    __syncthreads();
+  }
+}
+
 template <typename T, int V>
 struct __attribute__((packed)) Loose {
   T v[V];
@@ -478,8 +496,8 @@ struct Stage {
   Tail<T> tail;
   // `step` elements between rows, at most 2^24 of either sign.
   __device__ __forceinline__ Stage(int64_t step, int width)
-      : row(static_cast<int>(threadIdx.x) / kPieces),
-        there(width - static_cast<int>(threadIdx.x) % kPieces * kPer), tail(there, width) {
+      : row(head_thread<kThreads>() / kPieces),
+        there(width - head_thread<kThreads>() % kPieces * kPer), tail(there, width) {
     const int64_t rows = step >= 0 ? row * step : (kStep - 1 - row) * -step;
     offset = static_cast<uint32_t>(rows + (width - there) - (kWhole ? 0 : tail.back)) *
              static_cast<uint32_t>(sizeof(T));
@@ -499,7 +517,7 @@ struct Stage {
     }
   }
   __device__ __forceinline__ void put(char *tile) const {
-    char *p = tile + row * Tile<T, D>::kPitch + static_cast<int>(threadIdx.x) % kPieces * 16;
+    char *p = tile + row * Tile<T, D>::kPitch + head_thread<kThreads>() % kPieces * 16;
 #pragma unroll
     for (int i = 0; i < kCount; ++i)
       *reinterpret_cast<u32x4 *>(p + i * kStep * Tile<T, D>::kPitch) = raw[i];
@@ -569,7 +587,7 @@ struct Rows {
 template <typename T, int D, int C, int kThreads>
 __device__ __forceinline__ void clear_rows(char *tile) {
   constexpr int kPieces = D * static_cast<int>(sizeof(T)) / 16;
-  for (int q = kPieces + static_cast<int>(threadIdx.x); q < C * kPieces; q += kThreads)
+  for (int q = kPieces + head_thread<kThreads>(); q < C * kPieces; q += kThreads)
     *reinterpret_cast<u32x4 *>(tile + q / kPieces * Tile<T, D>::kPitch + q % kPieces * 16) =
         u32x4{0, 0, 0, 0};
 }
@@ -591,28 +609,41 @@ struct Shape {
   static constexpr int kK = C * Tile<T, KD>::kPitch, kV = C * Tile<T, kColumns>::kPitch;
   static constexpr int kS = kStates ? 0 : KB * W * kOperands * 1024;
   static constexpr int kLds = kK + kV + kS;
+  // Heads of a block: four of one wave each, so that a compute unit reads the whole
+  // lines that they share.
+  static constexpr int kHeads = W == 1 ? 4 : 1;
+  // Waves of a SIMD that the registers are shared out to.
+  static constexpr int kPerSimd =
+      KD == 32 ? (W == 1 && sizeof(T) == 4 ? 3 : 4) : KD == 64 ? 3 : KD == 128 ? 2 : 1;
 };
 
 template <typename T, int KD, int W, bool kStates, bool kWhole>
-__global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2 : 1) void decay_walk_kernel(
-    Walk w) {
+__global__ __launch_bounds__((64 * W * Shape<T, KD, W, kStates>::kHeads),
+                             (Shape<T, KD, W, kStates>::kPerSimd)) void decay_walk_kernel(Walk w) {
   using S = Shape<T, KD, W, kStates>;
   constexpr int C = S::C, kThreads = S::kThreads, KB = S::KB, JB = S::JB, kTiles = S::kTiles;
   constexpr int kFragment = S::kFragment, kPer = Tile<T, KD>::kPer, NT = S::NT, kRun = S::kRun;
   constexpr int kRows = 4 * kTiles;  // neighbouring rows of the state in a lane
   using U = typename Wide<T>::type;
   extern __shared__ __attribute__((aligned(16))) char s_tile[];
-  __shared__ int s_bad[2];
-  __shared__ float s_left[2 * C];
-  char *s_k = s_tile, *s_v = s_k + S::kK, *s_s = s_v + S::kV;
+  constexpr int kHeads = S::kHeads;
+  __shared__ int s_bads[kHeads][2];
+  __shared__ float s_lefts[kHeads][2 * C];
+  const int inner = kHeads > 1 ? static_cast<int>(wave_index()) : 0;  // head of the block
+  int *s_bad = s_bads[inner];
+  float *s_left = s_lefts[inner];
+  char *s_k = s_tile + inner * S::kLds, *s_v = s_k + S::kK, *s_s = s_v + S::kV;
 
   // Roles of the same tokens are neighbours, and neighbours share an XCD's cache.
   uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
   const Role &r = w.role[id % w.roles];
   id /= w.roles;
-  const uint32_t per_item = static_cast<uint32_t>(w.heads) * w.column_blocks;
+  const uint32_t head_blocks = static_cast<uint32_t>(w.heads + kHeads - 1) / kHeads;
+  const uint32_t per_item = head_blocks * w.column_blocks;
   const uint32_t item = id / per_item, inside = id - item * per_item;
-  const int head = static_cast<int>(inside / static_cast<uint32_t>(w.column_blocks));
+  const int head =
+      static_cast<int>(inside / static_cast<uint32_t>(w.column_blocks)) * kHeads + inner;
+  if (kHeads > 1 && head >= w.heads) return;
   const int block_column = static_cast<int>(inside % static_cast<uint32_t>(w.column_blocks)) *
                            S::kColumns;
   const int dk = r.dk, dv = r.dv;
@@ -629,7 +660,7 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
   T *y = static_cast<T *>(r.y);
   if (x.sequence >= w.cut.sequences) {  // behind the last sequence
     if constexpr (!kStates) {
-      for (int64_t i = threadIdx.x; i < x.count * width; i += kThreads)
+      for (int64_t i = head_thread<kThreads>(); i < x.count * width; i += kThreads)
         y[((x.lo + x.at + i / width) * w.heads + head) * dv + block_column + i % width] =
             static_cast<T>(0.0f);
     }
@@ -638,7 +669,7 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
   if (kStates && x.last) return;
 
   const int lane = static_cast<int>(lane_id()), i = lane % 16, g = lane / 16;
-  const int wave = static_cast<int>(wave_index());
+  const int wave = kHeads > 1 ? 0 : static_cast<int>(wave_index());  // of the head
   // Column tile c of the block holds, of each 16 NT columns, those 4 in every kRun
   // that make neighbours of a lane's outputs: lane i's is part_of(c) + i / 4 kRun + i % 4.
   auto part_of = [](int c) { return c / NT * (16 * NT) + c % NT * 4; };
@@ -696,7 +727,7 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
   }
   // What is left at the end of a chunk of its tokens, and nothing of those behind
   // it: token j of `count` is at C - count + j.
-  for (int j = threadIdx.x; j < 2 * C; j += kThreads)
+  for (int j = head_thread<kThreads>(); j < 2 * C; j += kThreads)
     s_left[j] = j < C ? r.scale_in * power(log2_decay, C - 1 - j + early) : 0.0f;
   const float keep_all = power(log2_decay, C);
 
@@ -740,10 +771,10 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
   // (3 heads of 33 x 45: 228 us forward and 247).
   auto none = [&](int kb) { return !kWhole && sizeof(T) == 4 && kb * kFragment >= dk; };
 
-  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+  if (head_thread<kThreads>() < 2) s_bad[head_thread<kThreads>()] = 0;
   load(0);
   if constexpr (!kStates) load_q(0);
-  __syncthreads();
+  head_sync<kThreads>();
   int turn = 0;
   for (int64_t pos = 0; pos < x.count; turn ^= 1) {
     if constexpr (!kStates) {
@@ -752,14 +783,14 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
     }
     k_stage.put(s_k);
     v_stage.put(s_v);
-    __syncthreads();
+    head_sync<kThreads>();
     int count = static_cast<int>(min(x.count - pos, static_cast<int64_t>(C)));
     if constexpr (!kStates) {
       if (s_bad[turn] != 0 && count > 1) {
         count = 1;
         clear_rows<T, KD, C, kThreads>(s_k);
         clear_rows<T, S::kColumns, C, kThreads>(s_v);
-        __syncthreads();
+        head_sync<kThreads>();
       }
     }
     load(pos + count);
@@ -873,8 +904,8 @@ __global__ __launch_bounds__(64 * W, KD == 32 ? 4 : KD == 64 ? 3 : KD == 128 ? 2
           state[kb][t] = multiply_split<T, true, true>(k_parts, fresh[b], state[kb][t]);
         }
       }
-    __syncthreads();
-    if (threadIdx.x == 0) s_bad[turn] = 0;
+    head_sync<kThreads>();
+    if (head_thread<kThreads>() == 0) s_bad[turn] = 0;
     pos += count;
   }
 
@@ -1016,18 +1047,19 @@ int64_t table_bytes(const Sizes &z, const Plan &p) {
 template <typename T, int KD, int W, bool kStates, bool kWhole>
 int launch_walk_as(const Walk &w, int64_t blocks, hipStream_t stream) {
   using S = Shape<T, KD, W, kStates>;
-  static_assert(S::kLds + 1024 <= 160 * 1024, "LDS of a CU");
-  if (S::kLds > 60 * 1024) {
+  constexpr int kLds = S::kLds * S::kHeads;
+  static_assert(kLds + 2048 <= 160 * 1024, "LDS of a CU");
+  if (kLds > 60 * 1024) {
     const hipError_t err = hipFuncSetAttribute(
         reinterpret_cast<const void *>(&decay_walk_kernel<T, KD, W, kStates, kWhole>),
-        hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
+        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (err != hipSuccess) {
-      set_error("decay_attention: %d bytes of LDS refused: %s", S::kLds, hipGetErrorString(err));
+      set_error("decay_attention: %d bytes of LDS refused: %s", kLds, hipGetErrorString(err));
       return R2S_EHIP;
     }
   }
   decay_walk_kernel<T, KD, W, kStates, kWhole>
-      <<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * W), S::kLds, stream>>>(w);
+      <<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * W * S::kHeads), kLds, stream>>>(w);
   return check_launch("decay_attention");
 }
 template <typename T, int KD, int W, bool kStates>
@@ -1046,7 +1078,7 @@ int walk(const Sizes &z, const Plan &p, Walk &w, int roles, hipStream_t stream) 
     columns = std::max<int64_t>(columns, ceil_div(w.role[i].dv, f.columns()));
   w.column_blocks = static_cast<int32_t>(columns);
   w.roles = static_cast<uint32_t>(roles);
-  const int64_t blocks = p.items * z.heads * columns * roles;
+  const int64_t blocks = p.items * (f.waves == 1 ? ceil_div(z.heads, 4) : z.heads) * columns * roles;
   if (blocks > kInt32Max) {
     set_error("decay_attention: %lld blocks exceed 2^31 - 1", static_cast<long long>(blocks));
     return R2S_ERANGE;
