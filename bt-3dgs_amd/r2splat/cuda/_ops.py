@@ -13,6 +13,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import operator
 import struct
 import threading
 import warnings
@@ -2197,6 +2198,10 @@ _POSITION_TYPES = {torch.float32: L.POSITION_F32, torch.int32: L.POSITION_I32,
                    torch.int64: L.POSITION_I64}
 
 
+_SECTIONS = [ctypes.c_int32 * axes for axes in range(L.ROTARY_MAX_AXES + 1)]
+_DENSE = torch.contiguous_format
+
+
 def _heads_3d(t: Tensor, name: str, n: int):
     """(tensor, token stride, head stride, heads) of [..., H, D] as [n, H, D]; a
     copy where a head's elements are not consecutive or the tokens have no one
@@ -2230,7 +2235,7 @@ def rotary_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, sections, bas
     kind = _POSITION_TYPES.get(positions.dtype)
     if kind is None:
         _fail("positions must be float32, int32 or int64, got ", positions.dtype)
-    sections = tuple(int(s) for s in sections)
+    sections = tuple(map(operator.index, sections))
     axes = len(sections)
     if not 1 <= axes <= L.ROTARY_MAX_AXES:
         _fail("sections must name 1 to ", L.ROTARY_MAX_AXES, " axes, got ", axes)
@@ -2244,10 +2249,10 @@ def rotary_axes(q: Tensor, k: Optional[Tensor], positions: Tensor, sections, bas
     positions = positions.contiguous()
     dev = q.device
     with _on(dev):
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+        q_out = torch.empty_like(q, memory_format=_DENSE)
+        k_out = None if k is None else torch.empty_like(k, memory_format=_DENSE)
         _call("r2s_rotary_axes", _ptr(qr), qt, qh, hq, _ptr(kr), kt, kh, hk, _ptr(positions), kind,
-              (ctypes.c_int32 * axes)(*sections), axes, bool(shared), float(base),
+              _SECTIONS[axes](*sections), axes, bool(shared), float(base),
               bool(interleaved), bool(inverse), code, n, d, _ptr(q_out), _ptr(k_out), _stream(dev))
     return q_out, k_out
 
@@ -2311,8 +2316,8 @@ def residual_norm_fwd(x: Tensor, update: Optional[Tensor], gate: Optional[Tensor
         x, update, gate, update_weight, weight, "residual_norm_fwd")
     dev = x.device
     with _on(dev):
-        y = x if update is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        u = None if weight is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        y = x if update is None else torch.empty_like(x, memory_format=_DENSE)
+        u = None if weight is None else torch.empty_like(x, memory_format=_DENSE)
         _call("r2s_residual_norm_fwd", _ptr(xr), xs, _ptr(ur), us, _ptr(gr), gs, kind, _ptr(w1),
               _ptr(w2), float(scale), float(eps), bool(centered), code, n, d,
               None if update is None else _ptr(y), _ptr(u), _stream(dev))
@@ -2487,8 +2492,8 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
         _fail("state must be given")
     dev = q.device
     with _on(dev):
-        y = torch.empty(v.shape, dtype=v.dtype, device=dev)
-        final = torch.empty(state.shape, dtype=torch.float32, device=dev)
+        y = torch.empty_like(v, memory_format=_DENSE)
+        final = torch.empty_like(state)
         _call("r2s_decay_attention_step", _ptr(qr), *qs, _ptr(kr), *ks, _ptr(vr), *vs,
               _ptr(log_decay.contiguous()), _ptr(state), b, heads, dk, dv, float(scale), code,
               _ptr(y), _ptr(final), _stream(dev))

@@ -1306,7 +1306,8 @@ int r2s_residual_norm_bwd(const void *x, int64_t x_stride, const void *update,
  * reverse: each sequence from its last token to its first.  A token's row of q, k
  * [heads, dk] and v [heads, dv] is found by the strides of its sequence (equal ones
  * alone; ragged tokens are counted from 0), its place in it and its head, in
- * elements; a head's elements are consecutive.  dk, dv at most 256.  log_decay
+ * elements; a head's elements are consecutive, tokens at most 2^24 elements
+ * apart.  dk, dv at most 256.  log_decay
  * [heads]; initial [sequences, heads, dk, dv] (may be NULL: zeros); final_state
  * likewise; y [n, heads, dv] dense.  kept [r2s_decay_attention_kept_states(...),
  * heads, dk, dv] receives states that the backward starts from (NULL where that
