@@ -82,8 +82,8 @@ constexpr int kRoles = 3;
 // How the sequences are cut.
 struct Cut {
   const int32_t *offsets;  // ragged
-  const int32_t *owner;    // ragged, several spans: each item's sequence
-  const int32_t *first;    // and each sequence's first item
+  const int64_t *order;    // ragged, several spans: items as they are taken, see below
+  const int32_t *first;    // and each sequence's first item, as places are counted
   int64_t n, sequences, length, span;
   int64_t carried;  // places for states between spans
   int32_t spans;    // of an equal sequence
@@ -95,6 +95,7 @@ struct Walk {
   Cut cut;
   int32_t heads, column_blocks;
   uint32_t roles;
+  uint32_t blocks, together;  // and how many of them one XCD takes in a row; 0: its share
 };
 
 // A block's span of its sequence: tokens [at, at + count) of the walk's order.
@@ -112,52 +113,76 @@ __device__ __forceinline__ int64_t bound(const Cut &c, int64_t s) {
 // False for an item that there is not.  Sequence `sequences` stands for the
 // tokens behind the last one.
 __device__ __forceinline__ bool find_span(const Cut &c, int64_t item, Span &x) {
-  int64_t index = 0, items = 1;
+  int64_t sequence = item, index = 0, items = 1, place = 0, lo = 0, length = c.length;
   if (c.offsets == nullptr) {
     const uint32_t which = static_cast<uint32_t>(item), spans = static_cast<uint32_t>(c.spans);
-    x.sequence = which / spans;
+    sequence = which / spans;
     index = which % spans;
     items = c.spans;
-    x.lo = x.sequence * c.length;
-    x.length = c.length;
-    x.place = x.sequence * (c.spans - 1) + index;
+    lo = sequence * length;
+    place = sequence * (items - 1) + index;
   } else {
-    x.sequence = item;
-    if (c.owner != nullptr) {
-      x.sequence = c.owner[item];
-      if (x.sequence < 0) return false;
-      index = item - c.first[x.sequence];
-      items = c.first[x.sequence + 1] - c.first[x.sequence];
+    if (c.order != nullptr) {
+      const int64_t which = c.order[item];
+      if (which < 0) return false;
+      sequence = which >> 32;
+      index = which & 0xFFFFFFFF;
+      const int64_t first = c.first[sequence];
+      items = c.first[sequence + 1] - first;
+      place = first + index - sequence;  // each sequence before has an item without a place
     }
-    x.lo = bound(c, x.sequence);
-    const int64_t hi = x.sequence < c.sequences ? bound(c, x.sequence + 1) : c.n;
-    x.length = max(hi - x.lo, int64_t{0});
-    x.place = item - x.sequence;  // each sequence before has an item without a place
+    lo = bound(c, sequence);
+    const int64_t hi = sequence < c.sequences ? bound(c, sequence + 1) : c.n;
+    length = max(hi - lo, int64_t{0});
   }
+  x.sequence = sequence;
+  x.lo = lo;
+  x.length = length;
+  x.place = place;
   x.at = index * c.span;
-  x.count = max(min(x.length - x.at, c.span), int64_t{0});
+  x.count = max(min(length - x.at, c.span), int64_t{0});
   x.first = index == 0;
   x.last = index + 1 >= items;
   // Offsets that do not ascend may ask for more places than there are.
-  return x.place >= 0 && (x.last || x.place < c.carried) &&
-         (x.first || (x.place > 0 && x.place <= c.carried));
+  return place >= 0 && (x.last || place < c.carried) &&
+         (x.first || (place > 0 && place <= c.carried));
 }
 
-// The items of ragged sequences: each sequence's spans, at least one; those of
-// the tokens behind the last; -1 for the others.
+// The items of ragged sequences, a sequence and the index of its span to each (the
+// upper and the lower half): every sequence's spans, at least one, those of the
+// tokens behind the last, and -1 for places left over.  The longest come first, in classes of an
+// eighth of a span: with short ones last, the device runs dry all at once (100k
+// tokens in 512 sequences, 3 heads of 33 x 45 float32: forward 166 us, in the order of
+// the sequences and in equal shares to the XCDs 231).
+constexpr uint32_t kClasses = 8;
 __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
-                                                           int32_t *__restrict__ owner,
+                                                           int64_t *__restrict__ order,
                                                            int32_t *__restrict__ first) {
   __shared__ int64_t s_total[16];
+  __shared__ uint32_t s_next[kClasses];
+  if (threadIdx.x < kClasses) s_next[threadIdx.x] = 0;
+  __syncthreads();
+  auto tokens_of = [&](int64_t s) {
+    const int64_t hi = s < c.sequences ? bound(c, s + 1) : c.n;
+    return max(hi - bound(c, s), int64_t{0});
+  };
+  // Of the tokens behind a sequence's whole spans, if there are any.
+  auto class_of = [&](int64_t rest) {
+    return kClasses - 1 - static_cast<uint32_t>((rest * kClasses - 1) / c.span);
+  };
   int64_t before = 0;
   for (int64_t s0 = 0; s0 <= c.sequences; s0 += 1024) {
     const int64_t s = s0 + threadIdx.x;
     int64_t items = 0;
     if (s <= c.sequences) {
-      const int64_t hi = s < c.sequences ? bound(c, s + 1) : c.n;
-      const int64_t tokens = max(hi - bound(c, s), int64_t{0});
-      items = (tokens + c.span - 1) / c.span;
-      if (s < c.sequences) items = max(items, int64_t{1});
+      const int64_t tokens = tokens_of(s), whole = tokens / c.span, rest = tokens - whole * c.span;
+      items = whole + (rest > 0 ? 1 : 0);
+      if (whole > 0) atomicAdd(&s_next[0], static_cast<uint32_t>(whole));
+      if (rest > 0) atomicAdd(&s_next[class_of(rest)], 1u);
+      if (s < c.sequences && items == 0) {
+        items = 1;
+        atomicAdd(&s_next[kClasses - 1], 1u);
+      }
     }
     const int64_t inside = wave_inclusive_scan(items);
     if (lane_id() == 63) s_total[wave_index()] = inside;
@@ -168,14 +193,40 @@ __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
       before += s_total[w];
     }
     // Offsets that do not ascend may name more items than there is room for.
-    at = min(at, most);
     before = min(before, most);
-    if (s <= c.sequences) first[s] = static_cast<int32_t>(at);
-    for (int64_t i = at; i < min(at + items, most); ++i) owner[i] = static_cast<int32_t>(s);
+    if (s <= c.sequences) first[s] = static_cast<int32_t>(min(at, most));
     __syncthreads();
   }
-  if (threadIdx.x == 0) first[c.sequences + 1] = static_cast<int32_t>(before);
-  for (int64_t i = before + threadIdx.x; i < most; i += 1024) owner[i] = -1;
+  if (threadIdx.x == 0) {
+    first[c.sequences + 1] = static_cast<int32_t>(before);
+    uint32_t sum = 0;
+    for (uint32_t i = 0; i < kClasses; ++i) {
+      const uint32_t own = s_next[i];
+      s_next[i] = sum;
+      sum += own;
+    }
+  }
+  __syncthreads();
+  auto put = [&](int64_t at, int64_t s, int64_t index) {
+    if (at < most) order[at] = s << 32 | index;
+  };
+  for (int64_t s0 = 0; s0 <= c.sequences; s0 += 1024) {
+    const int64_t s = s0 + threadIdx.x;
+    int64_t whole = 0, at = 0;
+    if (s <= c.sequences) {
+      const int64_t tokens = tokens_of(s), rest = tokens - tokens / c.span * c.span;
+      whole = tokens / c.span;
+      if (whole > 0) at = atomicAdd(&s_next[0], static_cast<uint32_t>(whole));
+      if (rest > 0) put(atomicAdd(&s_next[class_of(rest)], 1u), s, whole);
+      if (s < c.sequences && tokens == 0) put(atomicAdd(&s_next[kClasses - 1], 1u), s, 0);
+    }
+    for (uint64_t some = ballot(whole > 0); some != 0; some &= some - 1) {
+      const uint32_t from = static_cast<uint32_t>(__builtin_ctzll(some));
+      const int64_t spans = readlane_i64(whole, from), to = readlane_i64(at, from);
+      for (int64_t i = lane_id(); i < spans; i += 64) put(to + i, s - lane_id() + from, i);
+    }
+  }
+  for (int64_t i = before + threadIdx.x; i < most; i += 1024) order[i] = -1;
 }
 
 // The states behind `count` spans of a sequence from each span's own, from `now` on:
@@ -635,7 +686,15 @@ __global__ __launch_bounds__((64 * W * Shape<T, KD, W, kStates>::kHeads),
   char *s_k = s_tile + inner * S::kLds, *s_v = s_k + S::kK, *s_s = s_v + S::kV;
 
   // Roles of the same tokens are neighbours, and neighbours share an XCD's cache.
-  uint32_t id = xcd_swizzle(blockIdx.x, gridDim.x);
+  // Ragged items, long ones first, are dealt out to the XCDs in turn.
+  uint32_t id = blockIdx.x;
+  if (w.together == 0) {
+    id = xcd_swizzle(id, gridDim.x);
+  } else {
+    const uint32_t turn = id / 8;
+    id = (turn / w.together * 8 + id % 8) * w.together + turn % w.together;
+    if (id >= w.blocks) return;
+  }
   const Role &r = w.role[id % w.roles];
   id /= w.roles;
   const uint32_t head_blocks = static_cast<uint32_t>(w.heads + kHeads - 1) / kHeads;
@@ -911,10 +970,37 @@ __global__ __launch_bounds__((64 * W * Shape<T, KD, W, kStates>::kHeads),
 
   float *end = kStates ? r.carried : x.last ? r.final_state : nullptr;
   if (end == nullptr) return;
-  visit(end, kStates ? x.place : x.sequence, false,
-        [&](float &value, const float *at, bool there) {
-          if (there) *const_cast<float *>(at) = value;
-        });
+  if constexpr (kStates || W == 1) {
+    visit(end, kStates ? x.place : x.sequence, false, [&](float &value, const float *at, bool there) {
+      if (there) *const_cast<float *>(at) = value;
+    });
+  } else {
+    // By LDS, as whole rows (2000 sequences of 17 tokens, 8 heads of 64 bfloat16: 154 us,
+    // from the lanes 162).
+    float *z = reinterpret_cast<float *>(s_s);
+    static_assert(S::kS == KD * S::kColumns * 4, "the operands' room is the state's");
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          z[(kb * kFragment + row_of_lane + t * 4 + e) * S::kColumns + column_of_lane -
+            block_column] = state[kb][t][e];
+    head_sync<kThreads>();
+    float *to = end + (x.sequence * w.heads + head) * size + block_column;
+    constexpr int kWide = kWhole ? 4 : 1;  // floats of a store
+    constexpr int kAcross = S::kColumns / kWide;
+    const int column = head_thread<kThreads>() % kAcross * kWide;
+    if (column < width) {
+      for (int row = head_thread<kThreads>() / kAcross; row < dk; row += kThreads / kAcross) {
+        Loose<float, kWide> out;
+#pragma unroll
+        for (int e = 0; e < kWide; ++e) out.v[e] = z[row * S::kColumns + column + e];
+        *reinterpret_cast<Loose<float, kWide> *>(to + row * dv + column) = out;
+      }
+    }
+  }
 }
 
 // One token of every sequence: the state is read, decayed, added to, stored and
@@ -997,17 +1083,16 @@ int64_t blocks_at_once(const Form &f) {
   return 256 * (f.waves == 1 ? 16 : f.waves == 2 ? 8 : f.kd == 64 ? 3 : f.kd == 128 ? 2 : 1);
 }
 
-// Tokens of a span: as many as fill the device once (twice where the sequences'
-// lengths are not known, so that short ones even out the ends: 100k tokens in 512
-// sequences, 3 heads of 33 x 45 float32, 247 us forward and 269), but at least 256, so
-// that a span's own tokens outweigh its states.
+// Tokens of a span: as many as fill the device once, but at least 256, so that a
+// span's own tokens outweigh its states (200k tokens in 512 sequences, 4 heads of 64
+// bfloat16, backward: 306 us, twice as many spans 357; 20k tokens in 40, 8 heads, spans
+// of 128: 126, of 256: 98).
 int64_t span_of(const Sizes &z) {
   const Form f = form_of(z);
   const int64_t blocks = std::max<int64_t>(1, z.heads * ceil_div(std::max(z.dk, z.dv), f.columns()));
   const int64_t longest = z.ragged ? z.n : z.length;
   const int64_t sequences = z.ragged ? 1 : std::max<int64_t>(1, z.sequences);
-  const int64_t spans = std::max<int64_t>(
-      1, (z.ragged ? 2 : 1) * blocks_at_once(f) / (blocks * sequences));
+  const int64_t spans = std::max<int64_t>(1, blocks_at_once(f) / (blocks * sequences));
   const int64_t span = ceil_div(ceil_div(std::max<int64_t>(longest, 1), spans), 64) * 64;
   return std::max<int64_t>(256, span);
 }
@@ -1039,7 +1124,7 @@ Plan plan_of(const Sizes &z) {
 int64_t table_bytes(const Sizes &z, const Plan &p) {
   if (!z.ragged || !p.cut) return 0;
   Carver c(nullptr);
-  c.take<int32_t>(p.items);
+  c.take<int64_t>(p.items);
   c.take<int32_t>(z.sequences + 2);
   return static_cast<int64_t>(align_up(c.used, 256));
 }
@@ -1078,7 +1163,16 @@ int walk(const Sizes &z, const Plan &p, Walk &w, int roles, hipStream_t stream) 
     columns = std::max<int64_t>(columns, ceil_div(w.role[i].dv, f.columns()));
   w.column_blocks = static_cast<int32_t>(columns);
   w.roles = static_cast<uint32_t>(roles);
-  const int64_t blocks = p.items * (f.waves == 1 ? ceil_div(z.heads, 4) : z.heads) * columns * roles;
+  const int64_t heads = f.waves == 1 ? ceil_div(z.heads, 4) : z.heads;
+  int64_t blocks = p.items * heads * columns * roles;
+  w.blocks = static_cast<uint32_t>(blocks);
+  w.together = 0;
+  if (z.ragged) {
+    // All heads of an item, which may share lines; of few items, a head.
+    const int64_t together = columns * roles * (p.items >= 64 ? heads : 1);
+    w.together = static_cast<uint32_t>(together);
+    blocks = together == 0 ? 0 : ceil_div(blocks, 8 * together) * 8 * together;
+  }
   if (blocks > kInt32Max) {
     set_error("decay_attention: %lld blocks exceed 2^31 - 1", static_cast<long long>(blocks));
     return R2S_ERANGE;
@@ -1151,9 +1245,10 @@ int make_items(const Sizes &z, const Plan &p, Cut &cut, void *workspace, size_t 
     return R2S_EWORKSPACE;
   }
   Carver c(workspace);
-  int32_t *owner = c.take<int32_t>(p.items), *first = c.take<int32_t>(z.sequences + 2);
-  decay_items_kernel<<<dim3(1), dim3(1024), 0, stream>>>(cut, p.items, owner, first);
-  cut.owner = owner;
+  int64_t *order = c.take<int64_t>(p.items);
+  int32_t *first = c.take<int32_t>(z.sequences + 2);
+  decay_items_kernel<<<dim3(1), dim3(1024), 0, stream>>>(cut, p.items, order, first);
+  cut.order = order;
   cut.first = first;
   return check_launch("decay_attention items");
 }
