@@ -9,8 +9,10 @@
 // c' = m(v') where c is the mean, else 0.
 //
 // A row is held in registers by 8 to 512 lanes, 16 bytes of each input a lane (more
-// only where a row has over 512 such pieces), so each input is read once and each output written once, and the sums of squares are
-// of differences from the mean that was found first.  The backward makes the
+// only where a row has over 512 such pieces: two to each of 64 lanes took 503 us where
+// one to each of 128 took 216, 32k x 1024 bfloat16 both ways), so each input is read
+// once and each output written once, and the sums of squares are of differences from
+// the mean that was found first.  The backward makes the
 // forward's values again from its inputs, which costs no bytes.  Weights' gradients
 // are sums over rows: a lane group adds its rows, a block its groups, and a second
 // kernel the blocks, always in the same order.  Bound by the bytes.
@@ -149,23 +151,63 @@ struct Row {
   float v[E][V];
 };
 
-template <typename T, int E, bool kWide, int kThreads>
+// Where a lane's vectors are.  Rows are read by whole vectors alone, so that no load
+// waits at the end of a branch for the one before it (32k x 1024 bfloat16, backward:
+// 131 us, with a branch to each 154): the last vector of a row that ends inside it is
+// read from earlier elements on and moved (kTail), and vectors behind the row's end
+// are another's that count for nothing.  Such ends of float32 rows, of three elements
+// at most, are cheaper read by elements (300k x 45, backward: 71 us, moved 94), and so
+// are rows narrower than a vector (kElements).
+enum : int { kWhole = 0, kTail = 1, kElements = 2 };
+template <typename T, int E, bool kWide, int kThreads, int kEnd>
 struct RowOf {
   static constexpr int V = Row<T, E>::V;
   int first[E], count[E];
-  float share;  // 1 / d
+  int start[E];  // where a vector is read from
+  float share;   // 1 / d
   __device__ __forceinline__ RowOf(const Lanes<kWide, kThreads> &lanes, int d) : share(1.0f / d) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       first[e] = ((e << lanes.bits) + lanes.lane) * V;
       count[e] = max(0, min(V, d - first[e]));
+      start[e] = kEnd == kElements ? first[e] : min(first[e], d - V);
     }
   }
   __device__ __forceinline__ void load(const NormInput &in, int64_t row,
                                        Loose<T, V> (&raw)[E]) const {
     const T *p = static_cast<const T *>(in.p) + row * in.stride;
 #pragma unroll
-    for (int e = 0; e < E; ++e) raw[e] = load_row<T, V>(p + first[e], count[e]);
+    for (int e = 0; e < E; ++e) {
+      if constexpr (kEnd == kElements) {
+        raw[e] = load_row<T, V>(p + first[e], count[e]);
+      } else {
+        raw[e] = *reinterpret_cast<const Loose<T, V> *>(p + start[e]);
+      }
+    }
+  }
+  // A loaded row's own elements, and zeros past its end.
+  __device__ __forceinline__ void settle(Loose<T, V> (&raw)[E]) const {
+    if constexpr (kEnd == kElements) return;
+    using Words = __attribute__((ext_vector_type(4))) uint32_t;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      Words x = __builtin_bit_cast(Words, raw[e]);
+      if constexpr (kEnd == kTail) {
+        static_assert(sizeof(T) == 2, "two elements to a word");
+        const int back = first[e] - start[e];  // of the row's last vector
+#pragma unroll
+        for (int words = 2; words > 0; words /= 2)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            x[j] = (back & (2 * words)) != 0 ? (j + words < 4 ? x[j + words] : 0u) : x[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[j] = (back & 1) != 0 ? x[j] >> 16 | (j < 3 ? x[j + 1] << 16 : 0u) : x[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = count[e] > 0 ? x[j] : 0u;
+      raw[e] = __builtin_bit_cast(Loose<T, V>, x);
+    }
   }
   // A weight (ones without one), zeros past the row's end.
   __device__ __forceinline__ void load_weight(const void *w, Row<T, E> &out) const {
@@ -225,13 +267,15 @@ __device__ __forceinline__ void widen(const Loose<T, Row<T, E>::V> (&raw)[E], Ro
     for (int i = 0; i < Row<T, E>::V; ++i) x.v[e][i] = static_cast<float>(raw[e].v[i]);
 }
 
-// 32k x 1024 bf16 and 4k x 64 f32: the figures are those of the backward's comment.
-template <typename T, int E, bool kWide, int kThreads, int kGate>
+// 32k x 1024 bfloat16 with a gate of every row: 335 MB in 56 us (6.0 TB/s, some of it
+// from the last-level cache); 300k x 45 float32 37 us (5.8 TB/s); 4k x 64 float32 4 us,
+// the launch's own.  Bound by the bytes.
+template <typename T, int E, bool kWide, int kThreads, int kGate, int kEnd>
 __global__ __launch_bounds__(kThreads) void residual_norm_fwd_kernel(NormArgs a, int bits) {
   __shared__ float2 s_sums[2 * (kThreads / 64)];
   constexpr int V = Row<T, E>::V;
   Lanes<kWide, kThreads> lanes(bits, s_sums);
-  const RowOf<T, E, kWide, kThreads> at(lanes, a.d);
+  const RowOf<T, E, kWide, kThreads, kEnd> at(lanes, a.d);
   Row<T, E> w1, w2, all;
   at.load_weight(a.w1, w1);
   at.load_weight(a.w2, w2);
@@ -253,6 +297,9 @@ __global__ __launch_bounds__(kThreads) void residual_norm_fwd_kernel(NormArgs a,
     at.load(a.x, r, rx);
     if (a.update.p != nullptr) at.load(a.update, r, rf);
     if constexpr (kGate == kRowGate) at.load(a.gate, r, rg);
+    at.settle(rx);
+    if (a.update.p != nullptr) at.settle(rf);
+    if constexpr (kGate == kRowGate) at.settle(rg);
     Row<T, E> y;
     widen<T, E>(rx, y);
     if (a.update.p != nullptr) {
@@ -282,8 +329,8 @@ __global__ __launch_bounds__(kThreads) void residual_norm_fwd_kernel(NormArgs a,
 }
 
 // A block's sum of its groups' `sums`, into its part.
-template <typename T, int E, bool kWide, int kThreads>
-__device__ __forceinline__ void store_part(const RowOf<T, E, kWide, kThreads> &at, int bits, int d,
+template <typename T, int E, bool kWide, int kThreads, int kEnd>
+__device__ __forceinline__ void store_part(const RowOf<T, E, kWide, kThreads, kEnd> &at, int bits, int d,
                                            const Row<T, E> &sums, float *s_row, float *part) {
   constexpr int V = Row<T, E>::V;
   const int groups = kThreads >> bits;
@@ -303,14 +350,19 @@ __device__ __forceinline__ void store_part(const RowOf<T, E, kWide, kThreads> &a
   }
 }
 
-template <typename T, int E, bool kWide, int kThreads, int kGate>
+// 32k x 1024 bfloat16 with a gate of every row: 537 MB in 116 to 131 us (4.1 to 4.6
+// TB/s); 300k x 45 float32 71 us (4.6 TB/s).  Between a row's loads and its stores lie
+// four sums over its lanes in turn; with 16-bit rows' eight elements to a lane three
+// waves of a SIMD are what the registers hold to cover them (eight waves of four
+// elements: 234 us against 154).
+template <typename T, int E, bool kWide, int kThreads, int kGate, int kEnd>
 __global__ __launch_bounds__(kThreads, E > 1 ? 2 : sizeof(T) == 2 ? 3 : 4) void
 residual_norm_bwd_kernel(NormArgs a, int bits) {
   __shared__ float2 s_sums[2 * (kThreads / 64)];
   extern __shared__ float s_row[];  // [groups][d], of several groups
   constexpr int V = Row<T, E>::V;
   Lanes<kWide, kThreads> lanes(bits, s_sums);
-  const RowOf<T, E, kWide, kThreads> at(lanes, a.d);
+  const RowOf<T, E, kWide, kThreads, kEnd> at(lanes, a.d);
   const bool centered = a.centered != 0, update = a.update.p != nullptr;
   Row<T, E> w1, w2, all, v_w1{}, v_w2{}, v_all{};
   at.load_weight(a.w1, w1);
@@ -328,6 +380,11 @@ residual_norm_bwd_kernel(NormArgs a, int bits) {
     if constexpr (kGate == kRowGate) at.load(a.gate, r, rg);
     if (a.v_u.p != nullptr) at.load(a.v_u, r, ru);
     if (a.v_y.p != nullptr) at.load(a.v_y, r, ry);
+    at.settle(rx);
+    if (update) at.settle(rf);
+    if constexpr (kGate == kRowGate) at.settle(rg);
+    if (a.v_u.p != nullptr) at.settle(ru);
+    if (a.v_y.p != nullptr) at.settle(ry);
     Row<T, E> z, h;
     widen<T, E>(rx, z);
     float h_factor = 1.0f;
@@ -423,10 +480,10 @@ residual_norm_bwd_kernel(NormArgs a, int bits) {
     if (some && a.v_update != nullptr) at.store(a.v_update, r, a.d, v);
   }
   float *part = a.parts + static_cast<int64_t>(blockIdx.x) * 3 * a.d;
-  if (a.want_w1 != 0) store_part<T, E, kWide, kThreads>(at, bits, a.d, v_w1, s_row, part);
-  if (a.want_w2 != 0) store_part<T, E, kWide, kThreads>(at, bits, a.d, v_w2, s_row, part + a.d);
+  if (a.want_w1 != 0) store_part<T, E, kWide, kThreads, kEnd>(at, bits, a.d, v_w1, s_row, part);
+  if (a.want_w2 != 0) store_part<T, E, kWide, kThreads, kEnd>(at, bits, a.d, v_w2, s_row, part + a.d);
   if constexpr (kGate == kChannelGate)
-    if (a.want_gate != 0) store_part<T, E, kWide, kThreads>(at, bits, a.d, v_all, s_row, part + 2 * a.d);
+    if (a.want_gate != 0) store_part<T, E, kWide, kThreads, kEnd>(at, bits, a.d, v_all, s_row, part + 2 * a.d);
 }
 
 // The blocks' parts of up to three sums, 64 columns of one sum to a block, 16
@@ -468,32 +525,47 @@ int norm_threads(const NormForm &f) { return f.bits > 8 ? 512 : 256; }
 int64_t norm_blocks(int64_t n, const NormForm &f, int64_t most) {
   return std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(n, norm_threads(f) >> f.bits)));
 }
-// Blocks of the backward: six to a CU while their parts of the sums are few bytes
-// beside the rows, then three, then two.
+// Blocks of the backward: as many as a CU's registers hold at once, five (300k x 44
+// float32: 68 us, six 83) while their parts of the sums are few bytes beside the rows,
+// then three, then two.
 int64_t norm_parts(int64_t n, int64_t d, const NormForm &f) {
-  return norm_blocks(n, f, d <= 512 ? 1536 : d <= 1024 ? 768 : 512);
+  return norm_blocks(n, f, d <= 512 ? 1280 : d <= 1024 ? 768 : 512);
 }
 
-template <typename T, bool kBack, int E, bool kWide, int kThreads, int kGate>
+template <typename T, bool kBack, int E, bool kWide, int kThreads, int kGate, int kEnd>
 void launch_norm_gate(const NormArgs &a, const NormForm &f, int64_t blocks, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
   if constexpr (kBack) {
     const int groups = kThreads >> f.bits;
     const size_t lds = groups > 1 ? static_cast<size_t>(groups) * a.d * sizeof(float) : 0;
-    residual_norm_bwd_kernel<T, E, kWide, kThreads, kGate><<<grid, block, lds, stream>>>(a, f.bits);
+    residual_norm_bwd_kernel<T, E, kWide, kThreads, kGate, kEnd><<<grid, block, lds, stream>>>(a, f.bits);
   } else {
-    residual_norm_fwd_kernel<T, E, kWide, kThreads, kGate><<<grid, block, 0, stream>>>(a, f.bits);
+    residual_norm_fwd_kernel<T, E, kWide, kThreads, kGate, kEnd><<<grid, block, 0, stream>>>(a, f.bits);
   }
+}
+template <typename T, bool kBack, int E, bool kWide, int kThreads, int kEnd>
+int launch_norm_gates(const NormArgs &a, const NormForm &f, int64_t blocks, hipStream_t stream) {
+  if (a.gate_kind == kRowGate)
+    launch_norm_gate<T, kBack, E, kWide, kThreads, kRowGate, kEnd>(a, f, blocks, stream);
+  else if (a.gate_kind == kChannelGate)
+    launch_norm_gate<T, kBack, E, kWide, kThreads, kChannelGate, kEnd>(a, f, blocks, stream);
+  else
+    launch_norm_gate<T, kBack, E, kWide, kThreads, kNoGate, kEnd>(a, f, blocks, stream);
+  return check_launch("residual_norm");
 }
 template <typename T, bool kBack, int E, bool kWide, int kThreads>
 int launch_norm_as(const NormArgs &a, const NormForm &f, int64_t blocks, hipStream_t stream) {
-  if (a.gate_kind == kRowGate)
-    launch_norm_gate<T, kBack, E, kWide, kThreads, kRowGate>(a, f, blocks, stream);
-  else if (a.gate_kind == kChannelGate)
-    launch_norm_gate<T, kBack, E, kWide, kThreads, kChannelGate>(a, f, blocks, stream);
-  else
-    launch_norm_gate<T, kBack, E, kWide, kThreads, kNoGate>(a, f, blocks, stream);
-  return check_launch("residual_norm");
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  if (a.d % V == 0)
+    return launch_norm_gates<T, kBack, E, kWide, kThreads, kWhole>(a, f, blocks, stream);
+  if constexpr (sizeof(T) == 4) {
+    return launch_norm_gates<T, kBack, E, kWide, kThreads, kElements>(a, f, blocks, stream);
+  } else {
+    if constexpr (!kWide)
+      if (a.d < V)
+        return launch_norm_gates<T, kBack, E, kWide, kThreads, kElements>(a, f, blocks, stream);
+    return launch_norm_gates<T, kBack, E, kWide, kThreads, kTail>(a, f, blocks, stream);
+  }
 }
 template <typename T, bool kBack>
 int launch_norm(const NormArgs &a, const NormForm &f, int64_t blocks, hipStream_t stream) {
