@@ -164,6 +164,8 @@ assert _ENTRY.size == ctypes.sizeof(L.AdamwTensor)
 # The names of states in 32 bits, and in 8 with the scales of each run.
 _STATE_32 = ("exp_avg", "exp_avg_sq")
 _STATE_8 = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
+_WANTED_32 = ("master", *_STATE_32, None, None)
+_WANTED_8 = ("master", *_STATE_8[::2], *_STATE_8[1::2])
 
 
 class AdamW(torch.optim.Optimizer):
@@ -218,54 +220,26 @@ class AdamW(torch.optim.Optimizer):
                 state[name] = torch.zeros_like(p, dtype=torch.float32)
 
     @staticmethod
-    def _state_tensors(p: torch.Tensor, state: dict) -> tuple:
+    def _state_tensors(p: torch.Tensor, state: dict, n: int) -> tuple:
         """(master, average, second, their scales), None for those that are not
-        there, checked: the kernel takes their addresses."""
-        runs, n = (-(-p.numel() // _RUN),), p.shape
-        wanted = [("master", n, torch.float32) if p.dtype != torch.float32 else None]
+        there, checked at every step: the kernel takes their addresses."""
+        device, f32 = p.get_device(), torch.float32
         if "exp_avg_sq_root" in state:
-            wanted += [(name, n, torch.float8_e4m3fn) for name in _STATE_8[::2]]
-            wanted += [(name, runs, torch.float32) for name in _STATE_8[1::2]]
+            wanted, kinds, runs = _WANTED_8, torch.float8_e4m3fn, -(-n // _RUN)
         else:
-            wanted += [(name, n, torch.float32) for name in _STATE_32] + [None, None]
+            wanted, kinds, runs = _WANTED_32, f32, None
         out = []
-        for want in wanted:
-            t = None
-            if want is not None:
-                name, shape, dtype = want
-                t = state.get(name)
-                if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype \
-                        or t.device != p.device or not t.is_contiguous():
-                    raise RuntimeError(f"AdamW state {name!r} does not match its parameter")
+        for name in wanted:
+            if name is None or (name == "master" and p.dtype is f32):
+                out.append(None)
+                continue
+            t, scale = state.get(name), name.endswith("_scale")
+            if not isinstance(t, torch.Tensor) or t.get_device() != device \
+                    or t.dtype is not (kinds if name != "master" and not scale else f32) \
+                    or t.numel() != (runs if scale else n) or not t.is_contiguous():
+                raise RuntimeError(f"AdamW state {name!r} does not match its parameter")
             out.append(t)
-        return tuple(out)
-
-    def _checked(self, p: torch.Tensor, state: dict, seen: dict) -> tuple:
-        """(element type, the state's tensors) of a parameter that the kernel may
-        step.  What was found for the very same tensor objects at an earlier step is
-        not looked up again but for their sizes: that was most of a step's host time."""
-        before = seen.get(p)
-        if before is not None:
-            kind, names, tensors = before
-            n, runs = p.numel(), -(-p.numel() // _RUN)
-            for name, t, per in zip(names, tensors, (n, n, n, runs, runs)):
-                if t is not None and (state.get(name) is not t or t.numel() != per
-                                      or not t.is_contiguous()):
-                    break
-            else:
-                if p.is_contiguous():
-                    return kind, tensors
-        kind = _PARAM_TYPES.get(p.dtype)
-        if kind is None or not p.is_cuda:
-            raise NotImplementedError("the fused AdamW step needs float32, bfloat16 or float16 "
-                                      "CUDA parameters")
-        if not p.is_contiguous():
-            raise NotImplementedError("the fused AdamW step needs contiguous parameters")
-        second = "exp_avg_sq_root" if "exp_avg_sq_root" in state else "exp_avg_sq"
-        names = ("master", "exp_avg", second, "exp_avg_scale", "exp_avg_sq_root_scale")
-        tensors = self._state_tensors(p, state)
-        seen[p] = kind, names, tensors
-        return kind, tensors
+        return out
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -273,7 +247,6 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        seen = self.__dict__.setdefault("_seen", {})
         work: dict = {}  # device -> (packed entries, gradients kept until the launch)
         for group in self.param_groups:
             _check_options(group, ())
@@ -300,7 +273,14 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     self._new_state(p, group["state_bits"])
-                kind, (master, mean, second, scale, second_scale) = self._checked(p, state, seen)
+                kind = _PARAM_TYPES.get(p.dtype)
+                if kind is None or not p.is_cuda:
+                    raise NotImplementedError("the fused AdamW step needs float32, bfloat16 or "
+                                              "float16 CUDA parameters")
+                if not p.is_contiguous():
+                    raise NotImplementedError("the fused AdamW step needs contiguous parameters")
+                n = p.numel()
+                master, mean, second, scale, second_scale = self._state_tensors(p, state, n)
                 if not grad.is_contiguous():
                     grad = grad.contiguous()
                 state["step"] = step = int(state["step"]) + 1
@@ -310,7 +290,7 @@ class AdamW(torch.optim.Optimizer):
                 entries.append(_ENTRY.pack(
                     p.data_ptr(), grad.data_ptr(), 0 if master is None else master.data_ptr(),
                     mean.data_ptr(), second.data_ptr(), 0 if scale is None else scale.data_ptr(),
-                    0 if second_scale is None else second_scale.data_ptr(), p.numel(), *fixed,
+                    0 if second_scale is None else second_scale.data_ptr(), n, *fixed,
                     *scalars, kind, step & 0xFFFFFFFF))
                 kept.append(grad)
         lib = _backend.library() if work else None
@@ -328,7 +308,6 @@ class AdamW(torch.optim.Optimizer):
         """torch's, with the states in the types that they were saved in (torch
         casts them to their parameters')."""
         super().load_state_dict(state_dict)
-        self.__dict__.pop("_seen", None)
         saved = state_dict["state"]
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]

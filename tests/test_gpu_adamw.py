@@ -239,3 +239,30 @@ def test_refusals():
         q.grad = torch.ones_like(q)
         with pytest.raises(NotImplementedError, match=kind):
             optim.AdamW([q]).step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_changed_after_a_step(bits):
+    """The same parameter object with other memory behind it: another address is
+    followed, another type or device refused before anything is launched."""
+    p = torch.nn.Parameter(torch.ones(8192, device="cuda"))
+    optimizer = optim.AdamW([p], lr=1e-2, state_bits=bits)
+    p.grad = torch.ones_like(p)
+    optimizer.step()
+    before, old = p.detach().clone(), p.data
+    p.data = old.clone()
+    optimizer.step()
+    assert torch.equal(old, before) and bool((p < before).all())
+    p.data = p.data.half()
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="master"):
+        optimizer.step()
+    p.data = p.data.float().cpu()
+    p.grad = torch.ones_like(p)
+    with pytest.raises(NotImplementedError):
+        optimizer.step()
+    p.data = old
+    p.grad = torch.ones_like(p)
+    optimizer.state[p]["exp_avg"].data = torch.zeros(4096, device="cuda")
+    with pytest.raises(RuntimeError, match="exp_avg"):
+        optimizer.step()
