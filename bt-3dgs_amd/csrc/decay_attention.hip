@@ -82,11 +82,13 @@ constexpr int kRoles = 3;
 // How the sequences are cut.
 struct Cut {
   const int32_t *offsets;  // ragged
-  const int64_t *order;    // ragged, several spans: items as they are taken, see below
+  const int32_t *order;    // ragged, several spans: items as they are taken, see below
+  const int32_t *index;    // [wholes], the span of the first of them, -1: the last
   const int32_t *first;    // and each sequence's first item, as places are counted
   int64_t n, sequences, length, span;
   int64_t carried;  // places for states between spans
   int32_t spans;    // of an equal sequence
+  int32_t wholes;   // spans that ragged sequences may fill at most
 };
 
 struct Walk {
@@ -123,12 +125,12 @@ __device__ __forceinline__ bool find_span(const Cut &c, int64_t item, Span &x) {
     place = sequence * (items - 1) + index;
   } else {
     if (c.order != nullptr) {
-      const int64_t which = c.order[item];
-      if (which < 0) return false;
-      sequence = which >> 32;
-      index = which & 0xFFFFFFFF;
+      sequence = c.order[item];
+      if (sequence < 0) return false;
+      index = item < c.wholes ? c.index[item] : -1;
       const int64_t first = c.first[sequence];
       items = c.first[sequence + 1] - first;
+      if (index < 0) index = max(items - 1, int64_t{0});  // offsets may be anything
       place = first + index - sequence;  // each sequence before has an item without a place
     }
     lo = bound(c, sequence);
@@ -148,15 +150,16 @@ __device__ __forceinline__ bool find_span(const Cut &c, int64_t item, Span &x) {
          (x.first || (place > 0 && place <= c.carried));
 }
 
-// The items of ragged sequences, a sequence and the index of its span to each (the
-// upper and the lower half): every sequence's spans, at least one, those of the
-// tokens behind the last, and -1 for places left over.  The longest come first, in classes of an
-// eighth of a span: with short ones last, the device runs dry all at once (100k
-// tokens in 512 sequences, 3 heads of 33 x 45 float32: forward 166 us, in the order of
-// the sequences and in equal shares to the XCDs 231).
-constexpr uint32_t kClasses = 8;
+// The items of ragged sequences: every sequence's spans, at least one, those of the
+// tokens behind the last, and -1 for places left over.  Whole spans come first, then
+// each sequence's rest, the longest first in classes of an eighth of a span: with
+// short ones last, the device runs dry all at once (100k tokens in 512 sequences, 3
+// heads of 33 x 45 float32: forward 166 us, in the order of the sequences and in equal
+// shares to the XCDs 231).
+constexpr uint32_t kEighths = 8, kClasses = 1 + kEighths;
 __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
-                                                           int64_t *__restrict__ order,
+                                                           int32_t *__restrict__ order,
+                                                           int32_t *__restrict__ index,
                                                            int32_t *__restrict__ first) {
   __shared__ int64_t s_total[16];
   __shared__ unsigned long long s_next[kClasses];  // offsets that do not ascend add up to much
@@ -168,7 +171,7 @@ __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
   };
   // Of the tokens behind a sequence's whole spans, if there are any.
   auto class_of = [&](int64_t rest) {
-    return kClasses - 1 - static_cast<uint32_t>((rest * kClasses - 1) / c.span);
+    return kEighths - static_cast<uint32_t>((rest * kEighths - 1) / c.span);
   };
   int64_t before = 0;
   for (int64_t s0 = 0; s0 <= c.sequences; s0 += 1024) {
@@ -207,8 +210,9 @@ __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
     }
   }
   __syncthreads();
-  auto put = [&](int64_t at, int64_t s, int64_t index) {
-    if (at < most) order[at] = s << 32 | index;
+  auto put = [&](int64_t at, int64_t s, int64_t span) {
+    if (at < most) order[at] = static_cast<int32_t>(s);
+    if (at < min(most, static_cast<int64_t>(c.wholes))) index[at] = static_cast<int32_t>(span);
   };
   for (int64_t s0 = 0; s0 <= c.sequences; s0 += 1024) {
     const int64_t s = s0 + threadIdx.x;
@@ -217,8 +221,8 @@ __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,
       const int64_t tokens = tokens_of(s), rest = tokens - tokens / c.span * c.span;
       whole = tokens / c.span;
       if (whole > 0) at = atomicAdd(&s_next[0], static_cast<unsigned long long>(whole));
-      if (rest > 0) put(atomicAdd(&s_next[class_of(rest)], 1ull), s, whole);
-      if (s < c.sequences && tokens == 0) put(atomicAdd(&s_next[kClasses - 1], 1ull), s, 0);
+      if (rest > 0) put(atomicAdd(&s_next[class_of(rest)], 1ull), s, -1);
+      if (s < c.sequences && tokens == 0) put(atomicAdd(&s_next[kClasses - 1], 1ull), s, -1);
     }
     for (uint64_t some = ballot(whole > 0); some != 0; some &= some - 1) {
       const uint32_t from = static_cast<uint32_t>(__builtin_ctzll(some));
@@ -1135,7 +1139,8 @@ Plan plan_of(const Sizes &z) {
 int64_t table_bytes(const Sizes &z, const Plan &p) {
   if (!z.ragged || !p.cut) return 0;
   Carver c(nullptr);
-  c.take<int64_t>(p.items);
+  c.take<int32_t>(p.items);
+  c.take<int32_t>(p.carried);
   c.take<int32_t>(z.sequences + 2);
   return static_cast<int64_t>(align_up(c.used, 256));
 }
@@ -1256,10 +1261,12 @@ int make_items(const Sizes &z, const Plan &p, Cut &cut, void *workspace, size_t 
     return R2S_EWORKSPACE;
   }
   Carver c(workspace);
-  int64_t *order = c.take<int64_t>(p.items);
+  int32_t *order = c.take<int32_t>(p.items), *index = c.take<int32_t>(p.carried);
   int32_t *first = c.take<int32_t>(z.sequences + 2);
-  decay_items_kernel<<<dim3(1), dim3(1024), 0, stream>>>(cut, p.items, order, first);
+  cut.wholes = static_cast<int32_t>(p.carried);
+  decay_items_kernel<<<dim3(1), dim3(1024), 0, stream>>>(cut, p.items, order, index, first);
   cut.order = order;
+  cut.index = index;
   cut.first = first;
   return check_launch("decay_attention items");
 }
