@@ -154,7 +154,7 @@ __device__ __forceinline__ bool find_span(const Cut &c, int64_t item, Span &x) {
 // tokens behind the last, and -1 for places left over.  Whole spans come first, then
 // each sequence's rest, the longest first in classes of an eighth of a span: with
 // short ones last, the device runs dry all at once (100k tokens in 512 sequences, 3
-// heads of 33 x 45 float32: forward 166 us, in the order of the sequences and in equal
+// heads of 33 x 45 float32: forward 166 to 174 us, in the order of the sequences and in equal
 // shares to the XCDs 231).
 constexpr uint32_t kEighths = 8, kClasses = 1 + kEighths;
 __global__ __launch_bounds__(1024) void decay_items_kernel(Cut c, int64_t most,

@@ -442,3 +442,26 @@ def test_refusals():
     y, final, kept = W.decay_attention_fwd(q, q, v, g.detach())
     with pytest.raises(RuntimeError, match="kept"):
         W.decay_attention_bwd(q, q, v, g.detach(), None, None, state, v)
+
+
+@pytest.mark.parametrize("lengths", [
+    [0, 1, 255, 256, 257, 40, 600, 128] * 6,   # whole spans and rests of every eighth
+    [0, 1, 3, 2, 0, 5] * 250 + [700, 0],       # more sequences than a block has threads
+    [700, 3]], ids=["mixed", "many", "few"])
+@pytest.mark.parametrize("heads,dk,dv,dtype", [(5, 16, 16, torch.bfloat16),
+                                               (3, 33, 45, torch.float32),
+                                               (2, 64, 64, torch.float16)])
+def test_ragged_spans_taken_out_of_order(lengths, heads, dk, dv, dtype):
+    bounds = np.cumsum([0] + lengths).tolist()
+    case = _case(bounds[-1] + 7, heads, dk, dv, len(lengths), dtype, len(lengths) + dk)
+    exact = tuple(None if t is None else t[:bounds[-1]] if t.shape[0] == bounds[-1] + 7 else t
+                  for t in case)
+    got = _check(exact, bounds, True, dtype, True)
+    # Tokens behind the last sequence change nothing and get zeros.
+    q, k, v, log_decay, state, v_y, v_final = (t.to(DEV) for t in case)
+    offsets = torch.tensor(bounds, dtype=torch.int32, device=DEV)
+    y, final, kept = W.decay_attention_fwd(q, k, v, log_decay, state, offsets, True, 0.3)
+    grads = W.decay_attention_bwd(q, k, v, log_decay, state, offsets, kept, v_y, v_final, True, 0.3)
+    for a, b in zip(got, (y, final, *grads)):
+        assert torch.equal(a, b[:a.shape[0]])
+        assert not bool(b[a.shape[0]:].any())
