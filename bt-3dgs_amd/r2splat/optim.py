@@ -205,9 +205,9 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             _check_options(group, ())
 
-    def _new_state(self, p: torch.Tensor, bits: int) -> None:
-        state = self.state[p]
-        state["step"] = 0
+    @staticmethod
+    def _new_state(p: torch.Tensor, bits: int) -> dict:
+        state = {"step": 0}
         if p.dtype != torch.float32:
             state["master"] = p.detach().float()
         if bits == 8 and p.numel() >= _FEWEST_8BIT:
@@ -218,6 +218,7 @@ class AdamW(torch.optim.Optimizer):
         else:
             for name in _STATE_32:
                 state[name] = torch.zeros_like(p, dtype=torch.float32)
+        return state
 
     @staticmethod
     def _state_tensors(p: torch.Tensor, state: dict, n: int) -> tuple:
@@ -247,7 +248,9 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work: dict = {}  # device -> (packed entries, gradients kept until the launch)
+        # device -> (packed entries, gradients kept until the launch, what it counts).
+        # Nothing of the optimizer changes before every parameter has been looked over.
+        work: dict = {}
         for group in self.param_groups:
             _check_options(group, ())
             lr, (beta1, beta2) = group["lr"], group["betas"]
@@ -268,22 +271,20 @@ class AdamW(torch.optim.Optimizer):
                         with _ops._on(device):
                             if torch.cuda.is_current_stream_capturing():
                                 raise RuntimeError("AdamW.step cannot be captured into a graph")
-                    work[device] = [], []
-                entries, kept = work[device]
-                state = self.state[p]
-                if not state:
-                    self._new_state(p, group["state_bits"])
+                    work[device] = [], [], []
+                entries, kept, counted = work[device]
                 kind = _PARAM_TYPES.get(p.dtype)
                 if kind is None or not p.is_cuda:
                     raise NotImplementedError("the fused AdamW step needs float32, bfloat16 or "
                                               "float16 CUDA parameters")
                 if not p.is_contiguous():
                     raise NotImplementedError("the fused AdamW step needs contiguous parameters")
+                state = self.state.get(p) or self._new_state(p, group["state_bits"])
                 n = p.numel()
                 master, mean, second, scale, second_scale = self._state_tensors(p, state, n)
                 if not grad.is_contiguous():
                     grad = grad.contiguous()
-                state["step"] = step = int(state["step"]) + 1
+                step = int(state["step"]) + 1
                 if step != last:
                     last, scalars = step, ((1 - beta2 ** step) ** 0.5, eps,
                                            -lr / (1 - beta1 ** step))
@@ -293,14 +294,18 @@ class AdamW(torch.optim.Optimizer):
                     0 if second_scale is None else second_scale.data_ptr(), n, *fixed,
                     *scalars, kind, step & 0xFFFFFFFF))
                 kept.append(grad)
+                counted.append((p, state, step))
         lib = _backend.library() if work else None
-        for device, (entries, _) in work.items():
+        for device, (entries, _, counted) in work.items():
             table = b"".join(entries)
             with _ops._on(device):
                 rc = lib.r2s_adamw_step(table, len(entries), _ops._stream(device))
             if rc != 0:
                 raise RuntimeError(f"r2s_adamw_step failed ({rc}): "
                                    f"{lib.r2s_last_error().decode(errors='replace')}")
+            for p, state, step in counted:
+                state["step"] = step
+                self.state[p] = state
         return loss
 
     @torch.no_grad()

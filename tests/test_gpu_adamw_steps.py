@@ -1,0 +1,71 @@
+"""AdamW on the GPU: steps that are refused, and what they leave as it was."""
+
+import pytest
+import torch
+
+from r2splat import optim
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _held(opt):
+    """Every state's values, by parameter."""
+    return [{name: t.clone() if isinstance(t, torch.Tensor) else t
+             for name, t in opt.state.get(p, {}).items()}
+            for group in opt.param_groups for p in group["params"]]
+
+
+def _same(a, b):
+    bits = lambda t: t.view(torch.uint8) if t.element_size() == 1 else t  # noqa: E731
+    return len(a) == len(b) and all(
+        x.keys() == y.keys() and all(
+            torch.equal(bits(x[k]), bits(y[k])) if isinstance(x[k], torch.Tensor) else x[k] == y[k]
+            for k in x)
+        for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_refused_step_leaves_counts_states_and_parameters(dtype, bits):
+    """A later parameter is refused: the earlier ones, with and without a state, are
+    as they were, and going on after the mend is as if the step had not been tried."""
+    def make():
+        ps = [torch.full((n,), 0.5, device=DEV).to(dtype).requires_grad_(True)
+              for n in (6000, 50, 6000, 7)]
+        return ps, optim.AdamW([dict(params=ps[:2]), dict(params=ps[2:], lr=1e-2)],
+                               state_bits=bits)
+
+    (ps, opt), (others, other) = make(), make()
+    for qs, o in ((ps, opt), (others, other)):
+        for q in qs[::2]:
+            q.grad = torch.ones_like(q)
+        o.step()
+        for q in qs:  # two have no state yet
+            q.grad = torch.full_like(q, 0.25)
+    before, values = _held(opt), [p.detach().clone() for p in ps]
+    assert [bool(s) for s in before] == [True, False, True, False]
+
+    def refused(error, match):
+        with pytest.raises(error, match=match):
+            opt.step()
+        assert _same(_held(opt), before)
+        assert len(opt.state) == 2
+        assert all(torch.equal(p, v) for p, v in zip(ps, values))
+
+    good, ps[3].grad = ps[3].grad, None
+    ps[3].grad = torch.sparse_coo_tensor([[1]], [1.0], (7,), device=DEV).to(dtype)
+    refused(RuntimeError, "sparse")
+    ps[3].grad = good
+    opt.param_groups[1]["eps"] = torch.tensor(1e-8)
+    refused(NotImplementedError, "float eps")
+    opt.param_groups[1]["eps"] = 1e-8
+    kept = opt.state[ps[2]]["exp_avg"]
+    opt.state[ps[2]]["exp_avg"] = before[2]["exp_avg"] = kept[:10]
+    refused(RuntimeError, "'exp_avg' does not match")
+    opt.state[ps[2]]["exp_avg"] = kept
+    for o in (opt, other):
+        o.step()
+    assert _same(_held(opt), _held(other))
+    assert all(torch.equal(p, q) for p, q in zip(ps, others))
+    assert [opt.state[p]["step"] for p in ps] == [2, 1, 2, 1]
