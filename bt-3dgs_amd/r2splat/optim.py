@@ -168,6 +168,19 @@ _WANTED_32 = ("master", *_STATE_32, None, None)
 _WANTED_8 = ("master", *_STATE_8[::2], *_STATE_8[1::2])
 
 
+def _check_bits(bits) -> None:
+    if bits not in (8, 32):
+        raise ValueError(f"state_bits must be 8 or 32, got {bits}")
+
+
+def _check_adamw_group(group: dict) -> None:
+    _check_options(group, ("amsgrad", "maximize", "capturable", "differentiable"))
+    if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+        raise NotImplementedError("the fused AdamW step does not support "
+                                  "decoupled_weight_decay=False")
+    _check_bits(group["state_bits"])
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` over float32, bfloat16 and float16 CUDA parameters
     (gradients of their type), one launch for every 32 tensors of a device.
@@ -189,8 +202,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                  state_bits=32):
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        _check_bits(state_bits)
         if not isinstance(lr, torch.Tensor) and lr < 0.0:
             raise ValueError(f"Invalid learning rate: {lr}")
         if not isinstance(eps, torch.Tensor) and eps < 0.0:
@@ -202,8 +214,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"Invalid weight_decay value: {weight_decay}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                                       state_bits=state_bits))
-        for group in self.param_groups:
-            _check_options(group, ())
+
+    def add_param_group(self, param_group: dict) -> None:
+        _check_adamw_group({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     @staticmethod
     def _new_state(p: torch.Tensor, bits: int) -> dict:
@@ -252,7 +266,7 @@ class AdamW(torch.optim.Optimizer):
         # Nothing of the optimizer changes before every parameter has been looked over.
         work: dict = {}
         for group in self.param_groups:
-            _check_options(group, ())
+            _check_adamw_group(group)
             lr, (beta1, beta2) = group["lr"], group["betas"]
             fixed = beta1, 1 - beta1, beta2, 1 - beta2, 1 - lr * group["weight_decay"]
             eps = group["eps"]
@@ -311,7 +325,14 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """torch's, with the states in the types that they were saved in (torch
-        casts them to their parameters')."""
+        casts them to their parameters').  Groups saved by torch's AdamW keep the
+        ``state_bits`` that they have here; what the step does not do is refused."""
+        groups = [{"state_bits": own["state_bits"], **group}
+                  for own, group in zip(self.param_groups, state_dict["param_groups"])]
+        if len(groups) == len(state_dict["param_groups"]):  # else torch refuses it
+            for group in groups:
+                _check_adamw_group(group)
+            state_dict = {**state_dict, "param_groups": groups}
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
