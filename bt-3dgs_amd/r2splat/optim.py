@@ -327,17 +327,30 @@ class AdamW(torch.optim.Optimizer):
         """torch's, with the states in the types that they were saved in (torch
         casts them to their parameters').  Groups saved by torch's AdamW keep the
         ``state_bits`` that they have here; what the step does not do is refused."""
-        groups = [{"state_bits": own["state_bits"], **group}
-                  for own, group in zip(self.param_groups, state_dict["param_groups"])]
-        if len(groups) == len(state_dict["param_groups"]):  # else torch refuses it
-            for group in groups:
-                _check_adamw_group(group)
-            state_dict = {**state_dict, "param_groups": groups}
-        super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(ids, params):
-            for name, t in saved.get(i, {}).items():
-                if name != "step" and isinstance(t, torch.Tensor):
-                    self.state[p][name] = t.detach().to(p.device, copy=True).contiguous()
+        given: dict = {}
+
+        def settle(_, state_dict):  # behind the caller's hooks
+            groups = [{"state_bits": own["state_bits"], **group}
+                      for own, group in zip(self.param_groups, state_dict["param_groups"])]
+            if len(groups) == len(state_dict["param_groups"]):  # else torch refuses it
+                for group in groups:
+                    _check_adamw_group(group)
+                state_dict = {**state_dict, "param_groups": groups}
+            given.update(state_dict)
+            return state_dict
+
+        def restore(_):  # and before theirs
+            ids = [i for group in given["param_groups"] for i in group["params"]]
+            params = [p for group in self.param_groups for p in group["params"]]
+            for i, p in zip(ids, params):
+                for name, t in given["state"].get(i, {}).items():
+                    if name != "step" and isinstance(t, torch.Tensor):
+                        self.state[p][name] = t.detach().to(p.device, copy=True).contiguous()
+
+        hooks = (self.register_load_state_dict_pre_hook(settle),
+                 self.register_load_state_dict_post_hook(restore, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()

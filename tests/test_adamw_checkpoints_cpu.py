@@ -91,3 +91,59 @@ def test_bits_of_a_group():
         opt.load_state_dict(checkpoint)
     opt.add_param_group({"params": [p], "state_bits": 8})
     assert [g["state_bits"] for g in opt.param_groups] == [32, 8]
+
+
+def test_hooks_of_loading_see_and_change_what_is_loaded():
+    ps, opt = _mine()
+    seen = []
+
+    def half(optimizer, state_dict):
+        """The caller's own change, in a dictionary of its own."""
+        states = {i: {k: t * 0.5 if k == "exp_avg" else t for k, t in s.items()}
+                  for i, s in state_dict["state"].items()}
+        groups = [{**g, "lr": 7.0} for g in state_dict["param_groups"]]
+        return {**state_dict, "state": states, "param_groups": groups}
+
+    opt.register_load_state_dict_pre_hook(half)
+    opt.register_load_state_dict_post_hook(
+        lambda optimizer: seen.append({p: dict(s) for p, s in optimizer.state.items()}))
+    checkpoint = _torch_checkpoint(second=True)
+    wanted = {i: s["exp_avg"].clone() * 0.5 for i, s in checkpoint["state"].items()}
+    for times in (1, 2):  # nothing of a load stays behind for the next
+        opt.load_state_dict(checkpoint)
+        assert opt.param_groups[0]["lr"] == 7.0
+        for i, p in enumerate(ps):
+            assert torch.equal(opt.state[p]["exp_avg"], wanted[i])
+            assert opt.state[p]["exp_avg"] is seen[-1][p]["exp_avg"]
+        assert len(seen) == times
+
+    def bad(optimizer, state_dict):
+        state_dict["param_groups"] = [{**g, "maximize": True} for g in state_dict["param_groups"]]
+
+    handle = opt.register_load_state_dict_pre_hook(bad)
+    with pytest.raises(NotImplementedError, match="maximize"):
+        opt.load_state_dict(checkpoint)
+    handle.remove()
+    opt.load_state_dict(checkpoint)
+    assert len(seen) == 3 and not checkpoint["param_groups"][0]["maximize"]
+
+
+def test_post_hooks_see_the_types_that_were_saved():
+    """A 16-bit parameter's states are float32, before and after the hooks."""
+    def make():
+        p = torch.nn.Parameter(torch.ones(4, dtype=torch.bfloat16))
+        return p, optim.AdamW([p])
+
+    p, opt = make()
+    saved = opt.state_dict()
+    saved["state"] = {0: {"step": 3, "master": torch.full((4,), 1 + 2.0 ** -12),
+                          "exp_avg": torch.full((4,), 2.0 ** -20 + 1),
+                          "exp_avg_sq": torch.full((4,), 0.5)}}
+    q, other = make()
+    types = []
+    other.register_load_state_dict_post_hook(
+        lambda o: types.extend((k, t.dtype) for k, t in o.state[q].items() if k != "step"))
+    other.load_state_dict(saved)
+    assert types and all(t == torch.float32 for _, t in types)
+    assert torch.equal(other.state[q]["master"], saved["state"][0]["master"])
+    assert other.state[q]["master"] is not saved["state"][0]["master"]
