@@ -4,7 +4,9 @@
 //   p -= lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
 //
 // Parameters and gradients are float32, bfloat16 or float16; a 16-bit parameter
-// has a float32 master copy that the step is made on, and is its rounding.  The
+// has a float32 master copy that the step is made on, and is its rounding after it.
+// Where the parameter is something else before the step, it was written in between
+// (a checkpoint, a clamp), and the step goes on from that value.  The
 // states are float32, or 8 bits: float8 (e4m3) codes of m and of sqrt(v), each run
 // of 256 elements with a float32 scale that takes its largest element to 448.  The
 // root has half the exponent range of v, which e4m3's 2^18 covers; a nonzero one is
@@ -19,9 +21,11 @@
 // array moves in whole lines and the run's largest element is a reduction over the
 // wave; a block takes 16 runs of one tensor.  Tensors lie one behind another in
 // the grid, so small ones cost a block each and not a column of the largest's.
-// Bound by the bytes: 16 per element with 8-bit states, 28 with float32 (float32 200k
-// x 500 and 8-bit states: 1.65 GB in 303 to 352 us, 4.7 to 5.4 TB/s; 126 tensors of a
-// bfloat16 model, 1.38 GB, three launches in 313).
+// Bound by the bytes: 16 per float32 element with 8-bit states, 28 with float32 ones,
+// of 16-bit parameters 18 and 30 (two tables of 200k x 256 float32, 8-bit states: 1.65
+// GB in 314 to 316 us, 5.2 TB/s; the 76 tensors of twelve bfloat16 blocks of 512
+// channels, three launches: 1.56 GB in 349, 4.5 TB/s, of which reading the parameters
+// to see what was written to them is 35).
 #include <algorithm>
 
 #include "r2s_latent.h"
@@ -70,6 +74,10 @@ __device__ __forceinline__ float wave_max(float v) {
 
 __device__ __forceinline__ bool finite(float x) {
   return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
+}
+
+__device__ __forceinline__ bool same_bits(float a, float b) {
+  return __float_as_uint(a) == __float_as_uint(b);
 }
 
 // Four float8 codes <-> floats that are codes' values.
@@ -196,6 +204,13 @@ __device__ __forceinline__ void step_runs(const r2s_adamw_tensor_t &d, int64_t b
     float p[4], g[4], m[4], v[4];
     load4<T>(d.grad, i, d.n, vec, g);
     load4<float>(master, i, d.n, vec, p);
+    if constexpr (sizeof(T) == 2) {
+      float now[4];  // what the copy rounds to, or what was written since
+      load4<T>(d.param, i, d.n, vec, now);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        p[j] = same_bits(static_cast<float>(static_cast<T>(p[j])), now[j]) ? p[j] : now[j];
+    }
     if constexpr (!k8) {
       load4<float>(d.exp_avg, i, d.n, vec, m);
       load4<float>(d.second, i, d.n, vec, v);

@@ -187,7 +187,8 @@ class AdamW(torch.optim.Optimizer):
 
     The step is made in float32.  A 16-bit parameter keeps a float32 copy in its
     state (``master``), taken at its first step, and is that copy's rounding
-    after every step: what is written to the parameter in between is lost.  With
+    after every step; elements that are written in between are taken up by the
+    next, and go on from their new values.  With
     ``state_bits=32`` the states are torch's (``exp_avg``, ``exp_avg_sq``) and so
     is the arithmetic, bit for bit in float32.  With ``state_bits=8`` tensors of
     at least 4096 elements keep float8 codes of the average (``exp_avg``) and of

@@ -1129,7 +1129,8 @@ int r2s_adam_step_f32(const r2s_adam_tensor_t *tensors, int32_t n_tensors,
 
 /* One tensor of an AdamW step.  param and grad are of the element type;
  * master (float32) goes with a 16-bit param, which becomes its rounding, and is
- * NULL for a float32 one.  exp_avg and second are either float32 (the second the
+ * NULL for a float32 one; elements of param that are not the master's rounding
+ * before the step take their place in it.  exp_avg and second are either float32 (the second the
  * average of squares) with both scales NULL, or float8 e4m3 codes (the second
  * those of the square root of that average) with a float32 scale for every 256
  * elements: ceil(n / 256) each.  The step's scalars are the caller's:

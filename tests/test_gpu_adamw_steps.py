@@ -69,3 +69,43 @@ def test_a_refused_step_leaves_counts_states_and_parameters(dtype, bits):
     assert _same(_held(opt), _held(other))
     assert all(torch.equal(p, q) for p, q in zip(ps, others))
     assert [opt.state[p]["step"] for p in ps] == [2, 1, 2, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [50, 6001])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_what_is_written_to_a_16_bit_parameter_is_taken_up(dtype, n, bits):
+    """Between steps some elements are written, by whatever way, and the others keep
+    their copies' bits; a step after that goes on from the written values."""
+    g = torch.Generator().manual_seed(n + bits)
+    p = torch.randn(n, generator=g).to(dtype).to(DEV).requires_grad_(True)
+    opt = optim.AdamW([p], lr=1e-3, weight_decay=0.0, state_bits=bits)
+    for _ in range(3):
+        p.grad = torch.randn(n, generator=g).to(dtype).to(DEV)
+        opt.step()
+    master = opt.state[p]["master"]
+    assert not torch.equal(master, p.detach().float())  # holds more than the parameter
+    opt.param_groups[0]["lr"] = 0.0  # the step alone writes nothing now
+    p.grad = torch.zeros_like(p)
+    held, value = master.clone(), p.detach().clone()
+    opt.step()
+    assert torch.equal(master, held) and torch.equal(p.detach(), value)
+    written = torch.arange(n, device=DEV) % 7 == 3
+    with torch.no_grad():
+        p[written] = -2.5
+    p.data[0] = 0.0
+    p.data[5] = float("nan")
+    written[0] = written[5] = True
+    value = p.detach().clone()
+    opt.step()
+    want = torch.where(written, value.float(), held)
+    assert torch.equal(master.nan_to_num(9.0), want.nan_to_num(9.0))
+    assert torch.equal(p.detach().nan_to_num(9.0), value.nan_to_num(9.0))
+    # A model's checkpoint, loaded after the optimizer's.
+    fresh = torch.linspace(-3, 3, n, device=DEV).to(dtype)
+    with torch.no_grad():
+        p.copy_(fresh)
+    opt.step()
+    assert torch.equal(p.detach(), fresh)
+    same = held.to(dtype) == fresh  # there is nothing to tell these by
+    assert torch.equal(master[~same], fresh.float()[~same])
