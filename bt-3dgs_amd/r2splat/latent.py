@@ -70,8 +70,17 @@ class MixingBlock(torch.nn.Module):
         self.inward = new(4 * width, width)  # queries, keys, values, gates
         self.outward = new(width, width)
         self.post = torch.nn.Parameter(torch.ones(width, dtype=dtype))
-        reach = torch.linspace(5.0, 12.0, heads // 2).repeat(2)
+        reach = torch.linspace(5.0, 12.0, heads // 2, dtype=torch.float32).repeat(2)
         self.register_buffer("log_decay", torch.log1p(-torch.exp2(-reach)), persistent=False)
+
+    def _apply(self, fn, *args, **kwargs):
+        """Decays are float32 whatever the module is cast to: in eight bits a memory
+        of 4096 tokens would be one of another length, and the operator takes no other."""
+        decays = self.log_decay
+        super()._apply(fn, *args, **kwargs)
+        if self.log_decay.dtype != decays.dtype:
+            self.log_decay = decays.to(self.log_decay.device)
+        return self
 
     def forward(self, u: Tensor, positions: Tensor) -> Tuple[Tensor, Tensor]:
         n, width = u.shape
