@@ -85,7 +85,7 @@ class MixingBlock(torch.nn.Module):
     def forward(self, u: Tensor, positions: Tensor) -> Tuple[Tensor, Tensor]:
         n, width = u.shape
         q, k, v, gate = torch.nn.functional.linear(u, self.inward).split(width, dim=1)
-        q, k, v = (t.reshape(n, self.heads, -1) for t in (q, k, v))
+        q, k, v = (t.reshape(n, self.heads, width // self.heads) for t in (q, k, v))
         q, k = latent.rotary_axes(q, k, positions, self.sections)
         half = self.heads // 2
         mixed = [latent.decay_attention(*(t[None, :, part] for t in (q, k, v)),

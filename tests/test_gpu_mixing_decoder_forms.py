@@ -1,4 +1,5 @@
-"""A latent decoder with blocks on the GPU, cast after it was made."""
+"""A latent decoder with blocks on the GPU, cast after it was made and over an empty
+table."""
 
 import pytest
 import torch
@@ -34,3 +35,14 @@ def test_cast_after_it_was_made(dtype):
     grads = [torch.autograd.grad(o.float().square().sum(), list(m.parameters()))
              for o, m in zip(out, (decoder, made))]
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("blocks", [0, 2])
+def test_an_empty_table(blocks):
+    decoder = LatentDecoder(16, 3, width=24, heads=4, blocks=blocks).to(DEV)
+    out = decoder(*_inputs(0, 3, torch.float32))
+    assert out.shape == (0, 11)
+    grads = torch.autograd.grad(out.sum(), list(decoder.parameters()))
+    assert all(g.shape == p.shape and not g.any() for g, p in zip(grads, decoder.parameters()))
+    with torch.no_grad():
+        assert decoder(*_inputs(0, 3, torch.float32)).shape == (0, 11)
