@@ -1024,10 +1024,11 @@ __global__ __launch_bounds__((64 * W * Shape<T, KD, W, kStates>::kHeads),
 template <typename T, int V>
 __global__ __launch_bounds__(256) void decay_step_kernel(
     View q, View k, View v, const float *__restrict__ log_decay, const float *__restrict__ state,
-    int heads, int dk, int dv, float scale, T *__restrict__ y, float *__restrict__ next) {
+    int64_t first, int heads, int dk, int dv, float scale, T *__restrict__ y,
+    float *__restrict__ next) {
   __shared__ float s_q[kMostChannels], s_k[kMostChannels];
   __shared__ float s_sum[256 * V];
-  const int64_t which = blockIdx.x, sequence = which / heads;
+  const int64_t which = first + blockIdx.x, sequence = which / heads;
   const int head = static_cast<int>(which - sequence * heads);
   const T *qp = static_cast<const T *>(q.p) + sequence * q.token + head * q.head;
   const T *kp = static_cast<const T *>(k.p) + sequence * k.token + head * k.head;
@@ -1455,18 +1456,22 @@ int r2s_decay_attention_step(const void *q, int64_t q_token, int64_t q_head, con
     return R2S_ERANGE;
   }
   const bool wide = dv % 4 == 0 && (r2s::address(state) | r2s::address(next)) % 16 == 0;
-  const dim3 grid(static_cast<uint32_t>(sequences * heads));
   hipStream_t stream = r2s::as_stream(st);
   const int h = static_cast<int>(heads), a = static_cast<int>(dk), b = static_cast<int>(dv);
-  R2S_BY_TYPE(type, {
-    if (wide)
-      r2s::decay_step_kernel<T, 4><<<grid, dim3(256), 0, stream>>>(
-          vq, vk, vv, log_decay, state, h, a, b, scale, static_cast<T *>(y), next);
-    else
-      r2s::decay_step_kernel<T, 1><<<grid, dim3(256), 0, stream>>>(
-          vq, vk, vv, log_decay, state, h, a, b, scale, static_cast<T *>(y), next);
-  });
-  return r2s::check_launch("decay_attention_step");
+  constexpr int64_t kMost = r2s::most_blocks(256);
+  for (int64_t first = 0; first < sequences * heads; first += kMost) {
+    const dim3 grid(static_cast<uint32_t>(std::min(kMost, sequences * heads - first)));
+    R2S_BY_TYPE(type, {
+      if (wide)
+        r2s::decay_step_kernel<T, 4><<<grid, dim3(256), 0, stream>>>(
+            vq, vk, vv, log_decay, state, first, h, a, b, scale, static_cast<T *>(y), next);
+      else
+        r2s::decay_step_kernel<T, 1><<<grid, dim3(256), 0, stream>>>(
+            vq, vk, vv, log_decay, state, first, h, a, b, scale, static_cast<T *>(y), next);
+    });
+    R2S_RETURN_IF(r2s::check_launch("decay_attention_step"));
+  }
+  return R2S_OK;
 }
 
 }  // extern "C"

@@ -29,6 +29,9 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &x) {
   *reinterpret_cast<Pack<T, V> *>(p) = x;
 }
 
+// Blocks of one launch at most: a grid has fewer than 2^32 threads along a side.
+constexpr int64_t most_blocks(int threads) { return 0xFFFFFFFFll / threads; }
+
 inline int type_size(int type) { return type == R2S_TYPE_F32 ? 4 : 2; }
 inline bool known_type(int type) {
   return type == R2S_TYPE_F32 || type == R2S_TYPE_BF16 || type == R2S_TYPE_F16;

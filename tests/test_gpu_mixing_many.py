@@ -1,0 +1,31 @@
+"""The mixing operators where their blocks are more than one launch's grid has room
+for (2^32 threads): the same bits as the same call in two halves."""
+
+import pytest
+import torch
+
+from r2splat.ops import latent
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+GRID = 2 ** 32 // 256  # blocks of 256 threads that one launch does not hold
+
+
+@pytest.mark.parametrize("dv,dtype", [(4, torch.bfloat16), (1, torch.float32)])
+def test_step_of_more_states_than_a_grid_holds(dv, dtype):
+    h, dk = 8, 4
+    b = GRID // h + 3
+    torch.manual_seed(0)
+    q, k = (torch.randn(b, h, dk, device=DEV, dtype=dtype) for _ in range(2))
+    v = torch.randn(b, h, dv, device=DEV, dtype=dtype)
+    state = torch.randn(b, h, dk, dv, device=DEV)
+    log_decay = -torch.rand(h, device=DEV)
+    y, final = latent.decay_attention_step(q, k, v, log_decay, state)
+    for part in (slice(None, b // 2), slice(b // 2, None)):
+        y_part, final_part = latent.decay_attention_step(q[part], k[part], v[part], log_decay,
+                                                         state[part])
+        assert torch.equal(y[part], y_part) and torch.equal(final[part], final_part)
+    # The last sequence's, whose states are in the second launch.
+    want = torch.exp(log_decay)[:, None, None] * state[-1] + (
+        k[-1, :, :, None].float() * v[-1, :, None].float())
+    assert torch.allclose(final[-1], want, rtol=1e-6, atol=1e-6)
