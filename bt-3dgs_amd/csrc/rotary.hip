@@ -71,9 +71,9 @@ __device__ __forceinline__ double position(const void *p, int type, int64_t i) {
 template <typename T, int V>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(
     RotaryTensor q, RotaryTensor k, RotaryPlan plan, const void *__restrict__ positions,
-    int position_type, int64_t n, int tokens) {
+    int position_type, int64_t before, int64_t n, int tokens) {
   __shared__ float2 s_wheel[kRotaryPairs];
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * tokens;
+  const int64_t first = before + static_cast<int64_t>(blockIdx.x) * tokens;
   const int here = static_cast<int>(min(static_cast<int64_t>(tokens), n - first));
   const int pairs = plan.pairs;
   for (int i = threadIdx.x; i < here * pairs; i += kRotaryThreads) {
@@ -140,10 +140,14 @@ int launch_rotary(const RotaryTensor &q, const RotaryTensor &k, const RotaryPlan
   int64_t tokens = std::max<int64_t>(1, 8 * kRotaryThreads / std::max<int64_t>(items, 1));
   tokens = std::min<int64_t>(tokens, std::max<int64_t>(1, n / 1024));
   tokens = std::min<int64_t>(tokens, std::max(1, kRotaryPairs / std::max(plan.pairs, 1)));
-  rotary_kernel<T, V><<<dim3(static_cast<uint32_t>(ceil_div(n, tokens))), dim3(kRotaryThreads), 0,
-                        stream>>>(q, k, plan, positions, position_type, n,
-                                  static_cast<int>(tokens));
-  return check_launch("rotary_axes");
+  const int64_t blocks = ceil_div(n, tokens), most = most_blocks(kRotaryThreads);
+  for (int64_t b = 0; b < blocks; b += most) {
+    rotary_kernel<T, V><<<dim3(static_cast<uint32_t>(std::min(most, blocks - b))),
+                          dim3(kRotaryThreads), 0, stream>>>(
+        q, k, plan, positions, position_type, b * tokens, n, static_cast<int>(tokens));
+    R2S_RETURN_IF(check_launch("rotary_axes"));
+  }
+  return R2S_OK;
 }
 
 // The largest element of a tensor that is read, and whether it fits an address.

@@ -29,3 +29,20 @@ def test_step_of_more_states_than_a_grid_holds(dv, dtype):
     want = torch.exp(log_decay)[:, None, None] * state[-1] + (
         k[-1, :, :, None].float() * v[-1, :, None].float())
     assert torch.allclose(final[-1], want, rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+def test_rotary_of_more_tokens_than_a_grid_holds(dtype):
+    """A block to a token from 513 pairs on.  One row of queries for all tokens, so
+    that only the outputs (34 GB) are large."""
+    n, pairs = GRID + 40, 513
+    torch.manual_seed(1)
+    row = torch.randn(1, 1, 2 * pairs, device=DEV, dtype=dtype)
+    places = torch.randint(0, 1000, (n, 1), device=DEV, dtype=torch.int32)
+    out, _ = latent.rotary_axes(row.expand(n, 1, 2 * pairs), None, places, (pairs,))
+    for part in (slice(0, 50), slice(GRID // 2, GRID // 2 + 50), slice(GRID - 30, None)):
+        count = places[part].shape[0]
+        want, _ = latent.rotary_axes(row.expand(count, 1, 2 * pairs), None, places[part], (pairs,))
+        assert torch.equal(out[part], want)
+    del out
+    torch.cuda.empty_cache()
