@@ -98,6 +98,7 @@ struct Walk {
   int32_t heads, column_blocks;
   uint32_t roles;
   uint32_t blocks, together;  // and how many of them one XCD takes in a row; 0: its share
+  uint32_t first;             // block of this launch
 };
 
 // A block's span of its sequence: tokens [at, at + count) of the walk's order.
@@ -703,8 +704,9 @@ __global__ __launch_bounds__((64 * W * Shape<T, KD, W, kStates>::kHeads),
   // Ragged items, long ones first, are dealt out to the XCDs in turn.
   uint32_t id = blockIdx.x;
   if (w.together == 0) {
-    id = xcd_swizzle(id, gridDim.x);
+    id = w.first + xcd_swizzle(id, gridDim.x);
   } else {
+    id += w.first;
     const uint32_t turn = id / 8;
     id = (turn / w.together * 8 + id % 8) * w.together + turn % w.together;
     if (id >= w.blocks) return;
@@ -1147,7 +1149,7 @@ int64_t table_bytes(const Sizes &z, const Plan &p) {
 }
 
 template <typename T, int KD, int W, bool kStates, bool kWhole>
-int launch_walk_as(const Walk &w, int64_t blocks, hipStream_t stream) {
+int launch_walk_as(Walk w, int64_t blocks, hipStream_t stream) {
   using S = Shape<T, KD, W, kStates>;
   constexpr int kLds = S::kLds * S::kHeads;
   static_assert(kLds + 2048 <= 160 * 1024, "LDS of a CU");
@@ -1160,9 +1162,16 @@ int launch_walk_as(const Walk &w, int64_t blocks, hipStream_t stream) {
       return R2S_EHIP;
     }
   }
-  decay_walk_kernel<T, KD, W, kStates, kWhole>
-      <<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * W * S::kHeads), kLds, stream>>>(w);
-  return check_launch("decay_attention");
+  constexpr int kBlock = 64 * W * S::kHeads;
+  constexpr int64_t kMost = most_blocks(kBlock) / 8 * 8;  // whole turns of the XCDs
+  for (int64_t first = 0; first < blocks; first += kMost) {
+    w.first = static_cast<uint32_t>(first);
+    decay_walk_kernel<T, KD, W, kStates, kWhole>
+        <<<dim3(static_cast<uint32_t>(std::min(kMost, blocks - first))), dim3(kBlock), kLds,
+           stream>>>(w);
+    R2S_RETURN_IF(check_launch("decay_attention"));
+  }
+  return R2S_OK;
 }
 template <typename T, int KD, int W, bool kStates>
 int launch_walk(const Walk &w, int64_t blocks, hipStream_t stream) {

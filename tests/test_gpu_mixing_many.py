@@ -4,6 +4,7 @@ for (2^32 threads): the same bits as the same call in two halves."""
 import pytest
 import torch
 
+from r2splat.cuda import _wrapper as W
 from r2splat.ops import latent
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +47,29 @@ def test_rotary_of_more_tokens_than_a_grid_holds(dtype):
         assert torch.equal(out[part], want)
     del out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_of_more_sequences_than_a_grid_holds(ragged):
+    b, d = GRID + 21, 2
+    torch.manual_seed(2)
+    q, k, v, v_y = (torch.randn(b, 1, d, device=DEV) for _ in range(4))
+    log_decay, scale = torch.tensor([-0.3], device=DEV), 0.7
+
+    def both(part):
+        """Outputs, last states and gradients of some of the sequences, of a token each."""
+        args = [t[part] for t in (q, k, v, v_y)]
+        count = args[0].shape[0]
+        offsets = torch.arange(count + 1, device=DEV, dtype=torch.int32) if ragged else None
+        args = args if ragged else [t[:, None] for t in args]
+        y, final, kept = W.decay_attention_fwd(*args[:3], log_decay, None, offsets, False, scale)
+        grads = W.decay_attention_bwd(*args[:3], log_decay, None, offsets, kept, args[3], None,
+                                      False, scale)
+        return [t.reshape(count, -1) for t in (y, final, *grads)]
+
+    got = both(slice(None))
+    for part in (slice(None, b // 2), slice(b // 2, None)):
+        assert all(torch.equal(a[part], w) for a, w in zip(got, both(part)))
+    score = scale * (q * k).sum(-1)
+    assert torch.allclose(got[0], score * v[:, 0], rtol=1e-5, atol=1e-5)
+    assert torch.allclose(got[4], score * v_y[:, 0], rtol=1e-5, atol=1e-5)
