@@ -38,6 +38,7 @@ constexpr int kRun = 256;           // elements of a scale: four for each lane o
 constexpr int kRunsPerWave = 4;
 constexpr int kPerBlock = kRun * kRunsPerWave * (kThreads / 64);
 constexpr int kMostTensors = 32;    // of a launch
+constexpr int64_t kMostBlocks = most_blocks(kThreads);
 constexpr float kMostCode = 448.0f, kLeastCode = 0x1p-9f, kLeastNormal = 0x1p-6f;
 
 struct AdamwTable {
@@ -285,8 +286,9 @@ int r2s_adamw_step(const r2s_adamw_tensor_t *tensors, int32_t n_tensors, r2s_str
                 "adamw_step: tensor %d: 16-bit parameters have a master, float32 ones none", i);
     R2S_REQUIRE((t.exp_avg_scale == nullptr) == (t.second_scale == nullptr),
                 "adamw_step: tensor %d has one scale of two", i);
-    if (t.n > (int64_t{1} << 40)) {
-      r2s::set_error("adamw_step: tensor %d is too large", i);
+    if (t.n > r2s::kMostBlocks * r2s::kPerBlock) {
+      r2s::set_error("adamw_step: tensor %d is too large: more than %lld elements", i,
+                     static_cast<long long>(r2s::kMostBlocks * r2s::kPerBlock));
       return R2S_ERANGE;
     }
   }
@@ -296,7 +298,7 @@ int r2s_adamw_step(const r2s_adamw_tensor_t *tensors, int32_t n_tensors, r2s_str
     for (; next < n_tensors && table.count < r2s::kMostTensors; ++next) {
       const int64_t more = r2s::ceil_div(tensors[next].n, r2s::kPerBlock);
       if (more == 0) continue;
-      if (blocks + more > r2s::kInt32Max) break;
+      if (blocks + more > r2s::kMostBlocks) break;
       table.t[table.count] = tensors[next];
       table.first[table.count++] = static_cast<uint32_t>(blocks);
       blocks += more;
