@@ -24,8 +24,8 @@
 // Bound by the bytes: 16 per float32 element with 8-bit states, 28 with float32 ones,
 // of 16-bit parameters 18 and 30 (two tables of 200k x 256 float32, 8-bit states: 1.65
 // GB in 314 to 316 us, 5.2 TB/s; the 76 tensors of twelve bfloat16 blocks of 512
-// channels, three launches: 1.56 GB in 349, 4.5 TB/s, of which reading the parameters
-// to see what was written to them is 35).
+// channels, three launches: 1.56 GB in 336, 4.6 TB/s, two bytes of an element for
+// reading the parameters to see what was written to them).
 #include <algorithm>
 
 #include "r2s_latent.h"
@@ -184,7 +184,13 @@ __device__ __forceinline__ void step8(const r2s_adamw_tensor_t &d, float m_scale
   m = m * m_scale;
   m = d.beta1 * m + d.lerp_weight * g;
   r = r * r_scale;
-  r = sqrtf(d.beta2 * r * r + d.one_minus_beta2 * g * g);
+  const float square = d.beta2 * r * r + d.one_minus_beta2 * g * g;
+  if (square == __builtin_inff()) {  // the squares' sum, or an infinite gradient's root too
+    const float small = r * 0x1p-66f, g_small = g * 0x1p-66f;
+    r = sqrtf(d.beta2 * small * small + d.one_minus_beta2 * g_small * g_small) * 0x1p66f;
+  } else {
+    r = sqrtf(square);
+  }
 }
 
 template <typename T, bool k8>

@@ -109,3 +109,33 @@ def test_what_is_written_to_a_16_bit_parameter_is_taken_up(dtype, n, bits):
     assert torch.equal(p.detach(), fresh)
     same = held.to(dtype) == fresh  # there is nothing to tell these by
     assert torch.equal(master[~same], fresh.float()[~same])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_finite_gradients_leave_8_bit_states_finite(dtype):
+    """The square of a gradient beyond 1.8e19 is none of float32's numbers, its root is:
+    sqrt(beta2) to a step of it, times the codes' step at the least."""
+    p = torch.zeros(8192, device=DEV, dtype=dtype, requires_grad=True)
+    opt = optim.AdamW([p], lr=1e-2, betas=(0.9, 0.99), weight_decay=0.0, state_bits=8)
+    large = torch.tensor([1e19, 2e19, 1e25, 1e30, -3e38], device=DEV)
+    at = torch.tensor([300, 1000, 2001, 4100, 8000], device=DEV)  # runs of their own
+    root = torch.zeros(5, device=DEV, dtype=torch.float64)
+    mean = torch.zeros(5, device=DEV, dtype=torch.float64)
+    for step in range(3):
+        p.grad = torch.ones_like(p)
+        p.grad[at] = large.to(dtype) if step < 2 else torch.ones(5, device=DEV, dtype=dtype)
+        g = p.grad[at].double()
+        opt.step()
+        s = opt.state[p]
+        root = (0.99 * root ** 2 + 0.01 * g ** 2).sqrt()
+        mean = 0.9 * mean + 0.1 * g
+        for name, exact in (("exp_avg", mean), ("exp_avg_sq_root", root)):
+            assert torch.isfinite(s[name].float()).all() and torch.isfinite(s[name + "_scale"]).all()
+            found = s[name].float()[at].double() * s[name + "_scale"][at // 256].double()
+            # The largest of its run has the largest code, 448, and no chance: what is
+            # off is the scale's roundings alone, a few units of float32 a step.
+            assert ((found - exact).abs() <= (step + 1) * 16 * 2.0 ** -24 * exact.abs()).all(), name
+        assert torch.isfinite(p.detach()).all()
+    # lr mean / root, corrected: 0.1 / 0.1 in the first step.  (A root beyond 2^126 has
+    # no reciprocal among float32's normal numbers: no step.)
+    assert (p.detach()[at[:4]].float().abs() > 0.5e-2).all()
