@@ -21,20 +21,26 @@
 // decay a state behind its token, g^i and g^(C-j) above.  g R after the last token is
 // the first state's gradient.
 //
-// A block is one head and up to 16 W columns of v of one span of a sequence.  Each of
-// its W waves keeps the state's rows of 16 columns in registers and brings them up to
-// date; the outputs are shared out by tokens instead, so that each score is made
-// once, and every wave reads the state of all columns, as operands, from LDS.  The
-// products are made transposed (scores as k q^T, outputs as v^T p): then an
+// A block is one head and up to 16 W columns of v of one span of a sequence (of heads
+// up to 16 channels, four heads of a wave each).  Each of a head's W waves keeps the
+// state's rows of 16 columns in registers and brings them up to date; the outputs are
+// shared out by tokens instead, so that each score is made once for up to 64 columns,
+// and every wave reads the state of all the block's columns, as operands, from LDS.
+// The products are made transposed (scores as k q^T, outputs as v^T p): then an
 // accumulator's values are, lane by lane, the next product's operand, and a lane
 // ends with neighbouring columns of one token.
 //
 // Precision: the scores, the state and the decayed v are float32 values.  As
-// operands of 16-bit products they are split into a rounded part and a rounded
-// rest (the decayed v, which adds up in the state, into three), a product for
-// each, so that nothing is rounded to 16 bits but the outputs; float16 inputs
-// beside them, whose range does not hold those values, are split without loss into
-// bfloat16 parts.
+// operands of 16-bit products they are split into bfloat16 parts, each the rounding of
+// what the parts before leave, with a product for each.  The decayed v, which adds up
+// in the float32 state, has three, which hold its 24 bits.  Scores and state, whose
+// products end in a 16-bit output, have two: these leave out at most 2^-17 of a value,
+// where the output's own rounding is 2^-8 (bfloat16) or 2^-11 (float16).  Three there
+// take 335 us where two take 303 (8 x 4096 x 16 x 64 bfloat16, both ways) and 127
+// where 118 (500k x 4 x 16, forward).  float16 inputs beside them, whose range does not
+// hold those values, are split without loss into two bfloat16 parts, at a product more
+// for each: 446 us both ways of the former where bfloat16 takes 299, and 123 forward of
+// the latter where 98.
 //
 // A zero weight times a NaN or an infinity is a NaN: a chunk with such a v would
 // reach back to its earlier tokens.  Its tokens are walked one by one.
@@ -674,15 +680,17 @@ struct Shape {
 };
 
 // The walk.  8 sequences of 4096 tokens, 16 heads of 64 bfloat16: the spans' own
-// states 29 us, the forward's walk 61 (4.4 TB/s of q, k, v and y), the backward's three
-// roles 175.  What bounds it is not the memory: with all inputs in the cache the
+// states 29 to 34 us, the forward's walk 60 to 70 (3.8 to 4.5 TB/s of q, k, v and y), the
+// backward's three roles 164 to 188.  What bounds it is not the memory: with all inputs in the cache the
 // walk takes as long.  A wave issues some 330 vector, 65 LDS and 58 matrix
 // instructions for a chunk, between two barriers that three blocks of a CU have to
 // cover for each other; a fourth does not fit the registers (107 us for the whole
 // forward, with spills, against 99).  500k tokens of 4 heads of 16: 26 and 60 us, where
 // rows of 32 bytes and one wave to a head are the bound.  float32: the matrix cores,
 // at 1/8 of the 16-bit rate, are busy half of the time; three bfloat16 products in
-// place of a float32 one took 479 us at 8 x 4096 x 8 x 128, these 360.
+// place of a float32 one took 479 us at 8 x 4096 x 8 x 128, these 354 to 371.  Odd widths
+// above 128 in float32 are past the registers (272 bytes of scratch a lane): 4 x 4096 x
+// 4 x 131 takes 586 us forward, 132 channels 334.
 template <typename T, int KD, int W, bool kStates, bool kWhole>
 __global__ __launch_bounds__((64 * W * Shape<T, KD, W, kStates>::kHeads),
                              (Shape<T, KD, W, kStates>::kPerSimd)) void decay_walk_kernel(Walk w) {

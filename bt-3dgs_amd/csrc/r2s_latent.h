@@ -1,6 +1,6 @@
 // Shared pieces of the latent decoder's operators (lookup.hip, gated_scan.hip,
-// grouped.hip, rotary.hip, residual_norm.hip) and of adamw.hip: element types, vectors of them, and the
-// stable sort of ids that group.hip provides.
+// grouped.hip, rotary.hip, residual_norm.hip, decay_attention.hip) and of adamw.hip:
+// element types, vectors of them, and the stable sort of ids that group.hip provides.
 #pragma once
 
 #include <initializer_list>

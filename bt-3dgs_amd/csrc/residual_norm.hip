@@ -267,9 +267,9 @@ __device__ __forceinline__ void widen(const Loose<T, Row<T, E>::V> (&raw)[E], Ro
     for (int i = 0; i < Row<T, E>::V; ++i) x.v[e][i] = static_cast<float>(raw[e].v[i]);
 }
 
-// 32k x 1024 bfloat16 with a gate of every row: 335 MB in 56 us (6.0 TB/s, some of it
-// from the last-level cache); 300k x 45 float32 37 us (5.8 TB/s); 4k x 64 float32 4 us,
-// the launch's own.  Bound by the bytes.
+// 32k x 1024 bfloat16 with a gate of every row: 335 MB in 70 to 73 us (4.6 to 4.8 TB/s);
+// 300k x 45 float32 39 to 42 us (5.2 to 5.5 TB/s); 4k x 64 float32 4 us, the launch's
+// own.  Bound by the bytes.
 template <typename T, int E, bool kWide, int kThreads, int kGate, int kEnd>
 __global__ __launch_bounds__(kThreads) void residual_norm_fwd_kernel(NormArgs a, int bits) {
   __shared__ float2 s_sums[2 * (kThreads / 64)];
@@ -350,8 +350,10 @@ __device__ __forceinline__ void store_part(const RowOf<T, E, kWide, kThreads, kE
   }
 }
 
-// 32k x 1024 bfloat16 with a gate of every row: 537 MB in 116 to 131 us (4.1 to 4.6
-// TB/s); 300k x 45 float32 71 us (4.6 TB/s).  Between a row's loads and its stores lie
+// 32k x 1024 bfloat16 with a gate of every row: 537 MB in 117 to 131 us (4.1 to 4.6
+// TB/s); 300k x 45 float32 67 to 74 us (4.4 to 4.8 TB/s).  float32 rows of more than 4096
+// channels spill six registers, which the bytes cover (4096 x 8192: 245 us, as 8192 x
+// 4096).  Between a row's loads and its stores lie
 // four sums over its lanes in turn; with 16-bit rows' eight elements to a lane three
 // waves of a SIMD are what the registers hold to cover them (eight waves of four
 // elements: 234 us against 154).
