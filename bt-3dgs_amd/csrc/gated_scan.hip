@@ -1545,7 +1545,7 @@ int check_scan(const char *what, int type, const int32_t *offsets, int64_t n, in
 
 // The limits of a plan: grid sizes, and the 32-bit lane offsets of Rows.
 int check_plan(const char *what, int type, const Plan &p, std::initializer_list<int64_t> strides) {
-  bool fits = p.blocks * p.slices <= kInt32Max && p.c.strip < (1 << 23);
+  bool fits = p.blocks * p.slices <= most_blocks(p.threads) && p.c.strip < (1 << 23);
   for (int64_t s : strides)
     fits &= s * type_size(type) * p.c.strip * (64 >> p.c.lane_bits) <= 0xffffffffll;
   if (!fits) {
@@ -1557,10 +1557,17 @@ int check_plan(const char *what, int type, const Plan &p, std::initializer_list<
 
 int64_t states(const Tokens &c) { return static_cast<int64_t>(c.sequences) * c.width; }
 
+int check_states(int64_t blocks, int threads) {
+  if (blocks <= most_blocks(threads)) return R2S_OK;
+  set_error("gated_scan: more states than a grid of 2^32 threads holds");
+  return R2S_ERANGE;
+}
+
 // A launch for the sequences without a token, where there can be any.
 int empty_states(const Tokens &c, const float *in, float *out, hipStream_t stream) {
   const int64_t blocks = ceil_div(states(c), kThreads);
   if (out == nullptr || blocks == 0 || (c.offsets == nullptr && c.length > 0)) return R2S_OK;
+  R2S_RETURN_IF(check_states(blocks, kThreads));
   scan_empty_kernel<<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream>>>(c, in,
                                                                                          out);
   return check_launch("gated_scan empty sequences");
@@ -1573,13 +1580,14 @@ template <typename T, int V, bool kBack>
 int packed_maps(const Plan &p, const T *a, int64_t as, const T *b, int64_t bs, const float *state,
                 const float *empty_in, float *empty_out, const ScanSpace &s, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.blocks * p.slices));
+  const int64_t channel_blocks = ceil_div(p.c.width, kCarryCols);
+  const int64_t empty_blocks =
+      p.c.offsets != nullptr && empty_out != nullptr ? ceil_div(states(p.c), 1024) : 0;
+  R2S_RETURN_IF(check_states(channel_blocks + empty_blocks, 1024));
   scan_maps_kernel<T, V, kBack><<<grid, dim3(kThreads), kThreads * V * 2 * sizeof(float),
                                   stream>>>(a, as, b, bs, state, p.c, p.slices, s.strips,
                                             s.blocks);
   R2S_RETURN_IF(check_launch("gated_scan maps"));
-  const int64_t channel_blocks = ceil_div(p.c.width, kCarryCols);
-  const int64_t empty_blocks =
-      p.c.offsets != nullptr && empty_out != nullptr ? ceil_div(states(p.c), 1024) : 0;
   scan_carry_kernel<<<dim3(static_cast<uint32_t>(channel_blocks + empty_blocks)), dim3(1024), 0,
                       stream>>>(reinterpret_cast<const float2 *>(s.blocks),
                                 static_cast<int32_t>(p.blocks), p.c, kBack ? 1 : 0,
@@ -1597,7 +1605,7 @@ int scan_fwd(const Plan &p, const void *x, int64_t xs, const void *g, int64_t gs
   T *y = static_cast<T *>(y_);
   if (c.offsets == nullptr && c.length == 1) {
     const int64_t blocks = ceil_div(c.n * (c.width / V), kThreads);
-    if (blocks > kInt32Max) {
+    if (blocks > most_blocks(kThreads)) {
       set_error("gated_scan_fwd: too many tokens");
       return R2S_ERANGE;
     }

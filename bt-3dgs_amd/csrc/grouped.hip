@@ -814,7 +814,7 @@ int rows_launch(const T *in, int64_t stride, const T *weight, const T *bias, Gro
   const int64_t inner = kBack ? m : k, outer = kBack ? k : m;
   const int64_t col_tiles = ceil_div(outer, kCols);
   const int64_t blocks = (ceil_div(g.n, kRows) + g.count + 1) * col_tiles;
-  if (blocks > kInt32Max) {
+  if (blocks > most_blocks(kThreads)) {
     set_error("grouped_matmul: too many tiles");
     return R2S_ERANGE;
   }
@@ -862,7 +862,7 @@ int weights_launch(const T *x, int64_t x_stride, const T *v_y, int64_t v_stride,
   const int64_t slots = part_slots(g.n, k, m, g.count, sizeof(T));
   const uint32_t places = static_cast<uint32_t>(part_places(g.n, k, m, g.count, sizeof(T)));
   const int64_t m_tiles = ceil_div(m, kRows), k_tiles = ceil_div(std::max<int64_t>(k, 1), kCols);
-  if (slots * m_tiles * k_tiles > kInt32Max) {
+  if (slots * m_tiles * k_tiles > most_blocks(kThreads)) {
     set_error("grouped_matmul_bwd: too many tiles");
     return R2S_ERANGE;
   }

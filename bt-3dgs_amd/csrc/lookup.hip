@@ -317,7 +317,7 @@ int lookup_fwd(const void *table, int64_t stride, const void *ids, float scale, 
   static_assert(per_block <= 4096, "vector numbers of a block below 2^13");
   const int64_t vpr = ceil_div(width, V);
   const int64_t rows = std::max<int64_t>(per_block / vpr, 1), slices = ceil_div(vpr, per_block);
-  if (ceil_div(n, rows) > kInt32Max || slices > 65535) {
+  if (ceil_div(n, rows) > most_blocks(kThreads) || slices > 65535) {
     set_error("embedding_fwd: output too large");
     return R2S_ERANGE;
   }
@@ -333,8 +333,9 @@ int lookup_fwd(const void *table, int64_t stride, const void *ids, float scale, 
 }
 
 template <typename T, int V>
-int lookup_bwd(const void *v_out, int64_t stride, float scale, int64_t n, int64_t n_rows,
-               int64_t width_, void *v_table_, const BwdSpace &s, hipStream_t stream) {
+int lookup_bwd(const void *v_out, int64_t stride, const void *ids, bool wide, float scale,
+               int64_t n, int64_t n_rows, int64_t width_, void *v_table_, const BwdSpace &s,
+               hipStream_t stream) {
   T *v_table = static_cast<T *>(v_table_);
   const uint32_t width = static_cast<uint32_t>(width_), vpr = (width + V - 1) / V;
   uint32_t bits = 0;
@@ -343,6 +344,16 @@ int lookup_bwd(const void *v_out, int64_t stride, float scale, int64_t n, int64_
   const Sorted list{s.keys, s.order, s.offsets, static_cast<uint32_t>(n),
                     chunk_entries(n, int64_t{slices} << bits)};
   const int64_t chunks = ceil_div(n, list.chunk);
+  // Block b < n_long reads entry (b + 1) kLongRow chunk, the first of a chunk
+  // that there is.
+  const int64_t n_long = chunks > 0 ? (chunks - 1) / kLongRow : 0;
+  const int64_t row_blocks = n_long + ceil_div(n_rows, row_threads(V) >> bits);
+  if (ceil_div(chunks, kThreads >> bits) > most_blocks(kThreads) ||
+      row_blocks > most_blocks(row_threads(V))) {
+    set_error("embedding_bwd: more ids or rows than a grid of 2^32 threads holds");
+    return R2S_ERANGE;
+  }
+  R2S_RETURN_IF(sort_ids(ids, wide, n, n_rows, s.order, s.offsets, s.keys, s.sort, stream));
   if (n > 0) {
     lookup_bwd_chunks_kernel<T, V>
         <<<dim3(static_cast<uint32_t>(ceil_div(chunks, kThreads >> bits)), slices),
@@ -351,12 +362,8 @@ int lookup_bwd(const void *v_out, int64_t stride, float scale, int64_t n, int64_
                                         s.partial);
     R2S_RETURN_IF(check_launch("embedding_bwd"));
   }
-  // Block b < n_long reads entry (b + 1) kLongRow chunk, the first of a chunk
-  // that there is.
-  const int64_t n_long = chunks > 0 ? (chunks - 1) / kLongRow : 0;
   lookup_bwd_rows_kernel<T, V>
-      <<<dim3(static_cast<uint32_t>(n_long + ceil_div(n_rows, row_threads(V) >> bits)),
-              slices),
+      <<<dim3(static_cast<uint32_t>(row_blocks), slices),
          dim3(row_threads(V)), 0, stream>>>(list, scale, static_cast<uint32_t>(n_rows), width, bits,
                                          static_cast<uint32_t>(n_long), s.partial, v_table);
   return check_launch("embedding_bwd rows");
@@ -436,8 +443,6 @@ int r2s_embedding_bwd(const void *v_out, int64_t v_out_stride, const void *ids,
   Carver cv(ws);
   const BwdSpace s = carve_bwd(cv, n, n_rows, width);
   hipStream_t stream = as_stream(st);
-  R2S_RETURN_IF(
-      sort_ids(ids, ids_are_64 != 0, n, n_rows, s.order, s.offsets, s.keys, s.sort, stream));
   // Eight vectors to a row where it has them: 300k x 16 bf16 of 3000 rows, forward
   // and back, 45 us with vectors of 4 bytes and 52 with 16, 400k x 3 f32 45 with
   // 4 bytes and 52 with 8.
@@ -445,7 +450,8 @@ int r2s_embedding_bwd(const void *v_out, int64_t v_out_stride, const void *ids,
   int bytes = run_bytes(width, size);
   while (bytes > size && ceil_div(width * size, bytes) < 8) bytes /= 2;
   R2S_BY_TYPE(type, R2S_BY_VECTOR(T, bytes, {
-    return (lookup_bwd<T, V>(v_out, v_out_stride, scale, n, n_rows, width, v_table, s, stream));
+    return (lookup_bwd<T, V>(v_out, v_out_stride, ids, ids_are_64 != 0, scale, n, n_rows, width,
+                             v_table, s, stream));
   }));
   return R2S_OK;
 }
